@@ -9,6 +9,7 @@ Public surface (mirrors src/fields_official/reference/field_only_v4_chunked_trit
 * ``IndependentVacancyField``, ``FieldBlock``, ``RMSNorm``, ``PackedSwiGLU``
 * ``field_scan`` (with state_in / state_out) and ``field_decode_step`` (decode token loop)
 * ``field_scan_norm`` / ``field_decode_norm_step``: the same with the mixer's read_norm fused
+* ``token_logprobs`` (loss and scoring), ``grad_norm``, ``adamw_step`` / ``AdamW`` (the end of a training step)
 """
 from .field import (  # noqa: F401
     ScanPlan,
@@ -38,5 +39,7 @@ from .model import (  # noqa: F401,E402
     FieldTokenSystem,
     build_official_fields,
 )
+from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401,E402
+from .optim import AdamW, adamw_step, grad_norm  # noqa: F401,E402
 
 __version__ = "0.1.0"

@@ -8,6 +8,7 @@ There is no fallback: if the library is missing, every entry point raises Runtim
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import weakref
@@ -97,6 +98,16 @@ SIGNATURES = {
     "fl_softpatch_workspace_bytes": (_sz, [_i64] * 3),
     "fl_softpatch_scan": (_int, [_vp] * 3 + [_i64] * 3 + [_vp, _vp, _vp, _sz, _vp]),
     "fl_boundary_scan": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
+    "fl_token_logprobs_workspace_bytes": (_sz, [_i64] * 3),
+    "fl_token_logprobs": (_int, [_vp, _int] + [_i64] * 5 + [_vp] + [_i64] * 3 + [ctypes.c_float, _i64] + [_vp] * 6 +
+                          [_sz, _vp]),
+    "fl_token_logprobs_backward": (_int, [_vp, _int] + [_i64] * 5 + [_vp] + [_i64] * 3 + [ctypes.c_float, _i64] +
+                                   [_vp] * 8),
+    "fl_grad_norm_workspace_bytes": (_sz, [_i64, _vp]),
+    "fl_grad_norm": (_int, [_i64, _vp, _vp, _vp, ctypes.c_float, _int, _vp, _vp, _sz, _vp]),
+    "fl_adamw_workspace_bytes": (_sz, [_i64]),
+    "fl_adamw_step": (_int, [_i64, _vp, _vp, _int] + [_vp] * 6 + [ctypes.c_double, _vp] + [ctypes.c_double] * 4 +
+                      [_vp, _vp, _sz, _vp]),
     "fl_version": (ctypes.c_char_p, []),
 }
 
@@ -161,6 +172,13 @@ def stream_handle(device: torch.device) -> int:
     call costs 2 us, a tenth of an eager scan call's host time."""
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None
                                               else torch.cuda.current_device())
+
+
+def on(device: torch.device):
+    """``device`` as the current one for a launch; nothing where it is that already."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
 
 
 # Workspace header (the C ABI, include/fields_amd.h): bytes 128..131 the error word, 384..387 the

@@ -43,6 +43,7 @@ from . import _native as nat
 from ._dispatch import KERNEL_DTYPES, eager, free_rounding, no_grad_needed, plain_call, plain_linear
 from .field import (FieldBlock, RMSNorm, _linear_residual, boundary_scan, gate_residual_norm, rms_norm,
                     rms_norm_takes, swiglu)
+from .logprobs import TokenLogprobs, token_logprobs
 
 # api:72-91
 OFFICIAL_ARCHITECTURE: Mapping[str, Any] = {
@@ -1229,6 +1230,16 @@ class FieldsForCausalLM(nn.Module):
             raise TypeError("labels must match input_ids shape and use torch.long")
         raise NotImplementedError(
             "loss_and_stats (PCAF routing, training) is not rebuilt: this build is inference only")
+
+    @torch.no_grad()
+    def score(self, input_ids: torch.Tensor, *, temperature: float = 1.0, top_k: int = 0,
+              entropy: bool = False) -> TokenLogprobs:
+        """Log probability of every token but the first given the ones before it, [B, T - 1], with the
+        distributions' entropies and top alternatives where asked (:func:`token_logprobs`)."""
+        if input_ids.ndim != 2 or input_ids.dtype != torch.long:
+            raise TypeError("input_ids must be a rank-2 torch.long tensor [batch, time]")
+        logits = self.core_model.states_logits(input_ids)[1]
+        return token_logprobs(logits[:, :-1], input_ids[:, 1:], temperature=temperature, top_k=top_k, entropy=entropy)
 
     @torch.no_grad()
     def prefill(self, input_ids: torch.Tensor, max_len: int):

@@ -1,0 +1,275 @@
+"""What follows a training step's backward, on the HIP path only (``csrc/optimizer.hip``):
+
+* :func:`grad_norm`   the 2-norm over many gradients and the scale that clips it, in one pass over them;
+* :func:`adamw_step`  one AdamW step over many tensors, moments in fp32 or in 8 bits;
+* :class:`AdamW`      the optimizer around both.
+
+Nothing here waits for the device: norms and scales stay there, step counters too, so a step can be captured
+in a HIP graph and replayed.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as nat
+
+STATE_BLOCK = 256                   # values that share a scale in the 8-bit states
+STATE8_DTYPE = torch.float8_e4m3fn  # their codes
+
+_CODES = {torch.float32: nat.FL_DTYPE_F32, torch.bfloat16: nat.FL_DTYPE_BF16}
+
+
+def _addresses(tensors: Sequence[torch.Tensor]):
+    return (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+
+
+def _counts(tensors: Sequence[torch.Tensor]):
+    return (ctypes.c_int64 * len(tensors))(*[t.numel() for t in tensors])
+
+
+def _plain(t: torch.Tensor, what: str) -> torch.Tensor:
+    if t.layout != torch.strided:
+        raise TypeError(f"{what} must be dense")
+    return t
+
+
+@torch.no_grad()
+def grad_norm(grads: Iterable[torch.Tensor], max_norm: Optional[float] = None
+              ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """2-norm over all values of ``grads`` (fp32 / bf16, any mix, on one ROCm device): fp32 0-d, summed in
+    64 bits in a fixed order.
+
+    With ``max_norm`` also the scale that clips it, min(1, max_norm / (norm + 1e-6)), which
+    :func:`adamw_step` takes as ``grad_scale``; the gradients are not rewritten. The scale of a norm that is
+    not finite is NaN, on which :func:`adamw_step` leaves everything as it was.
+    """
+    lib = nat.load()
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no gradients")
+    device = grads[0].device
+    if device.type != "cuda":
+        raise RuntimeError("grad_norm requires a ROCm (cuda) device")
+    if max_norm is not None and not float(max_norm) >= 0.0:
+        raise ValueError(f"max_norm must be 0 or more, got {max_norm}")
+    codes = []
+    for i, g in enumerate(grads):
+        code = _CODES.get(g.dtype)
+        if code is None:
+            raise TypeError(f"gradients must be float32 or bfloat16, got {g.dtype}")
+        if g.device != device:
+            raise ValueError("the gradients must be on one device")
+        if not _plain(g, "gradients").is_contiguous():
+            grads[i] = g.contiguous()
+        codes.append(code)
+    numel = _counts(grads)
+    out = torch.empty(2, device=device, dtype=torch.float32)
+    ws = torch.empty(max(1, int(lib.fl_grad_norm_workspace_bytes(len(grads), numel))), device=device, dtype=torch.uint8)
+    with nat.on(device):
+        nat.check(lib.fl_grad_norm(
+            len(grads), _addresses(grads), (ctypes.c_int * len(codes))(*codes), numel,
+            0.0 if max_norm is None else float(max_norm), max_norm is not None, nat.ptr(out), nat.ptr(ws), ws.numel(),
+            nat.stream_handle(device)), "fl_grad_norm")
+    return out[0] if max_norm is None else (out[0], out[1])
+
+
+def _device_scalar(t: torch.Tensor, what: str, device: torch.device) -> int:
+    if t.numel() != 1 or t.dtype != torch.float32 or t.device != device:
+        raise ValueError(f"{what} must be one float32 value on {device}")
+    return t.data_ptr()
+
+
+def _check_hyper(lr, betas, eps, weight_decay) -> None:
+    if not isinstance(lr, torch.Tensor) and not (float(lr) >= 0.0 and math.isfinite(lr)):
+        raise ValueError(f"lr must be finite and 0 or more, got {lr}")
+    if not all(0.0 <= float(b) < 1.0 for b in betas):
+        raise ValueError(f"betas must lie in [0, 1), got {tuple(betas)}")
+    if not (float(eps) >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"eps must be finite and 0 or more, got {eps}")
+    if not (float(weight_decay) >= 0.0 and math.isfinite(weight_decay)):
+        raise ValueError(f"weight_decay must be finite and 0 or more, got {weight_decay}")
+
+
+@torch.no_grad()
+def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
+               exp_avg_sqs: Sequence[torch.Tensor], steps: Union[torch.Tensor, Sequence[torch.Tensor]], *,
+               lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, grad_scale: Optional[torch.Tensor] = None,
+               exp_avg_scales: Optional[Sequence[torch.Tensor]] = None,
+               exp_avg_sq_scales: Optional[Sequence[torch.Tensor]] = None) -> None:
+    """One AdamW step over all tensors, in place (``fl_adamw_step``). With g = grad * grad_scale and t the
+    tensor's step counter, advanced first:
+
+        m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v / (1 - beta2^t)) + eps)
+
+    params: contiguous, all fp32 or all bf16, on one ROCm device; grads of their shapes and type. Maths in
+    fp32, a bf16 parameter rounded once. steps: an int64 value per tensor, one tensor [N] or N of one value.
+    lr: a number, or one fp32 value on the device, read when the step runs.
+
+    Without scales exp_avgs / exp_avg_sqs are contiguous fp32 tensors of the parameters' sizes. With scales they
+    hold 8 bits a value: float8_e4m3fn codes of m and of sqrt(v) in blocks of 256 consecutive values, whose
+    largest magnitude / 448 is the block's fp32 scale ([ceil(numel / 256)]); zeros are a valid start. A root
+    that is not 0 keeps at least the smallest code. A non-finite value in a gradient spoils its block's states.
+
+    grad_scale: one fp32 value on the device (:func:`grad_norm`'s second), or None for 1. Where it is not finite the
+    call leaves parameters, states and step counters as they were.
+    """
+    lib = nat.load()
+    n = len(params)
+    if n == 0:
+        raise ValueError("no parameters")
+    eight = exp_avg_scales is not None
+    if eight != (exp_avg_sq_scales is not None):
+        raise ValueError("8-bit states need the scales of both moments")
+    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n
+            and (not eight or len(exp_avg_scales) == len(exp_avg_sq_scales) == n)):
+        raise ValueError("one gradient and one state of each kind per parameter")
+    _check_hyper(lr, betas, eps, weight_decay)
+    device, dtype = params[0].device, params[0].dtype
+    if device.type != "cuda":
+        raise RuntimeError("adamw_step requires a ROCm (cuda) device")
+    code = _CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
+    state_dtype = STATE8_DTYPE if eight else torch.float32
+    grads = list(grads)
+    numel = []
+    for i, (p, g, m, v) in enumerate(zip(params, grads, exp_avgs, exp_avg_sqs)):
+        if p.dtype != dtype or g.dtype != dtype:
+            raise TypeError(f"parameters and gradients must have one type, got {p.dtype} and {g.dtype} beside {dtype}")
+        if m.dtype != state_dtype or v.dtype != state_dtype:
+            raise TypeError(f"states must be {state_dtype}, got {m.dtype} and {v.dtype}")
+        if not (p.device == g.device == m.device == v.device == device):
+            raise ValueError("parameters, gradients and states must be on one device")
+        count = p.numel()
+        if g.shape != p.shape or m.numel() != count or v.numel() != count:
+            raise ValueError(f"parameter {i}: {tuple(p.shape)} with gradient {tuple(g.shape)} and states of "
+                             f"{m.numel()} and {v.numel()} values")
+        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
+            raise ValueError(f"parameter {i} and its states must be contiguous")
+        if not _plain(g, "gradients").is_contiguous():
+            grads[i] = g.contiguous()
+        numel.append(count)
+    if eight:
+        for i, (a, b) in enumerate(zip(exp_avg_scales, exp_avg_sq_scales)):
+            blocks = -(-numel[i] // STATE_BLOCK)
+            for s in (a, b):
+                if s.dtype != torch.float32 or s.device != device or s.numel() != blocks or not s.is_contiguous():
+                    raise ValueError(f"parameter {i}: scales must be {blocks} contiguous float32 values on {device}")
+    if isinstance(steps, torch.Tensor):
+        if steps.dtype != torch.int64 or steps.device != device or steps.shape != (n,) or not steps.is_contiguous():
+            raise ValueError(f"steps must be {n} int64 values on {device}")
+        first = steps.data_ptr()
+        step_list = list(range(first, first + 8 * n, 8))
+    else:
+        if len(steps) != n or not all(s.dtype == torch.int64 and s.device == device and s.numel() == 1 for s in steps):
+            raise ValueError(f"steps must be {n} int64 values on {device}")
+        step_list = [s.data_ptr() for s in steps]
+    param_list = [p.data_ptr() for p in params]
+    kept = [a for a, c in zip(param_list, numel) if c]
+    if len(set(kept)) != len(kept) or len(set(step_list)) != n:
+        raise ValueError("a parameter or a step counter occurs twice")
+    scale = None if grad_scale is None else _device_scalar(grad_scale, "grad_scale", device)
+    lr_ptr, lr_value = (_device_scalar(lr, "lr", device), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
+    array = ctypes.c_void_p * n
+    ws = torch.empty(int(lib.fl_adamw_workspace_bytes(n)), device=device, dtype=torch.uint8)
+    with nat.on(device):
+        nat.check(lib.fl_adamw_step(
+            n, array(*param_list), _addresses(grads), code, _addresses(exp_avgs), _addresses(exp_avg_sqs),
+            _addresses(exp_avg_scales) if eight else None, _addresses(exp_avg_sq_scales) if eight else None,
+            (ctypes.c_int64 * n)(*numel), array(*step_list), lr_value, lr_ptr, float(betas[0]), float(betas[1]),
+            float(eps), float(weight_decay), scale, nat.ptr(ws), ws.numel(), nat.stream_handle(device)),
+            "fl_adamw_step")
+    torch.autograd.graph.increment_version(params)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over :func:`adamw_step`: one call per parameter group and type.
+
+    ``state_bits`` 32 keeps both moments in fp32 (8 bytes a value), 8 in 8-bit blocks (2 bytes and 1 / 32).
+    ``max_grad_norm`` clips the norm over all groups' gradients inside the step, without rewriting them; the norm
+    stays in ``self.grad_norm`` (fp32, on the device), and a step whose norm is not finite changes nothing.
+    A parameter without a gradient is left alone and its step not counted. States are made at a parameter's
+    first step, which must not be under graph capture.
+    """
+
+    def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 max_grad_norm: Optional[float] = None) -> None:
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
+            raise ValueError(f"max_grad_norm must be 0 or more, got {max_grad_norm}")
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+
+    def add_param_group(self, param_group) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            _check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+            if group["state_bits"] not in (8, 32):
+                raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+            for p in group["params"]:
+                if p.dtype not in _CODES:
+                    raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
+
+    def _state(self, p: torch.Tensor, bits: int) -> dict:
+        st = self.state[p]
+        if not st:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("a parameter's first step makes its states and must not be under graph capture")
+            new = dict(device=p.device)
+            st["step"] = torch.zeros((), dtype=torch.int64, **new)
+            if bits == 32:
+                st["exp_avg"], st["exp_avg_sq"] = (torch.zeros(p.shape, dtype=torch.float32, **new) for _ in range(2))
+            else:
+                blocks = -(-p.numel() // STATE_BLOCK)
+                for name in ("exp_avg", "exp_avg_sq"):
+                    st[name] = torch.zeros(p.shape, dtype=torch.uint8, **new).view(STATE8_DTYPE)
+                    st[name + "_scale"] = torch.zeros(blocks, dtype=torch.float32, **new)
+        return st
+
+    def load_state_dict(self, state_dict) -> None:
+        """As the base class, but every state keeps the type it was saved in."""
+        super().load_state_dict(state_dict)
+        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
+        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
+            if i in state_dict["state"]:
+                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                 for k, v in state_dict["state"][i].items()}
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        work: List[Tuple[dict, List[torch.Tensor]]] = []
+        for group in self.param_groups:
+            for dtype in _CODES:
+                ps = [p for p in group["params"] if p.grad is not None and p.dtype == dtype]
+                if ps:
+                    work.append((group, ps))
+        if not work:
+            return loss
+        scale = None
+        if self.max_grad_norm is not None:
+            self.grad_norm, scale = grad_norm([p.grad for _, ps in work for p in ps], self.max_grad_norm)
+        for group, ps in work:
+            bits = group["state_bits"]
+            states = [self._state(p, bits) for p in ps]
+            names = ("exp_avg_scale", "exp_avg_sq_scale")
+            scales = [[s[k] for s in states] for k in names] if bits == 8 else (None, None)
+            adamw_step(ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
+                       [s["step"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], grad_scale=scale, exp_avg_scales=scales[0],
+                       exp_avg_sq_scales=scales[1])
+        return loss

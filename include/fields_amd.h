@@ -466,6 +466,63 @@ int fl_state_update(const float* decay, const float* xdt, const float* bm, int64
                     int64_t P, int64_t N, float* ssm, void* ssm16, void* stream);
 int fl_mix(const void* y, const void* g, const void* mix_logit, int mix_dtype, int64_t n, void* out, void* stream);
 
+/*
+ * Log probabilities of given tokens with entropy and top alternatives, and their gradient (no counterpart in
+ * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V logits of dtype at
+ * logits + (r / inner) * stride_outer + (r % inner) * stride_inner (elements), its token tokens[(r / inner) *
+ * token_outer + (r % inner) * token_inner]. With m = max x, d_v = (x_v - m) / temperature, s = sum e^{d_v}:
+ *   logprobs [rows] = d_token - ln s; 0 where the token is ignore_index, NaN where it is outside 0 .. V - 1;
+ *   entropy [rows] or NULL = ln s - (sum e^{d_v} d_v) / s;
+ *   top_tokens / top_logprobs [rows, top_k]: the top_k (0 .. 64) largest logits, largest first, of equal ones the
+ *     lowest index first, NaN above all;
+ *   stats [rows, 2] or NULL: m and ln s, for the backward.
+ * A row of -inf alone: log probabilities -inf, entropy 0, gradient 0. A row with NaN or +inf: NaN.
+ * workspace: fl_token_logprobs_workspace_bytes(rows, V, top_k) bytes, 16-byte aligned, no initial contents
+ * needed (0 bytes: NULL will do).
+ *
+ * The backward takes the forward's stats, entropy (if g_entropy) and top_tokens (if g_top), and writes g_logits
+ * [rows, V], contiguous, of dtype; any of g_logprobs, g_entropy [rows], g_top [rows, top_k] may be NULL. A row
+ * whose gradients are all 0 gets zeros without its logits being read.
+ */
+size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int64_t top_k);
+int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V, int64_t stride_outer,
+                      int64_t stride_inner, const int64_t* tokens, int64_t token_outer, int64_t token_inner,
+                      int64_t ignore_index, float temperature, int64_t top_k, float* logprobs, float* entropy,
+                      float* top_logprobs, int64_t* top_tokens, float* stats, void* workspace, size_t workspace_bytes,
+                      void* stream);
+int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V,
+                               int64_t stride_outer, int64_t stride_inner, const int64_t* tokens, int64_t token_outer,
+                               int64_t token_inner, int64_t ignore_index, float temperature, int64_t top_k,
+                               const float* stats, const float* entropy, const int64_t* top_tokens,
+                               const float* g_logprobs, const float* g_entropy, const float* g_top, void* g_logits,
+                               void* stream);
+
+/*
+ * The end of a training step over n tensors (no counterpart in the reference, which calls the stock clip and
+ * fused AdamW). The lists of addresses, types and value counts are HOST arrays, read before the call returns;
+ * what they point to, and every other pointer, is on the device. Empty tensors may have NULL addresses.
+ *
+ * fl_grad_norm: out[0] = 2-norm over all values (fp32; 64-bit sums in a fixed order); scaled: out[1] =
+ *   min(1, max_norm / (norm + 1e-6)), NaN where the norm is not finite. Workspace 8-byte aligned.
+ * fl_adamw_step: with t = ++*steps[i], g = grad * *grad_scale (NULL: 1),
+ *     m = beta1 m + (1 - beta1) g;  v = beta2 v + (1 - beta2) g^2;
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v / (1 - beta2^t)) + eps),
+ *   p and g of dtype, all maths fp32 in separate products and sums. Where *grad_scale is not finite nothing is
+ *   written. lr_ptr: one fp32 value on the device that stands for lr, or NULL. Scales NULL: m and v are fp32.
+ *   Otherwise both are e4m3 codes, of m and of sqrt(v), in blocks of 256 consecutive values with one fp32 scale
+ *   (largest magnitude / 448) each; a root that is not 0 keeps at least the smallest code.
+ *   Workspace 16-byte aligned, no initial contents needed.
+ */
+size_t fl_grad_norm_workspace_bytes(int64_t n, const int64_t* numel);
+int fl_grad_norm(int64_t n, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm, int scaled,
+                 float* out, void* workspace, size_t workspace_bytes, void* stream);
+size_t fl_adamw_workspace_bytes(int64_t n);
+int fl_adamw_step(int64_t n, void* const* params, const void* const* grads, int dtype, void* const* exp_avgs,
+                  void* const* exp_avg_sqs, float* const* exp_avg_scales, float* const* exp_avg_sq_scales,
+                  const int64_t* numel, int64_t* const* steps, double lr, const float* lr_ptr, double beta1, double beta2,
+                  double eps, double weight_decay, const float* grad_scale, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
 /* Library version string (host function). No counterpart in the reference. */
 const char* fl_version(void);
 

@@ -1,0 +1,406 @@
+"""GPU: token log probabilities, entropy, top alternatives and their gradients against a plain float64 form.
+
+Tolerances count roundings, u = 2^-24. With D the largest |d| = |x - max| / temperature among logits that weigh
+anything (e^d > 2^-40 of the row's sum; the others' errors vanish in it), a power e^d carries (4 D + 4) u: the
+difference, two products and the base-2 argument each move d by D u at most, the power itself rounds twice. A sum of V of them
+carries that and its own additions, at most V / 256 + 64 u for any order that adds in at least 256 lanes. So with
+E = (4 D + V / 256 + 72) u: ln s is off by E + 2 u |ln s|; a log probability by that and 4 u |d_t|; an entropy by
+E (2 + 2 D), its sum of e^d d over s being two such sums with terms up to D; a weight p (relative) by
+2 E + 8 u D. A gradient is a sum of terms (|g|, p |a|, p |h| (|ln p| + H)) each with that relative error, and is
+rounded to its type (half a step, eps / 2) at the end.
+"""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fields_lm_amd as fl
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm device")
+    return torch.device("cuda:0")
+
+
+def plain(x, t, temperature, k, ignore=-100):
+    """float64: (log p [R, V], log probabilities, entropy, top logprobs, top tokens, D per row)."""
+    x = x.double().cpu()
+    t = t.cpu()
+    empty = (x == float("-inf")).all(-1)
+    top = torch.where(empty, 0.0, x.amax(-1))[..., None]
+    d = (x - top) / temperature
+    s = d.exp().sum(-1, keepdim=True)
+    logp = torch.where(empty[..., None], float("-inf"), d - s.log())
+    p = logp.exp()
+    h = -torch.where(p > 0, p * logp, 0.0).sum(-1)
+    h = torch.where(x.isnan().any(-1) | (x == float("inf")).any(-1), float("nan"), h)
+    inside = (t >= 0) & (t < x.shape[-1])
+    lp = logp.gather(-1, torch.where(inside, t, 0)[..., None])[..., 0]
+    lp = torch.where(t == ignore, 0.0, torch.where(inside, lp, float("nan")))
+    order = torch.where(x.isnan(), float("inf"), x)  # NaN above +inf: sorted by (nan, value), stable
+    idx = torch.sort(order, dim=-1, descending=True, stable=True).indices
+    idx = idx.gather(-1, torch.sort(x.gather(-1, idx).isnan().int(), dim=-1, descending=True, stable=True).indices)[..., :k]
+    weighs = (logp > -40 * 0.6931471805599453)
+    big = torch.where(weighs, d.abs(), 0.0).amax(-1)
+    return logp, lp, h, logp.gather(-1, idx), idx, big
+
+
+def bounds(x, temperature, ref):
+    logp, lp, h, top, idx, big = ref
+    v = x.shape[-1]
+    e = (4 * big + v / 256 + 72) * U
+    x64 = x.double().cpu()
+    m = x64.amax(-1, keepdim=True)
+    logs = e + 2 * U * (big + 12)  # |ln s| <= ln V < 12 here
+    return e, logs, lambda values: logs[..., None] + 4 * U * ((m - values).abs() / temperature)
+
+
+def check(got, ref, tol, what):
+    got = got.double().cpu()
+    # (3e38 - -3e38 has no fp32 value but infinity)
+    ref = torch.where(ref.abs() > torch.finfo(torch.float32).max, ref.sign() * float("inf"), ref)
+    assert torch.equal(got.isnan(), ref.isnan()), what
+    special = ~ref.isfinite()
+    assert torch.equal(got[special & ~ref.isnan()], ref[special & ~ref.isnan()]), what
+    off = torch.where(special, 0.0, (got - ref).abs())
+    worst = (off - torch.where(special, 1.0, tol)).nan_to_num(1e300).flatten().argmax()
+    assert bool((off <= torch.where(special, 1.0, tol)).all()), \
+        (what, int(worst), *(float(z.expand_as(off).flatten()[worst]) for z in (got, ref, tol)))
+
+
+def check_forward(x, t, temperature, k, entropy, r, ignore=-100):
+    ref = logp, lp, h, top, idx, big = plain(x, t, temperature, k, ignore)
+    e, logs, lp_tol = bounds(x, temperature, ref)
+    xt = x.double().cpu().gather(-1, t.cpu().clamp(0, x.shape[-1] - 1)[..., None])
+    check(r.logprobs, lp, lp_tol(xt)[..., 0], "logprobs")
+    assert r.logprobs.dtype == torch.float32 and r.logprobs.shape == t.shape
+    if entropy:
+        check(r.entropy, h, (2 + 2 * big) * e + 4 * U * big + logs, "entropy")
+    else:
+        assert r.entropy is None
+    if k:
+        assert torch.equal(r.top_tokens.cpu(), idx), "top_tokens"
+        check(r.top_logprobs, top, lp_tol(x.double().cpu().gather(-1, idx)), "top_logprobs")
+    else:
+        assert r.top_tokens is None and r.top_logprobs is None
+    return ref
+
+
+def make(dev, rows, vocab, dtype, seed, spread=2.5):
+    g = torch.Generator(device=dev).manual_seed(seed)
+    x = torch.randn(rows, vocab, device=dev, generator=g) * spread
+    t = torch.randint(0, vocab, (rows,), device=dev, generator=g)
+    x.scatter_add_(-1, t[:, None], 8 * torch.rand(rows, 1, device=dev, generator=g))
+    return x.to(dtype), t
+
+
+# one logit; less than a vector, a wave and a block; odd; around the sizes that change the tile
+VOCABS = [1, 2, 7, 63, 65, 255, 257, 1000, 2047, 2049, 4096, 5003, 8191, 8193, 16384, 16385, 32767, 32769, 40001, 65537,
+          131073]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", VOCABS)
+def test_forward_over_vocabularies(dev, vocab, dtype):
+    print(f"[case] token_logprobs V={vocab} {dtype}", flush=True)
+    for rows, k, entropy, temperature in ((3, min(5, vocab), True, 1.0), (1, 0, False, 0.7), (2, min(64, vocab), False, 1.4)):
+        x, t = make(dev, rows, vocab, dtype, vocab + rows)
+        r = fl.token_logprobs(x, t, temperature=temperature, top_k=k, entropy=entropy)
+        check_forward(x, t, temperature, k, entropy, r)
+
+
+@pytest.mark.parametrize("rows,vocab", [(1, 16384), (64, 16384), (300, 16384), (700, 501), (5000, 33), (257, 12345), (40, 70000)])
+def test_forward_over_rows(dev, rows, vocab):
+    print(f"[case] token_logprobs rows={rows} V={vocab}", flush=True)
+    x, t = make(dev, rows, vocab, torch.bfloat16, rows)
+    check_forward(x, t, 1.0, 20, True, fl.token_logprobs(x, t, top_k=20, entropy=True))
+
+
+def test_forward_reads_slices_in_place(dev):
+    print("[case] token_logprobs, slices and strides", flush=True)
+    for dtype in (torch.bfloat16, torch.float32):
+        x, t = make(dev, 3 * 9, 1001, dtype, 5)
+        x, t = x.view(3, 9, 1001), t.view(3, 9)
+        for a, b in ((x[:, :-1], t[:, 1:]), (x.transpose(0, 1), t.t()), (x[:, ::2], t[:, ::2]), (x[..., 3:], t % 998),
+                     (x[1:2, 4], t[1:2, 4]), (x[0, 0], t[0, 0]), (x[..., ::2], t % 501), (x[:, :1].expand(3, 9, 1001), t)):
+            r = fl.token_logprobs(a, b, top_k=3, entropy=True)
+            check_forward(a.reshape(-1, a.shape[-1]), b.reshape(-1), 1.0, 3, True,
+                          fl.TokenLogprobs(r.logprobs.reshape(-1), r.entropy.reshape(-1), r.top_logprobs.reshape(-1, 3),
+                                           r.top_tokens.reshape(-1, 3)))
+            assert r.logprobs.shape == b.shape and r.top_tokens.shape == (*b.shape, 3)
+
+
+def special_rows(dev, vocab, dtype):
+    """Rows that go wrong first: masked, empty, equal, of the type's lowest value, infinite, NaN, large."""
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    x = (torch.randn(15, vocab, device=dev, generator=g) * 3).to(dtype)
+    low = torch.finfo(dtype).min
+    x[0, 1:] = float("-inf")                     # one token left
+    x[1] = float("-inf")                         # none left
+    x[2] = 0.0                                   # all equal
+    x[3] = low                                   # all masked by the type's lowest value
+    x[4, ::2] = low
+    x[5, vocab // 2] = float("nan")
+    x[6, vocab - 1] = float("inf")
+    x[7] = -0.0
+    x[7, ::3] = 0.0                              # both zeros are equal
+    x[8] = torch.arange(vocab, device=dev).to(dtype) / 64
+    x[9] = -torch.arange(vocab, device=dev).to(dtype) / 64
+    x[10] = x[10] * 1e4                          # large logits
+    x[11, : vocab // 2] = float("-inf")
+    x[12] = 3.0
+    x[12, vocab // 3] = torch.finfo(dtype).max   # the difference overflows to -inf
+    x[12, vocab // 4] = low
+    x[13, 0], x[13, vocab - 1] = float("inf"), float("nan")
+    x[14] = float("nan")
+    return x
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [3, 300, 8193, 70001])
+def test_forward_of_special_rows(dev, vocab, dtype):
+    print(f"[case] token_logprobs special rows V={vocab} {dtype}", flush=True)
+    x = special_rows(dev, vocab, dtype)
+    for k in sorted({min(vocab, n) for n in (1, 20, 64)}):
+        for at in (0, vocab - 1):
+            t = torch.full((15,), at, device=dev)
+            check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
+
+
+def test_tokens_outside_the_vocabulary_and_ignored_ones(dev):
+    print("[case] token_logprobs, tokens outside", flush=True)
+    x, _ = make(dev, 6, 400, torch.float32, 9)
+    t = torch.tensor([5, -100, 400, -1, 1 << 40, -(1 << 40)], device=dev)
+    check_forward(x, t, 1.0, 2, True, fl.token_logprobs(x, t, top_k=2, entropy=True))
+    x[1] = float("nan")
+    assert float(fl.token_logprobs(x, t).logprobs[1]) == 0.0
+    assert fl.token_logprobs(x, t, ignore_index=5).logprobs.cpu()[:2].isnan().tolist() == [False, True]
+
+
+def test_many_rows_past_32_bit_offsets(dev):
+    """Logits of more than 2^31 values: rows on both sides of the border."""
+    print("[case] token_logprobs past 2^31 values", flush=True)
+    vocab, rows = 16384, (1 << 17) + 3
+    x = torch.zeros(rows, vocab, device=dev, dtype=torch.bfloat16)
+    t = torch.arange(rows, device=dev) % vocab
+    at = torch.tensor([0, 1, (1 << 16) + 1, (1 << 17) - 1, 1 << 17, rows - 1], device=dev)
+    part, _ = make(dev, len(at), vocab, torch.bfloat16, 11)
+    x[at] = part
+    x.requires_grad_()
+    r = fl.token_logprobs(x, t, top_k=3, entropy=True)
+    check_forward(part, t[at], 1.0, 3, True, fl.TokenLogprobs(*[o.detach()[at] for o in r]))
+    w = torch.zeros(rows, device=dev)
+    w[at] = 1.0
+    grad, = torch.autograd.grad(r.logprobs, x, w)
+    check_grad(part, t[at], 1.0, 0, w[at], None, None, grad[at])
+    assert float(grad.float().abs().sum(-1)[(w == 0)].max()) == 0.0
+
+
+# ------------------------------------------------------------------ gradients
+def check_grad(x, t, temperature, k, g, h, gt, got, ignore=-100):
+    ref = logp, lp, ent, top, idx, big = plain(x, t, temperature, max(k, 1), ignore)
+    x64, t = x.double().cpu(), t.cpu()
+    p = logp.exp()
+    g = torch.where(t == ignore, 0.0, g.double().cpu()) if g is not None else torch.zeros(t.shape, dtype=torch.float64)
+    h = h.double().cpu() if h is not None else torch.zeros_like(g)
+    gt = gt.double().cpu() if gt is not None else torch.zeros(*t.shape, 0, dtype=torch.float64)
+    inside = (t >= 0) & (t < x.shape[-1])
+    up = torch.zeros_like(x64).scatter_add_(-1, torch.where(inside, t, 0)[..., None], torch.where(inside, g, 0.0)[..., None])
+    size = up.abs()
+    if gt.shape[-1]:
+        up.scatter_add_(-1, idx[..., :gt.shape[-1]], gt)
+        size.scatter_add_(-1, idx[..., :gt.shape[-1]], gt.abs())
+    a = g + gt.sum(-1)
+    inner = torch.where(p > 0, logp + ent[..., None], 0.0)
+    exp = (up - p * (a[..., None] + h[..., None] * inner)) / temperature
+    weight = (g.abs() + gt.abs().sum(-1))[..., None] \
+        + h.abs()[..., None] * (torch.where(p > 0, logp.abs(), 0.0) + ent.abs()[..., None])
+    size = (size + p * weight) / temperature
+    live = (g != 0) | (h != 0) | (gt != 0).any(-1)
+    empty = (x64 == float("-inf")).all(-1)
+    exp = torch.where((live & ~empty)[..., None], exp, 0.0)
+    exp = torch.where((live & ~empty & (g != 0) & ~inside)[..., None], float("nan"), exp)
+    e, logs, _ = bounds(x, temperature, ref)
+    rel = (2 * e + 8 * U * big + 8 * U)[..., None] + 8 * U * torch.where(p > 0, logp.abs(), 0.0)  # (small p: its own exponent)
+    # ln p + H cancels near p = e^-H: its parts' errors
+    part = (p * h.abs()[..., None] * (2 * logs + (2 + 2 * big) * e)[..., None]) / temperature
+    # a p below 2^-126 is 0 (the hardware's power has no subnormal results): up to 2^-126 of its factor, whose ln p is
+    # above -104 where fp32 has a value at all
+    flushed = 2.0 ** -126 * (1 + torch.where(p > 2.0 ** -150, weight, 0.0)) / temperature
+    tol = size * (rel + 8 * U) + part + exp.abs() * torch.finfo(x.dtype).eps / 2 + flushed
+    check(got, exp, tol, "grad")
+    assert got.dtype == x.dtype and got.shape == x.shape
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 2, 65, 501, 2048, 5003, 16384, 32769, 70001])
+def test_gradients(dev, vocab, dtype):
+    print(f"[case] token_logprobs gradients V={vocab} {dtype}", flush=True)
+    rows = 5
+    x, t = make(dev, rows, vocab, dtype, vocab)
+    t[1] = -100
+    k = min(7, vocab)
+    gen = torch.Generator(device=dev).manual_seed(1)
+    g, h, gt = (torch.randn(*s, device=dev, generator=gen) for s in ((rows,), (rows,), (rows, k)))
+    g[2] = h[2] = 0.0
+    gt[2] = 0.0  # a row that passes nothing
+    for temperature in (1.0, 0.6):
+        for use in ((1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 1)):
+            z = x.detach().clone().requires_grad_()
+            r = fl.token_logprobs(z, t, temperature=temperature, top_k=k if use[2] else 0, entropy=bool(use[1]))
+            outs = [o for o, u in zip((r.logprobs, r.entropy, r.top_logprobs), use) if u]
+            ups = [o for o, u in zip((g, h, gt), use) if u]
+            got, = torch.autograd.grad(outs, z, ups)
+            check_grad(x, t, temperature, k if use[2] else 0, *(o if u else None for o, u in zip((g, h, gt), use)), got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [3, 300, 8193])
+def test_gradients_of_special_rows(dev, vocab, dtype):
+    print(f"[case] token_logprobs gradients of special rows V={vocab} {dtype}", flush=True)
+    x = special_rows(dev, vocab, dtype)
+    t = torch.full((15,), vocab - 1, device=dev)
+    t[3], t[4] = vocab, -100
+    k = min(5, vocab)
+    g = torch.linspace(-1, 1, 15, device=dev) + 0.01
+    z = x.clone().requires_grad_()
+    r = fl.token_logprobs(z, t, top_k=k, entropy=True)
+    got, = torch.autograd.grad([r.logprobs, r.entropy], z, [g, g / 3])
+    check_grad(x, t, 1.0, 0, g, g / 3, None, got)
+    z = x.clone().requires_grad_()  # nothing flows: zeros, also from rows with NaN
+    got, = torch.autograd.grad(fl.token_logprobs(z, t).logprobs, z, torch.zeros(15, device=dev))
+    assert float(got.float().abs().max()) == 0.0
+
+
+def test_gradient_against_differences(dev):
+    print("[case] token_logprobs gradient against differences", flush=True)
+    x, t = make(dev, 3, 50, torch.float32, 2, spread=1.0)
+    w = torch.randn(3, 2, device=dev, generator=torch.Generator(device=dev).manual_seed(4))
+
+    def loss(z):
+        r = fl.token_logprobs(z, t, temperature=0.8, entropy=True)
+        return (w[:, 0] * r.logprobs + w[:, 1] * r.entropy).double().sum()
+
+    z = x.clone().requires_grad_()
+    got, = torch.autograd.grad(loss(z), z)
+    step = 2.0 ** -6
+    for i, j in [(0, int(t[0])), (0, 3), (1, 17), (2, 49)]:
+        d = torch.zeros_like(x)
+        d[i, j] = step
+        diff = float(loss(x + d) - loss(x - d)) / (2 * step)
+        # third derivatives of these sums below 60 (weights to 2.5, 1 / 0.8^3, entropy's up to 4 of p ln p): 10 step^2,
+        # and the two losses' roundings, 2^-20 each
+        assert abs(diff - float(got[i, j])) <= 10 * step ** 2 + 2 ** -20 / step, (i, j)
+
+
+def test_double_backward_matches_log_softmax(dev):
+    print("[case] token_logprobs double backward", flush=True)
+    x, t = make(dev, 4, 40, torch.float32, 6, spread=1.0)
+    t[2] = -100
+
+    def second(fn):
+        z = x.clone().requires_grad_()
+        g, = torch.autograd.grad(fn(z).square().sum(), z, create_graph=True)
+        return torch.autograd.grad(g.square().sum(), z)[0].double()
+
+    def stock(z):
+        lp = torch.log_softmax(z / 0.9, -1)
+        ent = -(lp.exp() * lp).sum(-1)
+        return torch.where(t == -100, 0.0, lp.gather(-1, t.clamp_min(0)[:, None])[:, 0]) + ent
+
+    def own(z):
+        r = fl.token_logprobs(z, t, temperature=0.9, entropy=True)
+        return r.logprobs + r.entropy
+
+    a, b = second(own), second(stock)
+    assert float((a - b).norm() / b.norm()) <= 1e-4  # two fp32 chains of some 40 roundings over sums of 40 terms
+
+
+def test_partial_outputs_and_no_gradient(dev):
+    print("[case] token_logprobs, parts of the outputs", flush=True)
+    x, t = make(dev, 3, 100, torch.bfloat16, 8)
+    with torch.no_grad():
+        assert not fl.token_logprobs(x.requires_grad_(), t).logprobs.requires_grad
+    r = fl.token_logprobs(x, t, top_k=4, entropy=True)
+    assert r.logprobs.requires_grad and r.entropy.requires_grad and r.top_logprobs.requires_grad
+    assert not r.top_tokens.requires_grad
+    got, = torch.autograd.grad(r.top_logprobs[:, 1].sum(), x)
+    gt = torch.zeros(3, 4, device=dev)
+    gt[:, 1] = 1
+    check_grad(x.detach(), t, 1.0, 4, None, None, gt, got)
+    changed = x.detach().clone().requires_grad_()
+    y = changed * 1.0
+    r = fl.token_logprobs(y, t)
+    y.add_(1.0)
+    with pytest.raises(RuntimeError):  # what the backward reads was changed in place
+        r.logprobs.sum().backward()
+
+
+def test_two_streams_and_graph_replays(dev):
+    """Calls on two streams at once, and two captured graphs replayed in turn with eager calls between."""
+    print("[case] token_logprobs on streams and in graphs", flush=True)
+    cases = [make(dev, r, v, torch.bfloat16, r + v) for r, v in ((64, 16384), (2, 131072))]
+    eager = [fl.token_logprobs(x, t, top_k=20, entropy=True) for x, t in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    outs = [[], []]
+    for _ in range(4):
+        for i, (s, (x, t)) in enumerate(zip(streams, cases)):
+            with torch.cuda.stream(s):
+                outs[i].append(fl.token_logprobs(x, t, top_k=20, entropy=True))
+    torch.cuda.synchronize()
+    for got, exp in zip(outs, eager):
+        for r in got:
+            assert all(torch.equal(a, b) for a, b in zip(r, exp))
+    graphs, results, inputs = [], [], []
+    for x, t in cases:
+        x = x.clone()
+        up = torch.ones(t.shape, device=dev)
+        z = x.requires_grad_()
+        side = torch.cuda.Stream()
+        with torch.cuda.stream(side):
+            torch.autograd.grad(fl.token_logprobs(z, t, top_k=20, entropy=True).logprobs, z, up)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            r = fl.token_logprobs(z, t, top_k=20, entropy=True)
+            grad, = torch.autograd.grad(r.logprobs, z, up)
+        graphs.append(g)
+        results.append((*(o.detach() for o in r), grad))
+        inputs.append((z, t, up))
+    for turn in range(3):
+        for z, _, _ in inputs:
+            with torch.no_grad():
+                z.copy_(z.flip(-1) if turn else z)
+        for g in graphs:
+            g.replay()
+        torch.cuda.synchronize()
+        for (z, t, up), got in zip(inputs, results):
+            r = fl.token_logprobs(z, t, top_k=20, entropy=True)
+            grad, = torch.autograd.grad(r.logprobs, z, up)
+            assert all(torch.equal(a, b) for a, b in zip(got, (*(o.detach() for o in r), grad))), turn
+
+
+def test_score_of_the_model_is_its_logits_log_softmax(dev):
+    print("[case] FieldsForCausalLM.score", flush=True)
+    from fields_lm_amd import model as M
+
+    torch.manual_seed(0)
+    core = M.FieldTokenSystem(vocab=211, dim=64, ff_hidden=96, refresh_windows=(64,), mamba_positions=(3,), layers=6, q_heads=4,
+                              kv_heads=2, latent_dim=16, landmark_chunk=32, softpatch_rank=8, late_ff_delta=0,
+                              mamba=dict(d_state=16, headdim=16, chunk_size=32)).to(dev)
+    lm = fl.FieldsForCausalLM(core, backend_name="test", source_audit={}, topology_audit={})
+    ids = torch.randint(0, 211, (2, 33), device=dev)
+    with torch.no_grad():
+        logits = lm(ids).logits[:, :-1]
+    r = lm.score(ids, top_k=3, entropy=True)
+    flat = fl.TokenLogprobs(*(o.reshape(-1, *o.shape[2:]) for o in r))
+    check_forward(logits.reshape(-1, 211), ids[:, 1:].reshape(-1), 1.0, 3, True, flat)
+    assert lm.score(ids[:, :1]).logprobs.shape == (2, 0)
+    with pytest.raises(TypeError):
+        lm.score(ids.int())

@@ -1,0 +1,472 @@
+"""GPU: gradient norm and AdamW against float64 formulas, the 8-bit states against the same steps on the CPU.
+
+Tolerances count roundings, u = 2^-24. m' = b1 m + c1 g is two products and a sum, of constants that are
+themselves rounded: 4 u (|b1 m| + |c1 g|), g's own scale one more. v' likewise with one product more: 6 u v'. The root of
+it then carries 4 u, the ratio m' / (root s + eps) beside m's error 8 u, the update one more for its step size (two more where
+the device's 64-bit powers round another way), and p' two products and a difference: 3 u (|p| + |update|). A bf16
+parameter is rounded once at the end (half a step, eps / 2). The 8-bit codes are compared bit for bit: every
+operation up to them is correctly rounded on both sides and they come in one order.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import fields_lm_amd as fl
+from fields_lm_amd.optim import STATE8_DTYPE
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+HYPER = dict(lr=3e-3, betas=(0.9, 0.98), eps=1e-8, weight_decay=0.1)
+
+
+@pytest.fixture(scope="module")
+def dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm device")
+    return torch.device("cuda:0")
+
+
+# ------------------------------------------------------------------ norm
+SIZES = [[1], [0, 5], [255, 256, 257], [4095, 4096, 4097, 0, 1], [7] * 200, [100003, 3, 65536], [0], [(1 << 22) + 5]]
+
+
+def tensors(dev, sizes, dtype, seed, scale=1.0, shift=0):
+    """Tensors of these sizes, each ``shift`` elements behind its allocation's start."""
+    g = torch.Generator(device=dev).manual_seed(seed)
+    return [(torch.randn(n + shift, device=dev, generator=g) * scale).to(dtype)[shift:] for n in sizes]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
+def test_grad_norm(dev, sizes, shift, dtype):
+    print(f"[case] grad_norm {sizes[:5]} shift={shift} {dtype}", flush=True)
+    grads = tensors(dev, sizes, dtype, len(sizes), 0.1, shift)
+    exp = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    norm, scale = fl.grad_norm(grads, 0.5)
+    assert norm.dtype == torch.float32 and norm.shape == () == scale.shape
+    assert abs(float(norm) - exp) <= 2 * U * exp
+    assert abs(float(scale) - min(1.0, 0.5 / (exp + 1e-6))) <= 6 * U * float(scale)
+    assert torch.equal(fl.grad_norm(grads), norm) and torch.equal(fl.grad_norm(grads, 0.5)[1], scale)
+
+
+def test_grad_norm_of_mixed_types_shapes_and_extremes(dev):
+    print("[case] grad_norm, mixed types", flush=True)
+    g = tensors(dev, [300, 64], torch.float32, 1) + tensors(dev, [129], torch.bfloat16, 2)
+    g[0] = g[0].view(30, 10).t()
+    exp = math.sqrt(sum(float(t.double().square().sum()) for t in g))
+    assert abs(float(fl.grad_norm(g)) - exp) <= 2 * U * exp
+    big = [torch.full((1000,), 1e30, device=dev), torch.full((3,), 1e-30, device=dev)]  # squares past fp32
+    exp = math.sqrt(sum(float(t.double().square().sum()) for t in big))
+    assert abs(float(fl.grad_norm(big)) - exp) <= 2 * U * exp
+    tiny = [torch.full((1000,), 1e-35, device=dev)]
+    exp = math.sqrt(float(tiny[0].double().square().sum()))
+    assert abs(float(fl.grad_norm(tiny)) - exp) <= 2 * U * exp
+    for bad in (float("inf"), float("nan")):
+        t = torch.zeros(5000, device=dev)
+        t[4321] = bad
+        norm, scale = fl.grad_norm([torch.ones(3, device=dev), t], 1.0)
+        assert not math.isfinite(float(norm)) and math.isnan(float(scale))
+    norm, scale = fl.grad_norm([torch.zeros(3, device=dev)], 0.0)
+    assert float(norm) == 0.0 == float(scale)
+    assert float(fl.grad_norm([torch.ones(4, device=dev)], float("inf"))[1]) == 1.0
+
+
+def test_grad_norm_refuses_on_the_device(dev):
+    print("[case] grad_norm refusals", flush=True)
+    with pytest.raises(TypeError):
+        fl.grad_norm([torch.ones(3, device=dev, dtype=torch.float16)])
+    with pytest.raises(ValueError):
+        fl.grad_norm([torch.ones(3, device=dev), torch.ones(3)])
+    with pytest.raises(ValueError):
+        fl.grad_norm([torch.ones(3, device=dev)], -1.0)
+    with pytest.raises(TypeError):
+        fl.grad_norm([torch.ones(3, device=dev).to_sparse()])
+
+
+# ------------------------------------------------------------------ AdamW, fp32 states
+def exact(p, g, m, v, t, gs=1.0, lr=3e-3, betas=(0.9, 0.98), eps=1e-8, weight_decay=0.1):
+    """One step in float64 with its tolerances: (p, m, v) and (tol_p, tol_m, tol_v)."""
+    p, g, m, v = (x.double() for x in (p, g, m, v))
+    g = g * gs
+    b1, b2 = betas
+    tol_m = 5 * U * ((b1 * m).abs() + ((1 - b1) * g).abs())
+    m = b1 * m + (1 - b1) * g
+    v = b2 * v + (1 - b2) * g * g
+    c = 1 / (1 - b1 ** t)
+    denom = (v / (1 - b2 ** t)).sqrt() + eps
+    update = lr * c * m / denom
+    tol_p = 3 * U * (p.abs() + update.abs()) + lr * c * (tol_m + 12 * U * m.abs()) / denom
+    return (p * (1 - lr * weight_decay) - update, m, v), (tol_p, tol_m + 1e-45, 8 * U * v + 1e-45)
+
+
+def near(got, exp, tol, what):
+    off = (got.double() - exp).abs()
+    tol = tol + exp.abs() * (torch.finfo(got.dtype).eps / 2 if got.dtype == torch.bfloat16 else 0)
+    assert bool((off <= tol).all()), (what, float((off / tol.clamp_min(1e-60)).max()))
+
+
+def start32(dev, sizes, dtype, seed, shift=0):
+    p, g = tensors(dev, sizes, dtype, seed, 0.5, shift), tensors(dev, sizes, dtype, seed + 1, 0.1, shift)
+    m = tensors(dev, sizes, torch.float32, seed + 2, 0.05, shift)
+    v = [x.square_() for x in tensors(dev, sizes, torch.float32, seed + 3, 0.1, shift)]
+    return p, g, m, v
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("sizes", SIZES, ids=lambda s: f"{len(s)}x{max(s)}")
+def test_adamw_step(dev, sizes, shift, dtype):
+    print(f"[case] adamw_step {sizes[:5]} shift={shift} {dtype}", flush=True)
+    p, g, m, v = start32(dev, sizes, dtype, len(sizes), shift)
+    before = [[t.clone() for t in l] for l in (p, g, m, v)]
+    steps = torch.arange(len(sizes), device=dev)
+    scale = torch.tensor(0.37, device=dev) if shift else None
+    fl.adamw_step(p, g, m, v, steps, grad_scale=scale, **HYPER)
+    assert torch.equal(steps, torch.arange(len(sizes), device=dev) + 1)
+    for i in range(len(sizes)):
+        if sizes[i] == 0:
+            continue
+        exp, tol = exact(*(l[i] for l in before), i + 1, float(scale) if shift else 1.0)
+        for got, e, t, what in zip((p[i], m[i], v[i]), exp, tol, "pmv"):
+            near(got, e, t, (i, what))
+        assert torch.equal(g[i], before[1][i])
+
+
+def test_adamw_neighbours_stay_as_they_were(dev):
+    """Values beside a tensor in its buffer (before it, after it, between blocks) are not written."""
+    print("[case] adamw_step leaves neighbours alone", flush=True)
+    for eight in (False, True):
+        for dtype in (torch.float32, torch.bfloat16):
+            n, total = 777, 2048
+            buf = [torch.full((total,), 3.0, device=dev, dtype=dtype) for _ in range(2)]
+            st = [torch.full((total,), 0.5, device=dev).to(STATE8_DTYPE if eight else torch.float32) for _ in range(2)]
+            sc = [torch.full((16,), 0.25, device=dev) for _ in range(2)]
+            cut = slice(5, 5 + n)
+            fl.adamw_step([buf[0][cut]], [buf[1][cut]], [st[0][cut]], [st[1][cut]], torch.zeros(1, dtype=torch.long, device=dev),
+                          **HYPER, **(dict(exp_avg_scales=[sc[0][3:7]], exp_avg_sq_scales=[sc[1][3:7]]) if eight else {}))
+            for t, old in [(buf[0], 3.0)] + [(s.float(), 0.5) for s in st]:
+                outside = torch.cat((t[:5], t[5 + n:]))
+                # inside, all change but a bf16 weight: m' / (1 - 0.9) = 7.5 over sqrt(v' / (1 - 0.98)) = 5.8 (v = 0.5) or
+                # less than 5.0 (8 bits: v = 1 / 64) makes a step below lr (2.5 + 0.3) = 0.0084 at most and 0.0048 with
+                # v = 0.5, around or below half a step of bf16 at 3, 2^-7
+                assert bool((outside == old).all()) and (t.dtype == torch.bfloat16 or not bool((t[cut] == old).all()))
+            if eight:
+                assert all(bool((torch.cat((s[:3], s[7:])) == 0.25).all()) for s in sc)
+
+
+def test_adamw_lr_and_scale_are_read_on_the_device(dev):
+    print("[case] adamw_step with lr on the device, and steps that are skipped", flush=True)
+    p, g, m, v = start32(dev, [1000, 3], torch.float32, 3)
+    q, g2, m2, v2 = ([t.clone() for t in l] for l in (p, g, m, v))
+    steps, steps2 = (torch.full((2,), 4, device=dev) for _ in range(2))
+    lr = torch.tensor(3e-3, device=dev)
+    fl.adamw_step(p, g, m, v, steps, **HYPER)
+    fl.adamw_step(q, g2, m2, v2, [steps2[0], steps2[1]], **{**HYPER, "lr": lr})
+    # the device's lr is the fp32 neighbour of the host's: 2^-24 of the update and of the decay
+    for a, b in zip(p, q):
+        assert float((a - b).abs().max()) <= 4 * U * float(a.abs().max())
+    assert all(torch.equal(a, b) for a, b in zip(m + v, m2 + v2)) and torch.equal(steps, steps2)
+    kept = [t.clone() for t in p + m + v]
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        fl.adamw_step(p, g, m, v, steps, grad_scale=torch.tensor(bad, device=dev), **HYPER)
+    assert all(torch.equal(a, b) for a, b in zip(kept, p + m + v)) and steps.tolist() == [5, 5]
+    fl.adamw_step(p, g, m, v, steps, grad_scale=torch.zeros((), device=dev), **HYPER)
+    assert steps.tolist() == [6, 6] and all(torch.equal(a, 0.9 * b) for a, b in zip(m, kept[2:4]))
+
+
+def test_adamw_first_step_and_edges_of_the_hyperparameters(dev):
+    print("[case] adamw_step, first step, betas 0, eps 0", flush=True)
+    for hyper in (dict(lr=1e-2, betas=(0.0, 0.0), eps=1e-8, weight_decay=0.0), dict(lr=0.0, betas=(0.9, 0.999), eps=1e-8,
+                  weight_decay=0.3), dict(lr=1e-2, betas=(0.9, 0.999), eps=0.0, weight_decay=0.0)):
+        p, g, m, v = start32(dev, [513], torch.float32, 9)
+        m[0].zero_(), v[0].zero_()
+        old = [t[0].clone() for t in (p, g, m, v)]
+        fl.adamw_step(p, g, m, v, torch.zeros(1, dtype=torch.long, device=dev), **hyper)
+        exp, tol = exact(*old, 1, **hyper)
+        for got, e, t in zip((p[0], m[0], v[0]), exp, tol):
+            near(got, e, t, hyper)
+
+
+def test_adamw_reads_gradients_of_any_strides_and_counts_as_a_write(dev):
+    print("[case] adamw_step, strides and versions", flush=True)
+    w = torch.nn.Parameter(torch.randn(6, 5, device=dev))
+    g = torch.randn(5, 6, device=dev).t()
+    a, b = w.detach().clone(), w.detach().clone()
+    zeros = [torch.zeros_like(w) for _ in range(4)]
+    fl.adamw_step([a], [g], zeros[:1], zeros[1:2], torch.zeros(1, dtype=torch.long, device=dev), **HYPER)
+    fl.adamw_step([b], [g.contiguous()], zeros[2:3], zeros[3:], torch.zeros(1, dtype=torch.long, device=dev), **HYPER)
+    assert torch.equal(a, b) and not torch.equal(a, w)
+    y = (w * w).sum()
+    fl.adamw_step([w], [g], zeros[:1], zeros[1:2], torch.zeros(1, dtype=torch.long, device=dev), **HYPER)
+    with pytest.raises(RuntimeError):  # w was changed after the product saved it
+        y.backward()
+
+
+def test_adamw_refuses_on_the_device(dev):
+    print("[case] adamw_step refusals", flush=True)
+    def one(dtype=torch.float32, n=4):
+        return torch.zeros(n, device=dev, dtype=dtype)
+
+    step = torch.zeros(1, dtype=torch.long, device=dev)
+    p = one()
+    for bad in (([one(torch.float16)], [one(torch.float16)], [one()], [one()], step),
+                ([p], [one(torch.bfloat16)], [one()], [one()], step),
+                ([p], [one()], [one(torch.bfloat16)], [one()], step),
+                ([p], [one().to_sparse()], [one()], [one()], step)):
+        with pytest.raises(TypeError):
+            fl.adamw_step(*bad)
+    for bad in (([p], [one(n=5)], [one()], [one()], step), ([p], [one()], [one(n=5)], [one()], step),
+                ([p], [torch.zeros(4)], [one()], [one()], step), ([p], [one()], [one()], [one()], step.int()),
+                ([p], [one()], [one()], [one()], [step[0], step[0]]), ([p], [one()], [one()], [one()], step.cpu()),
+                ([one(n=8)[::2]], [one()], [one()], [one()], step), ([p], [one()], [one(n=8)[::2]], [one()], step),
+                ([p, p], [one(), one()], [one(), one()], [one(), one()], torch.zeros(2, dtype=torch.long, device=dev)),
+                ([p, one()], [one(), one()], [one(), one()], [one(), one()], [step, step])):
+        with pytest.raises(ValueError):
+            fl.adamw_step(*bad)
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [one()], [one()], [one()], step, grad_scale=torch.zeros(2, device=dev))
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [one()], [one()], [one()], step, lr=torch.zeros((), dtype=torch.float64, device=dev))
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [one()], [one(STATE8_DTYPE)], [one(STATE8_DTYPE)], step, exp_avg_scales=[one(n=2)],
+                      exp_avg_sq_scales=[one(n=1)])
+    assert float(p.abs().sum()) == 0.0 and int(step) == 0
+
+
+# ------------------------------------------------------------------ AdamW, 8-bit states
+def quantised(x, root):
+    """Codes and scales of the flat fp32 x on the CPU, in the kernel's operations (numpy's reciprocal and root are
+    correctly rounded; torch's on the CPU are not: of 10^6 roots 6,558 came out next to the nearest float)."""
+    n = x.numel()
+    b = torch.zeros(-(-n // 256) * 256)
+    b[:n] = x
+    b = b.view(-1, 256)
+    top = b.abs().amax(1, keepdim=True)
+    held = top >= 1e-30
+    y = b * torch.where(held, torch.from_numpy(np.float32(1) / top.clamp_min(1e-38).numpy()) * 448.0, 0.0)
+    if root:
+        y = torch.where((y > 0) & (y < 2.0 ** -9), torch.tensor(2.0 ** -9), y)
+    return y.to(STATE8_DTYPE).view(-1)[:n], torch.where(held, top * (1.0 / 448.0), 0.0).view(-1)
+
+
+def step8(p, g, mc, ms, vc, vs, t, gs=1.0, lr=3e-3, betas=(0.9, 0.98), eps=1e-8, weight_decay=0.1):
+    """The 8-bit step on the CPU: (new codes and scales of both, exact p and its tolerance)."""
+    n = p.numel()
+
+    def back(code, scale):
+        return code.float() * scale.repeat_interleave(256)[:n]
+
+    m, v = back(mc, ms), back(vc, vs)
+    v = v * v
+    exp, tol = exact(p, g, m, v, t, gs, lr, betas, eps, weight_decay)
+    b1, b2 = betas
+    g = g.float() * torch.tensor(gs)
+    m = m * b1 + g * (1 - b1)
+    v = v * b2 + (g * (1 - b2)) * g
+    return (*quantised(m, False), *quantised(torch.from_numpy(np.sqrt(v.numpy())), True)), exp[0], tol[0]
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shift", [0, 1])
+@pytest.mark.parametrize("sizes", SIZES[:-2], ids=lambda s: f"{len(s)}x{max(s)}")
+def test_adamw_step_8_bits(dev, sizes, shift, dtype):
+    print(f"[case] adamw_step 8 bits {sizes[:5]} shift={shift} {dtype}", flush=True)
+    n = len(sizes)
+    p = tensors(dev, sizes, dtype, n, 0.5, shift)
+    blocks = [-(-s // 256) for s in sizes]
+    mc, vc = ([t.to(STATE8_DTYPE) for t in tensors(dev, sizes, torch.float32, 0, 0.0, shift)] for _ in range(2))
+    ms, vs = ([torch.zeros(b, device=dev) for b in blocks] for _ in range(2))
+    steps = torch.zeros(n, dtype=torch.long, device=dev)
+    for turn in range(3):
+        g = tensors(dev, sizes, dtype, n + turn, 1e-3, shift)
+        g = [x * torch.exp(3 * y) for x, y in zip(g, tensors(dev, sizes, dtype, 50 + turn, 1.0, shift))]  # over decades
+        before = [[t.cpu() for t in l] for l in (p, g, mc, ms, vc, vs)]
+        fl.adamw_step(p, g, mc, vc, steps, grad_scale=torch.tensor(0.7, device=dev) if shift else None, exp_avg_scales=ms,
+                      exp_avg_sq_scales=vs, **HYPER)
+        for i in range(n):
+            if sizes[i] == 0:
+                continue
+            (emc, ems, evc, evs), ep, tol = step8(*(l[i] for l in before), turn + 1, 0.7 if shift else 1.0)
+            near(p[i].cpu(), ep, tol, (turn, i, "p"))
+            for got, exp, what in ((ms[i], ems, "ms"), (vs[i], evs, "vs"), (mc[i].view(torch.uint8), emc.view(torch.uint8), "mc"),
+                                   (vc[i].view(torch.uint8), evc.view(torch.uint8), "vc")):
+                assert torch.equal(got.cpu(), exp), (turn, i, what)
+    assert bool((steps == 3).all())
+
+
+def test_adamw_8_bits_of_uneven_blocks(dev):
+    """Blocks of zeros, of one value, of values over all of fp32's range, of subnormals, of infinity."""
+    print("[case] adamw_step 8 bits, uneven blocks", flush=True)
+    g = torch.zeros(8, 256)
+    g[1, 17] = 2.0
+    g[2] = 10.0 ** torch.linspace(-18, 3, 256)
+    g[3] = 1e-38
+    g[4] = torch.where(torch.arange(256) % 2 == 0, 1.0, -1.0)
+    g[5] = 10.0 ** torch.linspace(0, 18, 256)
+    g[6, 3] = 1e-20
+    g = g.view(-1)
+    n = g.numel()
+    p = torch.randn(n, generator=torch.Generator().manual_seed(0))
+    state = [torch.zeros(n).to(STATE8_DTYPE), torch.zeros(8), torch.zeros(n).to(STATE8_DTYPE), torch.zeros(8)]
+    on = [t.to(dev) for t in (p, *state)]
+    steps = torch.zeros(1, dtype=torch.long, device=dev)
+    for turn in range(4):
+        grad = g if turn % 2 == 0 else torch.zeros(n)
+        (mc, ms, vc, vs), ep, tol = step8(p, grad, *state, turn + 1)
+        fl.adamw_step([on[0]], [grad.to(dev)], [on[1]], [on[3]], steps, exp_avg_scales=[on[2]], exp_avg_sq_scales=[on[4]], **HYPER)
+        near(on[0].cpu(), ep, tol, turn)
+        for got, exp in zip(on[1:], (mc, ms, vc, vs)):
+            assert torch.equal(got.cpu().view(torch.uint8), exp.view(torch.uint8)), turn
+        assert bool(on[0].isfinite().all())
+        # a root that is not 0 never rounds to 0 beside a moment that does not: no step without a gradient runs away
+        assert not bool(((mc.float() != 0) & (vc.float() == 0) & (vs.repeat_interleave(256) > 0)).any())
+        p, state = on[0].cpu(), [mc, ms, vc, vs]
+    bad = torch.zeros(n)
+    bad[300] = float("nan")
+    before = [t.clone() for t in on]
+    fl.adamw_step([on[0]], [bad.to(dev)], [on[1]], [on[3]], steps, exp_avg_scales=[on[2]], exp_avg_sq_scales=[on[4]], **HYPER)
+    nan = on[0].isnan().view(8, 256).any(1).tolist()
+    assert nan == [False, True] + [False] * 6 and before[0].isfinite().all()
+
+
+# ------------------------------------------------------------------ the optimizer, and a run of all together
+def stock_pair(dev, **kw):
+    torch.manual_seed(0)
+    own = torch.nn.Sequential(torch.nn.Linear(40, 300), torch.nn.SiLU(), torch.nn.Linear(300, 17, bias=False)).to(dev)
+    stock = torch.nn.Sequential(torch.nn.Linear(40, 300), torch.nn.SiLU(), torch.nn.Linear(300, 17, bias=False)).to(dev)
+    stock.load_state_dict(own.state_dict())
+    return own, stock
+
+
+def test_optimizer_matches_torch_adamw(dev):
+    """Groups, clipping, a parameter without a gradient for a while, a changed lr; ten steps."""
+    print("[case] AdamW against torch.optim.AdamW", flush=True)
+    own, stock = stock_pair(dev)
+    groups = lambda m: [dict(params=[m[0].weight, m[2].weight], weight_decay=0.2), dict(params=[m[0].bias], lr=1e-2)]  # noqa: E731
+    a = fl.AdamW(groups(own), lr=3e-3, betas=(0.9, 0.95), max_grad_norm=0.5)
+    b = torch.optim.AdamW(groups(stock), lr=3e-3, betas=(0.9, 0.95))
+    for turn in range(10):
+        x = torch.randn(32, 40, device=dev, generator=torch.Generator(device=dev).manual_seed(turn))
+        for m, opt in ((own, a), (stock, b)):
+            m[0].bias.requires_grad_(turn != 3)
+            opt.zero_grad(set_to_none=True)
+            (m(x).square().mean() * 30).backward()
+            opt.param_groups[0]["lr"] = 3e-3 / (1 + turn)
+        norm = torch.nn.utils.clip_grad_norm_(stock.parameters(), 0.5)
+        a.step()
+        b.step()
+        assert abs(float(a.grad_norm) - float(norm)) <= 1e-4 * float(norm)
+    for p, q in zip(own.parameters(), stock.parameters()):
+        # ten steps of at most 3e-3 / 1e-2 each; a gradient that differs by its own rounding noise moves its step by that share
+        assert float((p - q).abs().max()) <= 1e-3 * 10 * 1e-2
+    assert int(a.state[own[0].bias]["step"]) == 9 and int(a.state[own[0].weight]["step"]) == 10
+
+
+def test_optimizer_continues_from_its_checkpoint(dev):
+    print("[case] AdamW checkpoint", flush=True)
+    for bits in (32, 8):
+        own, other = stock_pair(dev)
+        a = fl.AdamW(own.parameters(), state_bits=bits)
+        grads = [[torch.randn_like(p) for p in own.parameters()] for _ in range(4)]
+
+        def take(model, opt, gs):
+            for p, g in zip(model.parameters(), gs):
+                p.grad = g.clone()
+            opt.step()
+
+        take(own, a, grads[0])
+        take(own, a, grads[1])
+        other.load_state_dict(own.state_dict())
+        b = fl.AdamW(other.parameters())
+        b.load_state_dict(a.state_dict())
+        for gs in grads[2:]:
+            take(own, a, gs)
+            take(other, b, gs)
+        assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters()))
+
+
+def test_optimizer_in_a_graph(dev):
+    """Norm, clip and step captured and replayed, with eager steps between, equal eager steps alone."""
+    print("[case] AdamW in a graph", flush=True)
+    for bits in (32, 8):
+        own, other = stock_pair(dev)
+        kw = dict(state_bits=bits, max_grad_norm=1.0, lr=torch.tensor(1e-2, device=dev))
+        a, b = fl.AdamW(own.parameters(), **kw), fl.AdamW(other.parameters(), **kw)
+        for p, q in zip(own.parameters(), other.parameters()):
+            p.grad, q.grad = torch.randn_like(p), torch.zeros_like(q)
+        fresh = fl.AdamW([torch.nn.Parameter(torch.zeros(3, device=dev))])
+        fresh.param_groups[0]["params"][0].grad = torch.ones(3, device=dev)
+        a.step()
+        g = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g):
+            a.step()
+            with pytest.raises(RuntimeError):
+                fresh.step()
+        for turn in range(6):
+            for p in own.parameters():
+                p.grad.normal_(generator=torch.Generator(device=dev).manual_seed(turn)) if turn else None
+            if turn == 4:
+                own[0].weight.grad[0, 0] = float("inf")  # skipped
+            kw["lr"].fill_(1e-2 / (turn + 1))
+            for p, q in zip(own.parameters(), other.parameters()):
+                q.grad.copy_(p.grad)
+            b.step()
+            if turn in (0, 3):
+                a.step() if turn else None
+            else:
+                g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters())), turn
+        assert int(a.state[own[0].weight]["step"]) == 5
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_training_step_of_field_blocks(dev, bits):
+    """Embedding, two Field blocks, head, token log probabilities as the loss, clip and AdamW: gradients against the
+    stock loss, and the step against torch's AdamW (fp32 states) or run for its result (8 bits)."""
+    print(f"[case] a training step of Field blocks, {bits} bits", flush=True)
+    torch.manual_seed(0)
+    vocab, dim = 501, 64
+    emb = torch.nn.Embedding(vocab, dim).to(dev)
+    blocks = torch.nn.ModuleList(fl.FieldBlock(dim, "triton", 32, 32, 64, 96) for _ in range(2)).to(dev)
+    head = torch.nn.Linear(dim, vocab, bias=False).to(dev)
+    params = [p for m in (emb, blocks, head) for p in m.parameters()]
+    ids = torch.randint(0, vocab, (3, 40), device=dev)
+    target = ids[:, 1:].clone()
+    target[1, 20:] = -100  # padding
+
+    def logits():
+        x = emb(ids)
+        for b in blocks:
+            x = b(x)
+        return head(x)
+
+    r = fl.token_logprobs(logits()[:, :-1], target, entropy=True)
+    kept = int((target != -100).sum())
+    loss = -r.logprobs.sum() / kept
+    stock = torch.nn.functional.cross_entropy(logits()[:, :-1].reshape(-1, vocab), target.reshape(-1))
+    assert abs(float(loss) - float(stock)) <= 1e-5 * float(stock)  # fp32 sums over 117 rows of 501
+    grads = torch.autograd.grad(loss, params)
+    for a, b in zip(grads, torch.autograd.grad(stock, params)):
+        assert float((a - b).norm()) <= 1e-4 * float(b.norm()) + 1e-9
+    opt = fl.AdamW(params, lr=1e-2, state_bits=bits, max_grad_norm=0.1)
+    before = [p.detach().clone() for p in params]
+    for p, g in zip(params, grads):
+        p.grad = g.clone()
+    opt.step()
+    norm = math.sqrt(sum(float(g.double().square().sum()) for g in grads))
+    assert abs(float(opt.grad_norm) - norm) <= 1e-6 * norm
+    for p, old, g in zip(params, before, grads):
+        exp, tol = exact(old, g, torch.zeros_like(g), torch.zeros_like(g), 1, min(1.0, 0.1 / (norm + 1e-6)), 1e-2,
+                         (0.9, 0.999), 1e-8, 1e-2)
+        # (the clip's own roundings move g by 4 u, which a first step's ratio hardly sees)
+        near(p.detach(), exp[0], 2 * tol[0], "p")
+        assert bool(p.isfinite().all())
+    again = fl.token_logprobs(logits()[:, :-1], target).logprobs
+    assert bool(again.isfinite().all()) and int(opt.state[params[0]]["step"]) == 1

@@ -1,0 +1,252 @@
+"""Token log probabilities, gradient norm and AdamW on the host: refusals (Python's and the C ABI's, none of which
+reaches a launch), how rows and strides are seen, the optimizer's bookkeeping and the stock form that a
+differentiable backward runs.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import fields_lm_amd as fl
+from fields_lm_amd import _native as nat
+from fields_lm_amd import logprobs as L
+
+
+# ------------------------------------------------------------------ token_logprobs
+class _OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on a device, for checks that come before any launch."""
+
+    @property
+    def is_cuda(self):
+        return True
+
+
+def _there(t):
+    return t.as_subclass(_OnDevice)
+
+
+def test_token_logprobs_refuses_what_it_does_not_take():
+    x, t = torch.randn(3, 7), torch.zeros(3, dtype=torch.long)
+    with pytest.raises(RuntimeError):
+        fl.token_logprobs(x, t)
+    with pytest.raises(TypeError):
+        fl.token_logprobs(_there(x.half()), t)
+    with pytest.raises(TypeError):
+        fl.token_logprobs(_there(x), t.int())
+    with pytest.raises(ValueError):
+        fl.token_logprobs(_there(x), t[:2])
+    with pytest.raises(ValueError):
+        fl.token_logprobs(_there(torch.randn(3, 0)), t)
+    for temperature in (0.0, -1.0, float("nan"), float("inf"), 1e-40):
+        with pytest.raises(ValueError):
+            fl.token_logprobs(_there(x), t, temperature=temperature)
+    for top_k in (-1, 8, 65):
+        with pytest.raises(ValueError):
+            fl.token_logprobs(_there(x), t, top_k=top_k)
+    with pytest.raises(ValueError):
+        fl.token_logprobs(_there(torch.randn(3, 100)), t, top_k=65)
+
+
+def test_token_logprobs_without_rows():
+    r = fl.token_logprobs(_there(torch.randn(4, 0, 7)), torch.zeros(4, 0, dtype=torch.long), top_k=3, entropy=True)
+    assert r.logprobs.shape == r.entropy.shape == (4, 0) and r.top_logprobs.shape == r.top_tokens.shape == (4, 0, 3)
+
+
+def _flat_rows(t, groups, dims):
+    """The elements (or rows) that (outer, inner, strides) reach, in order."""
+    outer, inner, so, si = groups
+    base = t.storage_offset()
+    at = torch.tensor([base + o * so + i * si for o in range(outer) for i in range(inner)])
+    store = torch.as_strided(t, (t.untyped_storage().nbytes() // t.element_size(),), (1,), 0)
+    if dims == t.ndim:
+        return store[at]
+    return store[at[:, None] + torch.arange(t.shape[-1])]
+
+
+@pytest.mark.parametrize("make", [
+    lambda: (torch.randn(5), torch.zeros((), dtype=torch.long)),
+    lambda: (torch.randn(6, 5), torch.arange(6)),
+    lambda: (torch.randn(6, 9)[:, 2:7], torch.arange(12)[::2]),
+    lambda: (torch.randn(3, 4, 5)[:, :-1], torch.arange(12).view(3, 4)[:, 1:]),
+    lambda: (torch.randn(3, 4, 5), torch.arange(12).view(3, 4)),
+    lambda: (torch.randn(3, 4, 5), torch.arange(12).view(4, 3).t()),
+    lambda: (torch.randn(4, 3, 5).transpose(0, 1), torch.arange(12).view(3, 4)),
+    lambda: (torch.randn(2, 3, 4, 5)[:, :, 1:], torch.arange(24).view(2, 3, 4)[:, :, 1:]),
+    lambda: (torch.randn(2, 3, 4, 5)[:, 1:, 1:], torch.arange(24).view(2, 3, 4)[:, 1:, 1:]),
+    lambda: (torch.randn(2, 3, 4, 5)[:, 1:], torch.arange(24).view(2, 3, 4)[:, :2]),
+    lambda: (torch.randn(2, 6, 4, 5)[:, ::2], torch.arange(48).view(2, 3, 8)[..., ::2]),
+    lambda: (torch.randn(1, 4, 5).expand(3, 4, 5), torch.arange(4).expand(3, 4)),
+    lambda: (torch.randn(5, 6).t(), torch.arange(6)),
+    lambda: (torch.randn(1, 1, 5), torch.arange(7)[3:4].view(1, 1)),
+])
+def test_rows_are_found_where_they_are(make):
+    x, t = make()
+    x2, t2, a, b = L._rows(x, t)
+    assert a[0] * a[1] == t.numel()
+    assert torch.equal(_flat_rows(x2, a, x2.ndim - 1), x.reshape(-1, x.shape[-1]))
+    assert torch.equal(_flat_rows(t2, (*a[:2], *b), t2.ndim), t.reshape(-1))
+
+
+def test_rows_of_a_slice_are_not_copied():
+    x, t = torch.randn(3, 4, 5), torch.arange(12).view(3, 4)
+    x2, t2, _, _ = L._rows(x[:, :-1], t[:, 1:])
+    assert x2.data_ptr() == x.data_ptr() and t2.data_ptr() == t[:, 1:].data_ptr()
+
+
+def test_stock_form_and_its_gradient():
+    """The form a differentiable backward runs, against log_softmax in float64 and against differences."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(4, 9, generator=g, dtype=torch.float64)
+    x[1, 3] = float("-inf")
+    t = torch.tensor([2, 5, -100, 0])
+    top = torch.topk(x, 3).indices
+    lp, ent, tops = L._ops(x.float(), t, top, 0.7, -100)
+    ref = torch.log_softmax(x / 0.7, -1)
+    assert torch.allclose(lp.double(), torch.where(t == -100, 0.0, ref.gather(-1, t.clamp_min(0)[:, None])[:, 0]), atol=1e-5)
+    assert torch.allclose(ent.double(), -(ref.exp() * ref.masked_fill(ref == float("-inf"), 0)).sum(-1), atol=1e-5)
+    assert torch.allclose(tops.double(), ref.gather(-1, top), atol=1e-5)
+    x32 = x.float().requires_grad_()
+    weights = [torch.randn(4, generator=g), torch.randn(4, generator=g), torch.randn(4, 3, generator=g)]
+
+    def loss(z):
+        return sum((w * o).sum() for w, o in zip(weights, L._ops(z, t, top, 0.7, -100)))
+
+    got, = torch.autograd.grad(loss(x32), x32)
+    step = 1e-2
+    for i, j in [(0, 2), (0, 7), (1, 5), (1, 0), (2, 4), (3, 0)]:
+        d = torch.zeros_like(x32)
+        d[i, j] = step
+        diff = (loss(x32.detach() + d) - loss(x32.detach() - d)) / (2 * step)
+        # the third derivative of these sums is below 30: 30 step^2 / 6, and 2^-22 of a loss below 30 over a step
+        assert abs(float(diff - got[i, j])) <= 5 * step ** 2 + 30 * 2 ** -22 / step
+    empty = torch.full((1, 9), float("-inf"), requires_grad=True)
+    lp, ent, tops = L._ops(empty, torch.tensor([1]), top[:1], 1.0, -100)
+    assert torch.autograd.grad(lp.sum() + ent.sum() + tops.sum(), empty)[0].abs().max() == 0
+
+
+def test_c_abi_token_logprobs_refusals():
+    lib = nat.load()
+
+    def call(logits=256, dtype=0, outer=1, inner=4, V=10, so=40, si=10, tokens=256, temperature=1.0, k=0, lp=256, ent=None,
+             top=None, tok=None, stats=None, ws=None, ws_bytes=0):
+        return lib.fl_token_logprobs(logits, dtype, outer, inner, V, so, si, tokens, 4, 1, -100, temperature, k, lp, ent, top,
+                                     tok, stats, ws, ws_bytes, None)
+
+    bad = nat.FL_ERR_INVALID_ARGUMENT
+    assert call(dtype=7) == nat.FL_ERR_DTYPE
+    for kw in (dict(logits=None), dict(logits=257), dict(outer=0), dict(inner=-1), dict(V=0), dict(V=1 << 31), dict(si=-1),
+               dict(tokens=None), dict(tokens=260), dict(temperature=0.0), dict(temperature=float("nan")),
+               dict(temperature=float("inf")), dict(k=-1), dict(k=65), dict(k=11, top=256, tok=256), dict(k=2), dict(lp=None),
+               dict(lp=258), dict(ent=258), dict(stats=258), dict(k=2, top=256), dict(k=2, top=256, tok=260),
+               dict(outer=1 << 40, inner=1 << 40)):
+        assert call(**kw) == bad, kw
+
+    def back(logits=256, dtype=0, V=10, k=0, stats=256, ent=None, tok=None, g=None, gh=None, gt=None, out=256, t=1.0):
+        return lib.fl_token_logprobs_backward(logits, dtype, 1, 4, V, 40, 10, 256, 4, 1, -100, t, k, stats, ent, tok, g, gh, gt,
+                                              out, None)
+
+    assert back(dtype=9) == nat.FL_ERR_DTYPE
+    for kw in (dict(logits=None), dict(V=-1), dict(stats=None), dict(out=None), dict(out=258), dict(gh=256), dict(gt=256),
+               dict(k=2, gt=256), dict(g=258), dict(t=-1.0)):
+        assert back(**kw) == bad, kw
+
+
+# ------------------------------------------------------------------ grad_norm, adamw_step
+def _array(*addresses):
+    return (ctypes.c_void_p * len(addresses))(*addresses)
+
+
+def test_grad_norm_refusals():
+    with pytest.raises(ValueError):
+        fl.grad_norm([])
+    with pytest.raises(RuntimeError):
+        fl.grad_norm([torch.randn(3)])
+    lib = nat.load()
+    n = (ctypes.c_int64 * 2)(5, 0)
+    codes = (ctypes.c_int * 2)(0, 1)
+
+    def call(count=2, grads=_array(256, None), codes=codes, n=n, most=1.0, scaled=1, out=256, ws=256, ws_bytes=1 << 20):
+        return lib.fl_grad_norm(count, grads, codes, n, most, scaled, out, ws, ws_bytes, None)
+
+    bad = nat.FL_ERR_INVALID_ARGUMENT
+    assert call(codes=(ctypes.c_int * 2)(0, 5)) == nat.FL_ERR_DTYPE
+    for kw in (dict(count=0), dict(grads=None), dict(codes=None), dict(n=None), dict(n=(ctypes.c_int64 * 2)(5, -1)),
+               dict(n=(ctypes.c_int64 * 2)(5, 1 << 35)), dict(grads=_array(None, None)), dict(grads=_array(258, None)),
+               dict(most=-1.0), dict(most=float("nan")), dict(out=None), dict(ws=260), dict(n=(ctypes.c_int64 * 2)(5, 3))):
+        assert call(**kw) == bad, kw
+    assert call(ws=None) == nat.FL_ERR_WORKSPACE == call(ws_bytes=4)
+    assert lib.fl_grad_norm_workspace_bytes(2, n) >= 8 and lib.fl_grad_norm_workspace_bytes(0, n) == 0
+
+
+def test_adamw_refusals_on_the_host():
+    p, g, m, v = (torch.zeros(4) for _ in range(4))
+    step = torch.zeros(1, dtype=torch.long)
+    with pytest.raises(RuntimeError):
+        fl.adamw_step([p], [g], [m], [v], step)
+    with pytest.raises(ValueError):
+        fl.adamw_step([], [], [], [], step)
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [g, g], [m], [v], step)
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [g], [m], [v], step, exp_avg_scales=[m])
+    for kw in (dict(lr=-1.0), dict(lr=float("nan")), dict(betas=(1.0, 0.9)), dict(betas=(0.9, -0.1)), dict(eps=-1e-8),
+               dict(eps=float("inf")), dict(weight_decay=-0.1)):
+        with pytest.raises(ValueError):
+            fl.adamw_step([p], [g], [m], [v], step, **kw)
+
+
+def test_c_abi_adamw_refusals():
+    lib = nat.load()
+    n = (ctypes.c_int64 * 1)(5)
+    one = _array(256)
+
+    def call(count=1, p=one, g=one, dtype=0, m=one, v=one, ms=None, vs=None, n=n, steps=one, lr_ptr=None, b1=0.9, b2=0.99,
+             eps=1e-8, gs=None, ws=256, ws_bytes=16):
+        return lib.fl_adamw_step(count, p, g, dtype, m, v, ms, vs, n, steps, 1e-3, lr_ptr, b1, b2, eps, 0.1, gs, ws, ws_bytes,
+                                 None)
+
+    bad = nat.FL_ERR_INVALID_ARGUMENT
+    assert call(dtype=3) == nat.FL_ERR_DTYPE
+    for kw in (dict(count=0), dict(p=None), dict(p=_array(None)), dict(p=_array(258)), dict(g=_array(None)), dict(m=None),
+               dict(v=_array(258)), dict(ms=one), dict(vs=one), dict(ms=one, vs=_array(None)), dict(n=None), dict(steps=None),
+               dict(n=(ctypes.c_int64 * 1)(-1)), dict(n=(ctypes.c_int64 * 1)((1 << 34) + 1)), dict(steps=_array(None)),
+               dict(steps=_array(260)), dict(lr_ptr=258), dict(b1=1.0), dict(b1=float("nan")), dict(b2=-0.5), dict(eps=-1.0),
+               dict(gs=258), dict(ws=264)):
+        assert call(**kw) == bad, kw
+    assert call(ws=None) == nat.FL_ERR_WORKSPACE == call(ws_bytes=15)
+
+
+def test_optimizer_refuses_groups_it_cannot_step():
+    w = torch.nn.Parameter(torch.zeros(3))
+    for kw in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(max_grad_norm=-1.0),
+               dict(max_grad_norm=float("nan"))):
+        with pytest.raises(ValueError):
+            fl.AdamW([w], **kw)
+    with pytest.raises(TypeError):
+        fl.AdamW([torch.nn.Parameter(torch.zeros(3, dtype=torch.float16))])
+    opt = fl.AdamW([w])
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(2))], eps=-1.0))
+    assert len(opt.param_groups) == 1 and opt.step() is None  # no gradients: nothing to do
+
+
+def test_optimizer_state_keeps_its_types_through_a_checkpoint(tmp_path):
+    """8-bit codes and 64-bit counters come back as they were saved, also beside bf16 parameters."""
+    ws = [torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(4, 5, dtype=torch.bfloat16))]
+    opt = fl.AdamW(ws, state_bits=8)
+    for w in ws:
+        n = w.numel()
+        opt.state[w] = dict(step=torch.tensor(7), exp_avg=torch.randn(w.shape).to(torch.float8_e4m3fn),
+                            exp_avg_sq=torch.rand(w.shape).to(torch.float8_e4m3fn),
+                            exp_avg_scale=torch.rand(-(-n // 256)), exp_avg_sq_scale=torch.rand(-(-n // 256)))
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    new = fl.AdamW(ws, state_bits=32)
+    new.load_state_dict(torch.load(tmp_path / "opt.pt", weights_only=True))
+    assert new.param_groups[0]["state_bits"] == 8
+    for w in ws:
+        for k, t in opt.state[w].items():
+            u = new.state[w][k]
+            assert u.dtype == t.dtype and u.shape == t.shape and u.data_ptr() != t.data_ptr()
+            assert torch.equal(u.float(), t.float())
