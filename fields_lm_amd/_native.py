@@ -98,7 +98,7 @@ SIGNATURES = {
     "fl_softpatch_workspace_bytes": (_sz, [_i64] * 3),
     "fl_softpatch_scan": (_int, [_vp] * 3 + [_i64] * 3 + [_vp, _vp, _vp, _sz, _vp]),
     "fl_boundary_scan": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp]),
-    "fl_token_logprobs_workspace_bytes": (_sz, [_i64] * 3),
+    "fl_token_logprobs_workspace_bytes": (_sz, [_i64, _i64, _int, _i64]),
     "fl_token_logprobs": (_int, [_vp, _int] + [_i64] * 5 + [_vp] + [_i64] * 3 + [ctypes.c_float, _i64] + [_vp] * 6 +
                           [_sz, _vp]),
     "fl_token_logprobs_backward": (_int, [_vp, _int] + [_i64] * 5 + [_vp] + [_i64] * 3 + [ctypes.c_float, _i64] +

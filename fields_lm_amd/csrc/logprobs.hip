@@ -13,6 +13,7 @@ namespace {
 using namespace fl;
 
 constexpr int kMaxTop = 64;
+constexpr float kMinTemperature = 9.5367431640625e-7f, kMaxTemperature = 1048576.0f;  // 2^-20, 2^20
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Rows {
@@ -32,133 +33,503 @@ __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
   return (uint64_t)b << 32 | (0xffffffffu - index);
 }
 
-template <typename V, typename Op>
-__device__ __forceinline__ V block_reduce(V v, V* s, Op op) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = op(v, __shfl_xor(v, d));
-  __syncthreads();  // s may still be read from the last reduction
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = s[0];
-  for (int i = 1; i < (int)(blockDim.x >> 6); ++i) v = op(v, s[i]);
-  return v;
+__device__ __forceinline__ float key_value(uint64_t key) {
+  const uint32_t b = (uint32_t)(key >> 32);
+  return b == 0xfffffffeu ? __uint_as_float(0x7fc00000u) : __uint_as_float(b & 0x80000000u ? b ^ 0x80000000u : ~b);
 }
 
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7fc00000u); }
 
-// One block to a row.
+// 16 bytes of logits at any element's address
+typedef unsigned int u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
+
 template <typename T>
-__global__ __launch_bounds__(256) void fl_token_logprobs_kernel(
-    const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, const int64_t* __restrict__ tokens,
-    int64_t ignore, float inv_t, int K, float* __restrict__ logprobs, float* __restrict__ entropy,
-    float* __restrict__ top_lp, int64_t* __restrict__ top_tok, float* __restrict__ stats) {
-  __shared__ float s_f[4];
-  __shared__ unsigned long long s_k[4];
-  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
-    const T* x = logits + rows.logits(row);
-    float top = -INFINITY, sum = 0.f, ent = 0.f;
-    bool nan = false;
-    for (int i = threadIdx.x; i < V; i += 256) {
-      const float v = load_as<T>(x + i);
-      nan |= v != v;
-      top = fmaxf(top, v);
-    }
-    top = block_reduce(nan ? INFINITY : top, s_f, [](float a, float b) { return fmaxf(a, b); });
-    const bool empty = top == -INFINITY;
-    const float base = empty ? 0.f : top;
-    for (int i = threadIdx.x; i < V; i += 256) {
-      const float d = (load_as<T>(x + i) - base) * inv_t, e = __builtin_amdgcn_exp2f(d * kLog2e);
-      sum += e;
-      if (e > 0.f) ent = fmaf(e, d, ent);
-    }
-    const auto add = [](float a, float b) { return a + b; };
-    sum = block_reduce(sum, s_f, add);
-    ent = block_reduce(ent, s_f, add);
-    const float log_sum = __builtin_amdgcn_logf(sum) * kLn2;
-    const auto lp_of = [&](float v) { return empty ? -INFINITY : (v - base) * inv_t - log_sum; };
-    if (threadIdx.x == 0) {
-      const int64_t t = tokens[rows.token(row)];
-      logprobs[row] = t == ignore ? 0.f : t >= 0 && t < V ? lp_of(load_as<T>(x + t)) : quiet_nan();
-      if (entropy) entropy[row] = empty ? 0.f : log_sum - ent / sum;
-      if (stats) {
-        stats[2 * row] = top;
-        stats[2 * row + 1] = log_sum;
-      }
-    }
-    unsigned long long last = ~0ull;
-    for (int k = 0; k < K; ++k) {
-      unsigned long long best = 0;
-      for (int i = threadIdx.x; i < V; i += 256) {
-        const unsigned long long key = rank_key(load_as<T>(x + i), (uint32_t)i);
-        if (key < last && key > best) best = key;
-      }
-      last = block_reduce(best, s_k, [](unsigned long long a, unsigned long long b) { return a > b ? a : b; });
-      if (threadIdx.x == 0) {
-        const uint32_t at = 0xffffffffu - (uint32_t)last;
-        top_tok[row * K + k] = at;
-        top_lp[row * K + k] = lp_of(load_as<T>(x + at));
-      }
-    }
+struct Pack;
+template <>
+struct Pack<bf16_bits> {
+  static constexpr int N = 8;
+  static constexpr uint32_t kNone = 0xff80ff80u;  // -inf
+  __device__ __forceinline__ static float get(const u32x4& v, int q) {
+    return q & 1 ? bf16_hi(v[q >> 1]) : bf16_lo(v[q >> 1]);
+  }
+};
+template <>
+struct Pack<float> {
+  static constexpr int N = 4;
+  static constexpr uint32_t kNone = 0xff800000u;
+  __device__ __forceinline__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
+};
+
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+// maximum over the wave, in every lane (the steps of wave_sum)
+__device__ __forceinline__ float wave_max(float v) {
+  v = dpp_max<0xb1>(v);
+  v = dpp_max<0x4e>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b.x), __uint_as_float(b.y));
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const uint64_t o = __shfl_xor((unsigned long long)v, d);
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+constexpr int kCand = 512;           // candidates for the alternatives that a block ranks
+constexpr float kPlainScale = 1048576.0f;  // below this |m| c, x c - fl(m c) is as good as (x - m) c
+
+// What a row's results are made of: m, log2 of s, the mean of d log2(e) under the distribution.
+struct RowStats {
+  float m, log2_s, mean;
+  bool empty;
+  float inv_t;
+  // from the sum: a row of -inf alone adds up to 0; one with NaN or +inf to NaN, which the maximum may have missed
+  __device__ __forceinline__ void settle(float sum) {
+    empty = sum == 0.f;
+    if (sum != sum) m = sum;
+    log2_s = __builtin_amdgcn_logf(sum);
+  }
+  __device__ __forceinline__ float log_sum() const { return log2_s * kLn2; }
+  __device__ __forceinline__ float logprob(float x) const {
+    return empty ? -INFINITY : (x - m) * inv_t - log2_s * kLn2;
+  }
+  __device__ __forceinline__ float entropy() const { return empty ? 0.f : (log2_s - mean) * kLn2; }
+};
+
+struct Outputs {
+  const int64_t* tokens;
+  int64_t ignore;
+  int K;
+  float* logprobs;
+  float* entropy;
+  float* top_lp;
+  int64_t* top_tok;
+  float* stats;
+};
+
+__device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const RowStats& st, int64_t t, int V, float xt) {
+  out.logprobs[row] = t == out.ignore ? 0.f : t >= 0 && t < V ? st.logprob(xt) : quiet_nan();
+  if (out.entropy) out.entropy[row] = st.entropy();
+  if (out.stats) {
+    out.stats[2 * row] = st.m;
+    out.stats[2 * row + 1] = st.log_sum();
   }
 }
 
-// Gradient of one row by one block. A row whose gradients are all 0 gets zeros whatever its logits hold.
+// One block to a row, or to a segment of one (gridDim.y of them): its logits stay in registers, NV packs of
+// 16 bytes to a thread, for the maximum, the sums and the alternatives.
+//
+// Alternatives: the threads' maxima, in 64 groups, give a value that at least K logits reach: their K-th
+// largest (to 16 bits). Only logits from there up are candidates, some K to 2 K of them in text; they are
+// ranked by counting. Rows that hold NaN or +inf, and rows with more candidates than fit (equal logits), are
+// searched K times instead.
+template <typename T, int THREADS, int NV, bool ENT, bool TOP>
+__global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
+    const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, int seg_len, float inv_t, Outputs out,
+    f32x4* __restrict__ part, uint64_t* __restrict__ part_keys) {
+  constexpr int N = Pack<T>::N, WAVES = THREADS / 64;
+  __shared__ float s_max[THREADS], s_sum[2 * WAVES];
+  __shared__ unsigned long long s_cand[kCand], s_best[WAVES];
+  __shared__ int s_n;
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), K = TOP ? out.K : 0;
+  const int lo = (int)blockIdx.y * seg_len, len = V - lo < seg_len ? V - lo : seg_len, packs = len / N;
+  const bool whole = gridDim.y == 1;
+  const float c = inv_t * kLog2e;
+  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
+    const int64_t t = out.tokens[rows.token(row)];
+    if (!TOP && !ENT && t == out.ignore) {  // nothing of this row is asked for
+      if (whole && tid == 0) {
+        out.logprobs[row] = 0.f;
+        if (out.stats) out.stats[2 * row] = out.stats[2 * row + 1] = 0.f;
+      }
+      continue;
+    }
+    const T* row_x = logits + rows.logits(row);
+    const T* x = row_x + lo;
+    float xt = 0.f;
+    if (whole && tid == 0 && t >= 0 && t < V) xt = load_as<T>(row_x + t);
+    u32x4 v[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int j = i * THREADS + tid;
+      v[i] = u32x4{Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
+      if (j < packs) v[i] = *reinterpret_cast<const u32x4_at2*>(x + (int64_t)j * N);
+    }
+    float rest = -INFINITY;  // the logits behind the last pack, one to a thread
+    if (tid < len - packs * N) rest = load_as<T>(x + packs * N + tid);
+    // f(logit, index in the row) of all the thread's logits, and of what stands in for those it lacks (-inf, >= V)
+    const auto each = [&](auto f) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        // (opaque, or the compiler keeps what one pass unpacked for the next: twice the registers)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(v[i][w]));
+#pragma unroll
+        for (int q = 0; q < N; ++q) f(Pack<T>::get(v[i], q), i, q);
+      }
+      f(rest, NV, 0);
+    };
+    const auto index_of = [&](int i, int q) {
+      int at = tid;
+      asm volatile("" : "+v"(at));  // (computed where it is wanted, not kept)
+      return i == NV ? (at < len - packs * N ? lo + packs * N + at : V)
+                     : (i * THREADS + at < packs ? lo + (i * THREADS + at) * N + q : V);
+    };
+    if (TOP && tid == 0) s_n = 0;
+    float mine = -INFINITY;
+    each([&](float a, int, int) { mine = fmaxf(mine, a); });
+    s_max[tid] = mine;
+    __syncthreads();
+    float group = s_max[lane];
+#pragma unroll
+    for (int w = 1; w < WAVES; ++w) group = fmaxf(group, s_max[w * 64 + lane]);
+    RowStats st;
+    st.inv_t = inv_t;
+    st.m = wave_max(group);
+    const float base = st.m == -INFINITY ? 0.f : st.m, shift = base * c;
+    float sum = 0.f, ent = 0.f, resid = 0.f;
+    const auto add = [&](float d) {
+      const float e = __builtin_amdgcn_exp2f(d);
+      sum += e;
+      if constexpr (ENT) ent = fmaf(e, fmaxf(d, -1000.f), ent);  // (0 times -inf is no number)
+    };
+    if (__builtin_fabsf(shift) < kPlainScale) {
+      resid = fmaf(base, c, -shift);
+      each([&](float a, int, int) { add(fmaf(a, c, -shift)); });
+    } else {
+      each([&](float a, int, int) { add((a - base) * c); });
+    }
+    sum = wave_sum(sum);
+    if constexpr (ENT) ent = wave_sum(ent);
+    if constexpr (WAVES > 1) {
+      if (lane == 0) {
+        s_sum[wave] = sum;
+        if constexpr (ENT) s_sum[WAVES + wave] = ent;
+      }
+      __syncthreads();
+      sum = s_sum[0];
+      if constexpr (ENT) ent = s_sum[WAVES];
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) {
+        sum += s_sum[w];
+        if constexpr (ENT) ent += s_sum[WAVES + w];
+      }
+    }
+    st.settle(sum);
+    st.log2_s -= resid;
+    st.mean = ENT ? ent / sum - resid : 0.f;
+    if (tid == 0) {
+      if (whole) write_row(out, row, st, t, V, xt);
+      else part[row * gridDim.y + blockIdx.y] = f32x4{st.m, st.log2_s, st.mean, 0.f};
+    }
+    if constexpr (TOP) {
+      const auto put = [&](int k, uint64_t key) {
+        if (whole) {
+          out.top_tok[row * K + k] = 0xffffffffu - (uint32_t)key;
+          out.top_lp[row * K + k] = st.logprob(key_value(key));
+        } else {
+          part_keys[(row * gridDim.y + blockIdx.y) * K + k] = key;
+        }
+      };
+      int n = kCand + 1;
+      if (sum == sum) {
+        uint32_t g = __float_as_uint(group), bound = 0;
+        g = (g & 0x80000000u ? ~g : g | 0x80000000u) >> 16;
+#pragma unroll
+        for (int bit = 15; bit >= 0; --bit) {
+          const uint32_t test = bound | 1u << bit;
+          if (__popcll(__ballot(g >= test)) >= K) bound = test;
+        }
+        const auto push = [&](float a, int i, int q) {
+          const int index = index_of(i, q);
+          if (index < V) {
+            const int at = atomicAdd(&s_n, 1);
+            if (at < kCand) s_cand[at] = rank_key(a, (uint32_t)index);
+          }
+        };
+        if (bound <= 0x007fu) {
+          // fewer than K groups hold a logit above -inf: all of those, and the masked ones of lowest index
+          each([&](float a, int i, int q) { if (a > -INFINITY || index_of(i, q) - lo < 2 * K) push(a, i, q); });
+        } else {
+          const float least = __uint_as_float(bound & 0x8000u ? bound << 16 ^ 0x80000000u : ~(bound << 16));
+          if (mine >= least) each([&](float a, int i, int q) { if (a >= least) push(a, i, q); });
+        }
+        __syncthreads();
+        n = s_n;
+      }
+      if (n <= kCand) {
+        for (int i = tid; i < n; i += THREADS) {
+          const uint64_t key = s_cand[i];
+          int rank = 0;
+          for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
+          if (rank < K) put(rank, key);
+        }
+        for (int k = n + tid; k < K; k += THREADS) put(k, 0);  // (a segment shorter than K)
+      } else {
+        uint64_t last = ~0ull;
+        for (int k = 0; k < K; ++k) {
+          uint64_t best = 0;
+          each([&](float a, int i, int q) {
+            const int index = index_of(i, q);
+            const uint64_t key = rank_key(a, (uint32_t)index);
+            if (index < V && key < last && key > best) best = key;
+          });
+          best = wave_max(best);
+          __syncthreads();
+          if (lane == 0) s_best[wave] = best;
+          __syncthreads();
+          for (int w = 0; w < WAVES; ++w) best = s_best[w] > best ? s_best[w] : best;
+          last = best;
+          if (tid == 0) put(k, best);
+          if (best == 0) last = 1;  // none left: nothing is below
+        }
+      }
+    }
+    __syncthreads();  // the next row takes the shared memory
+  }
+}
+
+// Joins a row's segments, one thread to a segment (at most THREADS): their sums relative to the row's maximum,
+// and K times the largest of their lists' heads.
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
+    const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, int segments, float inv_t, Outputs out,
+    const f32x4* __restrict__ part, const uint64_t* __restrict__ part_keys) {
+  constexpr int WAVES = THREADS / 64;
+  __shared__ float s_f[3 * WAVES];
+  __shared__ unsigned long long s_best[2][WAVES];
+  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), K = out.K;
+  const float c = inv_t * kLog2e;
+  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
+    const int64_t t = out.tokens[rows.token(row)];
+    float xt = 0.f;
+    if (tid == 0 && t >= 0 && t < V) xt = load_as<T>(logits + rows.logits(row) + t);
+    f32x4 p = {-INFINITY, -INFINITY, 0.f, 0.f};
+    if (tid < segments && !(t == out.ignore && K == 0 && !out.entropy)) p = part[row * segments + tid];
+    RowStats st;
+    st.inv_t = inv_t;
+    st.m = wave_max(p[0]);
+    if (lane == 0) s_f[wave] = st.m;
+    __syncthreads();
+    for (int w = 0; w < WAVES; ++w) st.m = fmaxf(st.m, s_f[w]);
+    // d log2(e) of the segment's own maximum; a segment of -inf alone adds nothing
+    const float d = (p[0] - st.m) * c;
+    const bool live = p[0] != -INFINITY;
+    const float s = live ? __builtin_amdgcn_exp2f(d + p[1]) : 0.f;
+    float sum = wave_sum(s), ent = wave_sum(live && s != 0.f ? s * (p[2] + d) : 0.f);
+    if (lane == 0) {
+      s_f[WAVES + wave] = sum;
+      s_f[2 * WAVES + wave] = ent;
+    }
+    __syncthreads();
+    sum = ent = 0.f;
+    for (int w = 0; w < WAVES; ++w) {
+      sum += s_f[WAVES + w];
+      ent += s_f[2 * WAVES + w];
+    }
+    st.settle(sum);
+    st.mean = ent / sum;
+    if (tid == 0) write_row(out, row, st, t, V, xt);
+    int at = 0;
+    uint64_t head = K > 0 && tid < segments ? part_keys[(row * segments + tid) * K] : 0;
+    for (int k = 0; k < K; ++k) {
+      uint64_t best = wave_max(head);
+      if constexpr (WAVES > 1) {
+        if (lane == 0) s_best[k & 1][wave] = best;
+        __syncthreads();
+        for (int w = 0; w < WAVES; ++w) best = s_best[k & 1][w] > best ? s_best[k & 1][w] : best;
+      }
+      if (head == best) {
+        ++at;
+        head = at < K ? part_keys[(row * segments + tid) * K + at] : 0;
+      }
+      if (tid == 0) {
+        out.top_tok[row * K + k] = 0xffffffffu - (uint32_t)best;
+        out.top_lp[row * K + k] = st.logprob(key_value(best));
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// Gradients: a block writes kBackPacks packs to a thread of one row, then puts in the logits that carry a
+// gradient of their own (the given token, the alternatives). With L = m c + log2 s (c = log2(e) / T) split into its
+// rounded value and the rest, p = 2^(x c - L) is one fused product and one power, and the row's constants make
+//   dx = -(p / T) (g + sum g_k + h (ln p + H))
+// two more operations, one without h. A row whose gradients are all 0 gets zeros whatever its logits hold.
+constexpr int kBackThreads = 256, kBackPacks = 4;
+
 template <typename T>
-__global__ __launch_bounds__(256) void fl_token_logprobs_backward_kernel(
+__device__ __forceinline__ void store_pack(T* p, const float* v);
+template <>
+__device__ __forceinline__ void store_pack<bf16_bits>(bf16_bits* p, const float* v) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<u32x4_at2*>(p) = w;
+}
+template <>
+__device__ __forceinline__ void store_pack<float>(float* p, const float* v) {
+  u32x4 w;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
+  *reinterpret_cast<u32x4_at2*>(p) = w;
+}
+
+template <typename T, bool ENT>
+__global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kernel(
     const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, const int64_t* __restrict__ tokens,
     int64_t ignore, float inv_t, int K, const float* __restrict__ stats, const float* __restrict__ entropy,
     const int64_t* __restrict__ top_tok, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
     const float* __restrict__ g_top, T* __restrict__ grad) {
+  constexpr int N = Pack<T>::N, kChunk = kBackThreads * kBackPacks * N;
+  const int tid = threadIdx.x, lo = (int)blockIdx.y * kChunk, len = V - lo < kChunk ? V - lo : kChunk, packs = len / N;
+  const float c = inv_t * kLog2e;
   for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
-    const T* x = logits + rows.logits(row);
-    T* out = grad + row * V;
+    const T* x = logits + rows.logits(row) + lo;
+    T* out = grad + row * V + lo;
     const int64_t t = tokens[rows.token(row)];
-    float g = g_lp && t != ignore ? g_lp[row] : 0.f;
-    const float h = g_ent ? g_ent[row] : 0.f;
+    const float g = g_lp && t != ignore ? g_lp[row] : 0.f;
+    const float h = ENT ? g_ent[row] : 0.f;
     float a = g;
     bool any = g != 0.f || h != 0.f;
-    for (int k = 0; k < (g_top ? K : 0); ++k) {
+    for (int k = 0; k < K; ++k) {
       const float gk = g_top[row * K + k];
       a += gk;
       any |= gk != 0.f;
     }
-    const float top = stats[2 * row], log_sum = stats[2 * row + 1];
-    if (!any || top == -INFINITY) {
-      for (int i = threadIdx.x; i < V; i += 256) store_as(out + i, 0.f);
+    const float m = stats[2 * row], ls2 = stats[2 * row + 1] * kLog2e;
+    if (!any || m == -INFINITY) {
+      const float zero[N] = {};
+#pragma unroll
+      for (int i = 0; i < kBackPacks; ++i)
+        if (i * kBackThreads + tid < packs) store_pack<T>(out + (i * kBackThreads + tid) * N, zero);
+      if (tid < len - packs * N) store_as(out + packs * N + tid, 0.f);
       continue;
     }
     if (g != 0.f && (t < 0 || t >= V)) a = quiet_nan();
-    const float ent = h != 0.f ? entropy[row] : 0.f;
-    const auto part = [&](float v) {  // -p (a + h (ln p + H))
-      const float lp = (v - top) * inv_t - log_sum, p = __builtin_amdgcn_exp2f(lp * kLog2e);
-      const float w = h != 0.f && p > 0.f ? fmaf(h, lp + ent, a) : a;
-      return -p * w;
+    // d = x c - L and -p (a + h (d ln 2 + H)) / T = 2^d (c0 + c1 d)
+    const float L = fmaf(m, c, ls2);
+    const bool plain = __builtin_fabsf(L) < kPlainScale;
+    const float rest_l = plain ? fmaf(m, c, -L) + ls2 : 0.f;  // L - its rounded value
+    const float scale = -inv_t * __builtin_amdgcn_exp2f(-rest_l);
+    const float c1 = ENT ? h * kLn2 * scale : 0.f;
+    const float c0 = ENT ? scale * fmaf(h, fmaf(rest_l, -kLn2, entropy[row]), a) : scale * a;
+    const auto power = [&](float v) { return plain ? fmaf(v, c, -L) : (v - m) * c - ls2; };
+    const auto part = [&](float d) {
+      const float p = __builtin_amdgcn_exp2f(d);
+      return ENT ? p * fmaf(c1, fmaxf(d, -1000.f), c0) : p * c0;
     };
-    for (int i = threadIdx.x; i < V; i += 256) {
-      float v = part(load_as<T>(x + i));
-      if (i == t) v += g;
-      for (int k = 0; k < (g_top ? K : 0); ++k)
-        if (i == top_tok[row * K + k]) v += g_top[row * K + k];
-      store_as(out + i, v * inv_t);
+    u32x4 v[kBackPacks];
+#pragma unroll
+    for (int i = 0; i < kBackPacks; ++i)
+      if (i * kBackThreads + tid < packs) v[i] = *reinterpret_cast<const u32x4_at2*>(x + (i * kBackThreads + tid) * N);
+#pragma unroll
+    for (int i = 0; i < kBackPacks; ++i) {
+      if (i * kBackThreads + tid < packs) {
+        float o[N];
+#pragma unroll
+        for (int q = 0; q < N; ++q) o[q] = part(power(Pack<T>::get(v[i], q)));
+        store_pack<T>(out + (i * kBackThreads + tid) * N, o);
+      }
     }
+    if (tid < len - packs * N) store_as(out + packs * N + tid, part(power(load_as<T>(x + packs * N + tid))));
+    __syncthreads();  // what follows writes over what other threads wrote
+    if (tid <= K) {
+      const int64_t at = tid < K ? top_tok[row * K + tid] : t;
+      float own = tid < K ? g_top[row * K + tid] : g;
+      bool mine = at >= lo && at < lo + len;
+      if (tid < K && at == t) own += g;
+      for (int k = 0; k < K; ++k)
+        if (tid == K && top_tok[row * K + k] == t) mine = false;  // the alternative's thread has it
+      if (mine) store_as(out + (at - lo), fmaf(own, inv_t, part(power(load_as<T>(x + (at - lo))))));
+    }
+    __syncthreads();
   }
 }
 
-constexpr int64_t kMaxBlocks = 1 << 20;
+constexpr int64_t kMaxBlocks = 1 << 20;  // rows of a launch that run at once
+constexpr int64_t kMaxVocab = (int64_t)1 << 25;
 
 bool shape_ok(int64_t outer, int64_t inner, int64_t V, int64_t so, int64_t si) {
-  return outer > 0 && inner > 0 && outer <= ((int64_t)1 << 40) / inner && V > 0 && V < ((int64_t)1 << 31) && so >= 0 && si >= 0;
+  return outer > 0 && inner > 0 && outer <= ((int64_t)1 << 40) / inner && V > 0 && V <= kMaxVocab && so >= 0 && si >= 0;
+}
+
+// The logits of a block: threads and packs of 16 bytes to each of them; segments of a row.
+struct Tile {
+  int threads, packs, segments;
+  int64_t seg_len;
+};
+
+Tile tile_of(int64_t rows, int64_t V, size_t size) {
+  const int64_t n = (int64_t)(16 / size);
+  const auto holds = [&](int threads, int packs) { return V <= threads * packs * n; };
+  if (holds(64, 4)) return {64, 4, 1, V};
+  if (holds(256, 4)) return {256, 4, 1, V};
+  if (holds(256, 8) && rows > 512) return {256, 8, 1, V};
+  if (holds(1024, 4)) return {1024, 4, 1, V};
+  if (holds(1024, 8) && rows > 128) return {1024, 8, 1, V};
+  const int64_t per = rows > 128 ? 1024 * 8 * n : 256 * 8 * n;
+  int64_t segments = cdiv(V, per);
+  if (segments > 1024) segments = 1024;
+  const int64_t len = cdiv(cdiv(V, segments), n) * n;  // at most 1024 threads' 8 packs: V <= 2^25
+  return {len <= 256 * 8 * n ? 256 : 1024, 8, (int)cdiv(V, len), len};
+}
+
+size_t part_bytes(int64_t rows, const Tile& tile, int64_t K) {
+  return tile.segments == 1 ? 0 : (size_t)rows * tile.segments * (16 + 8 * K);
+}
+
+template <typename T>
+int forward(const T* logits, const Rows& r, int64_t rows, int64_t V, float inv_t, const Outputs& out, void* workspace,
+            const Tile& tile, hipStream_t s) {
+  const dim3 grid((unsigned)(rows < kMaxBlocks ? rows : kMaxBlocks), (unsigned)tile.segments);
+  f32x4* part = static_cast<f32x4*>(workspace);
+  uint64_t* keys = reinterpret_cast<uint64_t*>(part + (tile.segments == 1 ? 0 : rows * tile.segments));
+#define FL_LP2(N, P, ENT, TOP)                                                                                     \
+  fl_token_logprobs_kernel<T, N, P, ENT, TOP><<<grid, N, 0, s>>>(logits, r, rows, (int)V, (int)tile.seg_len, inv_t, \
+                                                                 out, part, keys)
+#define FL_LP(N, P)                                                                                                \
+  if (tile.threads == N && tile.packs == P) {                                                                      \
+    if (out.entropy && out.K) FL_LP2(N, P, true, true);                                                            \
+    else if (out.entropy) FL_LP2(N, P, true, false);                                                               \
+    else if (out.K) FL_LP2(N, P, false, true);                                                                     \
+    else FL_LP2(N, P, false, false);                                                                               \
+  }
+  FL_LP(64, 4)
+  FL_LP(256, 4)
+  FL_LP(256, 8)
+  FL_LP(1024, 4)
+  FL_LP(1024, 8)
+#undef FL_LP
+#undef FL_LP2
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || tile.segments == 1) return hip_status(e);
+  if (tile.segments <= 64)
+    fl_token_logprobs_join_kernel<T, 64><<<grid.x, 64, 0, s>>>(logits, r, rows, (int)V, tile.segments, inv_t, out, part, keys);
+  else
+    fl_token_logprobs_join_kernel<T, 1024><<<grid.x, 1024, 0, s>>>(logits, r, rows, (int)V, tile.segments, inv_t, out, part,
+                                                                   keys);
+  return hip_status(hipGetLastError());
 }
 
 }  // namespace
 
 extern "C" {
 
-size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int64_t top_k) {
-  (void)rows;
-  (void)V;
-  (void)top_k;
-  return 0;
+size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int dtype, int64_t top_k) {
+  if (rows <= 0 || rows > (int64_t)1 << 40 || V <= 0 || V > kMaxVocab || top_k < 0 || top_k > kMaxTop || !dtype_ok(dtype))
+    return 0;
+  return part_bytes(rows, tile_of(rows, V, esize(dtype)), top_k);
 }
 
 int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V, int64_t stride_outer,
@@ -167,27 +538,25 @@ int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inne
                       float* top_logprobs, int64_t* top_tokens, float* stats, void* workspace, size_t workspace_bytes,
                       void* stream) {
   if (!dtype_ok(dtype)) return FL_ERR_DTYPE;
-  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature > 0.f) || !(1.0f / temperature > 0.f) ||
+  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
       top_k < 0 || top_k > kMaxTop || top_k > V)
     return FL_ERR_INVALID_ARGUMENT;
   if (!logits || !aligned(logits, esize(dtype)) || !tokens || !aligned(tokens, 8) || !logprobs || !aligned(logprobs, 4) ||
       !aligned(entropy, 4) || !aligned(stats, 4) ||
       (top_k && (!top_logprobs || !top_tokens || !aligned(top_logprobs, 4) || !aligned(top_tokens, 8))))
     return FL_ERR_INVALID_ARGUMENT;
-  (void)workspace;
-  (void)workspace_bytes;
   const int64_t rows = outer * inner;
+  const Tile tile = tile_of(rows, V, esize(dtype));
+  const size_t need = part_bytes(rows, tile, top_k);
+  if (need && (!workspace || workspace_bytes < need)) return FL_ERR_WORKSPACE;
+  if (need && !aligned(workspace, 16)) return FL_ERR_INVALID_ARGUMENT;
   const Rows r = {inner, stride_outer, stride_inner, token_outer, token_inner};
-  const unsigned blocks = (unsigned)(rows < kMaxBlocks ? rows : kMaxBlocks);
+  const Outputs out = {tokens, ignore_index, (int)top_k, logprobs, entropy, top_logprobs, top_tokens, stats};
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define FL_LP(T)                                                                                                  \
-  fl_token_logprobs_kernel<T><<<blocks, 256, 0, s>>>(static_cast<const T*>(logits), r, rows, (int)V, tokens,      \
-                                                     ignore_index, 1.0f / temperature, (int)top_k, logprobs,      \
-                                                     entropy, top_logprobs, top_tokens, stats)
-  if (dtype == FL_DTYPE_BF16) FL_LP(bf16_bits);
-  else FL_LP(float);
-#undef FL_LP
-  return hip_status(hipGetLastError());
+  const float inv_t = 1.0f / temperature;
+  return dtype == FL_DTYPE_BF16
+             ? forward(static_cast<const bf16_bits*>(logits), r, rows, V, inv_t, out, workspace, tile, s)
+             : forward(static_cast<const float*>(logits), r, rows, V, inv_t, out, workspace, tile, s);
 }
 
 int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V,
@@ -197,7 +566,7 @@ int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int
                                const float* g_logprobs, const float* g_entropy, const float* g_top, void* g_logits,
                                void* stream) {
   if (!dtype_ok(dtype)) return FL_ERR_DTYPE;
-  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature > 0.f) || !(1.0f / temperature > 0.f) ||
+  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
       top_k < 0 || top_k > kMaxTop || top_k > V)
     return FL_ERR_INVALID_ARGUMENT;
   if (!logits || !aligned(logits, esize(dtype)) || !tokens || !aligned(tokens, 8) || !stats || !aligned(stats, 4) ||
@@ -209,12 +578,19 @@ int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int
   const Rows r = {inner, stride_outer, stride_inner, token_outer, token_inner};
   const unsigned blocks = (unsigned)(rows < kMaxBlocks ? rows : kMaxBlocks);
   hipStream_t s = static_cast<hipStream_t>(stream);
-#define FL_LB(T)                                                                                                    \
-  fl_token_logprobs_backward_kernel<T><<<blocks, 256, 0, s>>>(                                                      \
-      static_cast<const T*>(logits), r, rows, (int)V, tokens, ignore_index, 1.0f / temperature, (int)top_k, stats,  \
-      entropy, top_tokens, g_logprobs, g_entropy, g_top, static_cast<T*>(g_logits))
-  if (dtype == FL_DTYPE_BF16) FL_LB(bf16_bits);
-  else FL_LB(float);
+  const int64_t chunk = (int64_t)kBackThreads * kBackPacks * (16 / esize(dtype));
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv(V, chunk));
+#define FL_LB(T, ENT)                                                                                              \
+  fl_token_logprobs_backward_kernel<T, ENT><<<grid, kBackThreads, 0, s>>>(                                         \
+      static_cast<const T*>(logits), r, rows, (int)V, tokens, ignore_index, 1.0f / temperature,                    \
+      g_top ? (int)top_k : 0, stats, entropy, top_tokens, g_logprobs, g_entropy, g_top, static_cast<T*>(g_logits))
+  if (dtype == FL_DTYPE_BF16) {
+    if (g_entropy) FL_LB(bf16_bits, true);
+    else FL_LB(bf16_bits, false);
+  } else {
+    if (g_entropy) FL_LB(float, true);
+    else FL_LB(float, false);
+  }
 #undef FL_LB
   return hip_status(hipGetLastError());
 }

@@ -3,7 +3,6 @@
 beside each token."""
 from __future__ import annotations
 
-import math
 from typing import NamedTuple, Optional, Tuple
 
 import torch
@@ -11,7 +10,8 @@ import torch
 from . import _native as nat
 from ._train import _stock_grads
 
-MAX_TOP = 64
+MAX_TOP, MAX_VOCAB = 64, 1 << 25
+MIN_TEMPERATURE, MAX_TEMPERATURE = 2.0 ** -20, 2.0 ** 20
 
 
 class TokenLogprobs(NamedTuple):
@@ -100,7 +100,7 @@ class _TokenLogprobs(torch.autograd.Function):
         top_tokens = new((*shape, top_k), torch.int64) if top_k else None
         stats = new((*shape, 2)) if grad else None
         x, t, (outer, inner, so, si), (to, ti) = _rows(logits, tokens)
-        nbytes = int(lib.fl_token_logprobs_workspace_bytes(tokens.numel(), vocab, top_k))
+        nbytes = int(lib.fl_token_logprobs_workspace_bytes(tokens.numel(), vocab, nat.dtype_code(logits.dtype), top_k))
         ws = new((nbytes,), torch.uint8) if nbytes else None
         with nat.on(dev):
             nat.check(lib.fl_token_logprobs(
@@ -168,10 +168,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     if logits.ndim < 1 or tokens.shape != logits.shape[:-1]:
         raise ValueError(f"tokens {tuple(tokens.shape)} must be the logits' rows {tuple(logits.shape)}")
     vocab, top_k, temperature = logits.shape[-1], int(top_k), float(temperature)
-    if not 0 < vocab < 1 << 31:
-        raise ValueError(f"a row must have 1 to 2^31 - 1 logits, got {vocab}")
-    if not (temperature > 0.0 and math.isfinite(temperature) and 1e-30 < temperature < 1e30):
-        raise ValueError(f"temperature must be positive and finite, got {temperature}")
+    if not 0 < vocab <= MAX_VOCAB:
+        raise ValueError(f"a row must have 1 to {MAX_VOCAB} logits, got {vocab}")
+    if not MIN_TEMPERATURE <= temperature <= MAX_TEMPERATURE:
+        raise ValueError(f"temperature must be {MIN_TEMPERATURE} to {MAX_TEMPERATURE}, got {temperature}")
     if not 0 <= top_k <= min(MAX_TOP, vocab):
         raise ValueError(f"top_k must be 0 to {min(MAX_TOP, vocab)}, got {top_k}")
     if tokens.numel() == 0:

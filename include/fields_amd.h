@@ -468,7 +468,7 @@ int fl_mix(const void* y, const void* g, const void* mix_logit, int mix_dtype, i
 
 /*
  * Log probabilities of given tokens with entropy and top alternatives, and their gradient (no counterpart in
- * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V logits of dtype at
+ * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V (at most 2^25) logits of dtype at
  * logits + (r / inner) * stride_outer + (r % inner) * stride_inner (elements), its token tokens[(r / inner) *
  * token_outer + (r % inner) * token_inner]. With m = max x, d_v = (x_v - m) / temperature, s = sum e^{d_v}:
  *   logprobs [rows] = d_token - ln s; 0 where the token is ignore_index, NaN where it is outside 0 .. V - 1;
@@ -476,15 +476,15 @@ int fl_mix(const void* y, const void* g, const void* mix_logit, int mix_dtype, i
  *   top_tokens / top_logprobs [rows, top_k]: the top_k (0 .. 64) largest logits, largest first, of equal ones the
  *     lowest index first, NaN above all;
  *   stats [rows, 2] or NULL: m and ln s, for the backward.
- * A row of -inf alone: log probabilities -inf, entropy 0, gradient 0. A row with NaN or +inf: NaN.
- * workspace: fl_token_logprobs_workspace_bytes(rows, V, top_k) bytes, 16-byte aligned, no initial contents
+ * temperature: 2^-20 to 2^20. A row of -inf alone: log probabilities -inf, entropy 0, gradient 0. A row with NaN or +inf: NaN.
+ * workspace: fl_token_logprobs_workspace_bytes(rows, V, dtype, top_k) bytes, 16-byte aligned, no initial contents
  * needed (0 bytes: NULL will do).
  *
  * The backward takes the forward's stats, entropy (if g_entropy) and top_tokens (if g_top), and writes g_logits
  * [rows, V], contiguous, of dtype; any of g_logprobs, g_entropy [rows], g_top [rows, top_k] may be NULL. A row
  * whose gradients are all 0 gets zeros without its logits being read.
  */
-size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int64_t top_k);
+size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int dtype, int64_t top_k);
 int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V, int64_t stride_outer,
                       int64_t stride_inner, const int64_t* tokens, int64_t token_outer, int64_t token_inner,
                       int64_t ignore_index, float temperature, int64_t top_k, float* logprobs, float* entropy,
