@@ -118,6 +118,27 @@ __device__ __forceinline__ float wave_sum(float v) {
   return __uint_as_float(b.x) + __uint_as_float(b.y);
 }
 
+// Maximum over the wave's 64 lanes, in every lane, by the same steps; NaN is passed over.
+template <int CTRL>
+__device__ __forceinline__ float dpp_max(float v) {
+  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = dpp_max<0xb1>(v);
+  v = dpp_max<0x4e>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b.x), __uint_as_float(b.y));
+}
+
+// 16, 8 and 4 bytes at the address of any element
+typedef unsigned int u32x4_any __attribute__((ext_vector_type(4), aligned(1)));
+typedef unsigned int u32x2_any __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned int u32_any __attribute__((aligned(1)));
+
 // 1 / (1 + e), subnormal results included: v_rcp_f32 gives 0 for those, so it takes a quarter of the
 // divisor, and the scale back is exact up to the subnormal's own rounding.
 __device__ __forceinline__ float rcp_one_plus(float e) {

@@ -40,9 +40,6 @@ __device__ __forceinline__ float key_value(uint64_t key) {
 
 __device__ __forceinline__ float quiet_nan() { return __uint_as_float(0x7fc00000u); }
 
-// 16 bytes of logits at any element's address
-typedef unsigned int u32x4_at2 __attribute__((ext_vector_type(4), aligned(2)));
-
 template <typename T>
 struct Pack;
 template <>
@@ -60,22 +57,7 @@ struct Pack<float> {
   __device__ __forceinline__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
 };
 
-template <int CTRL>
-__device__ __forceinline__ float dpp_max(float v) {
-  return fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true)));
-}
-// maximum over the wave, in every lane (the steps of wave_sum)
-__device__ __forceinline__ float wave_max(float v) {
-  v = dpp_max<0xb1>(v);
-  v = dpp_max<0x4e>(v);
-  v = dpp_max<0x141>(v);
-  v = dpp_max<0x140>(v);
-  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  v = fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
-  const u32x2 b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-  return fmaxf(__uint_as_float(b.x), __uint_as_float(b.y));
-}
-__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+__device__ __forceinline__ uint64_t key_max(uint64_t v) {
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) {
     const uint64_t o = __shfl_xor((unsigned long long)v, d);
@@ -162,7 +144,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     for (int i = 0; i < NV; ++i) {
       const int j = i * THREADS + tid;
       v[i] = u32x4{Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
-      if (j < packs) v[i] = *reinterpret_cast<const u32x4_at2*>(x + (int64_t)j * N);
+      if (j < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + (int64_t)j * N);
     }
     float rest = -INFINITY;  // the logits behind the last pack, one to a thread
     if (tid < len - packs * N) rest = load_as<T>(x + packs * N + tid);
@@ -283,7 +265,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
             const uint64_t key = rank_key(a, (uint32_t)index);
             if (index < V && key < last && key > best) best = key;
           });
-          best = wave_max(best);
+          best = key_max(best);
           __syncthreads();
           if (lane == 0) s_best[wave] = best;
           __syncthreads();
@@ -342,7 +324,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     int at = 0;
     uint64_t head = K > 0 && tid < segments ? part_keys[(row * segments + tid) * K] : 0;
     for (int k = 0; k < K; ++k) {
-      uint64_t best = wave_max(head);
+      uint64_t best = key_max(head);
       if constexpr (WAVES > 1) {
         if (lane == 0) s_best[k & 1][wave] = best;
         __syncthreads();
@@ -375,14 +357,14 @@ __device__ __forceinline__ void store_pack<bf16_bits>(bf16_bits* p, const float*
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-  *reinterpret_cast<u32x4_at2*>(p) = w;
+  *reinterpret_cast<u32x4_any*>(p) = w;
 }
 template <>
 __device__ __forceinline__ void store_pack<float>(float* p, const float* v) {
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
-  *reinterpret_cast<u32x4_at2*>(p) = w;
+  *reinterpret_cast<u32x4_any*>(p) = w;
 }
 
 template <typename T, bool ENT>
@@ -432,7 +414,7 @@ __global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kerne
     u32x4 v[kBackPacks];
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i)
-      if (i * kBackThreads + tid < packs) v[i] = *reinterpret_cast<const u32x4_at2*>(x + (i * kBackThreads + tid) * N);
+      if (i * kBackThreads + tid < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + (i * kBackThreads + tid) * N);
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i) {
       if (i * kBackThreads + tid < packs) {

@@ -14,7 +14,7 @@ namespace {
 using namespace fl;
 
 constexpr int kTensors = 64;      // tensors of a launch (an 8-bit table of 64 is 3.6 KiB of arguments)
-constexpr int kStepTensors = 256; // step counters of a launch
+constexpr int kStepTensors = 480; // step counters of a launch, one to a thread
 constexpr int kChunk = 4096;      // values of a block
 constexpr int kBlock = 256;       // values that share a scale in the 8-bit states
 constexpr int kMaxBlocks = 1 << 23;  // blocks of a launch
@@ -48,21 +48,56 @@ struct StepTable {
   int n;
 };
 
+// the tensor that `block` belongs to: as many end at or before it
 template <typename Table>
 __device__ __forceinline__ int tensor_of(const Table& t, int block) {
-  int i = 0;
-  while (i + 1 < t.n && t.first[i + 1] <= block) ++i;
-  return i;
+  const int lane = threadIdx.x & 63;
+  return __popcll(__ballot(lane < t.n && t.first[lane + 1] <= block));
 }
 
+// N consecutive values at any element's address
 template <typename T>
-__device__ double square_sum(const T* x, int64_t lo, int64_t hi) {
-  double acc = 0.0;
-  for (int64_t i = lo + threadIdx.x; i < hi; i += 256) {
-    const double v = load_as<T>(x + i);
-    acc = fma(v, v, acc);
+struct Values;
+template <>
+struct Values<float> {
+  static constexpr int N = 4;
+  __device__ __forceinline__ static float get(const u32x4& r, int q) { return __uint_as_float(r[q]); }
+};
+template <>
+struct Values<bf16_bits> {
+  static constexpr int N = 8;
+  __device__ __forceinline__ static float get(const u32x4& r, int q) {
+    return q & 1 ? bf16_hi(r[q >> 1]) : bf16_lo(r[q >> 1]);
   }
-  return acc;
+};
+
+// Four packs of 16 bytes a turn to a thread, each into a sum of its own.
+template <typename T>
+__device__ __forceinline__ double square_sum(const T* __restrict__ x, int64_t n) {
+  constexpr int N = Values<T>::N, U = 4;
+  const int64_t packs = n / N;
+  double acc[U] = {};
+  for (int64_t at = threadIdx.x; at < packs; at += 256 * U) {
+    u32x4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      r[u] = u32x4{0, 0, 0, 0};
+      if (at + 256 * u < packs) r[u] = *reinterpret_cast<const u32x4_any*>(x + (at + 256 * u) * N);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        const double v = Values<T>::get(r[u], q);
+        acc[u] = fma(v, v, acc[u]);
+      }
+    }
+  }
+  if (threadIdx.x < n - packs * N) {
+    const double v = load_as<T>(x + packs * N + threadIdx.x);
+    acc[0] = fma(v, v, acc[0]);
+  }
+  return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
 
 // sum over a block's threads, in thread 0
@@ -76,12 +111,12 @@ __device__ double block_sum(double v, double* s_sum) {
   return t;
 }
 
-__global__ __launch_bounds__(256) void fl_square_sum_kernel(const NormTable t, double* __restrict__ part) {
+__global__ __launch_bounds__(256) void fl_square_sum_kernel(const NormTable t, int chunk, double* __restrict__ part) {
   __shared__ double s_sum[4];
-  const int i = tensor_of(t, (int)blockIdx.x);
-  const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * kChunk, n = t.numel[i], hi = lo + kChunk < n ? lo + kChunk : n;
-  const double v = t.is_bf16[i] ? square_sum(static_cast<const bf16_bits*>(t.x[i]), lo, hi)
-                                : square_sum(static_cast<const float*>(t.x[i]), lo, hi);
+  const int i = uniform(tensor_of(t, (int)blockIdx.x));
+  const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * chunk, left = t.numel[i] - lo, n = left < chunk ? left : chunk;
+  const double v = t.is_bf16[i] ? square_sum(static_cast<const bf16_bits*>(t.x[i]) + lo, n)
+                                : square_sum(static_cast<const float*>(t.x[i]) + lo, n);
   const double sum = block_sum(v, s_sum);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
 }
@@ -91,6 +126,7 @@ __global__ __launch_bounds__(1024) void fl_norm_finish_kernel(const double* __re
                                                               float* __restrict__ out, int scaled) {
   __shared__ double s_sum[16];
   double acc = 0.0;
+#pragma unroll 4
   for (int64_t i = threadIdx.x; i < n; i += 1024) acc += part[i];
   const double sum = block_sum(acc, s_sum);
   if (threadIdx.x == 0) {
@@ -105,7 +141,7 @@ __global__ __launch_bounds__(1024) void fl_norm_finish_kernel(const double* __re
 
 // A tensor's factors of this step: hyper = {lr / (1 - b1^t), (1 - b2^t)^-1/2, 1 - lr decay, gradient scale},
 // and the step counted, or where the scale is not finite a scale of NaN and nothing counted.
-__global__ __launch_bounds__(256) void fl_adamw_factors_kernel(const StepTable t, double lr, const float* lr_ptr,
+__global__ __launch_bounds__(512) void fl_adamw_factors_kernel(const StepTable t, double lr, const float* lr_ptr,
                                                                double b1, double b2, double decay,
                                                                const float* __restrict__ grad_scale,
                                                                f32x4* __restrict__ hyper) {
@@ -139,17 +175,59 @@ __device__ __forceinline__ float adamw_value(float p, float g, float& m, float& 
 }
 
 template <typename T>
+__device__ __forceinline__ u32x4 pack_values(const float* v);
+template <>
+__device__ __forceinline__ u32x4 pack_values<float>(const float* v) {
+  return u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+}
+template <>
+__device__ __forceinline__ u32x4 pack_values<bf16_bits>(const float* v) {
+  return u32x4{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]), bf16_pair(v[4], v[5]), bf16_pair(v[6], v[7])};
+}
+
+// 16 bytes of parameters and gradients to a thread and turn, and their moments.
+template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw_kernel(const AdamTable<false> t, const f32x4* __restrict__ hyper,
                                                        float b1, float b1c, float b2, float b2c, float eps) {
-  const int i = tensor_of(t, (int)blockIdx.x);
+  constexpr int N = Values<T>::N;
+  const int i = uniform(tensor_of(t, (int)blockIdx.x));
   const f32x4 h = hyper[i];
   if (h[3] != h[3]) return;
   const Factors f = {h[0], h[1], h[2], h[3], b1, b1c, b2, b2c, eps};
-  const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * kChunk, n = t.numel[i], hi = lo + kChunk < n ? lo + kChunk : n;
-  T* p = static_cast<T*>(t.p[i]);
-  const T* g = static_cast<const T*>(t.g[i]);
-  float *ms = static_cast<float*>(t.m[i]), *vs = static_cast<float*>(t.v[i]);
-  for (int64_t k = lo + threadIdx.x; k < hi; k += 256) {
+  const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * kChunk, left = t.numel[i] - lo;
+  const int n = left < kChunk ? (int)left : kChunk, packs = n / N;
+  T* p = static_cast<T*>(t.p[i]) + lo;
+  const T* g = static_cast<const T*>(t.g[i]) + lo;
+  float *ms = static_cast<float*>(t.m[i]) + lo, *vs = static_cast<float*>(t.v[i]) + lo;
+#pragma unroll
+  for (int u = 0; u < kChunk / N / 256; ++u) {
+    const int at = u * 256 + (int)threadIdx.x;
+    if (at < packs) {
+      const u32x4 pr = *reinterpret_cast<const u32x4_any*>(p + at * N), gr = *reinterpret_cast<const u32x4_any*>(g + at * N);
+      u32x4 mr[N / 4], vr[N / 4];
+#pragma unroll
+      for (int w = 0; w < N / 4; ++w) {
+        mr[w] = *reinterpret_cast<const u32x4_any*>(ms + at * N + 4 * w);
+        vr[w] = *reinterpret_cast<const u32x4_any*>(vs + at * N + 4 * w);
+      }
+      float o[N];
+#pragma unroll
+      for (int q = 0; q < N; ++q) {
+        float m = __uint_as_float(mr[q / 4][q % 4]), v = __uint_as_float(vr[q / 4][q % 4]), root;
+        o[q] = adamw_value(Values<T>::get(pr, q), Values<T>::get(gr, q), m, v, root, f);
+        mr[q / 4][q % 4] = __float_as_uint(m);
+        vr[q / 4][q % 4] = __float_as_uint(v);
+      }
+      *reinterpret_cast<u32x4_any*>(p + at * N) = pack_values<T>(o);
+#pragma unroll
+      for (int w = 0; w < N / 4; ++w) {
+        *reinterpret_cast<u32x4_any*>(ms + at * N + 4 * w) = mr[w];
+        *reinterpret_cast<u32x4_any*>(vs + at * N + 4 * w) = vr[w];
+      }
+    }
+  }
+  const int k = packs * N + (int)threadIdx.x;
+  if (k < n) {
     float m = ms[k], v = vs[k], root;
     store_as(p + k, adamw_value(load_as<T>(p + k), load_as<T>(g + k), m, v, root, f));
     ms[k] = m;
@@ -157,62 +235,126 @@ __global__ __launch_bounds__(256) void fl_adamw_kernel(const AdamTable<false> t,
   }
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+// four values of a block of 256, 16 or 8 bytes
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  typedef u32x4 Reg;
+  __device__ __forceinline__ static Reg load(const float* p) { return *reinterpret_cast<const u32x4_any*>(p); }
+  __device__ __forceinline__ static void store(float* p, const float* v) { *reinterpret_cast<u32x4_any*>(p) = pack_values<float>(v); }
+  __device__ __forceinline__ static float get(const Reg& r, int q) { return __uint_as_float(r[q]); }
+  __device__ __forceinline__ static void set(Reg& r, int q, float v) { r[q] = __float_as_uint(v); }
+};
+template <>
+struct Four<bf16_bits> {
+  typedef u32x2 Reg;
+  __device__ __forceinline__ static Reg load(const bf16_bits* p) { return *reinterpret_cast<const u32x2_any*>(p); }
+  __device__ __forceinline__ static void store(bf16_bits* p, const float* v) {
+    *reinterpret_cast<u32x2_any*>(p) = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  }
+  __device__ __forceinline__ static float get(const Reg& r, int q) { return q & 1 ? bf16_hi(r[q >> 1]) : bf16_lo(r[q >> 1]); }
+  __device__ __forceinline__ static void set(Reg& r, int q, float v) {
+    const uint32_t b = bf16_bits_of(v);
+    r[q >> 1] = q & 1 ? (r[q >> 1] & 0xffffu) | b << 16 : (r[q >> 1] & 0xffff0000u) | b;
+  }
+};
+
+template <int Q>
+__device__ __forceinline__ float code_value(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, Q); }
+
+__device__ __forceinline__ uint32_t four_codes(const float* y) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
 }
 
-// One wave to a block of 256 values. m is held as the e4m3 code of m (448 / max|m|), v as that of its root
-// r (448 / max r), with max / 448 beside: a root keeps v's range in half the octaves, and one that is not 0
-// keeps at least the smallest code, since a v that rounds to 0 under an m that does not would let the next
-// step with a small gradient run away.
+// One wave to a block of 256 values, four of them to a lane, four blocks a wave with all their loads ahead of the
+// maths. m is held as the e4m3 code of m (448 / max|m|), v as that of its root r (448 / max r), with max / 448
+// beside: a root keeps v's range in half the octaves, and one that is not 0 keeps at least the smallest code,
+// since a v that rounds to 0 under an m that does not would let the next step with a small gradient run away.
 template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw8_kernel(const AdamTable<true> t, const f32x4* __restrict__ hyper,
                                                         float b1, float b1c, float b2, float b2c, float eps) {
-  const int i = tensor_of(t, (int)blockIdx.x);
+  constexpr int U = kChunk / kBlock / 4;
+  const int i = uniform(tensor_of(t, (int)blockIdx.x));
   const f32x4 h = hyper[i];
   if (h[3] != h[3]) return;
   const Factors f = {h[0], h[1], h[2], h[3], b1, b1c, b2, b2c, eps};
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t n = t.numel[i], lo = (int64_t)((int)blockIdx.x - t.first[i]) * kChunk;
-  T* p = static_cast<T*>(t.p[i]);
-  const T* g = static_cast<const T*>(t.g[i]);
-  uint8_t *mc = static_cast<uint8_t*>(t.m[i]), *vc = static_cast<uint8_t*>(t.v[i]);
-  for (int64_t at = lo + wave * kBlock; at < lo + kChunk && at < n; at += 4 * kBlock) {
-    const int64_t b = at / kBlock;
-    const float s_m = t.ms[i][b], s_v = t.vs[i][b];
-    float m[4], r[4], top_m = 0.f, top_r = 0.f;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * kChunk, left = t.numel[i] - lo;
+  const int n = left < kChunk ? (int)left : kChunk;
+  T* p = static_cast<T*>(t.p[i]) + lo;
+  const T* g = static_cast<const T*>(t.g[i]) + lo;
+  uint8_t *mc = static_cast<uint8_t*>(t.m[i]) + lo, *vc = static_cast<uint8_t*>(t.v[i]) + lo;
+  float *ms = t.ms[i] + lo / kBlock, *vs = t.vs[i] + lo / kBlock;
+  typename Four<T>::Reg pr[U] = {}, gr[U] = {};
+  uint32_t mr[U] = {}, vr[U] = {};
+  float sm[U] = {}, sv[U] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t k = at + 4 * lane + j;
-      m[j] = r[j] = 0.f;
-      if (k < n) {
-        m[j] = __builtin_amdgcn_cvt_f32_fp8((int)mc[k], 0) * s_m;
-        const float root = __builtin_amdgcn_cvt_f32_fp8((int)vc[k], 0) * s_v;
-        float v = root * root;
-        store_as(p + k, adamw_value(load_as<T>(p + k), load_as<T>(g + k), m[j], v, r[j], f));
-      }
-      top_m = fmaxf(top_m, fabsf(m[j]));
-      top_r = fmaxf(top_r, r[j]);
+  for (int u = 0; u < U; ++u) {
+    const int b = u * 4 + wave, k = b * kBlock + 4 * lane;
+    if (b * kBlock < n) {
+      sm[u] = ms[b];
+      sv[u] = vs[b];
     }
-    top_m = wave_max(top_m);
-    top_r = wave_max(top_r);
+    if (k + 4 <= n) {
+      pr[u] = Four<T>::load(p + k);
+      gr[u] = Four<T>::load(g + k);
+      mr[u] = *reinterpret_cast<const u32_any*>(mc + k);
+      vr[u] = *reinterpret_cast<const u32_any*>(vc + k);
+    } else if (k < n) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        if (k + q < n) {
+          Four<T>::set(pr[u], q, load_as<T>(p + k + q));
+          Four<T>::set(gr[u], q, load_as<T>(g + k + q));
+          mr[u] |= (uint32_t)mc[k + q] << (8 * q);
+          vr[u] |= (uint32_t)vc[k + q] << (8 * q);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int b = u * 4 + wave, k = b * kBlock + 4 * lane;
+    if (b * kBlock >= n) break;
+    float o[4], m[4], r[4];
+    const float m0[4] = {code_value<0>(mr[u]), code_value<1>(mr[u]), code_value<2>(mr[u]), code_value<3>(mr[u])};
+    const float r0[4] = {code_value<0>(vr[u]), code_value<1>(vr[u]), code_value<2>(vr[u]), code_value<3>(vr[u])};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {  // (behind the tensor's end all is 0 and stays 0)
+      m[q] = m0[q] * sm[u];
+      const float root = r0[q] * sv[u];
+      float v = root * root;
+      o[q] = adamw_value(Four<T>::get(pr[u], q), Four<T>::get(gr[u], q), m[q], v, r[q], f);
+    }
+    const float top_m = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
+    const float top_r = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
     const float inv_m = top_m >= kTiny ? 1.0f / top_m * kTopCode : 0.f, inv_r = top_r >= kTiny ? 1.0f / top_r * kTopCode : 0.f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t k = at + 4 * lane + j;
-      float y = r[j] * inv_r;
-      y = y > 0.f && y < kSmallest ? kSmallest : y;
-      const int codes = __builtin_amdgcn_cvt_pk_fp8_f32(m[j] * inv_m, y, 0, false);
-      if (k < n) {
-        mc[k] = (uint8_t)codes;
-        vc[k] = (uint8_t)(codes >> 8);
+    for (int q = 0; q < 4; ++q) {
+      m[q] *= inv_m;
+      r[q] *= inv_r;
+      if (r[q] > 0.f && r[q] < kSmallest) r[q] = kSmallest;
+    }
+    const uint32_t mo = four_codes(m), vo = four_codes(r);
+    if (k + 4 <= n) {
+      Four<T>::store(p + k, o);
+      *reinterpret_cast<u32_any*>(mc + k) = mo;
+      *reinterpret_cast<u32_any*>(vc + k) = vo;
+    } else if (k < n) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q) {
+        if (k + q < n) {
+          store_as(p + k + q, o[q]);
+          mc[k + q] = (uint8_t)(mo >> (8 * q));
+          vc[k + q] = (uint8_t)(vo >> (8 * q));
+        }
       }
     }
     if (lane == 0) {
-      t.ms[i][b] = top_m >= kTiny ? top_m * (1.0f / kTopCode) : 0.f;
-      t.vs[i][b] = top_r >= kTiny ? top_r * (1.0f / kTopCode) : 0.f;
+      ms[b] = top_m >= kTiny ? top_m * (1.0f / kTopCode) : 0.f;
+      vs[b] = top_r >= kTiny ? top_r * (1.0f / kTopCode) : 0.f;
     }
   }
 }
@@ -222,11 +364,11 @@ constexpr int64_t kMaxTensors = 1 << 20;
 
 // Fills `table` with tensors from `i` on, empty ones too; returns the index after the last one taken.
 template <typename Table, typename Put>
-int64_t fill_table(Table& table, int64_t n, const int64_t* numel, int64_t i, Put put) {
+int64_t fill_table(Table& table, int64_t n, const int64_t* numel, int64_t i, int chunk, Put put) {
   table.n = 0;
   table.first[0] = 0;
   for (; i < n && table.n < kTensors; ++i) {
-    const int64_t blocks = cdiv(numel[i], kChunk);
+    const int64_t blocks = cdiv(numel[i], chunk);
     if (table.first[table.n] + blocks > kMaxBlocks) break;
     put(table.n, i);
     table.numel[table.n] = numel[i];
@@ -244,7 +386,7 @@ int adamw_launch(int64_t n, void* const* params, const void* const* grads, void*
   for (int64_t i = 0; i < n;) {
     AdamTable<EIGHT> t = {};
     const f32x4* factors = hyper + i;
-    i = fill_table(t, n, numel, i, [&](int k, int64_t j) {
+    i = fill_table(t, n, numel, i, kChunk, [&](int k, int64_t j) {
       t.p[k] = params[j];
       t.g[k] = grads[j];
       t.m[k] = m[j];
@@ -273,6 +415,15 @@ bool list_ok(int64_t n, const int64_t* numel) {
   return true;
 }
 
+// Values of a block of the norm: 2,048 blocks or more where that leaves each 4,096, and at most 65,536.
+int norm_chunk(int64_t n, const int64_t* numel) {
+  int64_t total = 0;
+  for (int64_t i = 0; i < n; ++i) total += numel[i];
+  int chunk = kChunk;
+  while (chunk < 65536 && total / chunk > 4096) chunk *= 2;
+  return chunk;
+}
+
 // every non-empty tensor has an address, a multiple of its elements' size
 bool addresses_ok(int64_t n, const void* const* p, const int64_t* numel, size_t size) {
   if (!p) return false;
@@ -288,7 +439,8 @@ extern "C" {
 size_t fl_grad_norm_workspace_bytes(int64_t n, const int64_t* numel) {
   if (!list_ok(n, numel)) return 0;
   int64_t blocks = 0;
-  for (int64_t i = 0; i < n; ++i) blocks += cdiv(numel[i], kChunk);
+  const int chunk = norm_chunk(n, numel);
+  for (int64_t i = 0; i < n; ++i) blocks += cdiv(numel[i], chunk);
   return (size_t)(blocks > 0 ? blocks : 1) * sizeof(double);
 }
 
@@ -305,15 +457,16 @@ int fl_grad_norm(int64_t n, const void* const* grads, const int* dtypes, const i
   hipStream_t s = static_cast<hipStream_t>(stream);
   double* part = static_cast<double*>(workspace);
   int64_t done = 0;
+  const int chunk = norm_chunk(n, numel);
   for (int64_t i = 0; i < n;) {
     NormTable t = {};
-    i = fill_table(t, n, numel, i, [&](int k, int64_t j) {
+    i = fill_table(t, n, numel, i, chunk, [&](int k, int64_t j) {
       t.x[k] = grads[j];
       t.is_bf16[k] = dtypes[j] == FL_DTYPE_BF16;
     });
     const int blocks = t.first[t.n];
     if (blocks == 0) continue;
-    fl_square_sum_kernel<<<(unsigned)blocks, 256, 0, s>>>(t, part + done);
+    fl_square_sum_kernel<<<(unsigned)blocks, 256, 0, s>>>(t, chunk, part + done);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_status(e);
     done += blocks;
@@ -354,7 +507,7 @@ int fl_adamw_step(int64_t n, void* const* params, const void* const* grads, int 
     StepTable t = {};
     t.n = (int)(n - i < kStepTensors ? n - i : kStepTensors);
     for (int k = 0; k < t.n; ++k) t.step[k] = steps[i + k];
-    fl_adamw_factors_kernel<<<1, 256, 0, s>>>(t, lr, lr_ptr, beta1, beta2, weight_decay, grad_scale, hyper + i);
+    fl_adamw_factors_kernel<<<1, cdiv(t.n, 64) * 64, 0, s>>>(t, lr, lr_ptr, beta1, beta2, weight_decay, grad_scale, hyper + i);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_status(e);
   }

@@ -6,8 +6,10 @@ from __future__ import annotations
 from typing import NamedTuple, Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native as nat
+from ._dispatch import no_grad_needed
 from ._train import _stock_grads
 
 MAX_TOP, MAX_VOCAB = 64, 1 << 25
@@ -43,6 +45,8 @@ def _rows(logits: torch.Tensor, tokens: torch.Tensor):
     if logits.stride(-1) != 1 and logits.shape[-1] > 1:
         logits = logits.contiguous()
     dims = tokens.ndim
+    if logits.is_contiguous() and tokens.is_contiguous():
+        return logits, tokens, (1, tokens.numel(), 0, logits.shape[-1]), (0, 1)
     a, b = _strides(logits, dims), _strides(tokens, dims)
     if a is None:
         logits = logits.contiguous()
@@ -83,36 +87,42 @@ def _ops(logits, tokens, top_tokens, temperature, ignore_index):
     return got, entropy[..., 0], tops
 
 
+def _forward(logits, tokens, temperature, top_k, want_entropy, ignore_index, want_stats):
+    """(logprobs, entropy, top logprobs, top tokens, statistics for the backward), None where not wanted."""
+    lib, dev, vocab = nat.load(), logits.device, logits.shape[-1]
+
+    def new(shape, dtype=torch.float32):
+        return torch.empty(shape, device=dev, dtype=dtype)
+
+    shape = tuple(tokens.shape)
+    logprobs = new(shape)
+    entropy = new(shape) if want_entropy else None
+    top = new((*shape, top_k)) if top_k else None
+    top_tokens = new((*shape, top_k), torch.int64) if top_k else None
+    stats = new((*shape, 2)) if want_stats else None
+    x, t, (outer, inner, so, si), (to, ti) = _rows(logits, tokens)
+    code = nat.dtype_code(x.dtype)
+    nbytes = int(lib.fl_token_logprobs_workspace_bytes(outer * inner, vocab, code, top_k))
+    ws = new((nbytes,), torch.uint8) if nbytes else None
+    with nat.on(dev):
+        nat.check(lib.fl_token_logprobs(
+            nat.ptr(x), code, outer, inner, vocab, so, si, nat.ptr(t), to, ti, ignore_index, temperature, top_k,
+            nat.ptr(logprobs), nat.ptr(entropy), nat.ptr(top), nat.ptr(top_tokens), nat.ptr(stats), nat.ptr(ws), nbytes,
+            nat.stream_handle(dev)), "fl_token_logprobs")
+    return logprobs, entropy, top, top_tokens, stats
+
+
 class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, temperature, top_k, want_entropy, ignore_index):
-        lib, dev, vocab = nat.load(), logits.device, logits.shape[-1]
         ctx.set_materialize_grads(False)
-        grad = ctx.needs_input_grad[0]
-
-        def new(shape, dtype=torch.float32):
-            return torch.empty(shape, device=dev, dtype=dtype)
-
-        shape = tuple(tokens.shape)
-        logprobs = new(shape)
-        entropy = new(shape) if want_entropy else None
-        top = new((*shape, top_k)) if top_k else None
-        top_tokens = new((*shape, top_k), torch.int64) if top_k else None
-        stats = new((*shape, 2)) if grad else None
-        x, t, (outer, inner, so, si), (to, ti) = _rows(logits, tokens)
-        nbytes = int(lib.fl_token_logprobs_workspace_bytes(tokens.numel(), vocab, nat.dtype_code(logits.dtype), top_k))
-        ws = new((nbytes,), torch.uint8) if nbytes else None
-        with nat.on(dev):
-            nat.check(lib.fl_token_logprobs(
-                nat.ptr(x), nat.dtype_code(x.dtype), outer, inner, vocab, so, si, nat.ptr(t), to, ti, ignore_index,
-                temperature, top_k, nat.ptr(logprobs), nat.ptr(entropy), nat.ptr(top), nat.ptr(top_tokens), nat.ptr(stats),
-                nat.ptr(ws), nbytes, nat.stream_handle(dev)), "fl_token_logprobs")
-        if grad:
-            ctx.save_for_backward(logits, tokens, stats, entropy, top_tokens)
-            ctx.args = temperature, top_k, ignore_index
+        *outs, stats = _forward(logits, tokens, temperature, top_k, want_entropy, ignore_index, True)
+        _, entropy, _, top_tokens = outs
+        ctx.save_for_backward(logits, tokens, stats, entropy, top_tokens)
+        ctx.args = temperature, top_k, ignore_index
         if top_tokens is not None:
             ctx.mark_non_differentiable(top_tokens)
-        return logprobs, entropy, top, top_tokens
+        return tuple(outs)
 
     @staticmethod
     def backward(ctx, g_lp, g_entropy, g_top, _):
@@ -179,4 +189,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
         return TokenLogprobs(empty, empty.clone() if entropy else None,
                              empty[..., None].expand(*empty.shape, top_k).clone() if top_k else None,
                              tokens[..., None].expand(*tokens.shape, top_k).clone() if top_k else None)
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, temperature, top_k, bool(entropy), int(ignore_index)))
+    args = logits, tokens, temperature, top_k, bool(entropy), int(ignore_index)
+    if no_grad_needed(logits) and forward_ad._current_level < 0:  # (a tangent is refused by the function, not lost)
+        return TokenLogprobs(*_forward(*args, False)[:4])
+    return TokenLogprobs(*_TokenLogprobs.apply(*args))

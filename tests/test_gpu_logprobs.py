@@ -333,6 +333,10 @@ def test_partial_outputs_and_no_gradient(dev):
     gt = torch.zeros(3, 4, device=dev)
     gt[:, 1] = 1
     check_grad(x.detach(), t, 1.0, 4, None, None, gt, got)
+    import torch.autograd.forward_ad as fwad
+
+    with fwad.dual_level(), pytest.raises(NotImplementedError):  # a tangent is refused, not lost
+        fl.token_logprobs(fwad.make_dual(x.detach(), torch.ones_like(x)), t)
     changed = x.detach().clone().requires_grad_()
     y = changed * 1.0
     r = fl.token_logprobs(y, t)
