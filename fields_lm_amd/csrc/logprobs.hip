@@ -57,13 +57,28 @@ struct Pack<float> {
   __device__ __forceinline__ static float get(const u32x4& v, int q) { return __uint_as_float(v[q]); }
 };
 
+template <int CTRL>
+__device__ __forceinline__ uint64_t dpp_key_max(uint64_t v) {
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(v >> 32), CTRL, 0xf, 0xf, true);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+  const uint64_t o = (uint64_t)hi << 32 | lo;
+  return o > v ? o : v;
+}
+// largest key of the wave, in every lane (the steps of wave_max)
 __device__ __forceinline__ uint64_t key_max(uint64_t v) {
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) {
-    const uint64_t o = __shfl_xor((unsigned long long)v, d);
-    v = o > v ? o : v;
-  }
-  return v;
+  v = dpp_key_max<0xb1>(v);
+  v = dpp_key_max<0x4e>(v);
+  v = dpp_key_max<0x141>(v);
+  v = dpp_key_max<0x140>(v);
+  u32x2 h = __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  u32x2 l = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  uint64_t a = (uint64_t)h.x << 32 | l.x, b = (uint64_t)h.y << 32 | l.y;
+  v = a > b ? a : b;
+  h = __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false);
+  l = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  a = (uint64_t)h.x << 32 | l.x;
+  b = (uint64_t)h.y << 32 | l.y;
+  return a > b ? a : b;
 }
 
 constexpr int kCand = 512;           // candidates for the alternatives that a block ranks
@@ -122,11 +137,14 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
   __shared__ float s_max[THREADS], s_sum[2 * WAVES];
   __shared__ unsigned long long s_cand[kCand], s_best[WAVES];
   __shared__ int s_n;
-  const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), K = TOP ? out.K : 0;
+  const int K = TOP ? out.K : 0;
   const int lo = (int)blockIdx.y * seg_len, len = V - lo < seg_len ? V - lo : seg_len, packs = len / N;
   const bool whole = gridDim.y == 1;
   const float c = inv_t * kLog2e;
   for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));  // (what depends on it is computed where it is wanted, not kept over the rows)
+    const int lane = tid & 63, wave = uniform(tid >> 6);
     const int64_t t = out.tokens[rows.token(row)];
     if (!TOP && !ENT && t == out.ignore) {  // nothing of this row is asked for
       if (whole && tid == 0) {
@@ -148,27 +166,33 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     }
     float rest = -INFINITY;  // the logits behind the last pack, one to a thread
     if (tid < len - packs * N) rest = load_as<T>(x + packs * N + tid);
-    // f(logit, index in the row) of all the thread's logits, and of what stands in for those it lacks (-inf, >= V)
+    // f(logit, i, q) of all the thread's logits, and of -inf for those it lacks
     const auto each = [&](auto f) {
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        // (opaque, or the compiler keeps what one pass unpacked for the next: twice the registers)
 #pragma unroll
-        for (int w = 0; w < 4; ++w) asm volatile("" : "+v"(v[i][w]));
+        for (int w = 0; w < 4; ++w) {
+          // (opaque, or the compiler keeps what one pass unpacked for the next: twice the registers)
+          asm volatile("" : "+v"(v[i][w]));
 #pragma unroll
-        for (int q = 0; q < N; ++q) f(Pack<T>::get(v[i], q), i, q);
+          for (int q = w * N / 4; q < (w + 1) * N / 4; ++q) f(Pack<T>::get(v[i], q), i, q);
+        }
       }
       f(rest, NV, 0);
     };
-    const auto index_of = [&](int i, int q) {
-      int at = tid;
-      asm volatile("" : "+v"(at));  // (computed where it is wanted, not kept)
-      return i == NV ? (at < len - packs * N ? lo + packs * N + at : V)
-                     : (i * THREADS + at < packs ? lo + (i * THREADS + at) * N + q : V);
-    };
     if (TOP && tid == 0) s_n = 0;
-    float mine = -INFINITY;
-    each([&](float a, int, int) { mine = fmaxf(mine, a); });
+    float mine = rest, pack_top[TOP ? NV : 1];
+    if constexpr (TOP) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        pack_top[i] = Pack<T>::get(v[i], 0);
+#pragma unroll
+        for (int q = 1; q < N; ++q) pack_top[i] = fmaxf(pack_top[i], Pack<T>::get(v[i], q));
+        mine = fmaxf(mine, pack_top[i]);
+      }
+    } else {
+      each([&](float a, int, int) { mine = fmaxf(mine, a); });
+    }
     s_max[tid] = mine;
     __syncthreads();
     float group = s_max[lane];
@@ -231,40 +255,67 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
           const uint32_t test = bound | 1u << bit;
           if (__popcll(__ballot(g >= test)) >= K) bound = test;
         }
-        const auto push = [&](float a, int i, int q) {
-          const int index = index_of(i, q);
-          if (index < V) {
-            const int at = atomicAdd(&s_n, 1);
-            if (at < kCand) s_cand[at] = rank_key(a, (uint32_t)index);
-          }
+        const auto push = [&](float a, uint32_t at) {  // at: where in the segment
+          const int k = atomicAdd(&s_n, 1);
+          if (k < kCand) s_cand[k] = (uint64_t)__float_as_uint(a) << 32 | at;
         };
         if (bound <= 0x007fu) {
           // fewer than K groups hold a logit above -inf: all of those, and the masked ones of lowest index
-          each([&](float a, int i, int q) { if (a > -INFINITY || index_of(i, q) - lo < 2 * K) push(a, i, q); });
+          for (int i = tid; i < len; i += THREADS) {
+            const float a = load_as<T>(x + i);
+            if (a > -INFINITY || i < 2 * K) push(a, (uint32_t)i);
+          }
         } else {
           const float least = __uint_as_float(bound & 0x8000u ? bound << 16 ^ 0x80000000u : ~(bound << 16));
-          if (mine >= least) each([&](float a, int i, int q) { if (a >= least) push(a, i, q); });
+          uint32_t hit = 0;  // the packs that hold a candidate, read once more
+#pragma unroll
+          for (int i = 0; i < NV; ++i) hit |= pack_top[i] >= least ? 1u << i : 0u;
+          while (hit) {
+            const int at = (__builtin_ctz(hit) * THREADS + tid) * N;
+            hit &= hit - 1;
+            const u32x4 again = *reinterpret_cast<const u32x4_any*>(x + at);
+#pragma unroll
+            for (int q = 0; q < N; ++q) {
+              const float a = Pack<T>::get(again, q);
+              if (a >= least) push(a, (uint32_t)(at + q));
+            }
+          }
+          if (rest >= least) push(rest, (uint32_t)(packs * N + tid));
         }
         __syncthreads();
         n = s_n;
       }
-      if (n <= kCand) {
-        for (int i = tid; i < n; i += THREADS) {
-          const uint64_t key = s_cand[i];
+      const auto key_at = [&](int i) {
+        const uint64_t c = s_cand[i];
+        return rank_key(__uint_as_float((uint32_t)(c >> 32)), (uint32_t)lo + (uint32_t)c);
+      };
+      if (n <= 64) {  // one wave, a candidate to a lane
+        if (wave == 0) {
+          const uint64_t key = lane < n ? key_at(lane) : 0;
           int rank = 0;
-          for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
+          for (int j = 0; j < n; ++j) {
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), j);
+            const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)key, j);
+            rank += ((uint64_t)hi << 32 | low) > key;
+          }
+          if (lane < n && rank < K) put(rank, key);
+        }
+      } else if (n <= kCand) {
+        for (int i = tid; i < n; i += THREADS) {
+          const uint64_t key = key_at(i);
+          int rank = 0;
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) rank += key_at(j) > key;
           if (rank < K) put(rank, key);
         }
-        for (int k = n + tid; k < K; k += THREADS) put(k, 0);  // (a segment shorter than K)
       } else {
         uint64_t last = ~0ull;
         for (int k = 0; k < K; ++k) {
           uint64_t best = 0;
-          each([&](float a, int i, int q) {
-            const int index = index_of(i, q);
-            const uint64_t key = rank_key(a, (uint32_t)index);
-            if (index < V && key < last && key > best) best = key;
-          });
+          for (int i = tid; i < len; i += THREADS) {
+            const uint64_t key = rank_key(load_as<T>(x + i), (uint32_t)(lo + i));
+            if (key < last && key > best) best = key;
+          }
           best = key_max(best);
           __syncthreads();
           if (lane == 0) s_best[wave] = best;
@@ -275,6 +326,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
           if (best == 0) last = 1;  // none left: nothing is below
         }
       }
+      for (int k = n + tid; k < K; k += THREADS) put(k, 0);  // (a segment of fewer than K)
     }
     __syncthreads();  // the next row takes the shared memory
   }
@@ -288,7 +340,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     const f32x4* __restrict__ part, const uint64_t* __restrict__ part_keys) {
   constexpr int WAVES = THREADS / 64;
   __shared__ float s_f[3 * WAVES];
-  __shared__ unsigned long long s_best[2][WAVES];
+  __shared__ unsigned long long s_best[2][WAVES], s_keys[WAVES == 1 ? 64 * kMaxTop : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), K = out.K;
   const float c = inv_t * kLog2e;
   for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
@@ -321,8 +373,18 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     st.settle(sum);
     st.mean = ent / sum;
     if (tid == 0) write_row(out, row, st, t, V, xt);
+    const uint64_t* keys = part_keys + row * segments * K;
+    if constexpr (WAVES == 1) {
+      for (int i = tid; i < segments * K; i += 64) s_keys[i] = keys[i];
+      __syncthreads();
+    }
+    const auto key_of = [&](int k) -> uint64_t {
+      if (tid >= segments || k >= K) return 0;
+      if constexpr (WAVES == 1) return s_keys[tid * K + k];
+      else return keys[tid * K + k];
+    };
     int at = 0;
-    uint64_t head = K > 0 && tid < segments ? part_keys[(row * segments + tid) * K] : 0;
+    uint64_t head = key_of(0);
     for (int k = 0; k < K; ++k) {
       uint64_t best = key_max(head);
       if constexpr (WAVES > 1) {
@@ -330,10 +392,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
         __syncthreads();
         for (int w = 0; w < WAVES; ++w) best = s_best[k & 1][w] > best ? s_best[k & 1][w] : best;
       }
-      if (head == best) {
-        ++at;
-        head = at < K ? part_keys[(row * segments + tid) * K + at] : 0;
-      }
+      if (head == best) head = key_of(++at);
       if (tid == 0) {
         out.top_tok[row * K + k] = 0xffffffffu - (uint32_t)best;
         out.top_lp[row * K + k] = st.logprob(key_value(best));
@@ -376,7 +435,8 @@ __global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kerne
   constexpr int N = Pack<T>::N, kChunk = kBackThreads * kBackPacks * N;
   const int tid = threadIdx.x, lo = (int)blockIdx.y * kChunk, len = V - lo < kChunk ? V - lo : kChunk, packs = len / N;
   const float c = inv_t * kLog2e;
-  for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
+  for (int64_t at_row = blockIdx.x; at_row < n_rows; at_row += gridDim.x) {
+    const int64_t row = n_rows - 1 - at_row;  // the forward's last rows first: they may still be cached
     const T* x = logits + rows.logits(row) + lo;
     T* out = grad + row * V + lo;
     const int64_t t = tokens[rows.token(row)];
