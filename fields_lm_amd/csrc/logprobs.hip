@@ -407,7 +407,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
 // rounded value and the rest, p = 2^(x c - L) is one fused product and one power, and the row's constants make
 //   dx = -(p / T) (g + sum g_k + h (ln p + H))
 // two more operations, one without h. A row whose gradients are all 0 gets zeros whatever its logits hold.
-constexpr int kBackThreads = 256, kBackPacks = 4;
+constexpr int kBackPacks = 4;
 
 template <typename T>
 __device__ __forceinline__ void store_pack(T* p, const float* v);
@@ -416,45 +416,42 @@ __device__ __forceinline__ void store_pack<bf16_bits>(bf16_bits* p, const float*
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-  *reinterpret_cast<u32x4_any*>(p) = w;
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
 }
 template <>
 __device__ __forceinline__ void store_pack<float>(float* p, const float* v) {
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
-  *reinterpret_cast<u32x4_any*>(p) = w;
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
 }
 
-template <typename T, bool ENT>
-__global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kernel(
+template <typename T, int THREADS, bool ENT>
+__global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
     const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, const int64_t* __restrict__ tokens,
     int64_t ignore, float inv_t, int K, const float* __restrict__ stats, const float* __restrict__ entropy,
     const int64_t* __restrict__ top_tok, const float* __restrict__ g_lp, const float* __restrict__ g_ent,
     const float* __restrict__ g_top, T* __restrict__ grad) {
-  constexpr int N = Pack<T>::N, kChunk = kBackThreads * kBackPacks * N;
-  const int tid = threadIdx.x, lo = (int)blockIdx.y * kChunk, len = V - lo < kChunk ? V - lo : kChunk, packs = len / N;
+  constexpr int N = Pack<T>::N, kChunk = THREADS * kBackPacks * N;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int lo = (int)blockIdx.y * kChunk, len = V - lo < kChunk ? V - lo : kChunk, packs = len / N;
   const float c = inv_t * kLog2e;
   for (int64_t at_row = blockIdx.x; at_row < n_rows; at_row += gridDim.x) {
     const int64_t row = n_rows - 1 - at_row;  // the forward's last rows first: they may still be cached
     const T* x = logits + rows.logits(row) + lo;
     T* out = grad + row * V + lo;
     const int64_t t = tokens[rows.token(row)];
-    const float g = g_lp && t != ignore ? g_lp[row] : 0.f;
-    const float h = ENT ? g_ent[row] : 0.f;
-    float a = g;
-    bool any = g != 0.f || h != 0.f;
-    for (int k = 0; k < K; ++k) {
-      const float gk = g_top[row * K + k];
-      a += gk;
-      any |= gk != 0.f;
-    }
     const float m = stats[2 * row], ls2 = stats[2 * row + 1] * kLog2e;
+    const float h = ENT ? g_ent[row] : 0.f, ent = ENT ? entropy[row] : 0.f;
+    const float g = g_lp && t != ignore ? g_lp[row] : 0.f;
+    const float g_own = lane < K ? g_top[row * K + lane] : 0.f;  // the alternatives' gradients, one to a lane
+    float a = g + wave_sum(g_own);
+    const bool any = g != 0.f || h != 0.f || __ballot(g_own != 0.f) != 0;
     if (!any || m == -INFINITY) {
       const float zero[N] = {};
 #pragma unroll
       for (int i = 0; i < kBackPacks; ++i)
-        if (i * kBackThreads + tid < packs) store_pack<T>(out + (i * kBackThreads + tid) * N, zero);
+        if (i * THREADS + tid < packs) store_pack<T>(out + (i * THREADS + tid) * N, zero);
       if (tid < len - packs * N) store_as(out + packs * N + tid, 0.f);
       continue;
     }
@@ -465,7 +462,7 @@ __global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kerne
     const float rest_l = plain ? fmaf(m, c, -L) + ls2 : 0.f;  // L - its rounded value
     const float scale = -inv_t * __builtin_amdgcn_exp2f(-rest_l);
     const float c1 = ENT ? h * kLn2 * scale : 0.f;
-    const float c0 = ENT ? scale * fmaf(h, fmaf(rest_l, -kLn2, entropy[row]), a) : scale * a;
+    const float c0 = ENT ? scale * fmaf(h, fmaf(rest_l, -kLn2, ent), a) : scale * a;
     const auto power = [&](float v) { return plain ? fmaf(v, c, -L) : (v - m) * c - ls2; };
     const auto part = [&](float d) {
       const float p = __builtin_amdgcn_exp2f(d);
@@ -474,33 +471,31 @@ __global__ __launch_bounds__(kBackThreads) void fl_token_logprobs_backward_kerne
     u32x4 v[kBackPacks];
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i)
-      if (i * kBackThreads + tid < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + (i * kBackThreads + tid) * N);
+      if (i * THREADS + tid < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + (i * THREADS + tid) * N);
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i) {
-      if (i * kBackThreads + tid < packs) {
+      if (i * THREADS + tid < packs) {
         float o[N];
 #pragma unroll
         for (int q = 0; q < N; ++q) o[q] = part(power(Pack<T>::get(v[i], q)));
-        store_pack<T>(out + (i * kBackThreads + tid) * N, o);
+        store_pack<T>(out + (i * THREADS + tid) * N, o);
       }
     }
     if (tid < len - packs * N) store_as(out + packs * N + tid, part(power(load_as<T>(x + packs * N + tid))));
     __syncthreads();  // what follows writes over what other threads wrote
-    if (tid <= K) {
-      const int64_t at = tid < K ? top_tok[row * K + tid] : t;
-      float own = tid < K ? g_top[row * K + tid] : g;
-      bool mine = at >= lo && at < lo + len;
-      if (tid < K && at == t) own += g;
-      for (int k = 0; k < K; ++k)
-        if (tid == K && top_tok[row * K + k] == t) mine = false;  // the alternative's thread has it
-      if (mine) store_as(out + (at - lo), fmaf(own, inv_t, part(power(load_as<T>(x + (at - lo))))));
+    if (tid < 64) {
+      const auto put = [&](int64_t at, float own) {
+        if (at >= lo && at < lo + len) store_as(out + (at - lo), fmaf(own, inv_t, part(power(load_as<T>(x + (at - lo))))));
+      };
+      const int64_t at = lane < K ? top_tok[row * K + lane] : -1;
+      if (lane < K) put(at, at == t ? g_own + g : g_own);
+      if (__ballot(lane < K && at == t) == 0 && lane == 0) put(t, g);  // (else that alternative's lane had it)
     }
-    __syncthreads();
   }
 }
 
 constexpr int64_t kMaxBlocks = 1 << 20;  // rows of a launch that run at once
-constexpr int64_t kMaxVocab = (int64_t)1 << 25;
+constexpr int64_t kMaxVocab = (int64_t)1 << 23;  // 1,024 segments of 8,192 fp32 logits
 
 bool shape_ok(int64_t outer, int64_t inner, int64_t V, int64_t so, int64_t si) {
   return outer > 0 && inner > 0 && outer <= ((int64_t)1 << 40) / inner && V > 0 && V <= kMaxVocab && so >= 0 && si >= 0;
@@ -512,19 +507,12 @@ struct Tile {
   int64_t seg_len;
 };
 
-Tile tile_of(int64_t rows, int64_t V, size_t size) {
+Tile tile_of(int64_t V, size_t size) {
   const int64_t n = (int64_t)(16 / size);
-  const auto holds = [&](int threads, int packs) { return V <= threads * packs * n; };
-  if (holds(64, 4)) return {64, 4, 1, V};
-  if (holds(256, 4)) return {256, 4, 1, V};
-  if (holds(256, 8) && rows > 512) return {256, 8, 1, V};
-  if (holds(1024, 4)) return {1024, 4, 1, V};
-  if (holds(1024, 8) && rows > 128) return {1024, 8, 1, V};
-  const int64_t per = rows > 128 ? 1024 * 8 * n : 256 * 8 * n;
-  int64_t segments = cdiv(V, per);
-  if (segments > 1024) segments = 1024;
-  const int64_t len = cdiv(cdiv(V, segments), n) * n;  // at most 1024 threads' 8 packs: V <= 2^25
-  return {len <= 256 * 8 * n ? 256 : 1024, 8, (int)cdiv(V, len), len};
+  if (V <= 64 * 4 * n) return {64, 4, 1, V};
+  if (V <= 256 * 4 * n) return {256, 4, 1, V};
+  const int64_t segments = cdiv(V, 256 * 8 * n), len = cdiv(cdiv(V, segments), n) * n;
+  return {256, 8, (int)cdiv(V, len), len};
 }
 
 size_t part_bytes(int64_t rows, const Tile& tile, int64_t K) {
@@ -550,8 +538,6 @@ int forward(const T* logits, const Rows& r, int64_t rows, int64_t V, float inv_t
   FL_LP(64, 4)
   FL_LP(256, 4)
   FL_LP(256, 8)
-  FL_LP(1024, 4)
-  FL_LP(1024, 8)
 #undef FL_LP
 #undef FL_LP2
   const hipError_t e = hipGetLastError();
@@ -571,7 +557,7 @@ extern "C" {
 size_t fl_token_logprobs_workspace_bytes(int64_t rows, int64_t V, int dtype, int64_t top_k) {
   if (rows <= 0 || rows > (int64_t)1 << 40 || V <= 0 || V > kMaxVocab || top_k < 0 || top_k > kMaxTop || !dtype_ok(dtype))
     return 0;
-  return part_bytes(rows, tile_of(rows, V, esize(dtype)), top_k);
+  return part_bytes(rows, tile_of(V, esize(dtype)), top_k);
 }
 
 int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inner, int64_t V, int64_t stride_outer,
@@ -588,7 +574,7 @@ int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inne
       (top_k && (!top_logprobs || !top_tokens || !aligned(top_logprobs, 4) || !aligned(top_tokens, 8))))
     return FL_ERR_INVALID_ARGUMENT;
   const int64_t rows = outer * inner;
-  const Tile tile = tile_of(rows, V, esize(dtype));
+  const Tile tile = tile_of(V, esize(dtype));
   const size_t need = part_bytes(rows, tile, top_k);
   if (need && (!workspace || workspace_bytes < need)) return FL_ERR_WORKSPACE;
   if (need && !aligned(workspace, 16)) return FL_ERR_INVALID_ARGUMENT;
@@ -620,19 +606,25 @@ int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int
   const Rows r = {inner, stride_outer, stride_inner, token_outer, token_inner};
   const unsigned blocks = (unsigned)(rows < kMaxBlocks ? rows : kMaxBlocks);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int64_t chunk = (int64_t)kBackThreads * kBackPacks * (16 / esize(dtype));
-  const dim3 grid((unsigned)blocks, (unsigned)cdiv(V, chunk));
-#define FL_LB(T, ENT)                                                                                              \
-  fl_token_logprobs_backward_kernel<T, ENT><<<grid, kBackThreads, 0, s>>>(                                         \
+  // one wave to a row that it holds, four otherwise (8,192 rows of 1,000 bf16: see the figures above)
+  const int64_t pack = (int64_t)(kBackPacks * 16 / esize(dtype));
+  const int threads = V <= 64 * pack ? 64 : 256;
+  const dim3 grid((unsigned)blocks, (unsigned)cdiv(V, threads * pack));
+#define FL_LB2(T, N, ENT)                                                                                          \
+  fl_token_logprobs_backward_kernel<T, N, ENT><<<grid, N, 0, s>>>(                                                 \
       static_cast<const T*>(logits), r, rows, (int)V, tokens, ignore_index, 1.0f / temperature,                    \
       g_top ? (int)top_k : 0, stats, entropy, top_tokens, g_logprobs, g_entropy, g_top, static_cast<T*>(g_logits))
+#define FL_LB(T)                                                                                                   \
+  if (threads == 64 && g_entropy) FL_LB2(T, 64, true);                                                             \
+  else if (threads == 64) FL_LB2(T, 64, false);                                                                    \
+  else if (g_entropy) FL_LB2(T, 256, true);                                                                        \
+  else FL_LB2(T, 256, false);
   if (dtype == FL_DTYPE_BF16) {
-    if (g_entropy) FL_LB(bf16_bits, true);
-    else FL_LB(bf16_bits, false);
+    FL_LB(bf16_bits)
   } else {
-    if (g_entropy) FL_LB(float, true);
-    else FL_LB(float, false);
+    FL_LB(float)
   }
+#undef FL_LB2
 #undef FL_LB
   return hip_status(hipGetLastError());
 }

@@ -12,7 +12,7 @@ from . import _native as nat
 from ._dispatch import no_grad_needed
 from ._train import _stock_grads
 
-MAX_TOP, MAX_VOCAB = 64, 1 << 25
+MAX_TOP, MAX_VOCAB = 64, 1 << 23
 MIN_TEMPERATURE, MAX_TEMPERATURE = 2.0 ** -20, 2.0 ** 20
 
 

@@ -468,7 +468,7 @@ int fl_mix(const void* y, const void* g, const void* mix_logit, int mix_dtype, i
 
 /*
  * Log probabilities of given tokens with entropy and top alternatives, and their gradient (no counterpart in
- * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V (at most 2^25) logits of dtype at
+ * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V (at most 2^23) logits of dtype at
  * logits + (r / inner) * stride_outer + (r % inner) * stride_inner (elements), its token tokens[(r / inner) *
  * token_outer + (r % inner) * token_inner]. With m = max x, d_v = (x_v - m) / temperature, s = sum e^{d_v}:
  *   logprobs [rows] = d_token - ln s; 0 where the token is ignore_index, NaN where it is outside 0 .. V - 1;
