@@ -136,6 +136,22 @@ def load() -> ctypes.CDLL:
         return lib
 
 
+_lists = None
+
+
+def lists():
+    """The host module that reads lists of tensors (``csrc/lists.cpp``); opened once, no fallback."""
+    global _lists
+    if _lists is None:
+        try:
+            from . import _lists as module
+        except ImportError as e:
+            raise RuntimeError(f"host extension not built: {LIB_PATH.parent / '_lists.so'} "
+                               "(run `python -m fields_lm_amd.build` or __graft_entry__.build())") from e
+        _lists = module
+    return _lists
+
+
 def check(code: int, what: str) -> None:
     """Map a C-ABI return code to the exception type the reference raises for that failure."""
     if code == FL_OK:

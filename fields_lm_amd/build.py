@@ -1,4 +1,4 @@
-"""Build recipe for the gfx950 shared library ``libfields_amd.so``.
+"""Build recipe for the gfx950 shared library ``libfields_amd.so`` and the host module ``_lists.so``.
 
 The library is compiled in-tree with ``hipcc --offload-arch=gfx950`` and loaded with ctypes
 (:mod:`fields_lm_amd._native`). It links against the HIP runtime by SONAME
@@ -13,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 import tempfile
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
@@ -31,6 +32,9 @@ LIB_PATH = PKG_DIR / "libfields_amd.so"
 # the library behind the C ABI
 BENCH_SOURCES = [PKG_DIR / "csrc" / "copy_ceiling.hip"]
 BENCH_LIB_PATH = PKG_DIR / "libfields_bench.so"
+# the host module that reads lists of tensors (CPython and PyTorch headers, no device code)
+LISTS_SOURCE = PKG_DIR / "csrc" / "lists.cpp"
+LISTS_PATH = PKG_DIR / "_lists.so"
 ARCH = "gfx950"
 
 # -packed-fp32-ops: keep v_pk_{add,mul,fma}_f32 out of the generated code (the compiler would
@@ -85,7 +89,29 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None, out: Path
         raise RuntimeError(f"{target.name}: hipcc left {len(missing)} kernel launch stub(s) undefined, "
                            f"so the library would not load: {missing[0]}")
     os.replace(tmp, target)
+    if target == LIB_PATH:
+        build_lists(verbose)
     return target
+
+
+def build_lists(verbose: bool = False) -> Path:
+    """Compile ``csrc/lists.cpp`` into the extension module ``_lists.so`` with the host compiler."""
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    tmp = LISTS_PATH.with_suffix(".so.tmp")
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(arg for path in include_paths() for arg in ("-isystem", path)), f"-I{sysconfig.get_paths()['include']}",
+           str(LISTS_SOURCE), f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-o", str(tmp)]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, LISTS_PATH)
+    return LISTS_PATH
 
 
 def unresolved_kernel_stubs(lib: Path) -> list[str]:

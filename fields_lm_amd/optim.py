@@ -11,7 +11,6 @@ from __future__ import annotations
 
 import array
 import math
-import operator
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -21,28 +20,46 @@ from . import _native as nat
 STATE_BLOCK = 256                   # values that share a scale in the 8-bit states
 STATE8_DTYPE = torch.float8_e4m3fn  # their codes
 
-_CODES = {torch.float32: nat.FL_DTYPE_F32, torch.bfloat16: nat.FL_DTYPE_BF16}
+_TYPES = (torch.float32, torch.bfloat16)  # in the order of their codes
 
 
-# One attribute of many tensors at once: a step reads some twenty of each of a model's hundreds of tensors, and a
-# loop over them in Python costs twice what these do (266 tensors, both moments in 8 bits: 1.2 ms; now 0.4 ms).
-_dtype, _shape, _layout = (operator.attrgetter(name) for name in ("dtype", "shape", "layout"))
-_contiguous, _numel, _device, _address = (torch.Tensor.is_contiguous, torch.Tensor.numel, torch.Tensor.get_device,
-                                          torch.Tensor.data_ptr)
+class _Words:
+    """Host arrays of ``n`` 64-bit words each, for the library's calls: ``at(i)`` is where the i-th starts."""
+
+    def __init__(self, n: int, arrays: int) -> None:
+        self.n, self.words = n, array.array("q", bytes(8 * n * arrays))
+        self.start = self.words.buffer_info()[0]
+
+    def at(self, i: int) -> int:
+        return self.start + 8 * self.n * i
 
 
-def _dense(tensors: Sequence[torch.Tensor]) -> List[torch.Tensor]:
-    """The gradients as the kernels read them: dense, contiguous."""
-    if any(layout != torch.strided for layout in set(map(_layout, tensors))):
-        raise TypeError("gradients must be dense")
-    if all(map(_contiguous, tensors)):
-        return list(tensors)
-    return [t.detach().contiguous() for t in tensors]
-
-
-def _words(values: Iterable[int]) -> array.array:
-    """A host array of 64-bit words for one of the library's calls (addresses or counts)."""
-    return array.array("q", values)
+def _read(tensors, what: str, device: torch.device, dtypes, addresses: int, *, counts: int = 0, codes: int = 0,
+          expected: int = 0, block: int = 1):
+    """Addresses (and counts, type codes) of contiguous tensors of ``dtypes`` on ``device`` with the expected counts of
+    values. Gradients of other strides are copied; returns the tensors that were read."""
+    call = nat.lists().read
+    if not isinstance(tensors, (list, tuple)):
+        tensors = list(tensors)
+    bad = call(tensors, device.index, dtypes, addresses, counts, codes, expected, block)
+    if bad is not None and bad[1] == "contiguous" and what == "gradients":
+        tensors = [t if t.is_contiguous() else t.detach().contiguous() for t in tensors]
+        bad = call(tensors, device.index, dtypes, addresses, counts, codes, expected, block)
+    if bad is None:
+        return tensors
+    i, why = bad
+    t = tensors[i]
+    if why == "tensor":
+        raise TypeError(f"{what}: number {i} is no tensor")
+    if why == "dtype":
+        raise TypeError(f"{what} must be {' or '.join(map(str, dtypes))}, number {i} is {t.dtype}")
+    if why == "layout":
+        raise TypeError(f"{what} must be dense, number {i} is {t.layout}")
+    if why == "device":
+        raise ValueError(f"{what} must be on {device}, number {i} is on {t.device}")
+    if why == "count":
+        raise ValueError(f"{what}: number {i} has {t.numel()} values, not as many as it should")
+    raise ValueError(f"{what} must be contiguous, number {i} is not")
 
 
 def grad_norm(grads: Iterable[torch.Tensor], max_norm: Optional[float] = None
@@ -62,28 +79,18 @@ def grad_norm(grads: Iterable[torch.Tensor], max_norm: Optional[float] = None
         raise RuntimeError("grad_norm requires a ROCm (cuda) device")
     if max_norm is not None and not float(max_norm) >= 0.0:
         raise ValueError(f"max_norm must be 0 or more, got {max_norm}")
-    types = list(map(_dtype, grads))
-    for t in set(types):
-        if t not in _CODES:
-            raise TypeError(f"gradients must be float32 or bfloat16, got {t}")
-    if set(map(_device, grads)) != {device.index}:
-        raise ValueError("the gradients must be on one device")
-    grads = _dense(grads)
-    n, numel, codes = len(grads), _words(map(_numel, grads)), array.array("i", map(_CODES.get, types))
-    addresses = _words(map(_address, grads))
+    n = len(grads)
+    words = _Words(n, 3)  # addresses, counts, type codes (half their words)
+    grads = _read(grads, "gradients", device, _TYPES, words.at(0), counts=words.at(1), codes=words.at(2))
     lib = nat.load()
     out = torch.empty(2, device=device, dtype=torch.float32)
-    ws = torch.empty(int(lib.fl_grad_norm_workspace_bytes(n, _start(numel))), device=device, dtype=torch.uint8)
+    ws = torch.empty(int(lib.fl_grad_norm_workspace_bytes(n, words.at(1))), device=device, dtype=torch.uint8)
     with nat.on(device):
         nat.check(lib.fl_grad_norm(
-            n, _start(addresses), _start(codes), _start(numel), 0.0 if max_norm is None else float(max_norm),
+            n, words.at(0), words.at(2), words.at(1), 0.0 if max_norm is None else float(max_norm),
             max_norm is not None, nat.ptr(out), nat.ptr(ws), ws.numel(), nat.stream_handle(device)), "fl_grad_norm")
     norm, scale = out.unbind()
     return norm if max_norm is None else (norm, scale)
-
-
-def _start(words: array.array) -> int:
-    return words.buffer_info()[0]
 
 
 def _device_scalar(t: torch.Tensor, what: str, device: torch.device) -> int:
@@ -101,19 +108,6 @@ def _check_hyper(lr, betas, eps, weight_decay) -> None:
         raise ValueError(f"eps must be finite and 0 or more, got {eps}")
     if not (float(weight_decay) >= 0.0 and math.isfinite(weight_decay)):
         raise ValueError(f"weight_decay must be finite and 0 or more, got {weight_decay}")
-
-
-def _check_lists(device, lists, dtypes, counts, what: str) -> None:
-    """Contiguous tensors of one of the ``dtypes`` each list is to have, on ``device``, with ``counts`` values."""
-    for tensors, dtype in zip(lists, dtypes):
-        if set(map(_dtype, tensors)) != {dtype}:
-            raise TypeError(f"{what} must be {dtype}, got {set(map(_dtype, tensors))}")
-        if set(map(_device, tensors)) != {device.index}:
-            raise ValueError(f"{what} must be on {device}, with the first parameter")
-        if list(map(_numel, tensors)) != counts:
-            raise ValueError(f"{what} must have {counts} values, got {list(map(_numel, tensors))}")
-        if not all(map(_contiguous, tensors)):
-            raise ValueError(f"{what} must be contiguous")
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -153,46 +147,42 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     device, dtype = params[0].device, params[0].dtype
     if device.type != "cuda":
         raise RuntimeError("adamw_step requires a ROCm (cuda) device")
-    code = _CODES.get(dtype)
-    if code is None:
+    if dtype not in _TYPES:
         raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
-    grads = _dense(grads)
-    counts = list(map(_numel, params))
-    _check_lists(device, (params, grads), (dtype, dtype), counts, "parameters and gradients")
-    if list(map(_shape, params)) != list(map(_shape, grads)):
-        raise ValueError("gradients must have their parameters' shapes")
-    _check_lists(device, (exp_avgs, exp_avg_sqs), (STATE8_DTYPE if eight else torch.float32,) * 2, counts, "states")
+    words = _Words(n, 8)  # counts; addresses of parameters, gradients, the moments, their scales, the steps
+    counts, at = words.at(0), [words.at(i) for i in range(1, 8)]
+    _read(params, "parameters", device, (dtype,), at[0], counts=counts)
+    read_grads = _read(grads, "gradients", device, (dtype,), at[1], expected=counts)
+    i = nat.lists().same_shapes(params if isinstance(params, (list, tuple)) else list(params), read_grads)
+    if i >= 0:
+        raise ValueError(f"gradient {i} has the shape {tuple(grads[i].shape)}, its parameter {tuple(params[i].shape)}")
+    state_types = (STATE8_DTYPE if eight else torch.float32,)
+    _read(exp_avgs, "states", device, state_types, at[2], expected=counts)
+    _read(exp_avg_sqs, "states", device, state_types, at[3], expected=counts)
     if eight:
-        _check_lists(device, (exp_avg_scales, exp_avg_sq_scales), (torch.float32,) * 2,
-                     [-(-c // STATE_BLOCK) for c in counts], "scales")
+        for k, scales in ((4, exp_avg_scales), (5, exp_avg_sq_scales)):
+            _read(scales, "scales", device, (torch.float32,), at[k], expected=counts, block=STATE_BLOCK)
     if isinstance(steps, torch.Tensor):
         if steps.dtype != torch.int64 or steps.device != device or steps.shape != (n,) or not steps.is_contiguous():
             raise ValueError(f"steps must be {n} int64 values on {device}")
         first = steps.data_ptr()
-        step_at = _words(range(first, first + 8 * n, 8))
+        words.words[7 * n:] = array.array("q", range(first, first + 8 * n, 8))
     else:
-        if len(steps) != n or set(map(_dtype, steps)) != {torch.int64} or set(map(_device, steps)) != {device.index} \
-                or set(map(_numel, steps)) != {1}:
+        if len(steps) != n:
             raise ValueError(f"steps must be {n} int64 values on {device}")
-        step_at = _words(map(_address, steps))
-        if len(set(step_at)) != n:
-            raise ValueError("a step counter occurs twice")
-    lists = [_words(map(_address, ts)) for ts in (params, grads, exp_avgs, exp_avg_sqs)]
-    lists += [_words(map(_address, ts)) for ts in (exp_avg_scales, exp_avg_sq_scales)] if eight else [None, None]
-    kept = [a for a, c in zip(lists[0], counts) if c]
-    if len(set(kept)) != len(kept):
-        raise ValueError("a parameter occurs twice")
+        ones = array.array("q", (1,)) * n
+        _read(steps, "steps", device, (torch.int64,), at[6], expected=ones.buffer_info()[0])
+    if nat.lists().repeats(at[0], counts, n) or nat.lists().repeats(at[6], 0, n):
+        raise ValueError("a parameter or a step counter occurs twice")
     scale = None if grad_scale is None else _device_scalar(grad_scale, "grad_scale", device)
     lr_ptr, lr_value = (_device_scalar(lr, "lr", device), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
-    numel = _words(counts)
-    at = [None if words is None else _start(words) for words in lists]
     lib = nat.load()
     ws = torch.empty(int(lib.fl_adamw_workspace_bytes(n)), device=device, dtype=torch.uint8)
     with nat.on(device):
         nat.check(lib.fl_adamw_step(
-            n, at[0], at[1], code, at[2], at[3], at[4], at[5], _start(numel), _start(step_at), lr_value, lr_ptr,
-            float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale, nat.ptr(ws), ws.numel(),
-            nat.stream_handle(device)), "fl_adamw_step")
+            n, at[0], at[1], nat.dtype_code(dtype), at[2], at[3], at[4] if eight else None, at[5] if eight else None,
+            counts, at[6], lr_value, lr_ptr, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale,
+            nat.ptr(ws), ws.numel(), nat.stream_handle(device)), "fl_adamw_step")
     torch.autograd.graph.increment_version(params)
 
 
@@ -223,7 +213,7 @@ class AdamW(torch.optim.Optimizer):
             if group["state_bits"] not in (8, 32):
                 raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
             for p in group["params"]:
-                if p.dtype not in _CODES:
+                if p.dtype not in _TYPES:
                     raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
         except (TypeError, ValueError):
             self.param_groups.pop()
@@ -262,7 +252,7 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         work: List[Tuple[dict, List[torch.Tensor]]] = []
         for group in self.param_groups:
-            for dtype in _CODES:
+            for dtype in _TYPES:
                 ps = [p for p in group["params"] if p.grad is not None and p.dtype == dtype]
                 if ps:
                     work.append((group, ps))

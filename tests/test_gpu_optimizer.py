@@ -221,13 +221,17 @@ def test_adamw_refuses_on_the_device(dev):
         with pytest.raises(TypeError):
             fl.adamw_step(*bad)
     for bad in (([p], [one(n=5)], [one()], [one()], step), ([p], [one()], [one(n=5)], [one()], step),
-                ([p], [torch.zeros(4)], [one()], [one()], step), ([p], [one()], [one()], [one()], step.int()),
+                ([p], [torch.zeros(4)], [one()], [one()], step), ([p], [one()], [one()], [one()], step.int()), ([p], [one()], [one()], [one()], [step.expand(2)]),
                 ([p], [one()], [one()], [one()], [step[0], step[0]]), ([p], [one()], [one()], [one()], step.cpu()),
                 ([one(n=8)[::2]], [one()], [one()], [one()], step), ([p], [one()], [one(n=8)[::2]], [one()], step),
                 ([p, p], [one(), one()], [one(), one()], [one(), one()], torch.zeros(2, dtype=torch.long, device=dev)),
                 ([p, one()], [one(), one()], [one(), one()], [one(), one()], [step, step])):
         with pytest.raises(ValueError):
             fl.adamw_step(*bad)
+    with pytest.raises(TypeError):
+        fl.adamw_step([p], [one()], [one()], [one()], [step.int()])
+    with pytest.raises(TypeError):
+        fl.adamw_step([p], [3], [one()], [one()], step)
     with pytest.raises(ValueError):
         fl.adamw_step([p], [one()], [one()], [one()], step, grad_scale=torch.zeros(2, device=dev))
     with pytest.raises(ValueError):
