@@ -20,8 +20,13 @@ struct Rows {
   int64_t inner;                      // row r is (r / inner, r % inner)
   int64_t stride_outer, stride_inner; // of the logits, in elements
   int64_t token_outer, token_inner;   // of the tokens
-  __device__ __forceinline__ int64_t logits(int64_t r) const { return r / inner * stride_outer + r % inner * stride_inner; }
-  __device__ __forceinline__ int64_t token(int64_t r) const { return r / inner * token_outer + r % inner * token_inner; }
+  // where row r is; most callers have one group of rows, and a 64-bit division is 200 instructions ahead of the loads
+  __device__ __forceinline__ void find(int64_t r, int64_t& logit_at, int64_t& token_at) const {
+    const int64_t o = r < inner ? 0 : (uint64_t)r >> 32 || (uint64_t)inner >> 32 ? r / inner : (uint32_t)r / (uint32_t)inner;
+    const int64_t i = r - o * inner;
+    logit_at = o * stride_outer + i * stride_inner;
+    token_at = o * token_outer + i * token_inner;
+  }
 };
 
 // Order of the alternatives as an integer: larger values first, -0 as 0, NaN above all, then the lower index.
@@ -145,7 +150,9 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     int tid = threadIdx.x;
     asm volatile("" : "+v"(tid));  // (what depends on it is computed where it is wanted, not kept over the rows)
     const int lane = tid & 63, wave = uniform(tid >> 6);
-    const int64_t t = out.tokens[rows.token(row)];
+    int64_t logit_at, token_at;
+    rows.find(row, logit_at, token_at);
+    const int64_t t = out.tokens[token_at];
     if (!TOP && !ENT && t == out.ignore) {  // nothing of this row is asked for
       if (whole && tid == 0) {
         out.logprobs[row] = 0.f;
@@ -153,17 +160,22 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
       }
       continue;
     }
-    const T* row_x = logits + rows.logits(row);
+    const T* row_x = logits + logit_at;
     const T* x = row_x + lo;
     float xt = 0.f;
     if (whole && tid == 0 && t >= 0 && t < V) xt = load_as<T>(row_x + t);
     u32x4 v[NV];
     const auto load = [&](auto get) {
+      if (packs == NV * THREADS) {  // all of the tile: nothing to stand in for
+#pragma unroll
+        for (int i = 0; i < NV; ++i) v[i] = get(reinterpret_cast<const u32x4_any*>(x + (i * THREADS + tid) * N));
+        return;
+      }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int j = i * THREADS + tid;
         v[i] = u32x4{Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
-        if (j < packs) v[i] = get(reinterpret_cast<const u32x4_any*>(x + (int64_t)j * N));
+        if (j < packs) v[i] = get(reinterpret_cast<const u32x4_any*>(x + j * N));
       }
     };
     // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 42 us, and 48 through
@@ -350,9 +362,11 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
   const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), K = out.K;
   const float c = inv_t * kLog2e;
   for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
-    const int64_t t = out.tokens[rows.token(row)];
+    int64_t logit_at, token_at;
+    rows.find(row, logit_at, token_at);
+    const int64_t t = out.tokens[token_at];
     float xt = 0.f;
-    if (tid == 0 && t >= 0 && t < V) xt = load_as<T>(logits + rows.logits(row) + t);
+    if (tid == 0 && t >= 0 && t < V) xt = load_as<T>(logits + logit_at + t);
     f32x4 p = {-INFINITY, -INFINITY, 0.f, 0.f};
     if (tid < segments && !(t == out.ignore && K == 0 && !out.entropy)) p = part[row * segments + tid];
     RowStats st;
@@ -444,9 +458,11 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
   const float c = inv_t * kLog2e;
   for (int64_t at_row = blockIdx.x; at_row < n_rows; at_row += gridDim.x) {
     const int64_t row = n_rows - 1 - at_row;  // the forward's last rows first: they may still be cached
-    const T* x = logits + rows.logits(row) + lo;
+    int64_t logit_at, token_at;
+    rows.find(row, logit_at, token_at);
+    const T* x = logits + logit_at + lo;
     T* out = grad + row * V + lo;
-    const int64_t t = tokens[rows.token(row)];
+    const int64_t t = tokens[token_at];
     const float m = stats[2 * row], ls2 = stats[2 * row + 1] * kLog2e;
     const float h = ENT ? g_ent[row] : 0.f, ent = ENT ? entropy[row] : 0.f;
     const float g = g_lp && t != ignore ? g_lp[row] : 0.f;

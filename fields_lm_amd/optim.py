@@ -187,11 +187,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
 
 class AdamW(torch.optim.Optimizer):
-    """AdamW over :func:`adamw_step`: one call per parameter group and type.
+    """AdamW over :func:`adamw_step`: one call per parameter group, type and device.
 
     ``state_bits`` 32 keeps both moments in fp32 (8 bytes a value), 8 in 8-bit blocks (2 bytes and 1 / 32).
     ``max_grad_norm`` clips the norm over all groups' gradients inside the step, without rewriting them; the norm
-    stays in ``self.grad_norm`` (fp32, on the device), and a step whose norm is not finite changes nothing.
+    stays in ``self.grad_norm`` (fp32, on the device; all gradients on one), and a step whose norm is not finite changes
+    nothing.
     A parameter without a gradient is left alone and its step not counted. States are made at a parameter's
     first step, which must not be under graph capture.
     """
@@ -252,10 +253,11 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         work: List[Tuple[dict, List[torch.Tensor]]] = []
         for group in self.param_groups:
-            for dtype in _TYPES:
-                ps = [p for p in group["params"] if p.grad is not None and p.dtype == dtype]
-                if ps:
-                    work.append((group, ps))
+            kinds: dict = {}
+            for p in group["params"]:
+                if p.grad is not None:
+                    kinds.setdefault((p.dtype, p.device), []).append(p)
+            work += [(group, ps) for ps in kinds.values()]
         if not work:
             return loss
         scale = None

@@ -100,8 +100,8 @@ def make(dev, rows, vocab, dtype, seed, spread=2.5):
 
 
 # one logit; less than a vector, a wave and a block; odd; around the sizes that change the tile
-VOCABS = [1, 2, 7, 63, 65, 255, 257, 1000, 2047, 2049, 4096, 5003, 8191, 8193, 16384, 16385, 32767, 32769, 40001, 65537,
-          131073]
+VOCABS = [1, 2, 7, 63, 65, 255, 257, 1000, 1024, 1025, 2047, 2049, 4096, 4097, 5003, 8191, 8193, 16384, 16385, 32767, 32769,
+          40001, 65537, 131073, 600011]
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
@@ -112,6 +112,16 @@ def test_forward_over_vocabularies(dev, vocab, dtype):
         x, t = make(dev, rows, vocab, dtype, vocab + rows)
         r = fl.token_logprobs(x, t, temperature=temperature, top_k=k, entropy=entropy)
         check_forward(x, t, temperature, k, entropy, r)
+
+
+def test_forward_of_the_longest_row(dev):
+    """2^23 logits: 1,024 segments; with the largest in the last and equal ones in others."""
+    print("[case] token_logprobs V=2^23", flush=True)
+    x, t = make(dev, 2, 1 << 23, torch.float32, 3)
+    x[0, -1], x[1, 5], x[1, 1 << 22] = 30.0, 29.0, 29.0
+    check_forward(x, t, 1.0, 64, True, fl.token_logprobs(x, t, top_k=64, entropy=True))
+    with pytest.raises(ValueError):
+        fl.token_logprobs(torch.empty(1, (1 << 23) + 1, device=dev), t[:1])
 
 
 @pytest.mark.parametrize("rows,vocab", [(1, 16384), (64, 16384), (300, 16384), (700, 501), (5000, 33), (257, 12345), (40, 70000)])
@@ -275,6 +285,30 @@ def test_gradients_of_special_rows(dev, vocab, dtype):
     z = x.clone().requires_grad_()  # nothing flows: zeros, also from rows with NaN
     got, = torch.autograd.grad(fl.token_logprobs(z, t).logprobs, z, torch.zeros(15, device=dev))
     assert float(got.float().abs().max()) == 0.0
+
+
+def test_gradients_of_slices_and_broadcast_logits(dev):
+    print("[case] token_logprobs gradients of slices and broadcast logits", flush=True)
+    for dtype in (torch.bfloat16, torch.float32):
+        x, t = make(dev, 3 * 9, 1001, dtype, 5)
+        x, t = x.view(3, 9, 1001), t.view(3, 9)
+        g = torch.randn(3, 9, device=dev, generator=torch.Generator(device=dev).manual_seed(2))
+        z = x.clone().requires_grad_()
+        got, = torch.autograd.grad(fl.token_logprobs(z[:, :-1], t[:, 1:]).logprobs, z, g[:, 1:])
+        assert float(got[:, -1].float().abs().max()) == 0.0
+        check_grad(x[:, :-1].reshape(-1, 1001), t[:, 1:].reshape(-1), 1.0, 0, g[:, 1:].reshape(-1), None, None,
+                   got[:, :-1].reshape(-1, 1001))
+        one = x[:, :1].clone().requires_grad_()  # every position reads one row's logits
+        wide = one.expand(3, 9, 1001)
+        got, = torch.autograd.grad(fl.token_logprobs(wide, t).logprobs, wide, g)
+        check_grad(x[:, :1].expand(3, 9, 1001).reshape(-1, 1001), t.reshape(-1), 1.0, 0, g.reshape(-1), None, None,
+                   got.reshape(-1, 1001))
+        total, = torch.autograd.grad(fl.token_logprobs(one.expand(3, 9, 1001), t).logprobs, one, g)
+        assert total.shape == one.shape
+        z = x.clone().requires_grad_()  # gradients that are broadcast themselves (a mean's)
+        got, = torch.autograd.grad(fl.token_logprobs(z.transpose(0, 1), t.t()).logprobs.mean(), z)
+        check_grad(x.reshape(-1, 1001), t.reshape(-1), 1.0, 0, torch.full((27,), 1 / 27, device=dev), None, None,
+                   got.reshape(-1, 1001))
 
 
 def test_gradient_against_differences(dev):

@@ -159,6 +159,26 @@ def test_adamw_neighbours_stay_as_they_were(dev):
                 assert all(bool((torch.cat((s[:3], s[7:])) == 0.25).all()) for s in sc)
 
 
+@pytest.mark.parametrize("eight", [False, True])
+def test_one_tensor_past_2_to_31_values(dev, eight):
+    print(f"[case] adamw_step and grad_norm past 2^31 values, 8 bits: {eight}", flush=True)
+    n = (1 << 31) + 300
+    p, g = (torch.zeros(n, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    at = torch.tensor([0, 1, (1 << 31) - 1, 1 << 31, n - 1], device=dev)
+    p[at], g[at] = torch.tensor([1.0, -2.0, 3.0, -4.0, 5.0], device=dev).bfloat16(), torch.tensor([2.0, 1.0, -1.0, 3.0, -2.0],
+                                                                                                 device=dev).bfloat16()
+    assert abs(float(fl.grad_norm([g])) - math.sqrt(19.0)) <= 2 * U * math.sqrt(19.0)
+    new = (lambda: torch.zeros(n, device=dev, dtype=torch.uint8).view(STATE8_DTYPE)) if eight else lambda: torch.zeros(n, device=dev)
+    m, v = new(), new()
+    scales = [[torch.zeros(-(-n // 256), device=dev)] for _ in range(2)] if eight else [None, None]
+    old = p[at].clone()
+    fl.adamw_step([p], [g], [m], [v], torch.zeros(1, dtype=torch.long, device=dev), exp_avg_scales=scales[0],
+                  exp_avg_sq_scales=scales[1], **{**HYPER, "lr": 0.1})
+    exp, tol = exact(old, g[at], torch.zeros(5, device=dev), torch.zeros(5, device=dev), 1, **{**HYPER, "lr": 0.1})
+    near(p[at], exp[0], tol[0], "p")
+    assert int((p != 0).sum()) == 5 and int((m.view(torch.uint8) if eight else m).ne(0).sum()) == 5
+
+
 def test_adamw_lr_and_scale_are_read_on_the_device(dev):
     print("[case] adamw_step with lr on the device, and steps that are skipped", flush=True)
     p, g, m, v = start32(dev, [1000, 3], torch.float32, 3)
