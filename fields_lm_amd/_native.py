@@ -136,20 +136,26 @@ def load() -> ctypes.CDLL:
         return lib
 
 
-_lists = None
+_host = None
 
 
-def lists():
-    """The host module that reads lists of tensors (``csrc/lists.cpp``); opened once, no fallback."""
-    global _lists
-    if _lists is None:
+def host():
+    """The host side of some calls (``csrc/host.cpp``); opened and given the library's entry points once, no
+    fallback."""
+    global _host
+    if _host is None:
+        lib = load()
         try:
-            from . import _lists as module
+            from . import _host as module
         except ImportError as e:
-            raise RuntimeError(f"host extension not built: {LIB_PATH.parent / '_lists.so'} "
+            raise RuntimeError(f"host extension not built: {LIB_PATH.parent / '_host.so'} "
                                "(run `python -m fields_lm_amd.build` or __graft_entry__.build())") from e
-        _lists = module
-    return _lists
+        from .logprobs import stock_gradient
+
+        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "fl_token_logprobs_workspace_bytes", "fl_token_logprobs", "fl_token_logprobs_backward")), stock_gradient)
+        _host = module
+    return _host
 
 
 def check(code: int, what: str) -> None:

@@ -1,4 +1,4 @@
-"""Build recipe for the gfx950 shared library ``libfields_amd.so`` and the host module ``_lists.so``.
+"""Build recipe for the gfx950 shared library ``libfields_amd.so`` and the host module ``_host.so``.
 
 The library is compiled in-tree with ``hipcc --offload-arch=gfx950`` and loaded with ctypes
 (:mod:`fields_lm_amd._native`). It links against the HIP runtime by SONAME
@@ -32,9 +32,9 @@ LIB_PATH = PKG_DIR / "libfields_amd.so"
 # the library behind the C ABI
 BENCH_SOURCES = [PKG_DIR / "csrc" / "copy_ceiling.hip"]
 BENCH_LIB_PATH = PKG_DIR / "libfields_bench.so"
-# the host module that reads lists of tensors (CPython and PyTorch headers, no device code)
-LISTS_SOURCE = PKG_DIR / "csrc" / "lists.cpp"
-LISTS_PATH = PKG_DIR / "_lists.so"
+# the host side of some calls (CPython and PyTorch headers, no device code)
+HOST_SOURCE = PKG_DIR / "csrc" / "host.cpp"
+HOST_PATH = PKG_DIR / "_host.so"
 ARCH = "gfx950"
 
 # -packed-fp32-ops: keep v_pk_{add,mul,fma}_f32 out of the generated code (the compiler would
@@ -90,28 +90,30 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None, out: Path
                            f"so the library would not load: {missing[0]}")
     os.replace(tmp, target)
     if target == LIB_PATH:
-        build_lists(verbose)
+        build_host(verbose)
     return target
 
 
-def build_lists(verbose: bool = False) -> Path:
-    """Compile ``csrc/lists.cpp`` into the extension module ``_lists.so`` with the host compiler."""
+def build_host(verbose: bool = False) -> Path:
+    """Compile ``csrc/host.cpp`` into the extension module ``_host.so`` with the host compiler."""
     import torch
     from torch.utils.cpp_extension import include_paths
 
-    tmp = LISTS_PATH.with_suffix(".so.tmp")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+    tmp = HOST_PATH.with_suffix(".so.tmp")
+    rocm = Path(hipcc()).resolve().parents[1]
+    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(arg for path in include_paths() for arg in ("-isystem", path)), f"-I{sysconfig.get_paths()['include']}",
-           str(LISTS_SOURCE), f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-isystem", str(rocm / "include"), f"-I{INCLUDE_DIR}", str(HOST_SOURCE), f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
+           "-lc10_hip",
            "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
-    os.replace(tmp, LISTS_PATH)
-    return LISTS_PATH
+    os.replace(tmp, HOST_PATH)
+    return HOST_PATH
 
 
 def unresolved_kernel_stubs(lib: Path) -> list[str]:

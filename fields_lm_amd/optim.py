@@ -38,7 +38,7 @@ def _read(tensors, what: str, device: torch.device, dtypes, addresses: int, *, c
           expected: int = 0, block: int = 1):
     """Addresses (and counts, type codes) of contiguous tensors of ``dtypes`` on ``device`` with the expected counts of
     values. Gradients of other strides are copied; returns the tensors that were read."""
-    call = nat.lists().read
+    call = nat.host().read
     if not isinstance(tensors, (list, tuple)):
         tensors = list(tensors)
     bad = call(tensors, device.index, dtypes, addresses, counts, codes, expected, block)
@@ -153,7 +153,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     counts, at = words.at(0), [words.at(i) for i in range(1, 8)]
     _read(params, "parameters", device, (dtype,), at[0], counts=counts)
     read_grads = _read(grads, "gradients", device, (dtype,), at[1], expected=counts)
-    i = nat.lists().same_shapes(params if isinstance(params, (list, tuple)) else list(params), read_grads)
+    i = nat.host().same_shapes(params if isinstance(params, (list, tuple)) else list(params), read_grads)
     if i >= 0:
         raise ValueError(f"gradient {i} has the shape {tuple(grads[i].shape)}, its parameter {tuple(params[i].shape)}")
     state_types = (STATE8_DTYPE if eight else torch.float32,)
@@ -172,7 +172,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             raise ValueError(f"steps must be {n} int64 values on {device}")
         ones = array.array("q", (1,)) * n
         _read(steps, "steps", device, (torch.int64,), at[6], expected=ones.buffer_info()[0])
-    if nat.lists().repeats(at[0], counts, n) or nat.lists().repeats(at[6], 0, n):
+    if nat.host().repeats(at[0], counts, n) or nat.host().repeats(at[6], 0, n):
         raise ValueError("a parameter or a step counter occurs twice")
     scale = None if grad_scale is None else _device_scalar(grad_scale, "grad_scale", device)
     lr_ptr, lr_value = (_device_scalar(lr, "lr", device), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))

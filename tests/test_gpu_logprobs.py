@@ -192,6 +192,15 @@ def test_tokens_outside_the_vocabulary_and_ignored_ones(dev):
     assert fl.token_logprobs(x, t, ignore_index=5).logprobs.cpu()[:2].isnan().tolist() == [False, True]
 
 
+def test_no_rows(dev):
+    print("[case] token_logprobs without rows", flush=True)
+    x = torch.randn(4, 0, 7, device=dev, requires_grad=True)
+    r = fl.token_logprobs(x, torch.zeros(4, 0, dtype=torch.long, device=dev), top_k=3, entropy=True)
+    assert r.logprobs.shape == r.entropy.shape == (4, 0) and r.top_logprobs.shape == r.top_tokens.shape == (4, 0, 3)
+    assert r.top_tokens.dtype == torch.int64
+    assert torch.autograd.grad(r.logprobs.sum(), x)[0].shape == x.shape
+
+
 def test_many_rows_past_32_bit_offsets(dev):
     """Logits of more than 2^31 values: rows on both sides of the border."""
     print("[case] token_logprobs past 2^31 values", flush=True)
@@ -369,8 +378,14 @@ def test_partial_outputs_and_no_gradient(dev):
     check_grad(x.detach(), t, 1.0, 4, None, None, gt, got)
     import torch.autograd.forward_ad as fwad
 
-    with fwad.dual_level(), pytest.raises(NotImplementedError):  # a tangent is refused, not lost
-        fl.token_logprobs(fwad.make_dual(x.detach(), torch.ones_like(x)), t)
+    with fwad.dual_level():
+        for z in (x.detach(), x):
+            with pytest.raises(NotImplementedError):  # a tangent is refused, not lost
+                fl.token_logprobs(fwad.make_dual(z, torch.ones_like(x)), t)
+    with pytest.raises(RuntimeError):  # a transform's wrapper has no memory to read
+        torch.func.vmap(lambda a, b: fl.token_logprobs(a, b).logprobs)(x.detach(), t)
+    with pytest.raises(ValueError):
+        fl.token_logprobs(x, t.cpu())
     changed = x.detach().clone().requires_grad_()
     y = changed * 1.0
     r = fl.token_logprobs(y, t)
