@@ -31,11 +31,12 @@ struct Rows {
 
 // Order of the alternatives as an integer: larger values first, -0 as 0, NaN above all, then the lower index.
 // Every key lies strictly between 0 and ~0, which stand for none and for no limit.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t b = __float_as_uint(x + 0.0f);
+  return x != x ? 0xfffffffeu : b & 0x80000000u ? ~b : b | 0x80000000u;
+}
 __device__ __forceinline__ uint64_t rank_key(float x, uint32_t index) {
-  uint32_t b = __float_as_uint(x + 0.0f);
-  b = b & 0x80000000u ? ~b : b | 0x80000000u;
-  if (x != x) b = 0xfffffffeu;
-  return (uint64_t)b << 32 | (0xffffffffu - index);
+  return (uint64_t)order_of(x) << 32 | (0xffffffffu - index);
 }
 
 __device__ __forceinline__ float key_value(uint64_t key) {
@@ -86,7 +87,8 @@ __device__ __forceinline__ uint64_t key_max(uint64_t v) {
   return a > b ? a : b;
 }
 
-constexpr int kCand = 512;           // candidates for the alternatives that a block ranks
+constexpr int kCand = 512;    // candidates for the alternatives that a block ranks
+constexpr int kFewTop = 20;   // alternatives up to which 64 groups bound them (25 candidates for 20; 300 for 64)
 constexpr float kPlainScale = 1048576.0f;  // below this |m| c, x c - fl(m c) is as good as (x - m) c
 
 // What a row's results are made of: m, log2 of s, the mean of d log2(e) under the distribution.
@@ -130,18 +132,18 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
 // One block to a row, or to a segment of one (gridDim.y of them): its logits stay in registers, NV packs of
 // 16 bytes to a thread, for the maximum, the sums and the alternatives.
 //
-// Alternatives: the threads' maxima, in 64 groups, give a value that at least K logits reach: their K-th
-// largest (to 16 bits). Only logits from there up are candidates, some K to 2 K of them in text; they are
+// Alternatives: the threads' maxima (in 64 groups where K is small) give a value that at least K logits reach: their
+// K-th largest, to 16 bits. Only logits from there up are candidates, little more than K of them in text; they are
 // ranked by counting. Rows that hold NaN or +inf, and rows with more candidates than fit (equal logits), are
-// searched K times instead.
+// searched by halving instead: for the K-th largest value, then for the index up to which those equal to it count.
 template <typename T, int THREADS, int NV, bool ENT, bool TOP>
 __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, int seg_len, float inv_t, Outputs out,
     f32x4* __restrict__ part, uint64_t* __restrict__ part_keys) {
   constexpr int N = Pack<T>::N, WAVES = THREADS / 64;
   __shared__ float s_max[THREADS], s_sum[2 * WAVES];
-  __shared__ unsigned long long s_cand[kCand], s_best[WAVES];
-  __shared__ int s_n;
+  __shared__ unsigned long long s_cand[kCand];
+  __shared__ int s_n, s_count[WAVES];
   const int K = TOP ? out.K : 0;
   const int lo = (int)blockIdx.y * seg_len, len = V - lo < seg_len ? V - lo : seg_len, packs = len / N;
   const bool whole = gridDim.y == 1;
@@ -197,6 +199,16 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         }
       }
       f(rest, NV, 0);
+    };
+    // f(logit, place in the segment), places that it lacks from len up
+    const auto for_places = [&](auto f) {
+      for (int j = tid; __ballot(j < packs); j += THREADS) {
+        u32x4 again = {Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
+        if (j < packs) again = *reinterpret_cast<const u32x4_any*>(x + j * N);
+#pragma unroll
+        for (int q = 0; q < N; ++q) f(Pack<T>::get(again, q), j < packs ? j * N + q : len);
+      }
+      f(rest, tid < len - packs * N ? packs * N + tid : len);
     };
     if (TOP && tid == 0) s_n = 0;
     float mine = rest, pack_top[TOP ? NV : 1];
@@ -264,30 +276,37 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
           part_keys[(row * gridDim.y + blockIdx.y) * K + k] = key;
         }
       };
+      const auto push = [&](float a, int at) {  // at: where in the segment
+        const int k = atomicAdd(&s_n, 1);
+        if (k < kCand) s_cand[k] = (uint64_t)__float_as_uint(a) << 32 | (uint32_t)at;
+      };
       int n = kCand + 1;
+      uint32_t bound = 0;  // the upper half of order_of of a value that K logits reach
       if (sum == sum) {
-        uint32_t g = __float_as_uint(group), bound = 0;
-        g = (g & 0x80000000u ? ~g : g | 0x80000000u) >> 16;
+        if (WAVES > 1 && K > kFewTop) {
+          uint32_t g[WAVES];
 #pragma unroll
-        for (int bit = 15; bit >= 0; --bit) {
-          const uint32_t test = bound | 1u << bit;
-          if (__popcll(__ballot(g >= test)) >= K) bound = test;
-        }
-        const auto push = [&](float a, uint32_t at) {  // at: where in the segment
-          const int k = atomicAdd(&s_n, 1);
-          if (k < kCand) s_cand[k] = (uint64_t)__float_as_uint(a) << 32 | at;
-        };
-        if (bound <= 0x007fu) {
-          // fewer than K groups hold a logit above -inf: all of those, and the masked ones of lowest index
-          for (int i = tid; i < len; i += THREADS) {
-            const float a = load_as<T>(x + i);
-            if (a > -INFINITY || i < 2 * K) push(a, (uint32_t)i);
+          for (int w = 0; w < WAVES; ++w) g[w] = order_of(s_max[w * 64 + lane]) >> 16;
+          for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t test = bound | 1u << bit;
+            int reach = 0;
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) reach += __popcll(__ballot(g[w] >= test));
+            if (reach >= K) bound = test;
           }
         } else {
-          const float least = __uint_as_float(bound & 0x8000u ? bound << 16 ^ 0x80000000u : ~(bound << 16));
-          uint32_t hit = 0;  // the packs that hold a candidate, read once more
+          const uint32_t g = order_of(group) >> 16;
 #pragma unroll
-          for (int i = 0; i < NV; ++i) hit |= pack_top[i] >= least ? 1u << i : 0u;
+          for (int bit = 15; bit >= 0; --bit) {
+            const uint32_t test = bound | 1u << bit;
+            if (__popcll(__ballot(g >= test)) >= K) bound = test;
+          }
+        }
+        // The packs that hold a candidate are read once more.
+        const auto scan = [&](auto in_pack, auto is) {
+          uint32_t hit = 0;
+#pragma unroll
+          for (int i = 0; i < NV; ++i) hit |= in_pack(i) ? 1u << i : 0u;
           while (hit) {
             const int at = (__builtin_ctz(hit) * THREADS + tid) * N;
             hit &= hit - 1;
@@ -295,11 +314,58 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
 #pragma unroll
             for (int q = 0; q < N; ++q) {
               const float a = Pack<T>::get(again, q);
-              if (a >= least) push(a, (uint32_t)(at + q));
+              if (is(a, at + q)) push(a, at + q);
             }
           }
-          if (rest >= least) push(rest, (uint32_t)(packs * N + tid));
+        };
+        if (bound > 0x007fu) {
+          const float least = __uint_as_float(bound & 0x8000u ? bound << 16 ^ 0x80000000u : ~(bound << 16));
+          scan([&](int i) { return pack_top[i] >= least; }, [&](float a, int) { return a >= least; });
+          if (rest >= least) push(rest, packs * N + tid);
+        } else {
+          // fewer than K groups hold a logit above -inf: all of those, and the masked ones of lowest index
+          scan([&](int i) { return i * THREADS + tid < packs && (pack_top[i] > -INFINITY || (i * THREADS + tid) * N < 2 * K); },
+               [&](float a, int at) { return a > -INFINITY || at < 2 * K; });
+          const int at = packs * N + tid;
+          if (at < len && (rest > -INFINITY || at < 2 * K)) push(rest, at);
         }
+        __syncthreads();
+        n = s_n;
+      }
+      if (n > kCand) {  // (block-uniform)
+        const int want = K < len ? K : len;
+        // how many of the segment's logits fulfil is(order, place), over the block
+        const auto count = [&](auto is) {
+          int mine_n = 0;
+          for_places([&](float a, int at) { mine_n += __popcll(__ballot(at < len && is(order_of(a), at))); });
+          __syncthreads();
+          if (lane == 0) s_count[wave] = mine_n;
+          __syncthreads();
+          int all = s_count[0];
+#pragma unroll
+          for (int w = 1; w < WAVES; ++w) all += s_count[w];
+          return all;
+        };
+        uint32_t low = sum == sum ? bound << 16 : 0, high = sum == sum ? order_of(base) : 0xffffffffu;
+        while (low < high) {
+          const uint32_t mid = low + (high - low) / 2 + 1;
+          if (count([&](uint32_t o, int) { return o >= mid; }) >= want) low = mid;
+          else high = mid - 1;
+        }
+        const int need = want - count([&](uint32_t o, int) { return o > low; });
+        int last = len - 1;
+        for (int from = 0; from < last;) {
+          const int mid = (from + last) / 2;
+          if (count([&](uint32_t o, int at) { return o == low && at <= mid; }) >= need) last = mid;
+          else from = mid + 1;
+        }
+        __syncthreads();
+        if (tid == 0) s_n = 0;
+        __syncthreads();
+        for_places([&](float a, int at) {
+          const uint32_t o = order_of(a);
+          if (at < len && (o > low || (o == low && at <= last))) push(a, at);
+        });
         __syncthreads();
         n = s_n;
       }
@@ -318,30 +384,15 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
           }
           if (lane < n && rank < K) put(rank, key);
         }
-      } else if (n <= kCand) {
+      } else {
+        for (int i = tid; i < n; i += THREADS) s_cand[i] = key_at(i);
+        __syncthreads();
         for (int i = tid; i < n; i += THREADS) {
-          const uint64_t key = key_at(i);
+          const uint64_t key = s_cand[i];
           int rank = 0;
 #pragma unroll 4
-          for (int j = 0; j < n; ++j) rank += key_at(j) > key;
+          for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
           if (rank < K) put(rank, key);
-        }
-      } else {
-        uint64_t last = ~0ull;
-        for (int k = 0; k < K; ++k) {
-          uint64_t best = 0;
-          for (int i = tid; i < len; i += THREADS) {
-            const uint64_t key = rank_key(load_as<T>(x + i), (uint32_t)(lo + i));
-            if (key < last && key > best) best = key;
-          }
-          best = key_max(best);
-          __syncthreads();
-          if (lane == 0) s_best[wave] = best;
-          __syncthreads();
-          for (int w = 0; w < WAVES; ++w) best = s_best[w] > best ? s_best[w] : best;
-          last = best;
-          if (tid == 0) put(k, best);
-          if (best == 0) last = 1;  // none left: nothing is below
         }
       }
       for (int k = n + tid; k < K; k += THREADS) put(k, 0);  // (a segment of fewer than K)
@@ -422,8 +473,8 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
   }
 }
 
-// Gradients: a block writes kBackPacks packs to a thread of one row, then puts in the logits that carry a
-// gradient of their own (the given token, the alternatives). With L = m c + log2 s (c = log2(e) / T) split into its
+// Gradients: a block writes kBackPacks packs to a thread of one row, then the logits that carry a gradient of their
+// own (the given token, the alternatives). With L = m c + log2 s (c = log2(e) / T) split into its
 // rounded value and the rest, p = 2^(x c - L) is one fused product and one power, and the row's constants make
 //   dx = -(p / T) (g + sum g_k + h (ln p + H))
 // two more operations, one without h. A row whose gradients are all 0 gets zeros whatever its logits hold.
@@ -490,6 +541,9 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
       const float p = __builtin_amdgcn_exp2f(d);
       return ENT ? p * fmaf(c1, fmaxf(d, -1000.f), c0) : p * c0;
     };
+    const int64_t at = lane < K ? top_tok[row * K + lane] : -1;
+    const bool mine = at >= lo && at < lo + len;
+    const float x_own = mine ? load_as<T>(x + (at - lo)) : 0.f, x_t = t >= lo && t < lo + len ? load_as<T>(x + (t - lo)) : 0.f;
     u32x4 v[kBackPacks];
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i)
@@ -504,15 +558,18 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
       }
     }
     if (tid < len - packs * N) store_as(out + packs * N + tid, part(power(load_as<T>(x + packs * N + tid))));
-    __syncthreads();  // what follows writes over what other threads wrote
-    if (tid < 64) {
-      const auto put = [&](int64_t at, float own) {
-        if (at >= lo && at < lo + len) store_as(out + (at - lo), fmaf(own, inv_t, part(power(load_as<T>(x + (at - lo))))));
-      };
-      const int64_t at = lane < K ? top_tok[row * K + lane] : -1;
-      if (lane < K) put(at, at == t ? g_own + g : g_own);
-      if (__ballot(lane < K && at == t) == 0 && lane == 0) put(t, g);  // (else that alternative's lane had it)
+    // The logits with a gradient of their own, each put over by the thread that has just written it.
+    const auto owner_of = [&](int k) { return k < packs * N ? k / N % THREADS : k - packs * N; };
+    const float value = fmaf(at == t ? g_own + g : g_own, inv_t, part(power(x_own)));
+    const int k_own = (int)(at - lo), owner = owner_of(k_own);
+    for (uint64_t left = __ballot(mine && owner >> 6 == tid >> 6); left; left &= left - 1) {
+      const int i = __builtin_ctzll(left);
+      const int k = __builtin_amdgcn_readlane(k_own, i);
+      if (tid == __builtin_amdgcn_readlane(owner, i))
+        store_as(out + k, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(value), i)));
     }
+    if (t >= lo && t < lo + len && __ballot(at == t) == 0 && tid == owner_of((int)(t - lo)))
+      store_as(out + (t - lo), fmaf(g, inv_t, part(power(x_t))));  // (else it is among the alternatives)
   }
 }
 

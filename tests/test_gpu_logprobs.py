@@ -148,7 +148,7 @@ def test_forward_reads_slices_in_place(dev):
 def special_rows(dev, vocab, dtype):
     """Rows that go wrong first: masked, empty, equal, of the type's lowest value, infinite, NaN, large."""
     g = torch.Generator(device=dev).manual_seed(vocab)
-    x = (torch.randn(15, vocab, device=dev, generator=g) * 3).to(dtype)
+    x = (torch.randn(18, vocab, device=dev, generator=g) * 3).to(dtype)
     low = torch.finfo(dtype).min
     x[0, 1:] = float("-inf")                     # one token left
     x[1] = float("-inf")                         # none left
@@ -168,6 +168,10 @@ def special_rows(dev, vocab, dtype):
     x[12, vocab // 4] = low
     x[13, 0], x[13, vocab - 1] = float("inf"), float("nan")
     x[14] = float("nan")
+    x[15] = torch.randint(0, 3, (vocab,), device=dev, generator=g).to(dtype)  # a few values, many times each
+    x[16] = torch.where(torch.arange(vocab, device=dev) % 131 == 7, x[16], float("-inf"))  # few and far between
+    x[17, vocab // 3:vocab // 3 + 90] = float("-inf")
+    x[17, :vocab // 3] = float("-inf")
     return x
 
 
@@ -176,9 +180,9 @@ def special_rows(dev, vocab, dtype):
 def test_forward_of_special_rows(dev, vocab, dtype):
     print(f"[case] token_logprobs special rows V={vocab} {dtype}", flush=True)
     x = special_rows(dev, vocab, dtype)
-    for k in sorted({min(vocab, n) for n in (1, 20, 64)}):
+    for k in sorted({min(vocab, n) for n in (1, 20, 21, 64)}):
         for at in (0, vocab - 1):
-            t = torch.full((15,), at, device=dev)
+            t = torch.full((18,), at, device=dev)
             check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
 
 
@@ -283,16 +287,16 @@ def test_gradients(dev, vocab, dtype):
 def test_gradients_of_special_rows(dev, vocab, dtype):
     print(f"[case] token_logprobs gradients of special rows V={vocab} {dtype}", flush=True)
     x = special_rows(dev, vocab, dtype)
-    t = torch.full((15,), vocab - 1, device=dev)
+    t = torch.full((18,), vocab - 1, device=dev)
     t[3], t[4] = vocab, -100
     k = min(5, vocab)
-    g = torch.linspace(-1, 1, 15, device=dev) + 0.01
+    g = torch.linspace(-1, 1, 18, device=dev) + 0.01
     z = x.clone().requires_grad_()
     r = fl.token_logprobs(z, t, top_k=k, entropy=True)
     got, = torch.autograd.grad([r.logprobs, r.entropy], z, [g, g / 3])
     check_grad(x, t, 1.0, 0, g, g / 3, None, got)
     z = x.clone().requires_grad_()  # nothing flows: zeros, also from rows with NaN
-    got, = torch.autograd.grad(fl.token_logprobs(z, t).logprobs, z, torch.zeros(15, device=dev))
+    got, = torch.autograd.grad(fl.token_logprobs(z, t).logprobs, z, torch.zeros(18, device=dev))
     assert float(got.float().abs().max()) == 0.0
 
 
