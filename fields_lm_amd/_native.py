@@ -8,7 +8,6 @@ There is no fallback: if the library is missing, every entry point raises Runtim
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import weakref
@@ -153,7 +152,8 @@ def host():
         from .logprobs import stock_gradient
 
         module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "fl_token_logprobs_workspace_bytes", "fl_token_logprobs", "fl_token_logprobs_backward")), stock_gradient)
+            "fl_token_logprobs_workspace_bytes", "fl_token_logprobs", "fl_token_logprobs_backward",
+            "fl_grad_norm_workspace_bytes", "fl_grad_norm", "fl_adamw_workspace_bytes", "fl_adamw_step")), stock_gradient)
         _host = module
     return _host
 
@@ -194,13 +194,6 @@ def stream_handle(device: torch.device) -> int:
     call costs 2 us, a tenth of an eager scan call's host time."""
     return torch._C._cuda_getCurrentRawStream(device.index if device.index is not None
                                               else torch.cuda.current_device())
-
-
-def on(device: torch.device):
-    """``device`` as the current one for a launch; nothing where it is that already."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
 
 
 # Workspace header (the C ABI, include/fields_amd.h): bytes 128..131 the error word, 384..387 the

@@ -6,23 +6,15 @@
 // alternatives cost 15.7 us a call from Python, forward and gradient of a few rows 110 (an operator of PyTorch's own
 // and its gradient: 46).
 //
-// Lists of tensors: what the optimizer's calls read of them, in one pass and without a Python object per attribute.
-// A step reads some twenty attributes of each of a model's hundreds of tensors: through Python's accessors that is
-// 1.2 us a tensor.
-//
-// read(tensors, device_index, dtypes, addresses, counts, codes, expected, block) -> None, or (index, what is wrong)
-//   tensors: a list or tuple; dtypes: the torch dtypes taken, in the order of their codes; addresses, counts (int64)
-//   and codes (int32): host addresses of arrays that hold len(tensors) words, 0 for not wanted; expected: the same of
-//   the counts that the tensors must have, in blocks of `block` values (rounded up).
-// same_shapes(a, b) -> the index of the first pair that differs, or -1.
-// repeats(addresses, counts, n) -> whether two of the n addresses with a count that is not 0 are equal (counts 0: any).
+// grad_norm, adamw_step: their lists of tensors are read in one pass and without a Python object per attribute. A step
+// reads some twenty attributes of each of a model's hundreds of tensors: through Python's accessors that is 1.2 us a
+// tensor.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
-#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -43,9 +35,13 @@ using torch::autograd::variable_list;
 decltype(&fl_token_logprobs_workspace_bytes) workspace_bytes = nullptr;
 decltype(&fl_token_logprobs) logprobs_call = nullptr;
 decltype(&fl_token_logprobs_backward) logprobs_backward_call = nullptr;
+decltype(&fl_grad_norm_workspace_bytes) norm_bytes = nullptr;
+decltype(&fl_grad_norm) norm_call = nullptr;
+decltype(&fl_adamw_workspace_bytes) adamw_bytes = nullptr;
+decltype(&fl_adamw_step) adamw_call = nullptr;
 PyObject* stock_gradient = nullptr;
 
-constexpr int64_t kMaxTop = 64, kMaxVocab = (int64_t)1 << 23;
+constexpr int64_t kMaxTop = 64, kMaxVocab = (int64_t)1 << 23, kStateBlock = 256;
 constexpr double kMinTemperature = 0x1p-20, kMaxTemperature = 0x1p20;
 
 void check(int code, const char* what) {
@@ -311,109 +307,190 @@ PyObject* where(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the library's three entry points, the stock gradient)
+// bind(addresses of the library's entry points, the stock gradient)
 PyObject* bind(PyObject*, PyObject* args) {
-  unsigned long long a, b, c;
+  unsigned long long a[7];
   PyObject* stock;
-  if (!PyArg_ParseTuple(args, "KKKO", &a, &b, &c, &stock)) return nullptr;
-  workspace_bytes = reinterpret_cast<decltype(workspace_bytes)>(a);
-  logprobs_call = reinterpret_cast<decltype(logprobs_call)>(b);
-  logprobs_backward_call = reinterpret_cast<decltype(logprobs_backward_call)>(c);
+  if (!PyArg_ParseTuple(args, "KKKKKKKO", a, a + 1, a + 2, a + 3, a + 4, a + 5, a + 6, &stock)) return nullptr;
+  workspace_bytes = reinterpret_cast<decltype(workspace_bytes)>(a[0]);
+  logprobs_call = reinterpret_cast<decltype(logprobs_call)>(a[1]);
+  logprobs_backward_call = reinterpret_cast<decltype(logprobs_backward_call)>(a[2]);
+  norm_bytes = reinterpret_cast<decltype(norm_bytes)>(a[3]);
+  norm_call = reinterpret_cast<decltype(norm_call)>(a[4]);
+  adamw_bytes = reinterpret_cast<decltype(adamw_bytes)>(a[5]);
+  adamw_call = reinterpret_cast<decltype(adamw_call)>(a[6]);
   Py_INCREF(stock);
   Py_XDECREF(stock_gradient);
   stock_gradient = stock;
   Py_RETURN_NONE;
 }
 
-// Items of a list or tuple, borrowed.
-struct Items {
-  PyObject** at = nullptr;
-  Py_ssize_t n = 0;
-  bool of(PyObject* o) {
-    if (!PyList_Check(o) && !PyTuple_Check(o)) {
-      PyErr_SetString(PyExc_TypeError, "a list or tuple is wanted");
-      return false;
+// A Python list or tuple of tensors: contiguous, of one of `types` (their places are the type codes), on `device`, with
+// the counts of values that are expected. Gradients of other strides are copied.
+struct TensorList {
+  std::vector<void*> addresses;
+  std::vector<int64_t> counts;
+  std::vector<int> codes;
+  std::vector<Tensor> kept;  // copies that have to live until the launch
+  std::vector<at::IntArrayRef> shapes;
+
+  TensorList(PyObject* list, const char* what, at::Device device, std::initializer_list<at::ScalarType> types,
+             const std::vector<int64_t>* expected = nullptr, int64_t block = 1, bool copy = false) {
+    TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), what, " must be a list or tuple of tensors");
+    PyObject** items = PySequence_Fast_ITEMS(list);
+    const size_t n = (size_t)PySequence_Fast_GET_SIZE(list);
+    addresses.reserve(n);
+    counts.reserve(n);
+    codes.reserve(n);
+    shapes.reserve(n);
+    for (size_t i = 0; i < n; ++i) {
+      TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ": number ", i, " is no tensor");
+      const Tensor& t = THPVariable_Unpack(items[i]);
+      const auto at = std::find(types.begin(), types.end(), t.scalar_type());
+      TORCH_CHECK_TYPE(at != types.end(), what, " must be ", *types.begin(), types.size() > 1 ? " or another type of the list" : "",
+                       ", number ", i, " is ", t.scalar_type());
+      TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, " must be dense, number ", i, " is ", t.layout());
+      TORCH_CHECK_VALUE(t.device() == device, what, " must be on ", device, ", number ", i, " is on ", t.device());
+      const int64_t count = t.numel();
+      TORCH_CHECK_VALUE(!expected || count == ((*expected)[i] + block - 1) / block, what, ": number ", i, " has ", count,
+                        " values, ", ((*expected)[i] + block - 1) / block, " are wanted");
+      const bool plain = t.is_contiguous() && !t.is_neg();
+      TORCH_CHECK_VALUE(plain || copy, what, " must be contiguous, number ", i, " is not");
+      if (!plain) kept.push_back(t.detach().resolve_neg().contiguous());
+      addresses.push_back((plain ? t : kept.back()).data_ptr());
+      counts.push_back(count);
+      codes.push_back((int)(at - types.begin()));
+      shapes.push_back(t.sizes());
     }
-    at = PySequence_Fast_ITEMS(o);
-    n = PySequence_Fast_GET_SIZE(o);
-    return true;
   }
+  size_t size() const { return addresses.size(); }
 };
 
-PyObject* wrong(Py_ssize_t i, const char* what) { return Py_BuildValue("(ns)", i, what); }
+// whether an address of something with values occurs twice
+bool repeats(const std::vector<void*>& addresses, const std::vector<int64_t>& counts) {
+  std::vector<void*> at;
+  for (size_t i = 0; i < addresses.size(); ++i)
+    if (counts[i]) at.push_back(addresses[i]);
+  std::sort(at.begin(), at.end());
+  return std::adjacent_find(at.begin(), at.end()) != at.end();
+}
 
-PyObject* read(PyObject*, PyObject* args) {
-  PyObject *list, *types;
-  long long device, addresses, counts, codes, expected, block;
-  Items items, taken;
-  if (!PyArg_ParseTuple(args, "OLOLLLLL", &list, &device, &types, &addresses, &counts, &codes, &expected,
-                        &block) || !items.of(list) ||
-      !taken.of(types))
+// the first tensor of a list or tuple, whose device the others are to be on
+const Tensor& first_of(PyObject* list, const char* what) {
+  TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), what, " must be a list or tuple of tensors");
+  TORCH_CHECK_VALUE(PySequence_Fast_GET_SIZE(list) > 0, "no ", what);
+  PyObject* first = PySequence_Fast_ITEMS(list)[0];
+  TORCH_CHECK_TYPE(THPVariable_Check(first), what, ": number 0 is no tensor");
+  return THPVariable_Unpack(first);
+}
+
+// one fp32 value on the device, or none
+float* device_value(PyObject* o, const char* what, at::Device device) {
+  if (o == Py_None) return nullptr;
+  TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
+  const Tensor& t = THPVariable_Unpack(o);
+  TORCH_CHECK_VALUE(t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == device, what,
+                    " must be one float32 value on ", device);
+  return static_cast<float*>(t.data_ptr());
+}
+
+Tensor workspace_on(at::Device device, size_t bytes) {
+  return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(device));
+}
+
+// grad_norm(gradients, max_norm or a negative number for none) -> (norm, scale or None)
+PyObject* grad_norm(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject* list;
+  double max_norm;
+  if (!PyArg_ParseTuple(args, "Od", &list, &max_norm)) return nullptr;
+  const at::Device device = first_of(list, "gradients").device();
+  TORCH_CHECK(device.is_cuda(), "grad_norm requires a ROCm (cuda) device");
+  const TensorList grads(list, "gradients", device, {at::kFloat, at::kBFloat16}, nullptr, 1, true);
+  const c10::DeviceGuard guard(device);
+  const int64_t n = (int64_t)grads.size();
+  const bool scaled = !(max_norm < 0.0);
+  const Tensor out = at::empty({2}, at::TensorOptions().dtype(at::kFloat).device(device));
+  const size_t bytes = norm_bytes(n, grads.counts.data());
+  const Tensor ws = workspace_on(device, bytes);
+  check(norm_call(n, grads.addresses.data(), grads.codes.data(), grads.counts.data(), scaled ? (float)max_norm : 0.f,
+                  scaled, address<float>(out), address<void>(ws), bytes, stream_of(out)),
+        "fl_grad_norm");
+  PyObject *norm = THPVariable_Wrap(out.select(0, 0)), *scale = scaled ? THPVariable_Wrap(out.select(0, 1)) : Py_NewRef(Py_None);
+  return Py_BuildValue("(NN)", norm, scale);
+  END_HANDLE_TH_ERRORS
+}
+
+// adamw_step(parameters, gradients, first moments, second moments, steps (a list or one tensor), lr (a number or a
+// tensor), beta1, beta2, eps, weight decay, gradient scale or None, the moments' scales or None twice)
+PyObject* adamw_step(PyObject*, PyObject* args) {
+  HANDLE_TH_ERRORS
+  PyObject *params, *grads, *avgs, *sqs, *steps, *lr, *grad_scale, *avg_scales, *sq_scales;
+  double beta1, beta2, eps, decay;
+  if (!PyArg_ParseTuple(args, "OOOOOOddddOOO", &params, &grads, &avgs, &sqs, &steps, &lr, &beta1, &beta2, &eps, &decay,
+                        &grad_scale, &avg_scales, &sq_scales))
     return nullptr;
-  at::ScalarType wanted[8];
-  if (block < 1) return PyErr_Format(PyExc_ValueError, "a block has 1 value or more");
-  if (taken.n > 8) return PyErr_Format(PyExc_ValueError, "at most 8 types");
-  for (Py_ssize_t k = 0; k < taken.n; ++k) {
-    if (!THPDtype_Check(taken.at[k])) return PyErr_Format(PyExc_TypeError, "a dtype is wanted");
-    wanted[k] = reinterpret_cast<THPDtype*>(taken.at[k])->scalar_type;
+  const Tensor& first = first_of(params, "parameters");
+  const at::Device device = first.device();
+  const at::ScalarType type = first.scalar_type();
+  TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16, "parameters must be float32 or bfloat16, got ", type);
+  const bool eight = avg_scales != Py_None;
+  const auto as_long = [&](PyObject* o) {
+    return (!PyList_Check(o) && !PyTuple_Check(o)) || PySequence_Fast_GET_SIZE(o) == PySequence_Fast_GET_SIZE(params);
+  };
+  TORCH_CHECK_VALUE(as_long(grads) && as_long(avgs) && as_long(sqs) && as_long(steps) && as_long(avg_scales) && as_long(sq_scales),
+                    "one gradient, one state of each kind and one step per parameter");
+  TORCH_CHECK_VALUE(eight == (sq_scales != Py_None), "8-bit states need the scales of both moments");
+  TORCH_CHECK(device.is_cuda(), "adamw_step requires a ROCm (cuda) device");
+  const TensorList p(params, "parameters", device, {type});
+  const int64_t n = (int64_t)p.size();
+  const TensorList g(grads, "gradients", device, {type}, &p.counts, 1, true);
+  for (int64_t i = 0; i < n; ++i)
+    TORCH_CHECK_VALUE(p.shapes[i] == g.shapes[i], "gradient ", i, " has the shape ", g.shapes[i], ", its parameter ", p.shapes[i]);
+  const at::ScalarType state = eight ? at::kFloat8_e4m3fn : at::kFloat;
+  const TensorList m(avgs, "states", device, {state}, &p.counts), v(sqs, "states", device, {state}, &p.counts);
+  std::vector<void*> ms, vs;
+  if (eight) {
+    ms = TensorList(avg_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock).addresses;
+    vs = TensorList(sq_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock).addresses;
   }
-  try {
-    for (Py_ssize_t i = 0; i < items.n; ++i) {
-      if (!THPVariable_Check(items.at[i])) return wrong(i, "tensor");
-      const Tensor& t = THPVariable_Unpack(items.at[i]);
-      Py_ssize_t code = 0;
-      while (code < taken.n && wanted[code] != t.scalar_type()) ++code;
-      if (code == taken.n) return wrong(i, "dtype");
-      if (t.layout() != at::kStrided || t.is_neg()) return wrong(i, "layout");
-      if (!t.device().is_cuda() || t.device().index() != device) return wrong(i, "device");
-      if (!t.is_contiguous()) return wrong(i, "contiguous");
-      if (expected && t.numel() != (reinterpret_cast<const int64_t*>(expected)[i] + block - 1) / block) return wrong(i, "count");
-      if (addresses) reinterpret_cast<int64_t*>(addresses)[i] = reinterpret_cast<int64_t>(t.data_ptr());
-      if (counts) reinterpret_cast<int64_t*>(counts)[i] = t.numel();
-      if (codes) reinterpret_cast<int32_t*>(codes)[i] = (int32_t)code;
-    }
-  } catch (const std::exception& e) {  // a tensor without memory of its own (a wrapper of some transform)
-    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
+  const std::vector<int64_t> ones(n, 1);
+  std::vector<void*> step_at;
+  if (THPVariable_Check(steps)) {
+    const Tensor& t = THPVariable_Unpack(steps);
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == device && t.dim() == 1 && t.numel() == n && t.is_contiguous(),
+                      "steps must be ", n, " int64 values on ", device);
+    for (int64_t i = 0; i < n; ++i) step_at.push_back(static_cast<int64_t*>(t.data_ptr()) + i);
+  } else {
+    step_at = TensorList(steps, "steps", device, {at::kLong}, &ones).addresses;
+  }
+  TORCH_CHECK_VALUE(!repeats(p.addresses, p.counts) && !repeats(step_at, ones), "a parameter or a step counter occurs twice");
+  float* scale = device_value(grad_scale, "grad_scale", device);
+  float* lr_at = THPVariable_Check(lr) ? device_value(lr, "lr", device) : nullptr;
+  const double lr_value = lr_at ? 0.0 : PyFloat_AsDouble(lr);
+  if (PyErr_Occurred()) return nullptr;
+  const c10::DeviceGuard guard(device);
+  const size_t bytes = adamw_bytes(n);
+  const Tensor ws = workspace_on(device, bytes);
+  check(adamw_call(n, p.addresses.data(), g.addresses.data(), type == at::kBFloat16 ? FL_DTYPE_BF16 : FL_DTYPE_F32,
+                   m.addresses.data(), v.addresses.data(), eight ? reinterpret_cast<float* const*>(ms.data()) : nullptr,
+                   eight ? reinterpret_cast<float* const*>(vs.data()) : nullptr, p.counts.data(),
+                   reinterpret_cast<int64_t* const*>(step_at.data()), lr_value, lr_at, beta1, beta2, eps, decay, scale,
+                   address<void>(ws), bytes, stream_of(first)),
+        "fl_adamw_step");
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(params); ++i) {  // written in place: saved parameters are stale
+    const Tensor& t = THPVariable_Unpack(PySequence_Fast_ITEMS(params)[i]);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   }
   Py_RETURN_NONE;
-}
-
-PyObject* same_shapes(PyObject*, PyObject* args) {
-  PyObject *first, *second;
-  Items a, b;
-  if (!PyArg_ParseTuple(args, "OO", &first, &second) || !a.of(first) || !b.of(second)) return nullptr;
-  try {
-    for (Py_ssize_t i = 0; i < a.n; ++i) {
-      if (i >= b.n || !THPVariable_Check(a.at[i]) || !THPVariable_Check(b.at[i]) ||
-          THPVariable_Unpack(a.at[i]).sizes() != THPVariable_Unpack(b.at[i]).sizes())
-        return PyLong_FromSsize_t(i);
-    }
-  } catch (const std::exception& e) {
-    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
-  }
-  return PyLong_FromSsize_t(a.n == b.n ? -1 : a.n);
-}
-
-PyObject* repeats(PyObject*, PyObject* args) {
-  long long addresses, counts, n;
-  if (!PyArg_ParseTuple(args, "LLL", &addresses, &counts, &n)) return nullptr;
-  try {
-    std::vector<int64_t> at;
-    for (long long i = 0; i < n; ++i)
-      if (!counts || reinterpret_cast<const int64_t*>(counts)[i]) at.push_back(reinterpret_cast<const int64_t*>(addresses)[i]);
-    std::sort(at.begin(), at.end());
-    return PyBool_FromLong(std::adjacent_find(at.begin(), at.end()) != at.end());
-  } catch (const std::exception& e) {
-    return PyErr_Format(PyExc_RuntimeError, "%s", e.what());
-  }
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "the library's entry points and the stock gradient"},
                          {"token_logprobs", token_logprobs, METH_VARARGS, "the call"},
                          {"where", where, METH_VARARGS, "the rows of logits and tokens"},
-                         {"read", read, METH_VARARGS, "addresses, counts and types of a list of tensors"},
-                         {"same_shapes", same_shapes, METH_VARARGS, "first pair of unequal shapes"},
-                         {"repeats", repeats, METH_VARARGS, "whether an address occurs twice"},
+                         {"grad_norm", grad_norm, METH_VARARGS, "the call"},
+                         {"adamw_step", adamw_step, METH_VARARGS, "the call"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

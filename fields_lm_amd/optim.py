@@ -1,4 +1,5 @@
-"""What follows a training step's backward, on the HIP path only (``csrc/optimizer.hip``):
+"""What follows a training step's backward, on the HIP path only (``csrc/optimizer.hip``, host side
+``csrc/host.cpp``):
 
 * :func:`grad_norm`   the 2-norm over many gradients and the scale that clips it, in one pass over them;
 * :func:`adamw_step`  one AdamW step over many tensors, moments in fp32 or in 8 bits;
@@ -9,7 +10,6 @@ in a HIP graph and replayed.
 """
 from __future__ import annotations
 
-import array
 import math
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
@@ -20,46 +20,11 @@ from . import _native as nat
 STATE_BLOCK = 256                   # values that share a scale in the 8-bit states
 STATE8_DTYPE = torch.float8_e4m3fn  # their codes
 
-_TYPES = (torch.float32, torch.bfloat16)  # in the order of their codes
+_TYPES = (torch.float32, torch.bfloat16)
 
 
-class _Words:
-    """Host arrays of ``n`` 64-bit words each, for the library's calls: ``at(i)`` is where the i-th starts."""
-
-    def __init__(self, n: int, arrays: int) -> None:
-        self.n, self.words = n, array.array("q", bytes(8 * n * arrays))
-        self.start = self.words.buffer_info()[0]
-
-    def at(self, i: int) -> int:
-        return self.start + 8 * self.n * i
-
-
-def _read(tensors, what: str, device: torch.device, dtypes, addresses: int, *, counts: int = 0, codes: int = 0,
-          expected: int = 0, block: int = 1):
-    """Addresses (and counts, type codes) of contiguous tensors of ``dtypes`` on ``device`` with the expected counts of
-    values. Gradients of other strides are copied; returns the tensors that were read."""
-    call = nat.host().read
-    if not isinstance(tensors, (list, tuple)):
-        tensors = list(tensors)
-    bad = call(tensors, device.index, dtypes, addresses, counts, codes, expected, block)
-    if bad is not None and bad[1] == "contiguous" and what == "gradients":
-        tensors = [t if t.is_contiguous() else t.detach().contiguous() for t in tensors]
-        bad = call(tensors, device.index, dtypes, addresses, counts, codes, expected, block)
-    if bad is None:
-        return tensors
-    i, why = bad
-    t = tensors[i]
-    if why == "tensor":
-        raise TypeError(f"{what}: number {i} is no tensor")
-    if why == "dtype":
-        raise TypeError(f"{what} must be {' or '.join(map(str, dtypes))}, number {i} is {t.dtype}")
-    if why == "layout":
-        raise TypeError(f"{what} must be dense, number {i} is {t.layout}")
-    if why == "device":
-        raise ValueError(f"{what} must be on {device}, number {i} is on {t.device}")
-    if why == "count":
-        raise ValueError(f"{what}: number {i} has {t.numel()} values, not as many as it should")
-    raise ValueError(f"{what} must be contiguous, number {i} is not")
+def _listed(tensors):
+    return tensors if isinstance(tensors, (list, tuple)) else list(tensors)
 
 
 def grad_norm(grads: Iterable[torch.Tensor], max_norm: Optional[float] = None
@@ -71,32 +36,10 @@ def grad_norm(grads: Iterable[torch.Tensor], max_norm: Optional[float] = None
     :func:`adamw_step` takes as ``grad_scale``; the gradients are not rewritten. The scale of a norm that is
     not finite is NaN, on which :func:`adamw_step` leaves everything as it was. Neither is differentiable.
     """
-    grads = list(grads)
-    if not grads:
-        raise ValueError("no gradients")
-    device = grads[0].device
-    if device.type != "cuda":
-        raise RuntimeError("grad_norm requires a ROCm (cuda) device")
     if max_norm is not None and not float(max_norm) >= 0.0:
         raise ValueError(f"max_norm must be 0 or more, got {max_norm}")
-    n = len(grads)
-    words = _Words(n, 3)  # addresses, counts, type codes (half their words)
-    grads = _read(grads, "gradients", device, _TYPES, words.at(0), counts=words.at(1), codes=words.at(2))
-    lib = nat.load()
-    out = torch.empty(2, device=device, dtype=torch.float32)
-    ws = torch.empty(int(lib.fl_grad_norm_workspace_bytes(n, words.at(1))), device=device, dtype=torch.uint8)
-    with nat.on(device):
-        nat.check(lib.fl_grad_norm(
-            n, words.at(0), words.at(2), words.at(1), 0.0 if max_norm is None else float(max_norm),
-            max_norm is not None, nat.ptr(out), nat.ptr(ws), ws.numel(), nat.stream_handle(device)), "fl_grad_norm")
-    norm, scale = out.unbind()
+    norm, scale = nat.host().grad_norm(_listed(grads), -1.0 if max_norm is None else float(max_norm))
     return norm if max_norm is None else (norm, scale)
-
-
-def _device_scalar(t: torch.Tensor, what: str, device: torch.device) -> int:
-    if t.numel() != 1 or t.dtype != torch.float32 or t.device != device:
-        raise ValueError(f"{what} must be one float32 value on {device}")
-    return t.data_ptr()
 
 
 def _check_hyper(lr, betas, eps, weight_decay) -> None:
@@ -134,56 +77,12 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     grad_scale: one fp32 value on the device (:func:`grad_norm`'s second), or None for 1. Where it is not finite the
     call leaves parameters, states and step counters as they were.
     """
-    n = len(params)
-    if n == 0:
-        raise ValueError("no parameters")
-    eight = exp_avg_scales is not None
-    if eight != (exp_avg_sq_scales is not None):
-        raise ValueError("8-bit states need the scales of both moments")
-    if not (len(grads) == len(exp_avgs) == len(exp_avg_sqs) == n
-            and (not eight or len(exp_avg_scales) == len(exp_avg_sq_scales) == n)):
-        raise ValueError("one gradient and one state of each kind per parameter")
     _check_hyper(lr, betas, eps, weight_decay)
-    device, dtype = params[0].device, params[0].dtype
-    if device.type != "cuda":
-        raise RuntimeError("adamw_step requires a ROCm (cuda) device")
-    if dtype not in _TYPES:
-        raise TypeError(f"parameters must be float32 or bfloat16, got {dtype}")
-    words = _Words(n, 8)  # counts; addresses of parameters, gradients, the moments, their scales, the steps
-    counts, at = words.at(0), [words.at(i) for i in range(1, 8)]
-    _read(params, "parameters", device, (dtype,), at[0], counts=counts)
-    read_grads = _read(grads, "gradients", device, (dtype,), at[1], expected=counts)
-    i = nat.host().same_shapes(params if isinstance(params, (list, tuple)) else list(params), read_grads)
-    if i >= 0:
-        raise ValueError(f"gradient {i} has the shape {tuple(grads[i].shape)}, its parameter {tuple(params[i].shape)}")
-    state_types = (STATE8_DTYPE if eight else torch.float32,)
-    _read(exp_avgs, "states", device, state_types, at[2], expected=counts)
-    _read(exp_avg_sqs, "states", device, state_types, at[3], expected=counts)
-    if eight:
-        for k, scales in ((4, exp_avg_scales), (5, exp_avg_sq_scales)):
-            _read(scales, "scales", device, (torch.float32,), at[k], expected=counts, block=STATE_BLOCK)
-    if isinstance(steps, torch.Tensor):
-        if steps.dtype != torch.int64 or steps.device != device or steps.shape != (n,) or not steps.is_contiguous():
-            raise ValueError(f"steps must be {n} int64 values on {device}")
-        first = steps.data_ptr()
-        words.words[7 * n:] = array.array("q", range(first, first + 8 * n, 8))
-    else:
-        if len(steps) != n:
-            raise ValueError(f"steps must be {n} int64 values on {device}")
-        ones = array.array("q", (1,)) * n
-        _read(steps, "steps", device, (torch.int64,), at[6], expected=ones.buffer_info()[0])
-    if nat.host().repeats(at[0], counts, n) or nat.host().repeats(at[6], 0, n):
-        raise ValueError("a parameter or a step counter occurs twice")
-    scale = None if grad_scale is None else _device_scalar(grad_scale, "grad_scale", device)
-    lr_ptr, lr_value = (_device_scalar(lr, "lr", device), 0.0) if isinstance(lr, torch.Tensor) else (None, float(lr))
-    lib = nat.load()
-    ws = torch.empty(int(lib.fl_adamw_workspace_bytes(n)), device=device, dtype=torch.uint8)
-    with nat.on(device):
-        nat.check(lib.fl_adamw_step(
-            n, at[0], at[1], nat.dtype_code(dtype), at[2], at[3], at[4] if eight else None, at[5] if eight else None,
-            counts, at[6], lr_value, lr_ptr, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), scale,
-            nat.ptr(ws), ws.numel(), nat.stream_handle(device)), "fl_adamw_step")
-    torch.autograd.graph.increment_version(params)
+    nat.host().adamw_step(
+        _listed(params), _listed(grads), _listed(exp_avgs), _listed(exp_avg_sqs),
+        steps if isinstance(steps, torch.Tensor) else _listed(steps), lr, betas[0], betas[1], eps, weight_decay, grad_scale,
+        None if exp_avg_scales is None else _listed(exp_avg_scales),
+        None if exp_avg_sq_scales is None else _listed(exp_avg_sq_scales))
 
 
 class AdamW(torch.optim.Optimizer):

@@ -147,34 +147,6 @@ def test_c_abi_token_logprobs_refusals():
 
 
 # ------------------------------------------------------------------ grad_norm, adamw_step
-def test_lists_of_tensors_are_read_or_refused_by_number():
-    lists = nat.host()
-    n = 3
-    ts = [torch.zeros(4), torch.zeros(0), torch.zeros(2, 3)]
-    words = (ctypes.c_int64 * n)()
-    at = ctypes.addressof(words)
-
-    def read(tensors, dtypes=(torch.float32, torch.bfloat16), device=0, expected=0, block=1):
-        return lists.read(tensors, device, dtypes, at, 0, 0, expected, block)
-
-    assert read(ts) == (0, "device")  # (what is read is on a device; there is none here)
-    assert read([ts[0].double()]) == (0, "dtype") == read(ts, (torch.int64,)) and read([3]) == (0, "tensor")
-    assert read([ts[0].to_sparse()]) == (0, "layout") and read([]) is None
-    imag = torch.imag(torch.zeros(3, dtype=torch.complex64).conj())
-    assert imag.is_neg() and read([imag]) == (0, "layout")  # its memory holds the values' negatives
-    for bad in ((7,), (ts, (3,)), (ts, (torch.float32,) * 9), (ts, (torch.float32,), 0, 0, 0)):
-        with pytest.raises((TypeError, ValueError)):
-            read(*bad)
-    assert lists.same_shapes(ts, ts) == -1 and lists.same_shapes(ts, ts[:2]) == 2 == lists.same_shapes(ts[:2], ts)
-    assert lists.same_shapes(ts, [ts[0], ts[1], ts[2].t()]) == 2
-    with pytest.raises(TypeError):
-        lists.same_shapes(ts, 3)
-    a = (ctypes.c_int64 * 4)(256, 512, 256, 0)
-    c = (ctypes.c_int64 * 4)(1, 1, 0, 0)
-    assert lists.repeats(ctypes.addressof(a), 0, 4) and not lists.repeats(ctypes.addressof(a), ctypes.addressof(c), 4)
-    assert not lists.repeats(ctypes.addressof(a), 0, 2)
-
-
 def _array(*addresses):
     return (ctypes.c_void_p * len(addresses))(*addresses)
 
