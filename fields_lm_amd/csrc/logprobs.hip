@@ -145,7 +145,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
   __shared__ unsigned long long s_cand[kCand];
   __shared__ int s_n, s_count[WAVES];
   const int K = TOP ? out.K : 0;
-  const int lo = (int)blockIdx.y * seg_len, len = V - lo < seg_len ? V - lo : seg_len, packs = len / N;
+  const int lo = (int)blockIdx.y * seg_len, len = V - lo < seg_len ? V - lo : seg_len;
   const bool whole = gridDim.y == 1;
   const float c = inv_t * kLog2e;
   for (int64_t row = blockIdx.x; row < n_rows; row += gridDim.x) {
@@ -164,28 +164,33 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     }
     const T* row_x = logits + logit_at;
     const T* x = row_x + lo;
+    // packs from the first 16-byte border on (8,192 rows of 16,383 bf16 logits: 58 us from the row's start)
+    const int ahead = (int)(-(uintptr_t)x % 16 / sizeof(T)), head = ahead < len ? ahead : len;
+    const int packs = (len - head) / N, tail = head + packs * N;
     float xt = 0.f;
     if (whole && tid == 0 && t >= 0 && t < V) xt = load_as<T>(row_x + t);
     u32x4 v[NV];
     const auto load = [&](auto get) {
       if (packs == NV * THREADS) {  // all of the tile: nothing to stand in for
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = get(reinterpret_cast<const u32x4_any*>(x + (i * THREADS + tid) * N));
+        for (int i = 0; i < NV; ++i) v[i] = get(reinterpret_cast<const u32x4*>(x + head + (i * THREADS + tid) * N));
         return;
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int j = i * THREADS + tid;
         v[i] = u32x4{Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
-        if (j < packs) v[i] = get(reinterpret_cast<const u32x4_any*>(x + j * N));
+        if (j < packs) v[i] = get(reinterpret_cast<const u32x4*>(x + head + j * N));
       }
     };
     // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 42 us, and 48 through
     // them; where one follows the pair takes 139 us so, and 132 through them).
-    if (out.stats) load([](const u32x4_any* p) { return *p; });
-    else load([](const u32x4_any* p) { return __builtin_nontemporal_load(p); });
-    float rest = -INFINITY;  // the logits behind the last pack, one to a thread
-    if (tid < len - packs * N) rest = load_as<T>(x + packs * N + tid);
+    if (out.stats) load([](const u32x4* p) { return *p; });
+    else load([](const u32x4* p) { return __builtin_nontemporal_load(p); });
+    // the logits ahead of the first pack and behind the last, one to a thread (fewer than 8 each), len for none
+    const auto rest_place = [&](int t) { return t < head ? t : t >= 8 && t - 8 < len - tail ? tail + t - 8 : len; };
+    float rest = -INFINITY;
+    if (rest_place(tid) < len) rest = load_as<T>(x + rest_place(tid));
     // f(logit, i, q) of all the thread's logits, and of -inf for those it lacks
     const auto each = [&](auto f) {
 #pragma unroll
@@ -204,11 +209,11 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     const auto for_places = [&](auto f) {
       for (int j = tid; __ballot(j < packs); j += THREADS) {
         u32x4 again = {Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
-        if (j < packs) again = *reinterpret_cast<const u32x4_any*>(x + j * N);
+        if (j < packs) again = *reinterpret_cast<const u32x4*>(x + head + j * N);
 #pragma unroll
-        for (int q = 0; q < N; ++q) f(Pack<T>::get(again, q), j < packs ? j * N + q : len);
+        for (int q = 0; q < N; ++q) f(Pack<T>::get(again, q), j < packs ? head + j * N + q : len);
       }
-      f(rest, tid < len - packs * N ? packs * N + tid : len);
+      f(rest, rest_place(tid));
     };
     if (TOP && tid == 0) s_n = 0;
     float mine = rest, pack_top[TOP ? NV : 1];
@@ -308,9 +313,9 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
 #pragma unroll
           for (int i = 0; i < NV; ++i) hit |= in_pack(i) ? 1u << i : 0u;
           while (hit) {
-            const int at = (__builtin_ctz(hit) * THREADS + tid) * N;
+            const int at = head + (__builtin_ctz(hit) * THREADS + tid) * N;
             hit &= hit - 1;
-            const u32x4 again = *reinterpret_cast<const u32x4_any*>(x + at);
+            const u32x4 again = *reinterpret_cast<const u32x4*>(x + at);
 #pragma unroll
             for (int q = 0; q < N; ++q) {
               const float a = Pack<T>::get(again, q);
@@ -321,12 +326,15 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         if (bound > 0x007fu) {
           const float least = __uint_as_float(bound & 0x8000u ? bound << 16 ^ 0x80000000u : ~(bound << 16));
           scan([&](int i) { return pack_top[i] >= least; }, [&](float a, int) { return a >= least; });
-          if (rest >= least) push(rest, packs * N + tid);
+          if (rest >= least) push(rest, rest_place(tid));
         } else {
           // fewer than K groups hold a logit above -inf: all of those, and the masked ones of lowest index
-          scan([&](int i) { return i * THREADS + tid < packs && (pack_top[i] > -INFINITY || (i * THREADS + tid) * N < 2 * K); },
+          scan([&](int i) {
+                 const int j = i * THREADS + tid;
+                 return j < packs && (pack_top[i] > -INFINITY || head + j * N < 2 * K);
+               },
                [&](float a, int at) { return a > -INFINITY || at < 2 * K; });
-          const int at = packs * N + tid;
+          const int at = rest_place(tid);
           if (at < len && (rest > -INFINITY || at < 2 * K)) push(rest, at);
         }
         __syncthreads();
@@ -487,14 +495,14 @@ __device__ __forceinline__ void store_pack<bf16_bits>(bf16_bits* p, const float*
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = bf16_pair(v[2 * i], v[2 * i + 1]);
-  __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
 }
 template <>
 __device__ __forceinline__ void store_pack<float>(float* p, const float* v) {
   u32x4 w;
 #pragma unroll
   for (int i = 0; i < 4; ++i) w[i] = __float_as_uint(v[i]);
-  __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
+  __builtin_nontemporal_store(w, reinterpret_cast<u32x4*>(p));
 }
 
 template <typename T, int THREADS, bool ENT>
@@ -505,14 +513,19 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
     const float* __restrict__ g_top, T* __restrict__ grad) {
   constexpr int N = Pack<T>::N, kChunk = THREADS * kBackPacks * N;
   const int tid = threadIdx.x, lane = tid & 63;
-  const int lo = (int)blockIdx.y * kChunk, len = V - lo < kChunk ? V - lo : kChunk, packs = len / N;
   const float c = inv_t * kLog2e;
   for (int64_t at_row = blockIdx.x; at_row < n_rows; at_row += gridDim.x) {
     const int64_t row = n_rows - 1 - at_row;  // the forward's last rows first: they may still be cached
     int64_t logit_at, token_at;
     rows.find(row, logit_at, token_at);
-    const T* x = logits + logit_at + lo;
-    T* out = grad + row * V + lo;
+    const T* x = logits + logit_at;
+    T* out = grad + row * V;
+    // Chunks from the gradient row's first 128-byte line on, so that no line is written in parts (8,192 rows of 16,383
+    // bf16: 120 us from the row's start); the logits ahead of it are the first chunk's too.
+    const int ahead = (int)(-(uintptr_t)out % 128 / sizeof(T)), first = ahead + (int)blockIdx.y * kChunk;
+    const int lo = blockIdx.y ? first : 0, hi = V - first < kChunk ? V : first + kChunk;
+    const int packs = hi > first ? (hi - first) / N : 0, tail = first + packs * N;
+    if (lo >= hi) continue;  // (block-uniform)
     const int64_t t = tokens[token_at];
     const float m = stats[2 * row], ls2 = stats[2 * row + 1] * kLog2e;
     const float h = ENT ? g_ent[row] : 0.f, ent = ENT ? entropy[row] : 0.f;
@@ -524,8 +537,9 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
       const float zero[N] = {};
 #pragma unroll
       for (int i = 0; i < kBackPacks; ++i)
-        if (i * THREADS + tid < packs) store_pack<T>(out + (i * THREADS + tid) * N, zero);
-      if (tid < len - packs * N) store_as(out + packs * N + tid, 0.f);
+        if (i * THREADS + tid < packs) store_pack<T>(out + first + (i * THREADS + tid) * N, zero);
+      if (lo + tid < first && lo + tid < hi) store_as(out + lo + tid, 0.f);
+      if (tail + tid < hi) store_as(out + tail + tid, 0.f);
       continue;
     }
     if (g != 0.f && (t < 0 || t >= V)) a = quiet_nan();
@@ -542,34 +556,35 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_backward_kernel(
       return ENT ? p * fmaf(c1, fmaxf(d, -1000.f), c0) : p * c0;
     };
     const int64_t at = lane < K ? top_tok[row * K + lane] : -1;
-    const bool mine = at >= lo && at < lo + len;
-    const float x_own = mine ? load_as<T>(x + (at - lo)) : 0.f, x_t = t >= lo && t < lo + len ? load_as<T>(x + (t - lo)) : 0.f;
+    const bool mine = at >= lo && at < hi;
+    const float x_own = mine ? load_as<T>(x + at) : 0.f, x_t = t >= lo && t < hi ? load_as<T>(x + t) : 0.f;
     u32x4 v[kBackPacks];
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i)
-      if (i * THREADS + tid < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + (i * THREADS + tid) * N);
+      if (i * THREADS + tid < packs) v[i] = *reinterpret_cast<const u32x4_any*>(x + first + (i * THREADS + tid) * N);
 #pragma unroll
     for (int i = 0; i < kBackPacks; ++i) {
       if (i * THREADS + tid < packs) {
         float o[N];
 #pragma unroll
         for (int q = 0; q < N; ++q) o[q] = part(power(Pack<T>::get(v[i], q)));
-        store_pack<T>(out + (i * THREADS + tid) * N, o);
+        store_pack<T>(out + first + (i * THREADS + tid) * N, o);
       }
     }
-    if (tid < len - packs * N) store_as(out + packs * N + tid, part(power(load_as<T>(x + packs * N + tid))));
+    if (lo + tid < first && lo + tid < hi) store_as(out + lo + tid, part(power(load_as<T>(x + lo + tid))));
+    if (tail + tid < hi) store_as(out + tail + tid, part(power(load_as<T>(x + tail + tid))));
     // The logits with a gradient of their own, each put over by the thread that has just written it.
-    const auto owner_of = [&](int k) { return k < packs * N ? k / N % THREADS : k - packs * N; };
+    const auto owner_of = [&](int k) { return k < first ? k - lo : k < tail ? (k - first) / N % THREADS : k - tail; };
     const float value = fmaf(at == t ? g_own + g : g_own, inv_t, part(power(x_own)));
-    const int k_own = (int)(at - lo), owner = owner_of(k_own);
+    const int k_own = (int)at, owner = owner_of(k_own);
     for (uint64_t left = __ballot(mine && owner >> 6 == tid >> 6); left; left &= left - 1) {
       const int i = __builtin_ctzll(left);
       const int k = __builtin_amdgcn_readlane(k_own, i);
       if (tid == __builtin_amdgcn_readlane(owner, i))
         store_as(out + k, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(value), i)));
     }
-    if (t >= lo && t < lo + len && __ballot(at == t) == 0 && tid == owner_of((int)(t - lo)))
-      store_as(out + (t - lo), fmaf(g, inv_t, part(power(x_t))));  // (else it is among the alternatives)
+    if (t >= lo && t < hi && __ballot(at == t) == 0 && tid == owner_of((int)t))
+      store_as(out + t, fmaf(g, inv_t, part(power(x_t))));  // (else it is among the alternatives)
   }
 }
 
@@ -645,7 +660,8 @@ int fl_token_logprobs(const void* logits, int dtype, int64_t outer, int64_t inne
                       float* top_logprobs, int64_t* top_tokens, float* stats, void* workspace, size_t workspace_bytes,
                       void* stream) {
   if (!dtype_ok(dtype)) return FL_ERR_DTYPE;
-  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
+  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) ||
+      !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
       top_k < 0 || top_k > kMaxTop || top_k > V)
     return FL_ERR_INVALID_ARGUMENT;
   if (!logits || !aligned(logits, esize(dtype)) || !tokens || !aligned(tokens, 8) || !logprobs || !aligned(logprobs, 4) ||
@@ -673,7 +689,8 @@ int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int
                                const float* g_logprobs, const float* g_entropy, const float* g_top, void* g_logits,
                                void* stream) {
   if (!dtype_ok(dtype)) return FL_ERR_DTYPE;
-  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) || !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
+  if (!shape_ok(outer, inner, V, stride_outer, stride_inner) ||
+      !(temperature >= kMinTemperature && temperature <= kMaxTemperature) ||
       top_k < 0 || top_k > kMaxTop || top_k > V)
     return FL_ERR_INVALID_ARGUMENT;
   if (!logits || !aligned(logits, esize(dtype)) || !tokens || !aligned(tokens, 8) || !stats || !aligned(stats, 4) ||
