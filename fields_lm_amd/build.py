@@ -104,8 +104,8 @@ def build_host(verbose: bool = False) -> Path:
     cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(arg for path in include_paths() for arg in ("-isystem", path)), f"-I{sysconfig.get_paths()['include']}",
-           "-isystem", str(rocm / "include"), f"-I{INCLUDE_DIR}", str(HOST_SOURCE), f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10",
-           "-lc10_hip",
+           "-isystem", str(rocm / "include"), f"-I{INCLUDE_DIR}", str(HOST_SOURCE),
+           f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
            "-o", str(tmp)]
     if verbose:
         print(" ".join(cmd), flush=True)

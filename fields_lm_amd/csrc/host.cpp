@@ -15,12 +15,17 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <algorithm>
+#include <memory>
 #include <optional>
+#include <unordered_set>
+#include <utility>
 #include <vector>
 
 #include "fields_amd.h"
@@ -203,6 +208,27 @@ Tensor stock_backward(const Tensor& logits, const Tensor& tokens, const Tensor& 
   return out;
 }
 
+// A captured backward adds into the logits' leaves on the streams that their eager graphs, where one still lives,
+// were made on. The default stream cannot join a capture, which ends in an error that the engine does not survive.
+void check_leaves(const Tensor& logits) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  std::vector<std::shared_ptr<torch::autograd::Node>> todo = {
+      logits.grad_fn() ? logits.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(logits)};
+  std::unordered_set<torch::autograd::Node*> seen;
+  while (!todo.empty()) {
+    const std::shared_ptr<torch::autograd::Node> node = todo.back();
+    todo.pop_back();
+    if (!node || !seen.insert(node.get()).second) continue;
+    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
+      const std::optional<c10::Stream> stream = node->stream();
+      TORCH_CHECK(!stream || stream->id() != 0,
+                  "the logits' leaves hold an autograd graph made on the default stream: drop it (its outputs) before "
+                  "a backward pass is captured");
+    }
+    for (const auto& edge : node->next_edges()) todo.push_back(edge.function);
+  }
+}
+
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   // the outputs that are wanted, in the order log probabilities, entropy, alternatives' log probabilities and tokens
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
@@ -233,6 +259,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     if (o.top_k) g[2] = grads[o.entropy ? 2 : 1];
     variable_list out(6);
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
+    check_leaves(logits);
     out[0] = at::GradMode::is_enabled() ? stock_backward(logits, tokens, top_tokens, o, g)
                                         : ::backward(logits, tokens, stats, entropy, top_tokens, o, g);
     return out;
@@ -247,7 +274,8 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
   Options o;
   long long top_k, ignore_index;
   int entropy;
-  if (!PyArg_ParseTuple(args, "OOdLpL", &first, &second, &o.temperature, &top_k, &entropy, &ignore_index)) return nullptr;
+  if (!PyArg_ParseTuple(args, "OOdLpL", &first, &second, &o.temperature, &top_k, &entropy, &ignore_index))
+    return nullptr;
   o.top_k = top_k;
   o.entropy = entropy;
   o.ignore_index = ignore_index;
@@ -256,7 +284,8 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
   TORCH_CHECK_TYPE(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16,
                    "logits must be float32 or bfloat16, got ", logits.scalar_type());
   TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong, "tokens must be int64, got ", tokens.scalar_type());
-  TORCH_CHECK_TYPE(logits.layout() == at::kStrided && tokens.layout() == at::kStrided, "logits and tokens must be dense");
+  TORCH_CHECK_TYPE(logits.layout() == at::kStrided && tokens.layout() == at::kStrided,
+                   "logits and tokens must be dense");
   TORCH_CHECK_VALUE(logits.dim() >= 1 && tokens.sizes() == logits.sizes().slice(0, logits.dim() - 1), "tokens ",
                     tokens.sizes(), " must be the logits' rows ", logits.sizes());
   const int64_t vocab = logits.size(-1), most = std::min(kMaxTop, vocab);
@@ -294,7 +323,8 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// where(logits, tokens) -> (logits, tokens, outer, inner, the logits' strides, the tokens'): the rows as a call sees them
+// where(logits, tokens) -> (logits, tokens, outer, inner, the logits' strides, the tokens'): the rows as a call sees
+// them
 PyObject* where(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
   PyObject *first, *second;
@@ -347,12 +377,14 @@ struct TensorList {
       TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ": number ", i, " is no tensor");
       const Tensor& t = THPVariable_Unpack(items[i]);
       const auto at = std::find(types.begin(), types.end(), t.scalar_type());
-      TORCH_CHECK_TYPE(at != types.end(), what, " must be ", *types.begin(), types.size() > 1 ? " or another type of the list" : "",
+      TORCH_CHECK_TYPE(at != types.end(), what, " must be ", *types.begin(),
+                       types.size() > 1 ? " or another type of the list" : "",
                        ", number ", i, " is ", t.scalar_type());
       TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, " must be dense, number ", i, " is ", t.layout());
       TORCH_CHECK_VALUE(t.device() == device, what, " must be on ", device, ", number ", i, " is on ", t.device());
       const int64_t count = t.numel();
-      TORCH_CHECK_VALUE(!expected || count == ((*expected)[i] + block - 1) / block, what, ": number ", i, " has ", count,
+      TORCH_CHECK_VALUE(!expected || count == ((*expected)[i] + block - 1) / block, what, ": number ", i, " has ",
+                        count,
                         " values, ", ((*expected)[i] + block - 1) / block, " are wanted");
       const bool plain = t.is_contiguous() && !t.is_neg();
       TORCH_CHECK_VALUE(plain || copy, what, " must be contiguous, number ", i, " is not");
@@ -366,13 +398,21 @@ struct TensorList {
   size_t size() const { return addresses.size(); }
 };
 
-// whether an address of something with values occurs twice
-bool repeats(const std::vector<void*>& addresses, const std::vector<int64_t>& counts) {
-  std::vector<void*> at;
-  for (size_t i = 0; i < addresses.size(); ++i)
-    if (counts[i]) at.push_back(addresses[i]);
-  std::sort(at.begin(), at.end());
-  return std::adjacent_find(at.begin(), at.end()) != at.end();
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;  // of addresses, [first, last + 1)
+
+void add_ranges(Ranges& to, const TensorList& list, size_t size) {
+  for (size_t i = 0; i < list.size(); ++i) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(list.addresses[i]);
+    if (list.counts[i]) to.emplace_back(at, at + list.counts[i] * size);
+  }
+}
+
+// whether two ranges share an address, after sorting
+bool overlap(Ranges& ranges) {
+  std::sort(ranges.begin(), ranges.end());
+  for (size_t i = 1; i < ranges.size(); ++i)
+    if (ranges[i].first < ranges[i - 1].second) return true;
+  return false;
 }
 
 // the first tensor of a list or tuple, whose device the others are to be on
@@ -416,7 +456,8 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   check(norm_call(n, grads.addresses.data(), grads.codes.data(), grads.counts.data(), scaled ? (float)max_norm : 0.f,
                   scaled, address<float>(out), address<void>(ws), bytes, stream_of(out)),
         "fl_grad_norm");
-  PyObject *norm = THPVariable_Wrap(out.select(0, 0)), *scale = scaled ? THPVariable_Wrap(out.select(0, 1)) : Py_NewRef(Py_None);
+  PyObject* norm = THPVariable_Wrap(out.select(0, 0));
+  PyObject* scale = scaled ? THPVariable_Wrap(out.select(0, 1)) : Py_NewRef(Py_None);
   return Py_BuildValue("(NN)", norm, scale);
   END_HANDLE_TH_ERRORS
 }
@@ -438,7 +479,8 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   const auto as_long = [&](PyObject* o) {
     return (!PyList_Check(o) && !PyTuple_Check(o)) || PySequence_Fast_GET_SIZE(o) == PySequence_Fast_GET_SIZE(params);
   };
-  TORCH_CHECK_VALUE(as_long(grads) && as_long(avgs) && as_long(sqs) && as_long(steps) && as_long(avg_scales) && as_long(sq_scales),
+  TORCH_CHECK_VALUE(as_long(grads) && as_long(avgs) && as_long(sqs) && as_long(steps) && as_long(avg_scales) &&
+                        as_long(sq_scales),
                     "one gradient, one state of each kind and one step per parameter");
   TORCH_CHECK_VALUE(eight == (sq_scales != Py_None), "8-bit states need the scales of both moments");
   TORCH_CHECK(device.is_cuda(), "adamw_step requires a ROCm (cuda) device");
@@ -446,25 +488,47 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   const int64_t n = (int64_t)p.size();
   const TensorList g(grads, "gradients", device, {type}, &p.counts, 1, true);
   for (int64_t i = 0; i < n; ++i)
-    TORCH_CHECK_VALUE(p.shapes[i] == g.shapes[i], "gradient ", i, " has the shape ", g.shapes[i], ", its parameter ", p.shapes[i]);
+    TORCH_CHECK_VALUE(p.shapes[i] == g.shapes[i], "gradient ", i, " has the shape ", g.shapes[i], ", its parameter ",
+                      p.shapes[i]);
   const at::ScalarType state = eight ? at::kFloat8_e4m3fn : at::kFloat;
   const TensorList m(avgs, "states", device, {state}, &p.counts), v(sqs, "states", device, {state}, &p.counts);
+  Ranges written;
+  written.reserve(5 * n + n);
+  add_ranges(written, p, type == at::kFloat ? 4 : 2);
+  add_ranges(written, m, eight ? 1 : 4);
+  add_ranges(written, v, eight ? 1 : 4);
   std::vector<void*> ms, vs;
   if (eight) {
-    ms = TensorList(avg_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock).addresses;
-    vs = TensorList(sq_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock).addresses;
+    const TensorList m_scales(avg_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock);
+    const TensorList v_scales(sq_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock);
+    add_ranges(written, m_scales, 4);
+    add_ranges(written, v_scales, 4);
+    ms = m_scales.addresses;
+    vs = v_scales.addresses;
   }
-  const std::vector<int64_t> ones(n, 1);
   std::vector<void*> step_at;
   if (THPVariable_Check(steps)) {
     const Tensor& t = THPVariable_Unpack(steps);
-    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == device && t.dim() == 1 && t.numel() == n && t.is_contiguous(),
+    TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == device && t.dim() == 1 && t.numel() == n &&
+                          t.is_contiguous(),
                       "steps must be ", n, " int64 values on ", device);
     for (int64_t i = 0; i < n; ++i) step_at.push_back(static_cast<int64_t*>(t.data_ptr()) + i);
+    written.emplace_back(reinterpret_cast<uintptr_t>(step_at[0]), reinterpret_cast<uintptr_t>(step_at[0]) + n * 8);
   } else {
-    step_at = TensorList(steps, "steps", device, {at::kLong}, &ones).addresses;
+    const std::vector<int64_t> ones(n, 1);
+    const TensorList list(steps, "steps", device, {at::kLong}, &ones);
+    add_ranges(written, list, 8);
+    step_at = list.addresses;
   }
-  TORCH_CHECK_VALUE(!repeats(p.addresses, p.counts) && !repeats(step_at, ones), "a parameter or a step counter occurs twice");
+  TORCH_CHECK_VALUE(!overlap(written), "parameters, states or step counters share memory");
+  for (int64_t i = 0; i < n; ++i) {  // a gradient is read beside what others write
+    if (!p.counts[i]) continue;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(g.addresses[i]);
+    const auto next = std::upper_bound(written.begin(), written.end(), std::make_pair(at, UINTPTR_MAX));
+    TORCH_CHECK_VALUE((next == written.end() || next->first >= at + p.counts[i] * (type == at::kFloat ? 4 : 2)) &&
+                          (next == written.begin() || std::prev(next)->second <= at),
+                      "gradient ", i, " shares memory with a parameter, a state or a step counter");
+  }
   float* scale = device_value(grad_scale, "grad_scale", device);
   float* lr_at = THPVariable_Check(lr) ? device_value(lr, "lr", device) : nullptr;
   const double lr_value = lr_at ? 0.0 : PyFloat_AsDouble(lr);

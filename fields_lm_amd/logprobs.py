@@ -55,9 +55,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     """Log probabilities of ``tokens`` under softmax(logits / temperature), in one pass over the logits.
 
     logits [..., V] (V up to 2^23) fp32 or bf16 on a ROCm device, rows any distance apart (a slice of positions is
-    read in place); tokens [...] int64 on the same device. temperature: 2^-20 to 2^20. ``entropy`` adds each row's entropy, ``top_k`` (up to 64) its largest
-    logits' log probabilities and tokens: largest first, of equal ones the lowest index first, NaN above all.
-    Everything is computed and returned in fp32.
+    read in place); tokens [...] int64 on the same device. temperature: 2^-20 to 2^20. ``entropy`` adds each row's
+    entropy, ``top_k`` (up to 64) its largest logits' log probabilities and tokens: largest first, of equal ones the
+    lowest index first, NaN above all. Everything is computed and returned in fp32.
 
     A token equal to ``ignore_index`` has log probability 0 and passes no gradient; one outside the vocabulary has
     NaN, and so has its gradient. -inf masks a logit; a row of -inf alone has log probabilities -inf, entropy 0 and
@@ -65,5 +65,6 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     without their logits being read.
 
     Gradients flow to ``logits`` from the log probabilities, the entropy and the alternatives' log probabilities.
+    Under graph capture the backward pass is refused while a graph of the default stream holds the logits' leaves.
     """
     return TokenLogprobs(*nat.host().token_logprobs(logits, tokens, temperature, top_k, entropy, ignore_index))

@@ -80,8 +80,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     _check_hyper(lr, betas, eps, weight_decay)
     nat.host().adamw_step(
         _listed(params), _listed(grads), _listed(exp_avgs), _listed(exp_avg_sqs),
-        steps if isinstance(steps, torch.Tensor) else _listed(steps), lr, betas[0], betas[1], eps, weight_decay, grad_scale,
-        None if exp_avg_scales is None else _listed(exp_avg_scales),
+        steps if isinstance(steps, torch.Tensor) else _listed(steps), lr, betas[0], betas[1], eps, weight_decay,
+        grad_scale, None if exp_avg_scales is None else _listed(exp_avg_scales),
         None if exp_avg_sq_scales is None else _listed(exp_avg_sq_scales))
 
 

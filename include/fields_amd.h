@@ -468,15 +468,16 @@ int fl_mix(const void* y, const void* g, const void* mix_logit, int mix_dtype, i
 
 /*
  * Log probabilities of given tokens with entropy and top alternatives, and their gradient (no counterpart in
- * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V (at most 2^23) logits of dtype at
- * logits + (r / inner) * stride_outer + (r % inner) * stride_inner (elements), its token tokens[(r / inner) *
+ * the reference, whose loss takes the stock log-softmax). Row r of rows = outer * inner is V (at most 2^23) logits
+ * of dtype at logits + (r / inner) * stride_outer + (r % inner) * stride_inner (elements), its token tokens[(r / inner) *
  * token_outer + (r % inner) * token_inner]. With m = max x, d_v = (x_v - m) / temperature, s = sum e^{d_v}:
  *   logprobs [rows] = d_token - ln s; 0 where the token is ignore_index, NaN where it is outside 0 .. V - 1;
  *   entropy [rows] or NULL = ln s - (sum e^{d_v} d_v) / s;
  *   top_tokens / top_logprobs [rows, top_k]: the top_k (0 .. 64) largest logits, largest first, of equal ones the
  *     lowest index first, NaN above all;
  *   stats [rows, 2] or NULL: m and ln s, for the backward.
- * temperature: 2^-20 to 2^20. A row of -inf alone: log probabilities -inf, entropy 0, gradient 0. A row with NaN or +inf: NaN.
+ * temperature: 2^-20 to 2^20. A row of -inf alone: log probabilities -inf, entropy 0, gradient 0. A row with NaN
+ * or +inf: NaN.
  * workspace: fl_token_logprobs_workspace_bytes(rows, V, dtype, top_k) bytes, 16-byte aligned, no initial contents
  * needed (0 bytes: NULL will do).
  *
@@ -514,14 +515,14 @@ int fl_token_logprobs_backward(const void* logits, int dtype, int64_t outer, int
  *   Workspace 16-byte aligned, no initial contents needed.
  */
 size_t fl_grad_norm_workspace_bytes(int64_t n, const int64_t* numel);
-int fl_grad_norm(int64_t n, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm, int scaled,
-                 float* out, void* workspace, size_t workspace_bytes, void* stream);
+int fl_grad_norm(int64_t n, const void* const* grads, const int* dtypes, const int64_t* numel, float max_norm,
+                 int scaled, float* out, void* workspace, size_t workspace_bytes, void* stream);
 size_t fl_adamw_workspace_bytes(int64_t n);
 int fl_adamw_step(int64_t n, void* const* params, const void* const* grads, int dtype, void* const* exp_avgs,
                   void* const* exp_avg_sqs, float* const* exp_avg_scales, float* const* exp_avg_sq_scales,
-                  const int64_t* numel, int64_t* const* steps, double lr, const float* lr_ptr, double beta1, double beta2,
-                  double eps, double weight_decay, const float* grad_scale, void* workspace, size_t workspace_bytes,
-                  void* stream);
+                  const int64_t* numel, int64_t* const* steps, double lr, const float* lr_ptr, double beta1,
+                  double beta2, double eps, double weight_decay, const float* grad_scale, void* workspace,
+                  size_t workspace_bytes, void* stream);
 
 /* Library version string (host function). No counterpart in the reference. */
 const char* fl_version(void);

@@ -443,6 +443,43 @@ def test_two_streams_and_graph_replays(dev):
             assert all(torch.equal(a, b) for a, b in zip(got, (*(o.detach() for o in r), grad))), turn
 
 
+@pytest.mark.parametrize("leaf", [True, False])
+def test_captured_backward_refuses_leaves_of_a_living_eager_graph(dev, leaf):
+    """A graph of the default stream that holds the leaves: the captured backward raises; without it, it replays."""
+    print(f"[case] captured backward, a living eager graph, leaf {leaf}", flush=True)
+    x, t = make(dev, 8, 301, torch.float32, 5)
+    z = x.clone().requires_grad_()
+    up = torch.ones(8, device=dev)
+
+    def loss():
+        return fl.token_logprobs(z if leaf else z * 2.0, t, top_k=3).logprobs
+
+    living = loss()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        r = loss()
+        with pytest.raises(RuntimeError, match="default stream"):
+            r.backward(up)
+        del r
+    del living
+    torch.cuda.synchronize()
+    assert z.grad is None
+    z.grad = torch.zeros_like(z)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        z.grad.zero_()
+        loss().backward(up)
+    for turn in range(3):
+        with torch.no_grad():
+            z.add_(0.25 * turn).copy_(z.flip(-1))
+        g.replay()
+        torch.cuda.synchronize()
+        got = z.grad.clone()
+        exp, = torch.autograd.grad(loss(), z, up)
+        assert torch.equal(got, exp), turn
+
+
 def test_score_of_the_model_is_its_logits_log_softmax(dev):
     print("[case] FieldsForCausalLM.score", flush=True)
     from fields_lm_amd import model as M

@@ -147,8 +147,9 @@ def test_adamw_neighbours_stay_as_they_were(dev):
             st = [torch.full((total,), 0.5, device=dev).to(STATE8_DTYPE if eight else torch.float32) for _ in range(2)]
             sc = [torch.full((16,), 0.25, device=dev) for _ in range(2)]
             cut = slice(5, 5 + n)
-            fl.adamw_step([buf[0][cut]], [buf[1][cut]], [st[0][cut]], [st[1][cut]], torch.zeros(1, dtype=torch.long, device=dev),
-                          **HYPER, **(dict(exp_avg_scales=[sc[0][3:7]], exp_avg_sq_scales=[sc[1][3:7]]) if eight else {}))
+            step = torch.zeros(1, dtype=torch.long, device=dev)
+            fl.adamw_step([buf[0][cut]], [buf[1][cut]], [st[0][cut]], [st[1][cut]], step, **HYPER,
+                          **(dict(exp_avg_scales=[sc[0][3:7]], exp_avg_sq_scales=[sc[1][3:7]]) if eight else {}))
             for t, old in [(buf[0], 3.0)] + [(s.float(), 0.5) for s in st]:
                 outside = torch.cat((t[:5], t[5 + n:]))
                 # inside, all change but a bf16 weight: m' / (1 - 0.9) = 7.5 over sqrt(v' / (1 - 0.98)) = 5.8 (v = 0.5) or
@@ -168,7 +169,10 @@ def test_one_tensor_past_2_to_31_values(dev, eight):
     p[at], g[at] = torch.tensor([1.0, -2.0, 3.0, -4.0, 5.0], device=dev).bfloat16(), torch.tensor([2.0, 1.0, -1.0, 3.0, -2.0],
                                                                                                  device=dev).bfloat16()
     assert abs(float(fl.grad_norm([g])) - math.sqrt(19.0)) <= 2 * U * math.sqrt(19.0)
-    new = (lambda: torch.zeros(n, device=dev, dtype=torch.uint8).view(STATE8_DTYPE)) if eight else lambda: torch.zeros(n, device=dev)
+    def new():
+        return torch.zeros(n, device=dev, dtype=torch.uint8 if eight else torch.float32).view(
+            STATE8_DTYPE if eight else torch.float32)
+
     m, v = new(), new()
     scales = [[torch.zeros(-(-n // 256), device=dev)] for _ in range(2)] if eight else [None, None]
     old = p[at].clone()
@@ -241,7 +245,8 @@ def test_adamw_refuses_on_the_device(dev):
         with pytest.raises(TypeError):
             fl.adamw_step(*bad)
     for bad in (([p], [one(n=5)], [one()], [one()], step), ([p], [one()], [one(n=5)], [one()], step),
-                ([p], [torch.zeros(4)], [one()], [one()], step), ([p], [one()], [one()], [one()], step.int()), ([p], [one()], [one()], [one()], [step.expand(2)]),
+                ([p], [torch.zeros(4)], [one()], [one()], step), ([p], [one()], [one()], [one()], step.int()),
+                ([p], [one()], [one()], [one()], [step.expand(2)]),
                 ([p], [one()], [one()], [one()], [step[0], step[0]]), ([p], [one()], [one()], [one()], step.cpu()),
                 ([one(n=8)[::2]], [one()], [one()], [one()], step), ([p], [one()], [one(n=8)[::2]], [one()], step),
                 ([p, p], [one(), one()], [one(), one()], [one(), one()], torch.zeros(2, dtype=torch.long, device=dev)),
@@ -259,6 +264,21 @@ def test_adamw_refuses_on_the_device(dev):
     with pytest.raises(ValueError):
         fl.adamw_step([p], [one()], [one(STATE8_DTYPE)], [one(STATE8_DTYPE)], step, exp_avg_scales=[one(n=2)],
                       exp_avg_sq_scales=[one(n=1)])
+    shared, m, sc = one(n=12), one(), one(n=1)
+    codes = one(STATE8_DTYPE)
+    for bad in (([shared[:8], shared[4:]], [one(n=8), one(n=8)], [one(n=8), one(n=8)], [one(n=8), one(n=8)],
+                 torch.zeros(2, dtype=torch.long, device=dev)),   # two parameters overlap
+                ([p], [one()], [m], [m], step),                   # both moments are one
+                ([p], [one()], [p], [m], step),                   # a moment is the parameter
+                ([shared[:4]], [shared[2:6]], [m], [one()], step),  # a gradient lies in a parameter
+                ([p], [m], [m], [one()], step)):
+        with pytest.raises(ValueError):
+            fl.adamw_step(*bad)
+    with pytest.raises(ValueError):
+        fl.adamw_step([p], [one()], [codes], [one(STATE8_DTYPE)], step, exp_avg_scales=[sc], exp_avg_sq_scales=[sc])
+    grad = one()  # one gradient of two parameters is read twice
+    fl.adamw_step([one(), one()], [grad, grad], [one(), one()], [one(), one()],
+                  torch.zeros(2, dtype=torch.long, device=dev))
     assert float(p.abs().sum()) == 0.0 and int(step) == 0
 
 
