@@ -1,9 +1,9 @@
 // optimizer.hip — what follows a training step's backward, over many tensors at once: the 2-norm of all
 // gradients with the scale that clips it, and the AdamW step, its moments in fp32 or in 8 bits.
 //
-// The tensors' addresses travel in the kernel arguments (kTensors to a launch), so that a call copies nothing
-// to the device and can be captured; blocks find their tensor by the running count of blocks. Sums are taken
-// in a fixed order.
+// The tensors' addresses travel in the kernel arguments (kTensors, kNormTensors to a launch), so that a call copies
+// nothing to the device and can be captured; blocks find their tensor by the running count of blocks. Sums are
+// taken in a fixed order.
 //
 // Compiled without contraction: the 8-bit codes next to a border between two go by the bits of the moments,
 // which are those of separate products and sums.
@@ -13,7 +13,8 @@ namespace {
 
 using namespace fl;
 
-constexpr int kTensors = 64;      // tensors of a launch (an 8-bit table of 64 is 3.6 KiB of arguments)
+constexpr int kTensors = 64;      // tensors of a step's launch (an 8-bit table of 64 is 3.6 KiB of arguments)
+constexpr int kNormTensors = 192;  // tensors of the norm's (3.8 KiB)
 constexpr int kStepTensors = 480; // step counters of a launch, one to a thread
 constexpr int kChunk = 4096;      // values of a block
 constexpr int kBlock = 256;       // values that share a scale in the 8-bit states
@@ -23,15 +24,17 @@ constexpr int kMaxBlocks = 1 << 23;  // blocks of a launch
 constexpr float kTopCode = 448.0f, kSmallest = 0.001953125f, kTiny = 1e-30f;
 
 struct NormTable {
-  const void* x[kTensors];
-  int64_t numel[kTensors];
-  int first[kTensors + 1];  // running count of blocks
-  int is_bf16[kTensors];
+  static constexpr int kSize = kNormTensors;
+  const void* x[kSize];
+  int64_t numel[kSize];
+  int first[kSize + 1];  // running count of blocks
+  uint32_t is_bf16[kSize / 32];  // a bit to a tensor
   int n;
 };
 
 template <bool EIGHT>
 struct AdamTable {
+  static constexpr int kSize = kTensors;
   void* p[kTensors];
   const void* g[kTensors];
   void* m[kTensors];
@@ -52,7 +55,11 @@ struct StepTable {
 template <typename Table>
 __device__ __forceinline__ int tensor_of(const Table& t, int block) {
   const int lane = threadIdx.x & 63;
-  return __popcll(__ballot(lane < t.n && t.first[lane + 1] <= block));
+  int ended = 0;
+#pragma unroll
+  for (int i = 0; i < Table::kSize; i += 64)
+    ended += __popcll(__ballot(i + lane < t.n && t.first[i + lane + 1] <= block));
+  return ended;
 }
 
 // What a step touches once it touches past the caches' keeping (0.29 G values: the norm 222 us plain and 196
@@ -121,13 +128,14 @@ __device__ double block_sum(double v, double* s_sum) {
 }
 
 // Reads each gradient once and adds up squares in fp64: those of fp32 values are exact there, and nothing overflows
-// or is lost. The loads bound it: 0.29 G fp32 values take 197 us in a model's 200 tensors (5.9 TB/s).
+// or is lost. The loads bound it: 0.29 G fp32 values in a model's 200 tensors take 178 us with the last
+// sum (6.6 TB/s; a streaming read reaches 7.0), and 195 in launches of 64 tensors.
 __global__ __launch_bounds__(256) void fl_square_sum_kernel(const NormTable t, int chunk, double* __restrict__ part) {
   __shared__ double s_sum[4];
   const int i = uniform(tensor_of(t, (int)blockIdx.x));
   const int64_t lo = (int64_t)((int)blockIdx.x - t.first[i]) * chunk, left = t.numel[i] - lo;
   const int64_t n = left < chunk ? left : chunk;
-  const double v = t.is_bf16[i] ? square_sum(static_cast<const bf16_bits*>(t.x[i]) + lo, n)
+  const double v = t.is_bf16[i >> 5] >> (i & 31) & 1 ? square_sum(static_cast<const bf16_bits*>(t.x[i]) + lo, n)
                                 : square_sum(static_cast<const float*>(t.x[i]) + lo, n);
   const double sum = block_sum(v, s_sum);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -393,7 +401,7 @@ template <typename Table, typename Put>
 int64_t fill_table(Table& table, int64_t n, const int64_t* numel, int64_t i, int chunk, Put put) {
   table.n = 0;
   table.first[0] = 0;
-  for (; i < n && table.n < kTensors; ++i) {
+  for (; i < n && table.n < Table::kSize; ++i) {
     const int64_t blocks = cdiv(numel[i], chunk);
     if (table.first[table.n] + blocks > kMaxBlocks) break;
     put(table.n, i);
@@ -441,13 +449,13 @@ bool list_ok(int64_t n, const int64_t* numel) {
   return true;
 }
 
-// Values of a block of the norm: 4,096 up to 65,536, as many as leave 1,024 blocks (13 M values: 8,192 of them
-// 13.5 us, 4,096 of them 14.9).
+// Values of a block of the norm: 4,096 up to 32,768, as many as leave 1,024 blocks (13 M values: 8,192 of them
+// 13.5 us, 4,096 of them 14.9; 0.29 G: 16,384 of them 180 us, 32,768 178, 65,536 183, 131,072 201).
 int norm_chunk(int64_t n, const int64_t* numel) {
   int64_t total = 0;
   for (int64_t i = 0; i < n; ++i) total += numel[i];
   int chunk = kChunk;
-  while (chunk < 65536 && total / chunk > 2048) chunk *= 2;
+  while (chunk < 32768 && total / chunk > 2048) chunk *= 2;
   return chunk;
 }
 
@@ -489,7 +497,7 @@ int fl_grad_norm(int64_t n, const void* const* grads, const int* dtypes, const i
     NormTable t = {};
     i = fill_table(t, n, numel, i, chunk, [&](int k, int64_t j) {
       t.x[k] = grads[j];
-      t.is_bf16[k] = dtypes[j] == FL_DTYPE_BF16;
+      t.is_bf16[k >> 5] |= (uint32_t)(dtypes[j] == FL_DTYPE_BF16) << (k & 31);
     });
     const int blocks = t.first[t.n];
     if (blocks == 0) continue;

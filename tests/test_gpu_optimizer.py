@@ -54,6 +54,16 @@ def test_grad_norm(dev, sizes, shift, dtype):
     assert torch.equal(fl.grad_norm(grads), norm) and torch.equal(fl.grad_norm(grads, 0.5)[1], scale)
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 191, 192, 193, 500])
+def test_grad_norm_of_many_mixed_tensors(dev, n):
+    """Lists at and past a launch's tensors, types in turn of 1, 2, 3 and empty ones between."""
+    print(f"[case] grad_norm, {n} mixed tensors", flush=True)
+    sizes = [0 if i % 11 == 5 else 1 + 37 * i % 9000 for i in range(n)]
+    g = [t.bfloat16() if i % 6 in (1, 3, 4) else t for i, t in enumerate(tensors(dev, sizes, torch.float32, n))]
+    exp = math.sqrt(sum(float(t.double().square().sum()) for t in g))
+    assert abs(float(fl.grad_norm(g)) - exp) <= 2 * U * exp
+
+
 def test_grad_norm_of_mixed_types_shapes_and_extremes(dev):
     print("[case] grad_norm, mixed types", flush=True)
     g = tensors(dev, [300, 64], torch.float32, 1) + tensors(dev, [129], torch.bfloat16, 2)
