@@ -124,7 +124,8 @@ def test_forward_of_the_longest_row(dev):
         fl.token_logprobs(torch.empty(1, (1 << 23) + 1, device=dev), t[:1])
 
 
-@pytest.mark.parametrize("rows,vocab", [(1, 16384), (64, 16384), (300, 16384), (700, 501), (5000, 33), (257, 12345), (40, 70000)])
+@pytest.mark.parametrize("rows,vocab", [(1, 16384), (64, 16384), (300, 16384), (700, 501), (5000, 33), (257, 12345),
+                                        (40, 70000)])
 def test_forward_over_rows(dev, rows, vocab):
     print(f"[case] token_logprobs rows={rows} V={vocab}", flush=True)
     x, t = make(dev, rows, vocab, torch.bfloat16, rows)
@@ -184,6 +185,26 @@ def test_forward_of_special_rows(dev, vocab, dtype):
         for at in (0, vocab - 1):
             t = torch.full((18,), at, device=dev)
             check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
+
+
+@pytest.mark.parametrize("k", [1, 3, 20, 64])
+@pytest.mark.parametrize("vocab", [16388, 131072, 64 * 8192, 64 * 8192 + 1])
+def test_alternatives_of_long_rows(dev, vocab, k):
+    """Rows of several segments (fp32 segments of 8,192), up to 64 and one more: the largest logits in one of them, one in
+    each, equal in all, masked but in the last, fewer left than are wanted."""
+    print(f"[case] alternatives of long rows V={vocab} k={k}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(vocab + k)
+    x = torch.randn(8, vocab, device=dev, generator=g) * 3
+    x[1, 8192:8292] += 50
+    x[2, 17::8192] += 50
+    x[3] = 1.0
+    x[4, :-70] = float("-inf")
+    x[5] = float("-inf")
+    x[5, ::vocab // 2] = 2.0
+    x[6, -1] = float("nan")
+    x[7] = x[7].round()  # many equal ones
+    t = torch.randint(0, vocab, (8,), device=dev, generator=g)
+    check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
 
 
 def test_tokens_outside_the_vocabulary_and_ignored_ones(dev):
