@@ -418,10 +418,10 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
 }
 
 // Joins a row's segments, one thread to a segment: their sums relative to the row's maximum, and their sorted lists of
-// alternatives. SMALL, up to 64 segments: the K-th largest of the lists' first ceil(K / segments) keys is a key that K
+// alternatives. SMALL, up to 64 segments: the K-th largest of the lists' first K / segments + 1 keys is a key that K
 // reach; those that do, little more than K, are ranked by counting. Where they are more than fit, and for up to 1,024
-// segments, K times the largest of the lists' heads is taken (a row of 131,072 fp32 and 20 alternatives, both launches:
-// 13.6 us by heads alone).
+// segments, K times the largest of the lists' heads is taken. (A row of 131,072 fp32, both launches: with 20
+// alternatives 12.4 us, with 64 17.3; by heads alone 14.2 and 27.8.)
 template <typename T, int THREADS, bool SMALL>
 __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     const T* __restrict__ logits, Rows rows, int64_t n_rows, int V, int segments, float inv_t, Outputs out,
@@ -440,6 +440,15 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     if (tid == 0 && t >= 0 && t < V) xt = load_as<T>(logits + logit_at + t);
     f32x4 p = {-INFINITY, -INFINITY, 0.f, 0.f};
     if (tid < segments && !(t == out.ignore && K == 0 && !out.entropy)) p = part[row * segments + tid];
+    const uint64_t* keys = part_keys + row * segments * K;
+    if constexpr (SMALL) {
+#pragma unroll 2
+      for (int i = tid; i < segments * K; i += THREADS) s_keys[i] = keys[i];
+      if (tid == 0) {
+        s_n = 0;
+        s_bound = 1;  // (no list's filling of 0)
+      }
+    }
     RowStats st;
     st.inv_t = inv_t;
     st.m = wave_max(p[0]);
@@ -464,7 +473,6 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
     st.settle(sum);
     st.mean = ent / sum;
     if (tid == 0) write_row(out, row, st, t, V, xt);
-    const uint64_t* keys = part_keys + row * segments * K;
     const auto put = [&](int k, uint64_t key) {
       out.top_tok[row * K + k] = 0xffffffffu - (uint32_t)key;
       out.top_lp[row * K + k] = st.logprob(key_value(key));
@@ -474,13 +482,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
         __syncthreads();
         continue;
       }
-      for (int i = tid; i < segments * K; i += THREADS) s_keys[i] = keys[i];
-      if (tid == 0) {
-        s_n = 0;
-        s_bound = 1;  // (no list's filling of 0)
-      }
-      __syncthreads();
-      const int each = (K + segments - 1) / segments, some = segments * each;  // some < K + 64
+      const int each = K / segments + 1, some = segments * each;  // K < some <= K + 64, each <= K
       if (tid < some) {
         const uint64_t key = s_keys[tid / each * K + tid % each];
         int rank = 0;
