@@ -259,56 +259,67 @@ __global__ __launch_bounds__(256) void fl_adamw_kernel(const AdamTable<false> t,
   }
 }
 
-// four values of a block of 256, 16 or 8 bytes
-template <typename T>
-struct Four;
-template <>
-struct Four<float> {
-  typedef u32x4 Reg;
-  __device__ __forceinline__ static Reg load(const float* p) {
-    return load_once(reinterpret_cast<const u32x4_any*>(p));
-  }
-  __device__ __forceinline__ static void store(float* p, const float* v) {
-    store_once(reinterpret_cast<u32x4_any*>(p), pack_values<float>(v));
-  }
-  __device__ __forceinline__ static float get(const Reg& r, int q) { return __uint_as_float(r[q]); }
-  __device__ __forceinline__ static void set(Reg& r, int q, float v) { r[q] = __float_as_uint(v); }
-};
-template <>
-struct Four<bf16_bits> {
-  typedef u32x2 Reg;
-  __device__ __forceinline__ static Reg load(const bf16_bits* p) {
-    return load_once(reinterpret_cast<const u32x2_any*>(p));
-  }
-  __device__ __forceinline__ static void store(bf16_bits* p, const float* v) {
-    store_once(reinterpret_cast<u32x2_any*>(p), u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])});
-  }
-  __device__ __forceinline__ static float get(const Reg& r, int q) {
-    return q & 1 ? bf16_hi(r[q >> 1]) : bf16_lo(r[q >> 1]);
-  }
-  __device__ __forceinline__ static void set(Reg& r, int q, float v) {
-    const uint32_t b = bf16_bits_of(v);
-    r[q >> 1] = q & 1 ? (r[q >> 1] & 0xffffu) | b << 16 : (r[q >> 1] & 0xffff0000u) | b;
-  }
-};
-
-template <int Q>
-__device__ __forceinline__ float code_value(uint32_t codes) { return __builtin_amdgcn_cvt_f32_fp8((int)codes, Q); }
+__device__ __forceinline__ float code_value(uint32_t codes, int q) {  // (q a constant once unrolled)
+  return q == 0   ? __builtin_amdgcn_cvt_f32_fp8((int)codes, 0)
+         : q == 1 ? __builtin_amdgcn_cvt_f32_fp8((int)codes, 1)
+         : q == 2 ? __builtin_amdgcn_cvt_f32_fp8((int)codes, 2)
+                  : __builtin_amdgcn_cvt_f32_fp8((int)codes, 3);
+}
 
 __device__ __forceinline__ uint32_t four_codes(const float* y) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], lo, true);
 }
 
-// One wave to a block of 256 values, four of them to a lane, four blocks a wave with all their loads ahead of the
-// maths. m is held as the e4m3 code of m (448 / max|m|), v as that of its root r (448 / max r), with max / 448
-// beside: a root keeps v's range in half the octaves, and one that is not 0 keeps at least the smallest code,
-// since a v that rounds to 0 under an m that does not would let the next step with a small gradient run away.
-// Bound by the memory, 16 bytes an fp32 value: 0.29 G values take 785 us (6.0 TB/s).
+// value q of a pack, to be written
+__device__ __forceinline__ void set_value(u32x4& r, int q, float v) { r[q] = __float_as_uint(v); }
+__device__ __forceinline__ void set_value(u32x4& r, int q, bf16_bits v) {
+  r[q >> 1] = q & 1 ? (r[q >> 1] & 0xffffu) | (uint32_t)v << 16 : (r[q >> 1] & 0xffff0000u) | v;
+}
+
+// N codes, of 4 or 8 bytes
+template <int N>
+struct Codes;
+template <>
+struct Codes<4> {
+  uint32_t w[1] = {0};
+  __device__ __forceinline__ void load(const uint8_t* p) { w[0] = load_once(reinterpret_cast<const u32_any*>(p)); }
+  __device__ __forceinline__ void store(uint8_t* p) const { store_once(reinterpret_cast<u32_any*>(p), w[0]); }
+};
+template <>
+struct Codes<8> {
+  uint32_t w[2] = {0, 0};
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    const u32x2 v = load_once(reinterpret_cast<const u32x2_any*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
+  }
+  __device__ __forceinline__ void store(uint8_t* p) const {
+    store_once(reinterpret_cast<u32x2_any*>(p), u32x2{w[0], w[1]});
+  }
+};
+
+// largest of 64 or of each half's 32 lanes
+template <int LANES>
+__device__ __forceinline__ float lanes_max(float v) {
+  if constexpr (LANES == 64) return wave_max(v);
+  v = dpp_max<0xb1>(v);
+  v = dpp_max<0x4e>(v);
+  v = dpp_max<0x141>(v);
+  v = dpp_max<0x140>(v);
+  const u32x2 a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
+}
+
+// A block of 256 values to a wave (fp32) or to half of one (bf16), 16 bytes of them to a lane, 4,096 values to four
+// waves with all their loads ahead of the maths. m is held as the e4m3 code of m (448 / max|m|), v as that of its
+// root r (448 / max r), with max / 448 beside: a root keeps v's range in half the octaves, and one that is not 0 keeps
+// at least the smallest code, since a v that rounds to 0 under an m that does not would let the next step with a small
+// gradient run away. Bound by the memory, 16 bytes an fp32 value: 0.29 G values take 790 us (5.9 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw8_kernel(const AdamTable<true> t, const f32x4* __restrict__ hyper,
                                                         float b1, float b1c, float b2, float b2c, float eps) {
-  constexpr int U = kChunk / kBlock / 4;
+  constexpr int N = Values<T>::N, LANES = kBlock / N, GROUPS = 64 / LANES, U = kChunk / kBlock / 4 / GROUPS;
   const int i = uniform(tensor_of(t, (int)blockIdx.x));
   const f32x4 h = hyper[i];
   if (h[3] != h[3]) return;
@@ -320,73 +331,78 @@ __global__ __launch_bounds__(256) void fl_adamw8_kernel(const AdamTable<true> t,
   const T* g = static_cast<const T*>(t.g[i]) + lo;
   uint8_t *mc = static_cast<uint8_t*>(t.m[i]) + lo, *vc = static_cast<uint8_t*>(t.v[i]) + lo;
   float *ms = t.ms[i] + lo / kBlock, *vs = t.vs[i] + lo / kBlock;
-  typename Four<T>::Reg pr[U] = {}, gr[U] = {};
-  uint32_t mr[U] = {}, vr[U] = {};
+  u32x4 pr[U] = {}, gr[U] = {};
+  Codes<N> mr[U], vr[U];
   float sm[U] = {}, sv[U] = {};
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int b = u * 4 + wave, k = b * kBlock + 4 * lane;
+    const int b = (u * 4 + wave) * GROUPS + lane / LANES, k = b * kBlock + lane % LANES * N;
     if (b * kBlock < n) {
       sm[u] = ms[b];
       sv[u] = vs[b];
     }
-    if (k + 4 <= n) {
-      pr[u] = Four<T>::load(p + k);
-      gr[u] = Four<T>::load(g + k);
-      mr[u] = load_once(reinterpret_cast<const u32_any*>(mc + k));
-      vr[u] = load_once(reinterpret_cast<const u32_any*>(vc + k));
+    if (k + N <= n) {
+      pr[u] = load_once(reinterpret_cast<const u32x4_any*>(p + k));
+      gr[u] = load_once(reinterpret_cast<const u32x4_any*>(g + k));
+      mr[u].load(mc + k);
+      vr[u].load(vc + k);
     } else if (k < n) {
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
+      for (int q = 0; q < N - 1; ++q) {
         if (k + q < n) {
-          Four<T>::set(pr[u], q, load_as<T>(p + k + q));
-          Four<T>::set(gr[u], q, load_as<T>(g + k + q));
-          mr[u] |= (uint32_t)mc[k + q] << (8 * q);
-          vr[u] |= (uint32_t)vc[k + q] << (8 * q);
+          set_value(pr[u], q, p[k + q]);
+          set_value(gr[u], q, g[k + q]);
+          mr[u].w[q / 4] |= (uint32_t)mc[k + q] << (8 * (q % 4));
+          vr[u].w[q / 4] |= (uint32_t)vc[k + q] << (8 * (q % 4));
         }
       }
     }
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int b = u * 4 + wave, k = b * kBlock + 4 * lane;
-    if (b * kBlock >= n) break;
-    float o[4], m[4], r[4];
-    const float m0[4] = {code_value<0>(mr[u]), code_value<1>(mr[u]), code_value<2>(mr[u]), code_value<3>(mr[u])};
-    const float r0[4] = {code_value<0>(vr[u]), code_value<1>(vr[u]), code_value<2>(vr[u]), code_value<3>(vr[u])};
+    const int b = (u * 4 + wave) * GROUPS + lane / LANES, k = b * kBlock + lane % LANES * N;
+    if ((u * 4 + wave) * GROUPS * kBlock >= n) break;  // (wave-uniform)
+    float o[N], m[N], r[N], top_m = 0.f, top_r = 0.f;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {  // (behind the tensor's end all is 0 and stays 0)
-      m[q] = m0[q] * sm[u];
-      const float root = r0[q] * sv[u];
+    for (int q = 0; q < N; ++q) {  // (behind the tensor's end all is 0 and stays 0)
+      m[q] = code_value(mr[u].w[q / 4], q % 4) * sm[u];
+      const float root = code_value(vr[u].w[q / 4], q % 4) * sv[u];
       float v = root * root;
-      o[q] = adamw_value(Four<T>::get(pr[u], q), Four<T>::get(gr[u], q), m[q], v, r[q], f);
+      o[q] = adamw_value(Values<T>::get(pr[u], q), Values<T>::get(gr[u], q), m[q], v, r[q], f);
+      top_m = fmaxf(top_m, fabsf(m[q]));
+      top_r = fmaxf(top_r, r[q]);
     }
-    const float top_m = wave_max(fmaxf(fmaxf(fabsf(m[0]), fabsf(m[1])), fmaxf(fabsf(m[2]), fabsf(m[3]))));
-    const float top_r = wave_max(fmaxf(fmaxf(r[0], r[1]), fmaxf(r[2], r[3])));
+    top_m = lanes_max<LANES>(top_m);
+    top_r = lanes_max<LANES>(top_r);
     const float inv_m = top_m >= kTiny ? 1.0f / top_m * kTopCode : 0.f;
     const float inv_r = top_r >= kTiny ? 1.0f / top_r * kTopCode : 0.f;
+    Codes<N> mo, vo;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < N; ++q) {
       m[q] *= inv_m;
       r[q] *= inv_r;
       if (r[q] > 0.f && r[q] < kSmallest) r[q] = kSmallest;
     }
-    const uint32_t mo = four_codes(m), vo = four_codes(r);
-    if (k + 4 <= n) {
-      Four<T>::store(p + k, o);
-      store_once(reinterpret_cast<u32_any*>(mc + k), mo);
-      store_once(reinterpret_cast<u32_any*>(vc + k), vo);
+#pragma unroll
+    for (int w = 0; w < N / 4; ++w) {
+      mo.w[w] = four_codes(m + 4 * w);
+      vo.w[w] = four_codes(r + 4 * w);
+    }
+    if (k + N <= n) {
+      store_once(reinterpret_cast<u32x4_any*>(p + k), pack_values<T>(o));
+      mo.store(mc + k);
+      vo.store(vc + k);
     } else if (k < n) {
 #pragma unroll
-      for (int q = 0; q < 3; ++q) {
+      for (int q = 0; q < N - 1; ++q) {
         if (k + q < n) {
           store_as(p + k + q, o[q]);
-          mc[k + q] = (uint8_t)(mo >> (8 * q));
-          vc[k + q] = (uint8_t)(vo >> (8 * q));
+          mc[k + q] = (uint8_t)(mo.w[q / 4] >> (8 * (q % 4)));
+          vc[k + q] = (uint8_t)(vo.w[q / 4] >> (8 * (q % 4)));
         }
       }
     }
-    if (lane == 0) {
+    if (lane % LANES == 0 && b * kBlock < n) {
       ms[b] = top_m >= kTiny ? top_m * (1.0f / kTopCode) : 0.f;
       vs[b] = top_r >= kTiny ? top_r * (1.0f / kTopCode) : 0.f;
     }
