@@ -16,7 +16,8 @@ using namespace fl;
 constexpr int kTensors = 64;      // tensors of a step's launch (an 8-bit table of 64 is 3.6 KiB of arguments)
 constexpr int kNormTensors = 192;  // tensors of the norm's (3.8 KiB)
 constexpr int kStepTensors = 480; // step counters of a launch, one to a thread
-constexpr int kChunk = 4096;      // values of a block
+constexpr int kChunk = 2048;      // values of a step's block (the 8-bit step of 0.29 G bf16 values: 505 us; with 4,096
+                                  // 522, with 1,024 544; the 32-bit step of as many fp32 1,415, 1,480 and 1,413)
 constexpr int kBlock = 256;       // values that share a scale in the 8-bit states
 constexpr int kMaxBlocks = 1 << 23;  // blocks of a launch
 
@@ -208,7 +209,7 @@ __device__ __forceinline__ u32x4 pack_values<bf16_bits>(const float* v) {
 }
 
 // 16 bytes of parameters and gradients to a thread and turn, and their moments. Bound by the memory, 28 bytes an fp32
-// value: 0.29 G values take 1,445 us (5.6 TB/s; a streaming copy reaches 5.9).
+// value: 0.29 G values take 1,415 us (5.7 TB/s; a streaming copy reaches 5.9).
 template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw_kernel(const AdamTable<false> t, const f32x4* __restrict__ hyper,
                                                        float b1, float b1c, float b2, float b2c, float eps) {
@@ -311,11 +312,11 @@ __device__ __forceinline__ float lanes_max(float v) {
   return fmaxf(__uint_as_float(a.x), __uint_as_float(a.y));
 }
 
-// A block of 256 values to a wave (fp32) or to half of one (bf16), 16 bytes of them to a lane, 4,096 values to four
+// A block of 256 values to a wave (fp32) or to half of one (bf16), 16 bytes of them to a lane, 2,048 values to four
 // waves with all their loads ahead of the maths. m is held as the e4m3 code of m (448 / max|m|), v as that of its
 // root r (448 / max r), with max / 448 beside: a root keeps v's range in half the octaves, and one that is not 0 keeps
 // at least the smallest code, since a v that rounds to 0 under an m that does not would let the next step with a small
-// gradient run away. Bound by the memory, 16 bytes an fp32 value: 0.29 G values take 790 us (5.9 TB/s).
+// gradient run away. Bound by the memory, 16 bytes an fp32 value: 0.29 G values take 770 us (6.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw8_kernel(const AdamTable<true> t, const f32x4* __restrict__ hyper,
                                                         float b1, float b1c, float b2, float b2c, float eps) {
@@ -409,7 +410,7 @@ __global__ __launch_bounds__(256) void fl_adamw8_kernel(const AdamTable<true> t,
   }
 }
 
-constexpr int64_t kMaxNumel = (int64_t)1 << 34;  // 2^22 blocks: a tensor always fits a launch of 2^23
+constexpr int64_t kMaxNumel = (int64_t)1 << 34;  // 2^23 blocks: a tensor always fits a launch
 constexpr int64_t kMaxTensors = 1 << 20;
 
 // Fills `table` with tensors from `i` on, empty ones too; returns the index after the last one taken.
@@ -470,7 +471,7 @@ bool list_ok(int64_t n, const int64_t* numel) {
 int norm_chunk(int64_t n, const int64_t* numel) {
   int64_t total = 0;
   for (int64_t i = 0; i < n; ++i) total += numel[i];
-  int chunk = kChunk;
+  int chunk = 4096;
   while (chunk < 32768 && total / chunk > 2048) chunk *= 2;
   return chunk;
 }
