@@ -136,9 +136,9 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
 // 16 bytes to a thread, for the maximum, the sums and the alternatives, so that memory is read once. With the
 // segment's maximum known, e^d is one fused product and one power (x c - m c, c = log2(e) / T; the rounding error of
 // m c is put back into the log at the end), and no sum is ever rescaled. The memory bounds it where rows are many:
-// 8,192 rows of 16,384 bf16 take 41 us (6.5 TB/s; a streaming read reaches 7.0), with entropy and 20 alternatives
-// 62; the work between two rows' loads where they are short or carry alternatives; one row of 131,072 is two
-// launches and 13 us.
+// 8,192 rows of 16,384 bf16 take 41 us (6.5 TB/s; a streaming read reaches 7.0), 36 of which their vector instructions
+// fill too (5.5 a logit, 7.5 with entropy, of four cycles each and 16 for the power). With entropy and 20 alternatives
+// they take 60 and the instructions bound it (52). One row of 131,072 is two launches and 13 us.
 //
 // Alternatives: the threads' maxima (in 64 groups where K is small) give a value that at least K logits reach: their
 // K-th largest, to 16 bits. Only logits from there up are candidates, little more than K of them in text; they are
@@ -179,16 +179,21 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     if (whole && tid == 0 && t >= 0 && t < V) xt = load_as<T>(row_x + t);
     u32x4 v[NV];
     const auto load = [&](auto get) {
+      // (a uniform address and 32 bits beside: no address of its own to a lane and pack)
+      const auto place = [&](int i) {
+        const char* from = reinterpret_cast<const char*>(x + head + i * THREADS * N);
+        return reinterpret_cast<const u32x4*>(from + (uint32_t)tid * 16u);
+      };
       if (packs == NV * THREADS) {  // all of the tile: nothing to stand in for
 #pragma unroll
-        for (int i = 0; i < NV; ++i) v[i] = get(reinterpret_cast<const u32x4*>(x + head + (i * THREADS + tid) * N));
+        for (int i = 0; i < NV; ++i) v[i] = get(place(i));
         return;
       }
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
         const int j = i * THREADS + tid;
         v[i] = u32x4{Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone, Pack<T>::kNone};
-        if (j < packs) v[i] = get(reinterpret_cast<const u32x4*>(x + head + j * N));
+        if (j < packs) v[i] = get(place(i));
       }
     };
     // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 42 us, and 48 through
@@ -393,11 +398,12 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         if (wave == 0) {
           const uint64_t key = lane < n ? key_at(lane) : 0;
           int rank = 0;
-          for (int j = 0; j < n; ++j) {
-            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(key >> 32), j);
-            const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)key, j);
-            rank += ((uint64_t)hi << 32 | low) > key;
-          }
+          // (keys broadcast by the LDS: half the vector instructions of reading them from lanes, 64 us against 68 for
+          // 8,188 rows of 16,384 with 20 alternatives)
+          s_cand[lane] = key;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 4
+          for (int j = 0; j < n; ++j) rank += s_cand[j] > key;
           if (lane < n && rank < K) put(rank, key);
         }
       } else {
