@@ -20,6 +20,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <algorithm>
 #include <memory>
@@ -55,6 +56,16 @@ void check(int code, const char* what) {
   TORCH_CHECK(code != FL_ERR_WORKSPACE, what, ": workspace missing or too small");
   TORCH_CHECK(code < FL_ERR_HIP_BASE, what, ": HIP error ", code - FL_ERR_HIP_BASE);
   TORCH_CHECK(code == FL_OK, what, ": error code ", code);
+}
+
+// a trace would keep the results of its example as constants
+void check_not_traced(const char* what) {
+  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " reads addresses and cannot be traced");
+}
+
+// A tensor that dispatches to Python (a fake one, say) has no memory of its own behind its address.
+void check_plain(const Tensor& t, const char* what) {
+  TORCH_CHECK_TYPE(!t.key_set().has(c10::DispatchKey::Python), what, " must be plain tensors");
 }
 
 int dtype_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FL_DTYPE_BF16 : FL_DTYPE_F32; }
@@ -281,6 +292,8 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
   o.ignore_index = ignore_index;
   TORCH_CHECK_TYPE(THPVariable_Check(first) && THPVariable_Check(second), "logits and tokens must be tensors");
   const Tensor &logits = THPVariable_Unpack(first), &tokens = THPVariable_Unpack(second);
+  check_plain(logits, "logits");
+  check_plain(tokens, "tokens");
   TORCH_CHECK_TYPE(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16,
                    "logits must be float32 or bfloat16, got ", logits.scalar_type());
   TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong, "tokens must be int64, got ", tokens.scalar_type());
@@ -294,6 +307,7 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
                     kMinTemperature, " to ", kMaxTemperature, ", got ", o.temperature);
   TORCH_CHECK_VALUE(o.top_k >= 0 && o.top_k <= most, "top_k must be 0 to ", most, ", got ", o.top_k);
   TORCH_CHECK(logits.is_cuda(), "token_logprobs requires a ROCm (cuda) device");
+  check_not_traced("token_logprobs");
   TORCH_CHECK_VALUE(tokens.device() == logits.device(), "logits and tokens must be on one device");
   TORCH_CHECK_NOT_IMPLEMENTED(!logits._fw_grad(0).defined(), "token_logprobs has no forward-mode derivative");
   const Tensor x = logits.is_neg() ? logits.resolve_neg() : logits;
@@ -376,6 +390,7 @@ struct TensorList {
     for (size_t i = 0; i < n; ++i) {
       TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ": number ", i, " is no tensor");
       const Tensor& t = THPVariable_Unpack(items[i]);
+      check_plain(t, what);
       const auto at = std::find(types.begin(), types.end(), t.scalar_type());
       TORCH_CHECK_TYPE(at != types.end(), what, " must be ", *types.begin(),
                        types.size() > 1 ? " or another type of the list" : "",
@@ -429,6 +444,7 @@ float* device_value(PyObject* o, const char* what, at::Device device) {
   if (o == Py_None) return nullptr;
   TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
   const Tensor& t = THPVariable_Unpack(o);
+  check_plain(t, what);
   TORCH_CHECK_VALUE(t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == device, what,
                     " must be one float32 value on ", device);
   return static_cast<float*>(t.data_ptr());
@@ -446,6 +462,7 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   if (!PyArg_ParseTuple(args, "Od", &list, &max_norm)) return nullptr;
   const at::Device device = first_of(list, "gradients").device();
   TORCH_CHECK(device.is_cuda(), "grad_norm requires a ROCm (cuda) device");
+  check_not_traced("grad_norm");
   const TensorList grads(list, "gradients", device, {at::kFloat, at::kBFloat16}, nullptr, 1, true);
   const c10::DeviceGuard guard(device);
   const int64_t n = (int64_t)grads.size();
@@ -484,6 +501,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                     "one gradient, one state of each kind and one step per parameter");
   TORCH_CHECK_VALUE(eight == (sq_scales != Py_None), "8-bit states need the scales of both moments");
   TORCH_CHECK(device.is_cuda(), "adamw_step requires a ROCm (cuda) device");
+  check_not_traced("adamw_step");
   const TensorList p(params, "parameters", device, {type});
   const int64_t n = (int64_t)p.size();
   const TensorList g(grads, "gradients", device, {type}, &p.counts, 1, true);
@@ -509,6 +527,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   std::vector<void*> step_at;
   if (THPVariable_Check(steps)) {
     const Tensor& t = THPVariable_Unpack(steps);
+    check_plain(t, "steps");
     TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == device && t.dim() == 1 && t.numel() == n &&
                           t.is_contiguous(),
                       "steps must be ", n, " int64 values on ", device);

@@ -409,6 +409,18 @@ def test_partial_outputs_and_no_gradient(dev):
                 fl.token_logprobs(fwad.make_dual(z, torch.ones_like(x)), t)
     with pytest.raises(RuntimeError):  # a transform's wrapper has no memory to read
         torch.func.vmap(lambda a, b: fl.token_logprobs(a, b).logprobs)(x.detach(), t)
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda a: fl.token_logprobs(a, t).logprobs.sum())(x.detach())
+    with pytest.raises(RuntimeError):  # a trace would hold this call's results
+        torch.jit.trace(lambda a, b: fl.token_logprobs(a, b).logprobs, (x.detach(), t))
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    plain = x.detach()
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        with pytest.raises(TypeError):
+            fl.token_logprobs(x.detach(), t)  # a fake tensor
+        with pytest.raises(ValueError):  # outputs without memory
+            fl.token_logprobs(plain, t)
     with pytest.raises(ValueError):
         fl.token_logprobs(x, t.cpu())
     changed = x.detach().clone().requires_grad_()

@@ -286,6 +286,10 @@ def test_adamw_refuses_on_the_device(dev):
             fl.adamw_step(*bad)
     with pytest.raises(ValueError):
         fl.adamw_step([p], [one()], [codes], [one(STATE8_DTYPE)], step, exp_avg_scales=[sc], exp_avg_sq_scales=[sc])
+    with pytest.raises(RuntimeError):
+        torch.jit.trace(lambda g: fl.grad_norm([g]), (p,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda g: fl.grad_norm([g]))(one(n=8).view(2, 4))
     grad = one()  # one gradient of two parameters is read twice
     fl.adamw_step([one(), one()], [grad, grad], [one(), one()], [one(), one()],
                   torch.zeros(2, dtype=torch.long, device=dev))

@@ -14,6 +14,19 @@ from fields_lm_amd import _native as nat
 from fields_lm_amd import logprobs as L
 
 
+def test_fake_tensors_are_refused():
+    """Tensors that dispatch to Python have no memory behind their addresses."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, t = torch.empty(4, 9, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
+        step = torch.zeros(1, dtype=torch.long, device="cuda")
+    for call in (lambda: fl.token_logprobs(x[1:], t), lambda: fl.grad_norm([x[1:]]),
+                 lambda: fl.adamw_step([x], [x], [x], [x], step)):
+        with pytest.raises(TypeError):
+            call()
+
+
 # ------------------------------------------------------------------ token_logprobs
 def test_token_logprobs_refuses_what_it_does_not_take():
     x, t = torch.randn(3, 7), torch.zeros(3, dtype=torch.long)
