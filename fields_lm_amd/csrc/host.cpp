@@ -413,20 +413,41 @@ struct TensorList {
   size_t size() const { return addresses.size(); }
 };
 
-typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;  // of addresses, [first, last + 1)
+typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;  // of addresses, [first, last + 1), in their order
 
-void add_ranges(Ranges& to, const TensorList& list, size_t size) {
+Ranges ranges_of(const TensorList& list, size_t size) {
+  Ranges r;
+  r.reserve(list.size());
   for (size_t i = 0; i < list.size(); ++i) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(list.addresses[i]);
-    if (list.counts[i]) to.emplace_back(at, at + list.counts[i] * size);
+    if (list.counts[i]) r.emplace_back(at, at + list.counts[i] * size);
   }
+  if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
+  return r;
 }
 
-// whether two ranges share an address, after sorting
-bool overlap(Ranges& ranges) {
-  std::sort(ranges.begin(), ranges.end());
-  for (size_t i = 1; i < ranges.size(); ++i)
-    if (ranges[i].first < ranges[i - 1].second) return true;
+// Lists are mostly in order and apart from each other, so that sorting all of a step's ranges anew (16 us for 240
+// tensors with 8-bit states) is not needed.
+void merge(Ranges& to, const Ranges& r) {
+  if (r.empty()) return;
+  const bool ahead = !to.empty() && r.back() < to.front(), behind = to.empty() || to.back() < r.front();
+  const auto middle = to.insert(ahead ? to.begin() : to.end(), r.begin(), r.end());
+  if (!ahead && !behind) std::inplace_merge(to.begin(), middle, to.end());
+}
+
+bool overlap(const Ranges& r) {
+  for (size_t i = 1; i < r.size(); ++i)
+    if (r[i].first < r[i - 1].second) return true;
+  return false;
+}
+
+// whether one of a, which are apart, and one of b share an address
+bool meet(const Ranges& a, const Ranges& b) {
+  for (size_t i = 0, j = 0; i < a.size() && j < b.size();) {
+    if (a[i].second <= b[j].first) ++i;
+    else if (b[j].second <= a[i].first) ++j;
+    else return true;
+  }
   return false;
 }
 
@@ -511,16 +532,17 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   const at::ScalarType state = eight ? at::kFloat8_e4m3fn : at::kFloat;
   const TensorList m(avgs, "states", device, {state}, &p.counts), v(sqs, "states", device, {state}, &p.counts);
   Ranges written;
-  written.reserve(5 * n + n);
-  add_ranges(written, p, type == at::kFloat ? 4 : 2);
-  add_ranges(written, m, eight ? 1 : 4);
-  add_ranges(written, v, eight ? 1 : 4);
+  written.reserve(6 * n);
+  const size_t size = type == at::kFloat ? 4 : 2;
+  merge(written, ranges_of(p, size));
+  merge(written, ranges_of(m, eight ? 1 : 4));
+  merge(written, ranges_of(v, eight ? 1 : 4));
   std::vector<void*> ms, vs;
   if (eight) {
     const TensorList m_scales(avg_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock);
     const TensorList v_scales(sq_scales, "scales", device, {at::kFloat}, &p.counts, kStateBlock);
-    add_ranges(written, m_scales, 4);
-    add_ranges(written, v_scales, 4);
+    merge(written, ranges_of(m_scales, 4));
+    merge(written, ranges_of(v_scales, 4));
     ms = m_scales.addresses;
     vs = v_scales.addresses;
   }
@@ -532,22 +554,17 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                           t.is_contiguous(),
                       "steps must be ", n, " int64 values on ", device);
     for (int64_t i = 0; i < n; ++i) step_at.push_back(static_cast<int64_t*>(t.data_ptr()) + i);
-    written.emplace_back(reinterpret_cast<uintptr_t>(step_at[0]), reinterpret_cast<uintptr_t>(step_at[0]) + n * 8);
+    const uintptr_t at = reinterpret_cast<uintptr_t>(step_at[0]);
+    merge(written, {{at, at + n * 8}});
   } else {
     const std::vector<int64_t> ones(n, 1);
     const TensorList list(steps, "steps", device, {at::kLong}, &ones);
-    add_ranges(written, list, 8);
+    merge(written, ranges_of(list, 8));
     step_at = list.addresses;
   }
   TORCH_CHECK_VALUE(!overlap(written), "parameters, states or step counters share memory");
-  for (int64_t i = 0; i < n; ++i) {  // a gradient is read beside what others write
-    if (!p.counts[i]) continue;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(g.addresses[i]);
-    const auto next = std::upper_bound(written.begin(), written.end(), std::make_pair(at, UINTPTR_MAX));
-    TORCH_CHECK_VALUE((next == written.end() || next->first >= at + p.counts[i] * (type == at::kFloat ? 4 : 2)) &&
-                          (next == written.begin() || std::prev(next)->second <= at),
-                      "gradient ", i, " shares memory with a parameter, a state or a step counter");
-  }
+  TORCH_CHECK_VALUE(!meet(written, ranges_of(g, size)),
+                    "a gradient shares memory with a parameter, a state or a step counter");
   float* scale = device_value(grad_scale, "grad_scale", device);
   float* lr_at = THPVariable_Check(lr) ? device_value(lr, "lr", device) : nullptr;
   const double lr_value = lr_at ? 0.0 : PyFloat_AsDouble(lr);

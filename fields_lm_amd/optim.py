@@ -11,6 +11,7 @@ in a HIP graph and replayed.
 from __future__ import annotations
 
 import math
+from operator import itemgetter
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -21,6 +22,8 @@ STATE_BLOCK = 256                   # values that share a scale in the 8-bit sta
 STATE8_DTYPE = torch.float8_e4m3fn  # their codes
 
 _TYPES = (torch.float32, torch.bfloat16)
+_STATES = {32: itemgetter("step", "exp_avg", "exp_avg_sq"),
+           8: itemgetter("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
 
 def _listed(tensors):
@@ -150,25 +153,29 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        work: List[Tuple[dict, List[torch.Tensor]]] = []
+        work: List[Tuple[dict, List[torch.Tensor], List[torch.Tensor]]] = []  # a group's parameters and gradients
         for group in self.param_groups:
             kinds: dict = {}
             for p in group["params"]:
-                if p.grad is not None:
-                    kinds.setdefault((p.dtype, p.device), []).append(p)
-            work += [(group, ps) for ps in kinds.values()]
+                grad = p.grad
+                if grad is not None:
+                    key = (p.dtype, p.device)
+                    kind = kinds.get(key)
+                    if kind is None:
+                        kind = kinds[key] = (group, [], [])
+                    kind[1].append(p)
+                    kind[2].append(grad)
+            work += kinds.values()
         if not work:
             return loss
         scale = None
         if self.max_grad_norm is not None:
-            self.grad_norm, scale = grad_norm((p.grad for _, ps in work for p in ps), self.max_grad_norm)
-        for group, ps in work:
-            bits = group["state_bits"]
-            states = [self._state(p, bits) for p in ps]
-            names = ("exp_avg_scale", "exp_avg_sq_scale")
-            scales = [[s[k] for s in states] for k in names] if bits == 8 else (None, None)
-            adamw_step(ps, [p.grad for p in ps], [s["exp_avg"] for s in states], [s["exp_avg_sq"] for s in states],
-                       [s["step"] for s in states], lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                       weight_decay=group["weight_decay"], grad_scale=scale, exp_avg_scales=scales[0],
-                       exp_avg_sq_scales=scales[1])
+            self.grad_norm, scale = grad_norm([g for _, _, grads in work for g in grads], self.max_grad_norm)
+        for group, ps, grads in work:
+            bits, state = group["state_bits"], self.state
+            states = [state[p] or self._state(p, bits) for p in ps]
+            steps, avgs, sqs, *scales = zip(*map(_STATES[bits], states))
+            adamw_step(ps, grads, avgs, sqs, steps, lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                       weight_decay=group["weight_decay"], grad_scale=scale,
+                       **dict(zip(("exp_avg_scales", "exp_avg_sq_scales"), scales)))
         return loss
