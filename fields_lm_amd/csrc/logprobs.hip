@@ -196,8 +196,8 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         if (j < packs) v[i] = get(place(i));
       }
     };
-    // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 42 us, and 48 through
-    // them; where one follows the pair takes 139 us so, and 132 through them).
+    // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 45 us, and 51 through
+    // them; where one follows the pair takes 147 us so, and 137 through them).
     if (out.stats) load([](const u32x4* p) { return *p; });
     else load([](const u32x4* p) { return __builtin_nontemporal_load(p); });
     // the logits ahead of the first pack and behind the last, one to a thread (fewer than 8 each), len for none

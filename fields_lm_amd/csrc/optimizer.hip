@@ -63,8 +63,8 @@ __device__ __forceinline__ int tensor_of(const Table& t, int block) {
   return ended;
 }
 
-// What a step touches once it touches past the caches' keeping (0.29 G values: the norm 222 us plain and 196
-// streaming, the 32-bit step behind it 1,810 and 1,641 us in all, the 8-bit step 884 and 805).
+// What a step touches once it touches past the caches' keeping (0.29 G values: the norm 204 us plain and 179
+// streaming, the 32-bit step behind it 1,776 and 1,581 us in all, the 8-bit step 887 and 777).
 __device__ __forceinline__ u32x4 load_once(const u32x4_any* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ u32x2 load_once(const u32x2_any* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ uint32_t load_once(const u32_any* p) { return __builtin_nontemporal_load(p); }
@@ -187,7 +187,7 @@ struct Factors {
 };
 
 // One value: m and v in, m, v and its root out; the new parameter. The quotient of the update is a product with
-// v_rcp_f32 (an ulp; a correctly rounded division is ten operations more and the bf16 8-bit step 6 % slower): the
+// v_rcp_f32 (an ulp; a correctly rounded division is ten operations more and the bf16 8-bit step 8 % slower): the
 // update is small beside p. Roots are correctly rounded, the 8-bit codes go by them.
 __device__ __forceinline__ float adamw_value(float p, float g, float& m, float& v, float& root, const Factors& f) {
   g = g * f.gs;
