@@ -132,13 +132,13 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
   }
 }
 
-// One block to a row, or to a segment of one (gridDim.y of them): its logits stay in registers, NV packs of
-// 16 bytes to a thread, for the maximum, the sums and the alternatives, so that memory is read once. With the
-// segment's maximum known, e^d is one fused product and one power (x c - m c, c = log2(e) / T; the rounding error of
-// m c is put back into the log at the end), and no sum is ever rescaled. The memory bounds it where rows are many:
-// 8,192 rows of 16,384 bf16 take 41 us (6.5 TB/s; a streaming read reaches 7.0), 29 of which their vector instructions
-// fill too (5.5 a logit, 7.5 with entropy, of four cycles each and eight for the power). With entropy and 20
-// alternatives they take 60, of which the instructions fill 48 and the memory 39. One row of 131,072 is two launches and 13 us.
+// One block to a row, or to a segment of one (gridDim.y of them): its logits stay in registers, NV packs of 16 bytes
+// to a thread, for the maximum, the sums and the alternatives, so that memory is read once. With the segment's maximum
+// known, e^d is one fused product and one power (x c - m c, c = log2(e) / T; the rounding error of m c is put back
+// into the log at the end), and no sum is ever rescaled. The memory bounds it where rows are many: 8,192 rows of
+// 16,384 bf16 take 41 us (6.5 TB/s; a streaming read reaches 7.0), 29 of which their vector instructions fill too (5.5
+// a logit, 7.5 with entropy, of four cycles each and eight for the power). With entropy and 20 alternatives they take
+// 60, of which the instructions fill 48 and the memory 39. One row of 131,072 is two launches and 13 us.
 //
 // Alternatives: the threads' maxima (in 64 groups where K is small) give a value that at least K logits reach: their
 // K-th largest, to 16 bits. Only logits from there up are candidates, little more than K of them in text; they are
