@@ -531,3 +531,24 @@ def test_score_of_the_model_is_its_logits_log_softmax(dev):
     assert lm.score(ids[:, :1]).logprobs.shape == (2, 0)
     with pytest.raises(TypeError):
         lm.score(ids.int())
+
+
+@pytest.mark.parametrize("rows", [1, 5])
+def test_gradients_with_the_negative_flag(dev, rows):
+    """Upstream gradients whose memory holds their negative (the imaginary part of a conjugate), of one row and more."""
+    print(f"[case] token_logprobs gradients with the negative flag, rows {rows}", flush=True)
+    x, t = make(dev, rows, 300, torch.float32, rows)
+    gen = torch.Generator(device=dev).manual_seed(rows)
+    ups = [torch.randn(*s, device=dev, generator=gen) for s in ((rows,), (rows,), (rows, 4))]
+    z = x.clone().requires_grad_()
+    r = fl.token_logprobs(z, t, top_k=4, entropy=True)
+    outs = [r.logprobs, r.entropy, r.top_logprobs]
+    for use in ((0,), (1,), (2,), (0, 1, 2)):
+        o, g = [outs[i] for i in use], [ups[i] for i in use]
+        exp, = torch.autograd.grad(o, z, g, retain_graph=True)
+        got, = torch.autograd.grad(o, z, [torch._neg_view(-u) for u in g], retain_graph=True)
+        assert torch.equal(got, exp), use
+    lp = fl.token_logprobs(z, t).logprobs
+    exp, = torch.autograd.grad(2 * lp.sum(), z, retain_graph=True)
+    got, = torch.autograd.grad((torch.complex(torch.zeros_like(lp), lp).conj() * (1 + 2j)).real.sum(), z)
+    assert torch.equal(got, exp)
