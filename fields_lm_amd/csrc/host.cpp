@@ -310,9 +310,9 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
   check_not_traced("token_logprobs");
   TORCH_CHECK_VALUE(tokens.device() == logits.device(), "logits and tokens must be on one device");
   TORCH_CHECK_NOT_IMPLEMENTED(!logits._fw_grad(0).defined(), "token_logprobs has no forward-mode derivative");
-  const Tensor x = logits.is_neg() ? logits.resolve_neg() : logits;
+  const Tensor x = logits.resolve_neg(), t = tokens.resolve_neg();
   variable_list out;
-  if (tokens.numel() == 0) {  // no rows: empty outputs, on the logits' graph
+  if (t.numel() == 0) {  // no rows: empty outputs, on the logits' graph
     const Tensor none = x.sum(-1, false, at::kFloat);
     out = {none};
     if (o.entropy) out.push_back(none.clone());
@@ -320,12 +320,12 @@ PyObject* token_logprobs(PyObject*, PyObject* args) {
       std::vector<int64_t> shape = none.sizes().vec();
       shape.push_back(o.top_k);
       out.push_back(none.unsqueeze(-1).expand(shape).clone());
-      out.push_back(tokens.unsqueeze(-1).expand(shape).clone());
+      out.push_back(t.unsqueeze(-1).expand(shape).clone());
     }
   } else if (at::GradMode::is_enabled() && x.requires_grad()) {
-    out = TokenLogprobs::apply(x, tokens, o.temperature, o.top_k, o.entropy, o.ignore_index);
+    out = TokenLogprobs::apply(x, t, o.temperature, o.top_k, o.entropy, o.ignore_index);
   } else {
-    const Results r = forward(x, tokens, o, false);
+    const Results r = forward(x, t, o, false);
     out = {r.logprobs};
     if (o.entropy) out.push_back(r.entropy);
     if (o.top_k) out.insert(out.end(), {r.top_logprobs, r.top_tokens});

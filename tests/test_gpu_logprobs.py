@@ -552,3 +552,14 @@ def test_gradients_with_the_negative_flag(dev, rows):
     exp, = torch.autograd.grad(2 * lp.sum(), z, retain_graph=True)
     got, = torch.autograd.grad((torch.complex(torch.zeros_like(lp), lp).conj() * (1 + 2j)).real.sum(), z)
     assert torch.equal(got, exp)
+
+
+def test_tokens_with_the_negative_flag(dev):
+    print("[case] token_logprobs, tokens with the negative flag", flush=True)
+    x, t = make(dev, 6, 400, torch.float32, 9)
+    t[1], t[2] = -100, 400
+    z = x.clone().requires_grad_()
+    a, b = (fl.token_logprobs(z, s).logprobs for s in (t, torch._neg_view(-t)))
+    assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+    a, b = (torch.autograd.grad(o.sum(), z)[0].nan_to_num(7.0) for o in (a, b))
+    assert torch.equal(a, b)
