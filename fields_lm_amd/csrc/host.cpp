@@ -460,15 +460,15 @@ const Tensor& first_of(PyObject* list, const char* what) {
   return THPVariable_Unpack(first);
 }
 
-// one fp32 value on the device, or none
-float* device_value(PyObject* o, const char* what, at::Device device) {
-  if (o == Py_None) return nullptr;
+// one fp32 value on the device (a copy where its memory holds the negative), or none
+Tensor device_value(PyObject* o, const char* what, at::Device device) {
+  if (o == Py_None) return {};
   TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
   const Tensor& t = THPVariable_Unpack(o);
   check_plain(t, what);
   TORCH_CHECK_VALUE(t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == device, what,
                     " must be one float32 value on ", device);
-  return static_cast<float*>(t.data_ptr());
+  return t.is_neg() ? t.detach().resolve_neg() : t;
 }
 
 Tensor workspace_on(at::Device device, size_t bytes) {
@@ -551,8 +551,8 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
     const Tensor& t = THPVariable_Unpack(steps);
     check_plain(t, "steps");
     TORCH_CHECK_VALUE(t.scalar_type() == at::kLong && t.device() == device && t.dim() == 1 && t.numel() == n &&
-                          t.is_contiguous(),
-                      "steps must be ", n, " int64 values on ", device);
+                          t.is_contiguous() && !t.is_neg(),
+                      "steps must be ", n, " contiguous int64 values on ", device);
     for (int64_t i = 0; i < n; ++i) step_at.push_back(static_cast<int64_t*>(t.data_ptr()) + i);
     const uintptr_t at = reinterpret_cast<uintptr_t>(step_at[0]);
     merge(written, {{at, at + n * 8}});
@@ -565,9 +565,9 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   TORCH_CHECK_VALUE(!overlap(written), "parameters, states or step counters share memory");
   TORCH_CHECK_VALUE(!meet(written, ranges_of(g, size)),
                     "a gradient shares memory with a parameter, a state or a step counter");
-  float* scale = device_value(grad_scale, "grad_scale", device);
-  float* lr_at = THPVariable_Check(lr) ? device_value(lr, "lr", device) : nullptr;
-  const double lr_value = lr_at ? 0.0 : PyFloat_AsDouble(lr);
+  const Tensor scale = device_value(grad_scale, "grad_scale", device);
+  const Tensor lr_at = THPVariable_Check(lr) ? device_value(lr, "lr", device) : Tensor();
+  const double lr_value = lr_at.defined() ? 0.0 : PyFloat_AsDouble(lr);
   if (PyErr_Occurred()) return nullptr;
   const c10::DeviceGuard guard(device);
   const size_t bytes = adamw_bytes(n);
@@ -575,8 +575,8 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   check(adamw_call(n, p.addresses.data(), g.addresses.data(), type == at::kBFloat16 ? FL_DTYPE_BF16 : FL_DTYPE_F32,
                    m.addresses.data(), v.addresses.data(), eight ? reinterpret_cast<float* const*>(ms.data()) : nullptr,
                    eight ? reinterpret_cast<float* const*>(vs.data()) : nullptr, p.counts.data(),
-                   reinterpret_cast<int64_t* const*>(step_at.data()), lr_value, lr_at, beta1, beta2, eps, decay, scale,
-                   address<void>(ws), bytes, stream_of(first)),
+                   reinterpret_cast<int64_t* const*>(step_at.data()), lr_value, address<float>(lr_at), beta1, beta2, eps, decay,
+                   address<float>(scale), address<void>(ws), bytes, stream_of(first)),
         "fl_adamw_step");
   for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(params); ++i) {  // written in place: saved parameters are stale
     const Tensor& t = THPVariable_Unpack(PySequence_Fast_ITEMS(params)[i]);

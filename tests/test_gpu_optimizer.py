@@ -528,3 +528,22 @@ def test_a_training_step_of_field_blocks(dev, bits):
         assert bool(p.isfinite().all())
     again = fl.token_logprobs(logits()[:, :-1], target).logprobs
     assert bool(again.isfinite().all()) and int(opt.state[params[0]]["step"]) == 1
+
+
+def test_adamw_values_with_the_negative_flag(dev):
+    """lr and grad_scale whose memory holds their negative are read as they are; step counters are refused."""
+    print("[case] adamw_step, values with the negative flag", flush=True)
+    p, g, m, v = start32(dev, [100], torch.float32, 5)
+    lr, scale = torch.tensor(3e-3, device=dev), torch.tensor(0.5, device=dev)
+    results = []
+    for a, b in ((lr, scale), (torch._neg_view(-lr), torch._neg_view(-scale)),
+                 (torch.complex(lr, -lr).conj().imag, torch.complex(scale, -scale).conj().imag)):
+        q, m2, v2 = ([t.clone() for t in l] for l in (p, m, v))
+        fl.adamw_step(q, g, m2, v2, torch.zeros(1, dtype=torch.long, device=dev), grad_scale=b, **{**HYPER, "lr": a})
+        results.append(q + m2 + v2)
+    for other in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(results[0], other))
+    steps = torch._neg_view(torch.zeros(1, dtype=torch.long, device=dev))
+    for bad in (steps, [steps]):
+        with pytest.raises(ValueError):
+            fl.adamw_step(p, g, m, v, bad, **HYPER)
