@@ -182,8 +182,11 @@ Tensor backward(const Tensor& logits, const Tensor& tokens, const Tensor& stats,
                 const Tensor& top_tokens, const Options& o, const Tensor* grads) {
   const c10::DeviceGuard guard(logits.device());
   Tensor g[3];
-  for (int i = 0; i < 3; ++i)
-    if (grads[i].defined()) g[i] = grads[i].resolve_neg().contiguous();
+  for (int i = 0; i < 3; ++i) {
+    if (!grads[i].defined()) continue;
+    check_plain(grads[i], "the upstream gradients");
+    g[i] = grads[i].resolve_neg().contiguous();
+  }
   Tensor out = at::empty(logits.sizes(), at::TensorOptions().dtype(logits.scalar_type()).device(logits.device()));
   const Located at = locate(logits, tokens);
   check(logprobs_backward_call(address<void>(at.logits), dtype_code(logits), at.at.outer, at.at.inner, logits.size(-1),

@@ -563,3 +563,34 @@ def test_tokens_with_the_negative_flag(dev):
     assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
     a, b = (torch.autograd.grad(o.sum(), z)[0].nan_to_num(7.0) for o in (a, b))
     assert torch.equal(a, b)
+
+
+def test_upstream_gradients_without_memory_are_refused(dev):
+    """What follows in the graph may hand over a gradient that dispatches to Python, with no memory at its address."""
+    print("[case] token_logprobs, upstream gradients without memory", flush=True)
+    x, t = make(dev, 3, 20, torch.float32, 1)
+
+    class Wrapped(torch.Tensor):
+        @staticmethod
+        def __new__(cls, like):
+            return torch.Tensor._make_wrapper_subclass(cls, like.shape, dtype=like.dtype, device=like.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return func(*(torch.ones(a.shape, dtype=a.dtype, device=a.device) if isinstance(a, cls) else a for a in args),
+                        **(kwargs or {}))
+
+    class Hands(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, a):
+            return a.clone()
+
+        @staticmethod
+        def backward(ctx, g):
+            return Wrapped(g)
+
+    for entropy in (False, True):
+        z = x.clone().requires_grad_()
+        r = fl.token_logprobs(z, t, entropy=entropy)
+        with pytest.raises(TypeError):
+            torch.autograd.grad(Hands.apply(r.entropy if entropy else r.logprobs).sum(), z)
