@@ -471,6 +471,7 @@ Tensor device_value(PyObject* o, const char* what, at::Device device) {
   check_plain(t, what);
   TORCH_CHECK_VALUE(t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == device, what,
                     " must be one float32 value on ", device);
+  TORCH_CHECK_VALUE(t.data_ptr(), what, " has no memory");  // (an address of 0 stands for no value)
   return t.is_neg() ? t.detach().resolve_neg() : t;
 }
 

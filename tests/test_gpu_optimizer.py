@@ -547,3 +547,16 @@ def test_adamw_values_with_the_negative_flag(dev):
     for bad in (steps, [steps]):
         with pytest.raises(ValueError):
             fl.adamw_step(p, g, m, v, bad, **HYPER)
+
+
+def test_adamw_refuses_values_without_memory(dev):
+    """A scale of zero that torch holds without memory is no missing scale."""
+    print("[case] adamw_step, values without memory", flush=True)
+    p, g, m, v = start32(dev, [10], torch.float32, 5)
+    before = p[0].clone()
+    zero = torch._efficientzerotensor((), device=dev)
+    step = torch.zeros(1, dtype=torch.long, device=dev)
+    for kw in (dict(grad_scale=zero), dict(lr=zero)):
+        with pytest.raises(ValueError):
+            fl.adamw_step(p, g, m, v, step, **{**HYPER, **kw})
+    assert torch.equal(p[0], before) and int(step) == 0
