@@ -32,7 +32,8 @@ def _ops(logits, tokens, top_tokens, temperature, ignore_index):
     inside = (at >= 0) & (at < logits.shape[-1])
     got = lp.gather(-1, torch.where(inside, at, 0)[..., None])[..., 0]
     # (a product with NaN, not a choice of it: the gradient of a token outside the vocabulary is NaN)
-    got = torch.where(kept & ~empty[..., 0], got * torch.where(inside, 1.0, float("nan")), 0.0)
+    factor = torch.where(inside | empty[..., 0], 1.0, float("nan"))
+    got = torch.where(kept & ~empty[..., 0], got * factor, 0.0)
     live = e > 0
     entropy = torch.log(total) - torch.where(live, e * torch.where(live, d, 0.0), 0.0).sum(-1, keepdim=True) / total
     tops = torch.where(empty, 0.0, lp.gather(-1, top_tokens)) if top_tokens is not None else None
@@ -40,14 +41,28 @@ def _ops(logits, tokens, top_tokens, temperature, ignore_index):
 
 
 def stock_gradient(logits, tokens, top_tokens, temperature, ignore_index, *grads) -> Optional[torch.Tensor]:
-    """The logits' gradient in stock ops, for a backward that must itself be differentiable."""
-    given = [(i, g) for i, g in enumerate(grads) if g is not None]
+    """The logits' gradient in stock ops, for a backward that must itself be differentiable. Its zeros are the kernel's:
+    a row whose gradients are all 0 passes nothing whatever its logits hold, and neither does a gradient of 0 for a token
+    outside the vocabulary."""
+    g, h, top = grads
+    quiet = torch.ones(tokens.shape, dtype=torch.bool, device=tokens.device)
+    if g is not None:
+        quiet = (g == 0) | (tokens == ignore_index)
+        tokens = torch.where(quiet & ((tokens < 0) | (tokens >= logits.shape[-1])), ignore_index, tokens)
+    if h is not None:
+        quiet = quiet & (h == 0)
+    if top is not None:
+        quiet = quiet & (top == 0).all(-1)
+    # Only rows with NaN or +inf are hidden (0 times those is no 0): the others' zeros come about, and stay a function
+    # of the gradients.
+    hidden = (quiet & ~(logits.detach().amax(-1) < float("inf")))[..., None]
+    given = [(i, o) for i, o in enumerate(grads) if o is not None]
 
     def fn(x):
-        outs = _ops(x, tokens, top_tokens, temperature, ignore_index)
+        outs = _ops(torch.where(hidden, 0.0, x), tokens, top_tokens, temperature, ignore_index)
         return tuple(outs[i] for i, _ in given)
 
-    return _stock_grads(fn, (logits,), tuple(g for _, g in given))[0]
+    return _stock_grads(fn, (logits,), tuple(o for _, o in given))[0]
 
 
 def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: float = 1.0, top_k: int = 0,

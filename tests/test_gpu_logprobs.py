@@ -594,3 +594,33 @@ def test_upstream_gradients_without_memory_are_refused(dev):
         r = fl.token_logprobs(z, t, entropy=entropy)
         with pytest.raises(TypeError):
             torch.autograd.grad(Hands.apply(r.entropy if entropy else r.logprobs).sum(), z)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_differentiable_gradients_of_special_rows(dev, dtype):
+    """A backward that can be differentiated again has the plain backward's zeros and NaN: rows that pass nothing, ignored
+    and outside tokens, rows of -inf, NaN and +inf."""
+    print(f"[case] token_logprobs differentiable gradients of special rows {dtype}", flush=True)
+    x = special_rows(dev, 300, dtype)
+    for turn, (token, use) in enumerate([(299, (1, 0, 0)), (-100, (1, 0, 0)), (300, (1, 0, 0)), (300, (1, 1, 1)),
+                                         (-100, (0, 1, 1)), (0, (1, 1, 1))]):
+        t = torch.full((18,), token, device=dev)
+        gen = torch.Generator(device=dev).manual_seed(turn)
+        ups = [torch.randn(*s, device=dev, generator=gen) for s in ((18,), (18,), (18, 5))]
+        for u in ups:
+            u[turn % 2::2] = 0.0
+        z = x.clone().requires_grad_()
+        r = fl.token_logprobs(z, t, top_k=5, entropy=True)
+        o, g = ([a for a, u in zip(l, use) if u] for l in ((r.logprobs, r.entropy, r.top_logprobs), ups))
+        exp, = torch.autograd.grad(o, z, g, retain_graph=True)
+        got, = torch.autograd.grad(o, z, g, create_graph=True)
+        got, weights = got.detach(), [u if w else None for u, w in zip(ups, use)]
+        if weights[0] is not None:
+            weights[0] = torch.where(t == -100, 0.0, weights[0])
+        quiet = torch.stack([(u.view(18, -1) == 0).all(-1) for u in weights if u is not None]).all(0)
+        for grad in (exp, got):
+            assert bool((grad[quiet] == 0).all()), (token, use)
+            assert bool((grad[1] == 0).all())  # -inf alone
+            if not bool(quiet.all()):
+                check_grad(x[~quiet], t[~quiet], 1.0, 5 * use[2], *(None if u is None else u[~quiet] for u in weights),
+                           grad[~quiet])

@@ -132,6 +132,44 @@ def test_stock_form_and_its_gradient():
     assert torch.autograd.grad(lp.sum() + ent.sum() + tops.sum(), empty)[0].abs().max() == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_stock_gradient_of_rows_that_pass_nothing(dtype):
+    """The kernel's zeros and NaN: rows that pass nothing whatever they hold, tokens outside with and without a gradient."""
+    g = torch.Generator().manual_seed(2)
+    nan, inf = float("nan"), float("inf")
+    x = torch.randn(10, 9, generator=g).to(dtype)
+    x[1], x[2, 4], x[3, 0], x[6], x[8], x[9] = nan, inf, nan, nan, -inf, -inf
+    t = torch.tensor([1, -100, 2, 3, 9, -1, -100, 40, 9, -100])
+    up = torch.tensor([1.0, 2.0, 0.0, -0.0, 0.0, 0.5, 1.0, 0.0, 1.0, 1.0])
+    x.requires_grad_()
+    got = L.stock_gradient(x, t, None, 0.8, -100, up, None, None).detach()
+    assert got.dtype == dtype and bool(got[5].isnan().all()) and bool(got[0].isfinite().all()) and float(got[0].abs().max()) > 0
+    assert all(float(got[i].abs().max()) == 0.0 for i in (1, 2, 3, 4, 6, 7, 8, 9))
+    h = torch.zeros(10)
+    h[6] = h[7] = 1.0  # an ignored and an outside token's row passes its entropy
+    got = L.stock_gradient(x, t, None, 0.8, -100, up, h, None).detach()
+    assert bool(got[6].isnan().all()) and bool(got[7].isfinite().all()) and float(got[7].abs().max()) > 0
+    top = torch.topk(x.detach().float().nan_to_num(0.0), 2).indices
+    gt = torch.zeros(10, 2)
+    gt[0, 1] = gt[2, 0] = 1.0
+    got = L.stock_gradient(x, t, top, 0.8, -100, None, None, gt).detach()
+    assert bool(got[2].isnan().all()) and float(got[[1, 3, 4, 5, 6, 7, 8, 9]].abs().max()) == 0.0
+    assert float(L.stock_gradient(x, t, top, 0.8, -100, 0 * up, 0 * h, 0 * gt).abs().max()) == 0.0
+
+
+def test_stock_gradient_can_be_differentiated_by_a_gradient_of_zero():
+    """A product with the Jacobian by two backward passes: the first one's upstream gradient is zero everywhere."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(4, 9, generator=g).requires_grad_()
+    t = torch.tensor([2, 5, -100, 0])
+    up, v = torch.zeros(4, requires_grad=True), torch.randn(4, 9, generator=g)
+    got, = torch.autograd.grad(L.stock_gradient(x, t, None, 0.7, -100, up, None, None), up, v)
+    p = torch.softmax(x.detach().double() / 0.7, -1)
+    exp = (v.double().gather(-1, t.clamp_min(0)[:, None])[:, 0] - (p * v).sum(-1)) / 0.7
+    # sums of nine products below 4: 40 roundings of 2^-24
+    assert float((got.double() - torch.where(t == -100, 0.0, exp)).abs().max()) <= 40 * 4 * 2 ** -24
+
+
 def test_c_abi_token_logprobs_refusals():
     lib = nat.load()
 
