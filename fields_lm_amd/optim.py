@@ -139,13 +139,26 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def load_state_dict(self, state_dict) -> None:
-        """As the base class, but every state keeps the type it was saved in."""
-        super().load_state_dict(state_dict)
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(saved, (p for g in self.param_groups for p in g["params"])):
-            if i in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+        """As the base class, hooks included, but every state keeps the type it was saved in."""
+        loaded: dict = {}
+
+        def last(_, final) -> None:  # behind the other pre-hooks: what the base class is about to load
+            loaded.update(final)
+
+        def first(_) -> None:  # ahead of the other post-hooks: the base class has cast states to their parameters' type
+            ids = [i for g in loaded["param_groups"] for i in g["params"]]
+            for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
+                if i in loaded["state"]:
+                    self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
+                                     for k, v in loaded["state"][i].items()}
+
+        hooks = (self.register_load_state_dict_pre_hook(last),
+                 self.register_load_state_dict_post_hook(first, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
 
     @torch.no_grad()
     def step(self, closure=None):

@@ -294,3 +294,41 @@ def test_optimizer_state_keeps_its_types_through_a_checkpoint(tmp_path):
             u = new.state[w][k]
             assert u.dtype == t.dtype and u.shape == t.shape and u.data_ptr() != t.data_ptr()
             assert torch.equal(u.float(), t.float())
+
+
+def _with_state(ws, bits, step=7):
+    """An optimizer whose states are as after some steps, without a device."""
+    opt = fl.AdamW(ws, state_bits=bits)
+    code = torch.float8_e4m3fn if bits == 8 else torch.float32
+    for w in ws:
+        opt.state[w] = dict(step=torch.tensor(step), exp_avg=torch.randn(w.shape).to(code), exp_avg_sq=torch.rand(w.shape).to(code))
+        if bits == 8:
+            opt.state[w].update({k: torch.rand(-(-w.numel() // 256)) for k in ("exp_avg_scale", "exp_avg_sq_scale")})
+    return opt
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_optimizer_loads_through_its_hooks(bits):
+    """What pre-hooks return and what post-hooks write is what the optimizer holds; types are kept all the same."""
+    ws = [torch.nn.Parameter(torch.zeros(300, dtype=torch.bfloat16)), torch.nn.Parameter(torch.zeros(4, dtype=torch.bfloat16))]
+    saved = _with_state(ws, bits).state_dict()
+    new, seen = fl.AdamW(ws), []
+
+    def replace(opt, d):
+        state = {i: {**s, "step": torch.tensor(40 + i)} for i, s in d["state"].items()}
+        return {**d, "state": state, "param_groups": [{**g, "lr": 0.5} for g in d["param_groups"]]}
+
+    def look(opt):
+        seen.append([int(opt.state[w]["step"]) for w in ws])
+        opt.state[ws[1]]["step"] = torch.tensor(99)
+
+    new.register_load_state_dict_pre_hook(replace)
+    new.register_load_state_dict_post_hook(look, prepend=True)
+    for _ in range(2):  # the hooks stay those that were registered
+        new.load_state_dict(saved)
+    assert seen == [[40, 41]] * 2 and new.param_groups[0]["lr"] == 0.5
+    assert int(new.state[ws[0]]["step"]) == 40 and int(new.state[ws[1]]["step"]) == 99
+    for i, w in enumerate(ws):
+        assert {k: t.dtype for k, t in new.state[w].items()} == {k: t.dtype for k, t in saved["state"][i].items()}
+        assert all(torch.equal(new.state[w][k].float(), t.float()) for k, t in saved["state"][i].items() if k != "step")
+    assert int(saved["state"][0]["step"]) == 7
