@@ -22,6 +22,7 @@ STATE_BLOCK = 256                   # values that share a scale in the 8-bit sta
 STATE8_DTYPE = torch.float8_e4m3fn  # their codes
 
 _TYPES = (torch.float32, torch.bfloat16)
+_GROUP = ("lr", "betas", "eps", "weight_decay", "state_bits")  # what a step reads of its group
 _STATES = {32: itemgetter("step", "exp_avg", "exp_avg_sq"),
            8: itemgetter("step", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 
@@ -54,6 +55,25 @@ def _check_hyper(lr, betas, eps, weight_decay) -> None:
         raise ValueError(f"eps must be finite and 0 or more, got {eps}")
     if not (float(weight_decay) >= 0.0 and math.isfinite(weight_decay)):
         raise ValueError(f"weight_decay must be finite and 0 or more, got {weight_decay}")
+
+
+def _check_group(group: dict) -> None:
+    _check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
+    if group["state_bits"] not in (8, 32):
+        raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+
+
+def _check_state(state: dict, p: torch.Tensor, bits: int) -> None:
+    """A saved state of ``p`` is one that a step can go on from."""
+    n, blocks, code = p.numel(), -(-p.numel() // STATE_BLOCK), torch.float32 if bits == 32 else STATE8_DTYPE
+    wanted = dict(step=(torch.int64, 1), exp_avg=(code, n), exp_avg_sq=(code, n))
+    if bits == 8:
+        wanted.update(exp_avg_scale=(torch.float32, blocks), exp_avg_sq_scale=(torch.float32, blocks))
+    for name, (dtype, count) in wanted.items():
+        t = state.get(name)
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() != count:
+            got = f"{t.numel()} of {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
+            raise ValueError(f"{name} of a parameter of {n} values must be {count} of {dtype} ({bits}-bit states), got {got}")
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor],
@@ -112,9 +132,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         group = self.param_groups[-1]
         try:
-            _check_hyper(group["lr"], group["betas"], group["eps"], group["weight_decay"])
-            if group["state_bits"] not in (8, 32):
-                raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+            _check_group(group)
             for p in group["params"]:
                 if p.dtype not in _TYPES:
                     raise TypeError(f"parameters must be float32 or bfloat16, got {p.dtype}")
@@ -139,10 +157,18 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def load_state_dict(self, state_dict) -> None:
-        """As the base class, hooks included, but every state keeps the type it was saved in."""
+        """As the base class, hooks included, but every state keeps the type it was saved in. What no step can go on from
+        (another optimizer's checkpoint, states of other types or sizes) is refused before anything is changed."""
         loaded: dict = {}
 
         def last(_, final) -> None:  # behind the other pre-hooks: what the base class is about to load
+            for group, own in zip(final["param_groups"], self.param_groups):
+                if missing := [k for k in _GROUP if k not in group]:
+                    raise ValueError(f"no checkpoint of this optimizer: a group lacks {', '.join(missing)}")
+                _check_group(group)
+                for i, p in zip(group["params"], own["params"]):
+                    if final["state"].get(i):
+                        _check_state(final["state"][i], p, group["state_bits"])
             loaded.update(final)
 
         def first(_) -> None:  # ahead of the other post-hooks: the base class has cast states to their parameters' type

@@ -154,7 +154,8 @@ def test_stock_gradient_of_rows_that_pass_nothing(dtype):
     gt[0, 1] = gt[2, 0] = 1.0
     got = L.stock_gradient(x, t, top, 0.8, -100, None, None, gt).detach()
     assert bool(got[2].isnan().all()) and float(got[[1, 3, 4, 5, 6, 7, 8, 9]].abs().max()) == 0.0
-    assert float(L.stock_gradient(x, t, top, 0.8, -100, 0 * up, 0 * h, 0 * gt).abs().max()) == 0.0
+    got = L.stock_gradient(x, t, top, 0.8, -100, 0 * up, 0 * h, 0 * gt).detach()
+    assert float(got.abs().max()) == 0.0
 
 
 def test_stock_gradient_can_be_differentiated_by_a_gradient_of_zero():
@@ -332,3 +333,39 @@ def test_optimizer_loads_through_its_hooks(bits):
         assert {k: t.dtype for k, t in new.state[w].items()} == {k: t.dtype for k, t in saved["state"][i].items()}
         assert all(torch.equal(new.state[w][k].float(), t.float()) for k, t in saved["state"][i].items() if k != "step")
     assert int(saved["state"][0]["step"]) == 7
+
+
+def test_optimizer_refuses_checkpoints_it_cannot_go_on_from():
+    """Another optimizer's, and states of other types, sizes and kinds: refused at once, with nothing changed."""
+    ws = [torch.nn.Parameter(torch.zeros(300)), torch.nn.Parameter(torch.zeros(4))]
+    stock = torch.optim.AdamW(ws)
+    for w in ws:
+        w.grad = torch.ones_like(w)
+    stock.step()
+    good = {bits: _with_state(ws, bits).state_dict() for bits in (8, 32)}
+    own = _with_state(ws, 32, step=3)
+    before = own.state_dict()
+
+    def changed(bits, name, value):
+        d = good[bits]
+        return {**d, "state": {**d["state"], 1: {k: v for k, v in {**d["state"][1], name: value}.items() if v is not None}}}
+
+    def regrouped(**kw):
+        return {**good[32], "param_groups": [{**g, **kw} for g in good[32]["param_groups"]]}
+
+    bad = [stock.state_dict(), regrouped(state_bits=8), regrouped(state_bits=16), regrouped(lr=-1.0), regrouped(eps=float("nan")),
+           changed(32, "step", torch.tensor(7.0)), changed(32, "step", 7), changed(32, "exp_avg", None),
+           changed(32, "exp_avg_sq", torch.zeros(5)), changed(32, "exp_avg", torch.zeros(4, dtype=torch.bfloat16)),
+           changed(8, "exp_avg_scale", None), changed(8, "exp_avg_sq_scale", torch.zeros(2)),
+           changed(8, "exp_avg", torch.zeros(4)), {**good[32], "param_groups": []}]
+    for d in bad:
+        with pytest.raises(ValueError):
+            own.load_state_dict(d)
+        after = own.state_dict()
+        assert after["param_groups"] == before["param_groups"]
+        assert all(after["state"][i][k] is t for i, s in before["state"].items() for k, t in s.items())
+    for bits in (8, 32):
+        own.load_state_dict(good[bits])
+        assert own.param_groups[0]["state_bits"] == bits and int(own.state[ws[1]]["step"]) == 7
+    own.load_state_dict({**good[32], "state": {0: good[32]["state"][0], 1: {}}})  # one that has not stepped yet
+    assert int(own.state[ws[0]]["step"]) == 7 and not own.state[ws[1]]
