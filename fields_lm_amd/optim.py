@@ -128,6 +128,10 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: Optional[torch.Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
+    def __getstate__(self) -> dict:
+        """What copies and pickles hold: the base class's, and the clip."""
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "grad_norm": self.grad_norm}
+
     def add_param_group(self, param_group) -> None:
         super().add_param_group(param_group)
         group = self.param_groups[-1]

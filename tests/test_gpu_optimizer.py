@@ -9,6 +9,7 @@ operation up to them is correctly rounded on both sides and they come in one ord
 """
 from __future__ import annotations
 
+import copy
 import math
 
 import numpy as np
@@ -560,3 +561,21 @@ def test_adamw_refuses_values_without_memory(dev):
         with pytest.raises(ValueError):
             fl.adamw_step(p, g, m, v, step, **{**HYPER, **kw})
     assert torch.equal(p[0], before) and int(step) == 0
+
+
+def test_optimizer_copy_steps_as_its_original(dev):
+    print("[case] AdamW, a deep copy", flush=True)
+    own, _ = stock_pair(dev)
+    a = fl.AdamW(own.parameters(), state_bits=8, max_grad_norm=0.1, lr=1e-2)
+
+    def step(model, opt, seed):
+        for i, p in enumerate(model.parameters()):
+            p.grad = torch.randn(p.shape, device=dev, generator=torch.Generator(device=dev).manual_seed(seed + i))
+        opt.step()
+
+    step(own, a, 0)
+    other, b = copy.deepcopy((own, a))
+    for model, opt in ((own, a), (other, b)):
+        step(model, opt, 10)
+    assert torch.equal(a.grad_norm, b.grad_norm)
+    assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters()))

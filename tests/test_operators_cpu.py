@@ -4,7 +4,9 @@ differentiable backward runs.
 """
 from __future__ import annotations
 
+import copy
 import ctypes
+import pickle
 
 import pytest
 import torch
@@ -369,3 +371,12 @@ def test_optimizer_refuses_checkpoints_it_cannot_go_on_from():
         assert own.param_groups[0]["state_bits"] == bits and int(own.state[ws[1]]["step"]) == 7
     own.load_state_dict({**good[32], "state": {0: good[32]["state"][0], 1: {}}})  # one that has not stepped yet
     assert int(own.state[ws[0]]["step"]) == 7 and not own.state[ws[1]]
+
+
+def test_optimizer_copies_keep_the_clip():
+    ws = [torch.nn.Parameter(torch.zeros(3))]
+    for most in (None, 0.5):
+        opt = fl.AdamW(ws, max_grad_norm=most)
+        for new in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+            assert new.max_grad_norm == most and new.grad_norm is None and new.step() is None
+            assert new.param_groups[0]["state_bits"] == 32
