@@ -161,7 +161,8 @@ class AdamW(torch.optim.Optimizer):
         return st
 
     def load_state_dict(self, state_dict) -> None:
-        """As the base class, hooks included, but every state keeps the type it was saved in. What no step can go on from
+        """As the base class, hooks included, but every state keeps the type it was saved in, and a learning rate held in
+        a tensor comes to the parameters' device, as states do. What no step can go on from
         (another optimizer's checkpoint, states of other types or sizes) is refused before anything is changed."""
         loaded: dict = {}
 
@@ -176,6 +177,9 @@ class AdamW(torch.optim.Optimizer):
             loaded.update(final)
 
         def first(_) -> None:  # ahead of the other post-hooks: the base class has cast states to their parameters' type
+            for group in self.param_groups:
+                if isinstance(group["lr"], torch.Tensor) and group["params"]:
+                    group["lr"] = group["lr"].to(group["params"][0].device)
             ids = [i for g in loaded["param_groups"] for i in g["params"]]
             for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
                 if i in loaded["state"]:

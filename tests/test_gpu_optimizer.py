@@ -579,3 +579,26 @@ def test_optimizer_copy_steps_as_its_original(dev):
         step(model, opt, 10)
     assert torch.equal(a.grad_norm, b.grad_norm)
     assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters()))
+
+
+def test_optimizer_continues_from_a_checkpoint_read_on_the_host(dev, tmp_path):
+    """As a program resumes: saved, read with its tensors on the host, loaded; the learning rate lies on the device."""
+    print("[case] AdamW checkpoint by way of the host", flush=True)
+    own, other = stock_pair(dev)
+    kw = dict(state_bits=8, max_grad_norm=1.0)
+    a = fl.AdamW(own.parameters(), lr=torch.tensor(1e-2, device=dev), **kw)
+    grads = [[torch.randn_like(p) for p in own.parameters()] for _ in range(2)]
+
+    def take(model, opt, gs):
+        for p, g in zip(model.parameters(), gs):
+            p.grad = g.clone()
+        opt.step()
+
+    take(own, a, grads[0])
+    torch.save(a.state_dict(), tmp_path / "opt.pt")
+    other.load_state_dict(own.state_dict())
+    b = fl.AdamW(other.parameters(), lr=torch.tensor(1.0, device=dev), **kw)
+    b.load_state_dict(torch.load(tmp_path / "opt.pt", map_location="cpu", weights_only=True))
+    for model, opt in ((own, a), (other, b)):
+        take(model, opt, grads[1])
+    assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters()))

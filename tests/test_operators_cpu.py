@@ -380,3 +380,18 @@ def test_optimizer_copies_keep_the_clip():
         for new in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
             assert new.max_grad_norm == most and new.grad_norm is None and new.step() is None
             assert new.param_groups[0]["state_bits"] == 32
+
+
+def test_optimizer_loads_a_learning_rate_onto_the_parameters_device():
+    """A checkpoint read on the host, as most are: its tensors come to the parameters' device."""
+    ws = [torch.nn.Parameter(torch.zeros(3))]
+    saved = _with_state(ws, 32).state_dict()
+    for g in saved["param_groups"]:
+        g["lr"] = torch.tensor(0.25)
+    new = fl.AdamW([torch.nn.Parameter(torch.zeros(3, device="meta"))])
+    new.load_state_dict(saved)
+    p, = new.param_groups[0]["params"]
+    assert {t.device.type for t in (new.param_groups[0]["lr"], *new.state[p].values())} == {"meta"}
+    here = fl.AdamW(ws)
+    here.load_state_dict(saved)
+    assert float(here.param_groups[0]["lr"]) == 0.25 and here.param_groups[0]["lr"] is not saved["param_groups"][0]["lr"]
