@@ -504,6 +504,17 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+// Tensors (one, a list or tuple, or None) that were written in place: what autograd saved of them is stale.
+void count_writes(PyObject* o) {
+  const auto count = [](PyObject* item) {
+    const Tensor& t = THPVariable_Unpack(item);
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  if (o == Py_None) return;
+  if (THPVariable_Check(o)) return count(o);
+  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); ++i) count(PySequence_Fast_ITEMS(o)[i]);
+}
+
 // adamw_step(parameters, gradients, first moments, second moments, steps (a list or one tensor), lr (a number or a
 // tensor), beta1, beta2, eps, weight decay, gradient scale or None, the moments' scales or None twice)
 PyObject* adamw_step(PyObject*, PyObject* args) {
@@ -582,10 +593,7 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
                    reinterpret_cast<int64_t* const*>(step_at.data()), lr_value, address<float>(lr_at), beta1, beta2, eps, decay,
                    address<float>(scale), address<void>(ws), bytes, stream_of(first)),
         "fl_adamw_step");
-  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(params); ++i) {  // written in place: saved parameters are stale
-    const Tensor& t = THPVariable_Unpack(PySequence_Fast_ITEMS(params)[i]);
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  }
+  for (PyObject* list : {params, avgs, sqs, steps, avg_scales, sq_scales}) count_writes(list);
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }

@@ -602,3 +602,24 @@ def test_optimizer_continues_from_a_checkpoint_read_on_the_host(dev, tmp_path):
     for model, opt in ((own, a), (other, b)):
         take(model, opt, grads[1])
     assert all(torch.equal(p, q) for p, q in zip(own.parameters(), other.parameters()))
+
+
+def test_adamw_counts_as_a_write_of_states_and_counters(dev):
+    """A product that saved a moment, a scale or a step counter does not take the stepped one for it in its backward."""
+    print("[case] adamw_step, versions of states", flush=True)
+    for eight in (False, True):
+        for listed in (False, True):
+            p, g, m, v = start32(dev, [300], torch.float32, 5)
+            scales = [torch.ones(2, device=dev) for _ in range(2)] if eight else []
+            if eight:
+                m, v = ([t.to(STATE8_DTYPE) for t in l] for l in (m, v))
+            step = torch.zeros(1, dtype=torch.long, device=dev)
+            w = torch.ones((), device=dev, requires_grad=True)
+            sums = [(w * t).sum() for t in (*([] if eight else [m[0], v[0]]), step, *scales)]
+            before = [t._version for t in (p[0], m[0], v[0])]
+            fl.adamw_step(p, g, m, v, [step] if listed else step, **HYPER,
+                          **(dict(exp_avg_scales=scales[:1], exp_avg_sq_scales=scales[1:]) if eight else {}))
+            assert all(t._version > n for t, n in zip((p[0], m[0], v[0]), before))
+            for y in sums:
+                with pytest.raises(RuntimeError):
+                    y.backward()
