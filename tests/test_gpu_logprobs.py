@@ -624,3 +624,100 @@ def test_differentiable_gradients_of_special_rows(dev, dtype):
             if not bool(quiet.all()):
                 check_grad(x[~quiet], t[~quiet], 1.0, 5 * use[2], *(None if u is None else u[~quiet] for u in weights),
                            grad[~quiet])
+
+
+def flat_bounds(x, big, temperature=1.0):
+    """(ln s, entropy) tolerances of rows whose additions are counted one by one: up to 8 packs and one logit to a
+    thread (at most 65), 6 in a wave, 3 between waves, and where segments are joined 6 and 16 more: 96 with the
+    roundings of each segment's ln and of its shift (three of at most 40 each in base 2, 120 u) beside."""
+    e = (4 * big + 96 + 120 + 8) * U
+    logs = e + 2 * U * (big + 16)  # |ln s| <= ln 2^23 < 16
+    return logs, (2 + 2 * big) * e + 4 * U * big + logs
+
+
+def test_sums_of_the_longest_row(dev):
+    """2^23 logits in 1,024 segments, each of which weighs: all equal, a small spread, and all the weight in one
+    segment, early, late or last. A lost segment of equal logits would move ln s by 2^-10."""
+    print("[case] token_logprobs, sums of V=2^23", flush=True)
+    vocab, seg = 1 << 23, 8192
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.zeros(6, vocab, device=dev)
+    x[1] = 0.1 * torch.randn(vocab, device=dev, generator=g)
+    for row, at in ((2, 3), (3, 130), (4, 700), (5, 1023)):
+        x[row, at * seg:(at + 1) * seg] = 20.0 + 0.01 * torch.randn(seg, device=dev, generator=g)
+    t = torch.tensor([5, vocab - 1, 3 * seg + 1, 130 * seg + 7, 0, vocab - 2], device=dev)
+    r = fl.token_logprobs(x, t, entropy=True, top_k=3)
+    _, lp, h, top, idx, _ = plain(x, t, 1.0, 3)
+    big = torch.tensor([0.0, 1.2, 20.1, 20.1, 20.1, 20.1], dtype=torch.float64)  # (outside the heavy segment too)
+    logs, ent = flat_bounds(x, big)
+    assert float(logs.max()) < 3e-5  # far below what a segment weighs
+    check(r.logprobs, lp, logs + 4 * U * big, "logprobs")
+    check(r.entropy, h, ent, "entropy")
+    assert torch.equal(r.top_tokens.cpu(), idx)
+    check(r.top_logprobs, top, (logs + 4 * U * big)[:, None], "top_logprobs")
+
+
+@pytest.mark.parametrize("dtype,vocab,k", [(torch.float32, 9, 3), (torch.bfloat16, 600, 20), (torch.float32, 1025, 5),
+                                           (torch.float32, 1030, 40), (torch.bfloat16, 8200, 20), (torch.float32, 8193, 5),
+                                           (torch.float32, 8199, 64)])
+def test_rows_past_one_launch(dev, dtype, vocab, k):
+    """More than 2^20 rows, so that blocks take a second one: overlapping windows of one long tensor, against the same
+    rows in calls that hold them at once, bit for bit, and some of them in 64 bits."""
+    print(f"[case] token_logprobs, 2^20 + 9 rows of {vocab} {dtype}", flush=True)
+    rows, half = (1 << 20) + 9, 1 << 19
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    line = (torch.randn(rows + vocab, device=dev, generator=g) * 3).to(dtype)
+    line[half:half + 2 * vocab] = float("-inf")  # windows of -inf alone, and few logits left beside
+    line[rows - 3 - vocab // 2] = float("nan")   # the last rows, that their blocks' first rows are far from
+    x = line.as_strided((rows, vocab), (1, 1))
+    t = torch.randint(0, vocab, (rows,), device=dev, generator=g)
+    t[::7] = -100
+    outs = fl.token_logprobs(x, t, top_k=k, entropy=True)
+    parts = [fl.token_logprobs(x[lo:hi], t[lo:hi], top_k=k, entropy=True)
+             for lo, hi in ((0, half), (half, 2 * half), (2 * half, rows))]
+    for a, *b in zip(outs, *parts):
+        assert torch.equal(a.view(torch.int32), torch.cat(b).view(torch.int32))
+    at = torch.tensor([0, 1, 8, half - 1, 2 * half - 1, 2 * half, 2 * half + 1, rows - 1], device=dev)
+    check_forward(x[at], t[at], 1.0, k, True, fl.TokenLogprobs(*(o[at] for o in outs)))
+
+
+@pytest.mark.parametrize("dtype,vocab", [(torch.float32, 9), (torch.bfloat16, 600), (torch.float32, 1030)])
+def test_gradients_of_rows_past_one_launch(dev, dtype, vocab):
+    print(f"[case] token_logprobs gradients, 2^20 + 9 rows of {vocab} {dtype}", flush=True)
+    rows, half = (1 << 20) + 9, 1 << 19
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    x = (torch.randn(rows + vocab, device=dev, generator=g) * 3).to(dtype).as_strided((rows, vocab), (1, 1))
+    t = torch.randint(0, vocab, (rows,), device=dev, generator=g)
+    t[::7] = -100
+    ups = [torch.randn(*s, device=dev, generator=g) for s in ((rows,), (rows,), (rows, 3))]
+
+    def grad(lo, hi):
+        z = x[lo:hi].detach().requires_grad_()
+        r = fl.token_logprobs(z, t[lo:hi], top_k=3, entropy=True)
+        return torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], z, [u[lo:hi] for u in ups])[0]
+
+    whole = grad(0, rows)
+    for lo, hi in ((0, half), (half, 2 * half), (2 * half, rows)):
+        assert torch.equal(whole[lo:hi], grad(lo, hi)), lo
+    at = torch.tensor([0, 1, 8, 2 * half - 1, 2 * half, 2 * half + 1, rows - 1], device=dev)
+    check_grad(x[at], t[at], 1.0, 3, *(u[at] for u in ups), whole[at])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [3, 300, 8193])
+def test_gradients_of_alternatives_of_special_rows(dev, vocab, dtype):
+    """Masked alternatives, ties, fewer logits left than alternatives, with tokens among the alternatives and ignored."""
+    print(f"[case] token_logprobs gradients of special rows' alternatives V={vocab} {dtype}", flush=True)
+    x = special_rows(dev, vocab, dtype)
+    for k in sorted({min(vocab, n) for n in (1, 5, 64)}):
+        gen = torch.Generator(device=dev).manual_seed(k)
+        g, h, gt = (torch.randn(*s, device=dev, generator=gen) for s in ((18,), (18,), (18, k)))
+        for token in (0, vocab - 1, -100):
+            t = torch.full((18,), token, device=dev)
+            for use in ((0, 0, 1), (1, 1, 1)):
+                z = x.clone().requires_grad_()
+                r = fl.token_logprobs(z, t, top_k=k, entropy=True)
+                outs, ups = ([a for a, u in zip(l, use) if u]
+                             for l in ((r.logprobs, r.entropy, r.top_logprobs), (g, h, gt)))
+                got, = torch.autograd.grad(outs, z, ups)
+                check_grad(x, t, 1.0, k, *(o if u else None for o, u in zip((g, h, gt), use)), got)

@@ -623,3 +623,39 @@ def test_adamw_counts_as_a_write_of_states_and_counters(dev):
             for y in sums:
                 with pytest.raises(RuntimeError):
                     y.backward()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_adamw_8_bit_moments_are_the_formulas(dev, dtype):
+    """Code times scale against the moments in 64 bits, step by step from the held ones: a first moment is off by half a
+    step of e4m3 (2^-4 of itself, or half of the smallest code, 2^-10 of a block's largest over 448), a root by as much
+    or raised to the smallest code, both by their roundings before (16 u)."""
+    print(f"[case] adamw_step 8 bits, moments in 64 bits {dtype}", flush=True)
+    n, (b1, b2) = 5000, HYPER["betas"]
+    gen = torch.Generator(device=dev).manual_seed(7)
+    p = torch.randn(n, device=dev, generator=gen).to(dtype)
+    mc, vc = (torch.zeros(n, device=dev).to(STATE8_DTYPE) for _ in range(2))
+    ms, vs = (torch.zeros(-(-n // 256), device=dev) for _ in range(2))
+    steps = torch.zeros(1, dtype=torch.long, device=dev)
+
+    def held(code, scale):
+        return code.double() * scale.double().repeat_interleave(256)[:n]
+
+    def largest(x):
+        full = torch.zeros(ms.numel() * 256, device=dev, dtype=torch.float64)
+        full[:n] = x.abs()
+        return full.view(-1, 256).amax(1).repeat_interleave(256)[:n]
+
+    for turn in range(4):
+        g = (torch.randn(n, device=dev, generator=gen) * torch.exp(2 * torch.randn(n, device=dev, generator=gen))).to(dtype)
+        parts = b1 * held(mc, ms), (1 - b1) * g.double()
+        m = parts[0] + parts[1]
+        root = (b2 * held(vc, vs) ** 2 + (1 - b2) * g.double() ** 2).sqrt()
+        fl.adamw_step([p], [g], [mc], [vc], steps, exp_avg_scales=[ms], exp_avg_sq_scales=[vs], **HYPER)
+        low = 2.0 ** -10 / 448 * largest(m)
+        off = (held(mc, ms) - m).abs()
+        assert bool((off <= 2.0 ** -4 * m.abs() + low + 16 * U * (parts[0].abs() + parts[1].abs() + largest(m))).all()), turn
+        small = 2.0 ** -9 / 448 * largest(root)  # a root that is not 0 keeps at least this
+        off = (held(vc, vs) - root).abs()
+        assert bool((off <= torch.maximum(2.0 ** -4 * root + small / 2, small - root) + 16 * U * largest(root)).all()), turn
+        assert bool((held(vc, vs)[root > 0] > 0).all())
