@@ -721,3 +721,19 @@ def test_gradients_of_alternatives_of_special_rows(dev, vocab, dtype):
                              for l in ((r.logprobs, r.entropy, r.top_logprobs), (g, h, gt)))
                 got, = torch.autograd.grad(outs, z, ups)
                 check_grad(x, t, 1.0, k, *(o if u else None for o, u in zip((g, h, gt), use)), got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("vocab", [300, 8193, 70001])
+def test_alternatives_around_the_groups_that_bound_them(dev, vocab, dtype):
+    """The largest number of alternatives that 64 groups bound, and one more: special rows, ordinary ones, and logits
+    that lie in a few groups alone."""
+    print(f"[case] 32 and 33 alternatives V={vocab} {dtype}", flush=True)
+    g = torch.Generator(device=dev).manual_seed(vocab)
+    x = torch.cat((special_rows(dev, vocab, dtype), (torch.randn(6, vocab, device=dev, generator=g) * 3).to(dtype)))
+    x[20, :200] += 40
+    x[21, torch.arange(vocab, device=dev) % 64 < 31] += 40
+    x[22, torch.arange(vocab, device=dev) // 8 % 64 < 32] += 40
+    t = torch.randint(0, vocab, (24,), device=dev, generator=g)
+    for k in (32, 33):
+        check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
