@@ -90,10 +90,10 @@ __device__ __forceinline__ uint64_t key_max(uint64_t v) {
 }
 
 constexpr int kCand = 512;    // candidates for the alternatives that a block ranks
-// Alternatives up to which 64 groups bound them, all 256 threads' maxima above: fewer ballots against more candidates (of
-// normal logits about 25 for 20, 45 for 32, 65 for 40, 300 for 64). 8,188 rows of 16,384 bf16 with entropy take 55 us
-// with 5 and 60 by 256 groups, 61 and 64 with 20, 66 and 67 with 32, 70 and 69 with 40, 75 and 71 with 48, 378 and 77
-// with 64; 999 rows of 32,001 fp32 and 64 of 16,384 cross between 32 and 40 as well.
+// Alternatives up to which 64 groups bound them, all 256 threads' maxima above: fewer ballots against more
+// candidates (of normal logits about 25 for 20, 45 for 32, 65 for 40, 300 for 64). 8,188 rows of 16,384 bf16 with
+// entropy take 55 us with 5 and 60 by 256 groups, 61 and 64 with 20, 66 and 67 with 32, 70 and 69 with 40, 75 and 71
+// with 48, 378 and 77 with 64; 999 rows of 32,001 fp32 and 64 of 16,384 cross between 32 and 40 as well.
 constexpr int kFewTop = 32;
 constexpr float kPlainScale = 1048576.0f;  // below this |m| c, x c - fl(m c) is as good as (x - m) c
 
@@ -109,6 +109,7 @@ struct RowStats {
     log2_s = __builtin_amdgcn_logf(sum);
   }
   __device__ __forceinline__ float log_sum() const { return log2_s * kLn2; }
+  // (a product with the rounded 1 / T: up to 2^-24 |d| more than a quotient is off by, as every d of the sum has)
   __device__ __forceinline__ float logprob(float x) const {
     return empty ? -INFINITY : (x - m) * inv_t - log2_s * kLn2;
   }
@@ -140,9 +141,9 @@ __device__ __forceinline__ void write_row(const Outputs& out, int64_t row, const
 // to a thread, for the maximum, the sums and the alternatives, so that memory is read once. With the segment's maximum
 // known, e^d is one fused product and one power (x c - m c, c = log2(e) / T; the rounding error of m c is put back
 // into the log at the end), and no sum is ever rescaled. The memory bounds it where rows are many: 8,192 rows of
-// 16,384 bf16 take 41 us (6.5 TB/s; a streaming read reaches 7.0), 29 of which their vector instructions fill too (5.5
+// 16,384 bf16 take 42 us (6.4 TB/s; a streaming read reaches 7.0), 29 of which their vector instructions fill too (5.5
 // a logit, 7.5 with entropy, of four cycles each and eight for the power). With entropy and 20 alternatives they take
-// 60, of which the instructions fill 48 and the memory 39. One row of 131,072 is two launches and 13 us.
+// 61, of which the instructions fill 48 and the memory 39. One row of 131,072 is two launches and 12 us.
 //
 // Alternatives: the threads' maxima (in 64 groups where K is small) give a value that at least K logits reach: their
 // K-th largest, to 16 bits. Only logits from there up are candidates, little more than K of them in text; they are
@@ -176,7 +177,7 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
     }
     const T* row_x = logits + logit_at;
     const T* x = row_x + lo;
-    // packs from the first 16-byte border on (8,192 rows of 16,383 bf16 logits: 58 us from the row's start)
+    // packs from the first 16-byte border on (8,192 rows of 16,383 bf16 logits: 43 us, and 58 from the row's start)
     const int ahead = (int)(-(uintptr_t)x % 16 / sizeof(T)), head = ahead < len ? ahead : len;
     const int packs = (len - head) / N, tail = head + packs * N;
     float xt = 0.f;
@@ -200,8 +201,8 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         if (j < packs) v[i] = get(place(i));
       }
     };
-    // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 45 us, and 51 through
-    // them; where one follows the pair takes 147 us so, and 137 through them).
+    // Logits that no backward will read again pass the caches by (8,192 rows of 16,384 bf16: 42 us, and 48 through
+    // them; where one follows the pair with entropy takes 141 us so, and 133 through them).
     if (out.stats) load([](const u32x4* p) { return *p; });
     else load([](const u32x4* p) { return __builtin_nontemporal_load(p); });
     // the logits ahead of the first pack and behind the last, one to a thread (fewer than 8 each), len for none
@@ -402,8 +403,8 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_kernel(
         if (wave == 0) {
           const uint64_t key = lane < n ? key_at(lane) : 0;
           int rank = 0;
-          // (keys broadcast by the LDS: half the vector instructions of reading them from lanes, 64 us against 68 for
-          // 8,188 rows of 16,384 with 20 alternatives)
+          // (keys broadcast by the LDS: half the vector instructions of reading them from lanes, 61.6 us against 63.3
+          // for 8,188 rows of 16,384 bf16 with entropy and 20 alternatives)
           s_cand[lane] = key;
           __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 4
@@ -552,9 +553,9 @@ __global__ __launch_bounds__(THREADS) void fl_token_logprobs_join_kernel(
 //   dx = -(p / T) (g + sum g_k + h (ln p + H))
 // two more operations, one without h. A row whose gradients are all 0 gets zeros whatever its logits hold.
 // Bound by the memory: 8,192 rows of 16,384 bf16 take 92 us (5.8 TB/s of reads and writes; a streaming copy reaches
-// 5.9), 999 of 32,001 fp32 with entropy and 8 alternatives 53. 4 packs to a thread: with 2 those take 91 and 55 (104
-// and 115 with 20 alternatives), with 8 93 and 149. At least six waves to a SIMD (79 registers): 58 us for the
-// 999 rows at the compiler's own five, and 120 for the 8,192 at eight.
+// 6.1 with four packs to a thread and 6.7 with one), 999 of 32,001 fp32 with entropy and 8 alternatives 53. 4 packs
+// to a thread: with 2 those take 91 and 55 (104 and 115 with 20 alternatives), with 8 93 and 149. At least six waves
+// to a SIMD (79 registers): 58 us for the 999 rows at the compiler's own five, and 120 for the 8,192 at eight.
 constexpr int kBackPacks = 4;
 
 template <typename T>
@@ -590,7 +591,7 @@ __global__ __launch_bounds__(THREADS, 6) void fl_token_logprobs_backward_kernel(
     const T* x = logits + logit_at;
     T* out = grad + row * V;
     // Chunks from the gradient row's first 128-byte line on, so that no line is written in parts (8,192 rows of 16,383
-    // bf16: 120 us from the row's start); the logits ahead of it are the first chunk's too.
+    // bf16: 93 us, and 120 from the row's start); the logits ahead of it are the first chunk's too.
     const int ahead = (int)(-(uintptr_t)out % 128 / sizeof(T)), first = ahead + (int)blockIdx.y * kChunk;
     const int lo = blockIdx.y ? first : 0, hi = V - first < kChunk ? V : first + kChunk;
     const int packs = hi > first ? (hi - first) / N : 0, tail = first + packs * N;
@@ -667,7 +668,8 @@ bool shape_ok(int64_t outer, int64_t inner, int64_t V, int64_t so, int64_t si) {
 // The logits of a block: threads and packs of 16 bytes to each of them; segments of a row. One wave to a row that it
 // holds (8,192 rows of 1,000 bf16: 7.2 us, 17.9 with four waves); 4 packs to a thread where they hold the row (4,096
 // rows of 8,192: 14.1 us, 17.4 with 8 packs that half the threads fill) and 8 where they do not (8,192 rows of 16,384:
-// 48 us in one segment, 61 in two of 4 packs).
+// 42 us in one segment, 64 in two of 4 packs). A row just above a block's logits is two segments that half fill it:
+// 4,096 rows of 16,385 take 42 us and in three segments of 4 packs 40, of 20,000 42 and 43, of 32,768 54 and 56.
 struct Tile {
   int threads, packs, segments;
   int64_t seg_len;

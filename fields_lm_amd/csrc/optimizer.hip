@@ -64,7 +64,8 @@ __device__ __forceinline__ int tensor_of(const Table& t, int block) {
 }
 
 // What a step touches once it touches past the caches' keeping (0.29 G values: the norm 204 us plain and 179
-// streaming, the 32-bit step behind it 1,776 and 1,581 us in all, the 8-bit step 887 and 777).
+// streaming, the 32-bit step behind it 1,776 and 1,581 us in all, the 8-bit step 887 and 777; bf16 weights with 32-bit
+// states alone lose, 1,166 and 1,207).
 __device__ __forceinline__ u32x4 load_once(const u32x4_any* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ u32x2 load_once(const u32x2_any* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ uint32_t load_once(const u32_any* p) { return __builtin_nontemporal_load(p); }
@@ -209,7 +210,7 @@ __device__ __forceinline__ u32x4 pack_values<bf16_bits>(const float* v) {
 }
 
 // 16 bytes of parameters and gradients to a thread and turn, and their moments. Bound by the memory, 28 bytes an fp32
-// value: 0.29 G values take 1,415 us (5.7 TB/s; a streaming copy reaches 5.9).
+// value: 0.29 G values take 1,415 us (5.7 TB/s; four streams read and three written without arithmetic reach 6.1).
 template <typename T>
 __global__ __launch_bounds__(256) void fl_adamw_kernel(const AdamTable<false> t, const f32x4* __restrict__ hyper,
                                                        float b1, float b1c, float b2, float b2c, float eps) {

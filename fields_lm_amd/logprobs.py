@@ -79,7 +79,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, temperature: f
     gradient 0; NaN or +inf in a row make its results NaN. Rows whose incoming gradients are all 0 get zeros
     without their logits being read.
 
-    Gradients flow to ``logits`` from the log probabilities, the entropy and the alternatives' log probabilities.
+    Gradients flow to ``logits`` from the log probabilities, the entropy and the alternatives' log probabilities. A
+    backward that is to be differentiated itself (``create_graph``) runs stock operations, with the same zeros and NaN.
     Under graph capture the backward pass is refused while a graph of the default stream holds the logits' leaves.
     """
     return TokenLogprobs(*nat.host().token_logprobs(logits, tokens, temperature, top_k, entropy, ignore_index))

@@ -98,7 +98,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     that is not 0 keeps at least the smallest code. A non-finite value in a gradient spoils its block's states.
 
     grad_scale: one fp32 value on the device (:func:`grad_norm`'s second), or None for 1. Where it is not finite the
-    call leaves parameters, states and step counters as they were.
+    call leaves parameters, states and step counters as they were. To autograd the call is a write of all of them.
     """
     _check_hyper(lr, betas, eps, weight_decay)
     nat.host().adamw_step(
