@@ -737,3 +737,66 @@ def test_alternatives_around_the_groups_that_bound_them(dev, vocab, dtype):
     t = torch.randint(0, vocab, (24,), device=dev, generator=g)
     for k in (32, 33):
         check_forward(x, t, 1.0, k, True, fl.token_logprobs(x, t, top_k=k, entropy=True))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [2.0 ** -20, 2.0 ** -9, 2.0 ** 9, 2.0 ** 20])
+def test_temperatures_at_the_ends_of_their_range(dev, temperature, dtype):
+    print(f"[case] token_logprobs T={temperature} {dtype}", flush=True)
+    for vocab in (501, 16385):
+        x, t = make(dev, 6, vocab, dtype, vocab)
+        z = x.clone().requires_grad_()
+        r = fl.token_logprobs(z, t, temperature=temperature, top_k=5, entropy=True)
+        check_forward(x, t, temperature, 5, True, fl.TokenLogprobs(*(o.detach() for o in r)))
+        g = torch.Generator(device=dev).manual_seed(1)
+        ups = [torch.randn(*s, device=dev, generator=g) for s in ((6,), (6,), (6, 5))]
+        got, = torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], z, ups)
+        check_grad(x, t, temperature, 5, *ups, got)
+
+
+@pytest.mark.parametrize("vocab", [501, 8193])
+def test_logits_far_from_zero(dev, vocab):
+    """A maximum on both sides of 2^20 over log2(e) / T, where the difference is taken another way: differences of a few
+    units, in steps of 1 / 16, keep their digits."""
+    print(f"[case] token_logprobs, logits far from zero V={vocab}", flush=True)
+    base = 2.0 ** 20 / 1.4426950408889634
+    offsets = torch.tensor([0.5 * base, base - 20, base - 1, base + 20, 1.4 * base, -base - 20, -base + 20, 0.0], device=dev)
+    x, t = make(dev, 8, vocab, torch.float32, vocab)
+    x = x + offsets[:, None]
+    g = torch.Generator(device=dev).manual_seed(1)
+    ups = [torch.randn(*s, device=dev, generator=g) for s in ((8,), (8,), (8, 5))]
+    for temperature in (1.0, 0.75):
+        z = x.clone().requires_grad_()
+        r = fl.token_logprobs(z, t, temperature=temperature, top_k=5, entropy=True)
+        check_forward(x, t, temperature, 5, True, fl.TokenLogprobs(*(o.detach() for o in r)))
+        got, = torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], z, ups)
+        check_grad(x, t, temperature, 5, *ups, got)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gradient_of_the_longest_row(dev, dtype):
+    print(f"[case] token_logprobs gradient V=2^23 {dtype}", flush=True)
+    vocab = 1 << 23
+    x, t = make(dev, 2, vocab, dtype, 5)
+    x[1, : vocab // 2] = float("-inf")
+    t[0] = vocab - 1
+    ups = [torch.randn(*s, device=dev, generator=torch.Generator(device=dev).manual_seed(1)) for s in ((2,), (2,), (2, 5))]
+    z = x.clone().requires_grad_()
+    r = fl.token_logprobs(z, t, top_k=5, entropy=True)
+    check_forward(x, t, 1.0, 5, True, fl.TokenLogprobs(*(o.detach() for o in r)))
+    got, = torch.autograd.grad([r.logprobs, r.entropy, r.top_logprobs], z, ups)
+    check_grad(x, t, 1.0, 5, *ups, got)
+
+
+def test_rows_past_32_bits(dev):
+    """More than 2^32 rows in two groups, which all read one of three rows: where a row lies is a 64-bit quotient."""
+    print("[case] token_logprobs, 3 x (2^31 - 5) rows", flush=True)
+    inner = (1 << 31) - 5
+    line = torch.tensor([0.5, -1.0, 2.0, 0.25], device=dev)
+    x = line.as_strided((3, inner, 2), (1, 0, 1))
+    t = torch.ones(1, 1, dtype=torch.long, device=dev).expand(3, inner)
+    got = fl.token_logprobs(x, t).logprobs
+    exp = torch.log_softmax(line.double().unfold(0, 2, 1), -1)[:, 1]
+    for i in range(3):
+        low, high = float(got[i].min()), float(got[i].max())
+        assert low == high and abs(low - float(exp[i])) <= 16 * U * (1 + abs(float(exp[i]))), i

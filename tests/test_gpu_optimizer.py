@@ -659,3 +659,69 @@ def test_adamw_8_bit_moments_are_the_formulas(dev, dtype):
         off = (held(vc, vs) - root).abs()
         assert bool((off <= torch.maximum(2.0 ** -4 * root + small / 2, small - root) + 16 * U * largest(root)).all()), turn
         assert bool((held(vc, vs)[root > 0] > 0).all())
+
+
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("n", [479, 480, 481, 1000])
+def test_adamw_step_of_many_tensors(dev, n, eight):
+    """Past one launch's step counters and many of its tables: each tensor's step is that of a call of its own."""
+    print(f"[case] adamw_step, {n} tensors, 8 bits: {eight}", flush=True)
+    sizes = [0 if i % 13 == 7 else 1 + 37 * i % 5000 for i in range(n)]
+    p, g, m, v = start32(dev, sizes, torch.float32, n)
+    if eight:
+        m, v = ([t.clamp(-1, 1).to(STATE8_DTYPE) for t in l] for l in (m, v))
+    scales = [[torch.rand(-(-s // 256), device=dev) for s in sizes] for _ in range(2)] if eight else [None, None]
+
+    def call(pick, steps, lists):
+        lists = [None if l is None else [l[i] for i in pick] for l in lists]
+        fl.adamw_step(*lists[:4], steps, exp_avg_scales=lists[4], exp_avg_sq_scales=lists[5],
+                      grad_scale=torch.tensor(0.5, device=dev), **HYPER)
+
+    steps = torch.arange(n, device=dev) % 50
+    checked = sorted({*range(0, n, 97), 478, n - 1})
+    lists = [p, g, m, v, *scales]
+    alone = [None if l is None else [t.clone() for t in l] for l in lists]
+    for i in checked:
+        counter = steps[i:i + 1].clone()
+        call([i], counter, alone)
+        assert int(counter) == int(steps[i]) + 1
+    call(range(n), steps, lists)
+    assert torch.equal(steps, torch.arange(n, device=dev) % 50 + 1)
+    for i in checked:
+        for a, b in zip(lists, alone):
+            assert a is None or torch.equal(a[i].view(torch.uint8), b[i].view(torch.uint8)), i
+    for i in range(0, n, 5):  # the others are no longer what they were
+        assert sizes[i] == 0 or not torch.equal(p[i], alone[0][i]) or i in checked
+
+
+def test_one_tensor_of_the_most_values(dev):
+    """2^34 bf16 values with 8-bit states (106 GB): as many blocks as a launch takes, behind a small tensor's own."""
+    print("[case] adamw_step and grad_norm of 2^34 values", flush=True)
+    n = 1 << 34
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 130 << 30:
+        pytest.skip("needs 130 GiB of free device memory")
+    at = torch.tensor([0, 1, (1 << 31) - 1, 1 << 32, (1 << 33) + 255, n - 257, n - 1], device=dev)
+    vals = torch.tensor([2.0, 1.0, -1.0, 3.0, -2.0, 0.5, 4.0], device=dev).bfloat16()
+    p, g = (torch.zeros(n, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    m, v = (torch.zeros(n, device=dev, dtype=torch.uint8).view(STATE8_DTYPE) for _ in range(2))
+    ms, vs = (torch.zeros(n // 256, device=dev) for _ in range(2))
+    p[at], g[at] = -vals, vals
+    small = [torch.ones(3, device=dev, dtype=torch.bfloat16) for _ in range(2)]
+    codes = [torch.zeros(3, device=dev, dtype=torch.uint8).view(STATE8_DTYPE) for _ in range(2)]
+    tops = [torch.zeros(1, device=dev) for _ in range(2)]
+    norm = math.sqrt(float(vals.double().square().sum()) + 3)
+    assert abs(float(fl.grad_norm([small[1], g])) - norm) <= 2 * U * norm
+    hyper = {**HYPER, "lr": 0.1}
+    fl.adamw_step([small[0], p], [small[1], g], [codes[0], m], [codes[1], v], torch.zeros(2, dtype=torch.long, device=dev),
+                  exp_avg_scales=[tops[0], ms], exp_avg_sq_scales=[tops[1], vs], **hyper)
+    exp, tol = exact(-vals, vals, *(torch.zeros(7, device=dev) for _ in range(2)), 1, **hyper)
+    near(p[at], exp[0], tol[0], "p")
+    held = m[at].float() * ms[at // 256]
+    assert bool(((held - 0.1 * vals.float()).abs() <= 2.0 ** -4 * 0.1 * vals.float().abs() + 1e-6).all())
+    assert bool((small[0] != 1).all())
+    assert sum(int(c.count_nonzero()) for c in p.split(1 << 31)) == 7
+    assert sum(int(c.count_nonzero()) for c in m.view(torch.uint8).split(1 << 31)) == 7 == int(ms.count_nonzero()) + 1
+    del p, g, m, v, ms, vs
+    torch.cuda.empty_cache()
