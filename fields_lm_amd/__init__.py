@@ -9,7 +9,9 @@ Public surface (mirrors src/fields_official/reference/field_only_v4_chunked_trit
 * ``IndependentVacancyField``, ``FieldBlock``, ``RMSNorm``, ``PackedSwiGLU``
 * ``field_scan`` (with state_in / state_out) and ``field_decode_step`` (decode token loop)
 * ``field_scan_norm`` / ``field_decode_norm_step``: the same with the mixer's read_norm fused
-* ``token_logprobs`` (loss and scoring), ``grad_norm``, ``adamw_step`` / ``AdamW`` (the end of a training step)
+* ``embedding`` and ``gated_scan`` with their gradients (the model's beginning, the softpatch's recurrence)
+* ``token_logprobs`` (loss and scoring), ``grad_norm``, ``adamw_step`` / ``AdamW``, ``orthogonalize``, ``muon_step`` /
+  ``Muon`` (the end of a training step)
 """
 from .field import (  # noqa: F401
     ScanPlan,
@@ -26,6 +28,7 @@ from .field import (  # noqa: F401
     field_scan_backward,
     field_scan_norm,
     gate_residual_norm,
+    gated_scan,
     swiglu,
     fused_field_read,
     state_to_complex,
@@ -39,7 +42,8 @@ from .model import (  # noqa: F401,E402
     FieldTokenSystem,
     build_official_fields,
 )
+from .embedding import embedding  # noqa: F401,E402
 from .logprobs import TokenLogprobs, token_logprobs  # noqa: F401,E402
-from .optim import AdamW, adamw_step, grad_norm  # noqa: F401,E402
+from .optim import AdamW, Muon, adamw_step, grad_norm, muon_step, orthogonalize  # noqa: F401,E402
 
 __version__ = "0.1.0"

@@ -107,6 +107,18 @@ SIGNATURES = {
     "fl_adamw_workspace_bytes": (_sz, [_i64]),
     "fl_adamw_step": (_int, [_i64, _vp, _vp, _int] + [_vp] * 6 + [ctypes.c_double, _vp] + [ctypes.c_double] * 4 +
                       [_vp, _vp, _sz, _vp]),
+    "fl_embedding": (_int, [_vp, _i64, _vp, _int] + [_i64] * 3 + [ctypes.c_float, _int, _i64, _vp, _int, _vp]),
+    "fl_embedding_backward_workspace_bytes": (_sz, [_i64] * 3),
+    "fl_embedding_backward": (_int, [_vp, _i64, _vp, _int] + [_i64] * 3 + [ctypes.c_float, _vp, _int, _vp, _sz, _vp]),
+    "fl_gated_scan_tile": (_i64, []),
+    "fl_gated_scan_workspace_bytes": (_sz, [_i64] * 3 + [_int]),
+    "fl_gated_scan": (_int, [_vp, _int, _int, _i64, _i64, _vp, _int] + [_i64] * 5 + [_vp] * 5 + [_sz, _vp]),
+    "fl_gated_scan_backward": (_int, [_vp, _int, _int, _i64, _i64, _vp, _int] + [_i64] * 5 + [_vp] * 7 + [_sz, _vp]),
+    "fl_orthogonalize_check": (_int, [_int] + [ctypes.c_double] * 3),
+    "fl_orthogonalize_workspace_bytes": (_sz, [_i64, _vp, _vp]),
+    "fl_orthogonalize": (_int, [_i64, _vp, _int, _vp, _vp, _int] + [ctypes.c_double] * 4 + [_vp, _vp, _sz, _vp]),
+    "fl_muon_step": (_int, [_i64, _vp, _vp, _int, _vp, _vp, _vp, ctypes.c_double, _vp, _vp, ctypes.c_double, _int,
+                            ctypes.c_double, _int] + [ctypes.c_double] * 4 + [_vp, _vp, _sz, _vp]),
     "fl_version": (ctypes.c_char_p, []),
 }
 
@@ -149,11 +161,20 @@ def host():
         except ImportError as e:
             raise RuntimeError(f"host extension not built: {LIB_PATH.parent / '_host.so'} "
                                "(run `python -m fields_lm_amd.build` or __graft_entry__.build())") from e
+        from ._train import stock_scan_gradients
         from .logprobs import stock_gradient
 
-        module.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        def addresses(*names):
+            return [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names]
+
+        module.bind(*addresses(
             "fl_token_logprobs_workspace_bytes", "fl_token_logprobs", "fl_token_logprobs_backward",
-            "fl_grad_norm_workspace_bytes", "fl_grad_norm", "fl_adamw_workspace_bytes", "fl_adamw_step")), stock_gradient)
+            "fl_grad_norm_workspace_bytes", "fl_grad_norm", "fl_adamw_workspace_bytes", "fl_adamw_step"), stock_gradient)
+        module.bind_train(*addresses(
+            "fl_embedding", "fl_embedding_backward_workspace_bytes", "fl_embedding_backward",
+            "fl_gated_scan_workspace_bytes", "fl_gated_scan", "fl_gated_scan_backward", "fl_orthogonalize_check",
+            "fl_orthogonalize_workspace_bytes", "fl_orthogonalize", "fl_muon_step"), lib.fl_gated_scan_tile(),
+            stock_scan_gradients)
         _host = module
     return _host
 

@@ -158,6 +158,35 @@ def transition_ops(radius_logit, theta):
     return (radius * torch.cos(theta)).contiguous(), (radius * torch.sin(theta)).contiguous(), gamma.contiguous()
 
 
+def gated_scan_ops(gate, drive, state):
+    """(all states, the last one) of the gated scan in stock ops, by doubling: after k rounds a step holds what the last
+    2^k steps make of it."""
+    p = (gate if gate.ndim == 3 else gate[..., None]).float()
+    s = drive.float()
+    if state is not None:
+        s = torch.cat(((p[:, 0] * state + s[:, 0])[:, None], s[:, 1:]), 1)
+    reach = 1
+    while reach < s.shape[1]:
+        s = torch.cat((s[:, :reach], p[:, reach:] * s[:, :-reach] + s[:, reach:]), 1)
+        p = torch.cat((p[:, :reach], p[:, reach:] * p[:, :-reach]), 1)
+        reach *= 2
+    return s.to(drive.dtype), s[:, -1]
+
+
+def stock_scan_gradients(gate, drive, state, g_out, g_last):
+    """The gradients of gate, drive and state (or None) in stock ops, for a backward that must itself be
+    differentiable; an upstream gradient may be None."""
+    given = [(i, g) for i, g in enumerate((g_out, g_last)) if g is not None]
+
+    def fn(a, u, *first):
+        outs = gated_scan_ops(a, u, *(first or (None,)))
+        return tuple(outs[i] for i, _ in given)
+
+    inputs = (gate, drive) if state is None else (gate, drive, state)
+    got = _stock_grads(fn, inputs, tuple(g for _, g in given))
+    return (*got, *[None] * (3 - len(got)))
+
+
 class Transition(torch.autograd.Function):
     """The transition parameters, fp32 [C] each, from fp32 radius_logit and theta."""
 

@@ -22,7 +22,7 @@ PKG_DIR = Path(__file__).resolve().parent
 REPO_DIR = PKG_DIR.parent
 SOURCES = [PKG_DIR / "csrc" / name for name in ("field_scan.hip", "block_tail.hip", "field_params.hip", "mamba.hip",
                                                  "attention.hip", "boundary.hip", "linear.hip", "train.hip", "exact.hip",
-                                                 "logprobs.hip", "optimizer.hip")]
+                                                 "logprobs.hip", "optimizer.hip", "embedding.hip", "gated_scan.hip", "muon.hip")]
 # what a source needs beside HIP_FLAGS (a later flag of a kind replaces an earlier one)
 SOURCE_FLAGS = {"field_params.hip": ["-ffp-contract=on"], "exact.hip": ["-ffp-contract=on"],
                 "optimizer.hip": ["-ffp-contract=off"]}
@@ -33,7 +33,7 @@ LIB_PATH = PKG_DIR / "libfields_amd.so"
 BENCH_SOURCES = [PKG_DIR / "csrc" / "copy_ceiling.hip"]
 BENCH_LIB_PATH = PKG_DIR / "libfields_bench.so"
 # the host side of some calls (CPython and PyTorch headers, no device code)
-HOST_SOURCE = PKG_DIR / "csrc" / "host.cpp"
+HOST_SOURCES = [PKG_DIR / "csrc" / name for name in ("host.cpp", "host_train.cpp")]
 HOST_PATH = PKG_DIR / "_host.so"
 ARCH = "gfx950"
 
@@ -95,23 +95,30 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None, out: Path
 
 
 def build_host(verbose: bool = False) -> Path:
-    """Compile ``csrc/host.cpp`` into the extension module ``_host.so`` with the host compiler."""
+    """Compile ``HOST_SOURCES`` into the extension module ``_host.so`` with the host compiler."""
     import torch
     from torch.utils.cpp_extension import include_paths
 
     tmp = HOST_PATH.with_suffix(".so.tmp")
     rocm = Path(hipcc()).resolve().parents[1]
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           *(arg for path in include_paths() for arg in ("-isystem", path)), f"-I{sysconfig.get_paths()['include']}",
-           "-isystem", str(rocm / "include"), f"-I{INCLUDE_DIR}", str(HOST_SOURCE),
-           f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_hip",
-           "-o", str(tmp)]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+    flags = ["-O2", "-std=c++17", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+             *(arg for path in include_paths() for arg in ("-isystem", path)), f"-I{sysconfig.get_paths()['include']}",
+             "-isystem", str(rocm / "include"), f"-I{INCLUDE_DIR}"]
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"g++ failed ({proc.returncode}):\n{proc.stdout}\n{proc.stderr}")
+
+    with tempfile.TemporaryDirectory() as work:
+        objects = [str(Path(work) / f"{s.stem}.o") for s in HOST_SOURCES]
+        with ThreadPoolExecutor(max_workers=4) as pool:
+            list(pool.map(run, [["g++", *flags, "-c", str(s), "-o", o] for s, o in zip(HOST_SOURCES, objects)]))
+        run(["g++", "-shared", *objects, f"-L{Path(torch.__file__).parent / 'lib'}", "-ltorch_python", "-ltorch_cpu",
+             "-lc10", "-lc10_hip", "-o", str(tmp)])
     os.replace(tmp, HOST_PATH)
     return HOST_PATH
 

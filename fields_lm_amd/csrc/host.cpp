@@ -9,33 +9,13 @@
 // grad_norm, adamw_step: their lists of tensors are read in one pass and without a Python object per attribute. A step
 // reads some twenty attributes of each of a model's hundreds of tensors: through Python's accessors that is 1.2 us a
 // tensor.
-#define PY_SSIZE_T_CLEAN
-#include <Python.h>
-
-#include <ATen/ATen.h>
-#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPGraphsC10Utils.h>
-#include <torch/csrc/Exceptions.h>
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
-#include <torch/csrc/autograd/python_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
-
-#include <algorithm>
-#include <memory>
-#include <optional>
-#include <unordered_set>
-#include <utility>
-#include <vector>
-
-#include "fields_amd.h"
+//
+// The calls of host_train.cpp are this module's too.
+#include "host_common.h"
 
 namespace {
 
-using at::Tensor;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace host;
 
 // The library's entry points, which the loader of the library hands over, and the stock form of the gradient.
 decltype(&fl_token_logprobs_workspace_bytes) workspace_bytes = nullptr;
@@ -49,31 +29,6 @@ PyObject* stock_gradient = nullptr;
 
 constexpr int64_t kMaxTop = 64, kMaxVocab = (int64_t)1 << 23, kStateBlock = 256;
 constexpr double kMinTemperature = 0x1p-20, kMaxTemperature = 0x1p20;
-
-void check(int code, const char* what) {
-  TORCH_CHECK_VALUE(code != FL_ERR_INVALID_ARGUMENT, what, ": invalid shape, stride or pointer");
-  TORCH_CHECK_TYPE(code != FL_ERR_DTYPE, what, ": unsupported dtype");
-  TORCH_CHECK(code != FL_ERR_WORKSPACE, what, ": workspace missing or too small");
-  TORCH_CHECK(code < FL_ERR_HIP_BASE, what, ": HIP error ", code - FL_ERR_HIP_BASE);
-  TORCH_CHECK(code == FL_OK, what, ": error code ", code);
-}
-
-// a trace would keep the results of its example as constants
-void check_not_traced(const char* what) {
-  TORCH_CHECK(!torch::jit::tracer::isTracing(), what, " reads addresses and cannot be traced");
-}
-
-// A tensor that dispatches to Python (a fake one, say) has no memory of its own behind its address.
-void check_plain(const Tensor& t, const char* what) {
-  TORCH_CHECK_TYPE(!t.key_set().has(c10::DispatchKey::Python), what, " must be plain tensors");
-}
-
-int dtype_code(const Tensor& t) { return t.scalar_type() == at::kBFloat16 ? FL_DTYPE_BF16 : FL_DTYPE_F32; }
-
-void* stream_of(const Tensor& t) { return at::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream(); }
-
-template <typename T>
-T* address(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
 
 struct Grid {
   int64_t outer, inner, stride_outer, stride_inner;
@@ -222,27 +177,6 @@ Tensor stock_backward(const Tensor& logits, const Tensor& tokens, const Tensor& 
   return out;
 }
 
-// A captured backward adds into the logits' leaves on the streams that their eager graphs, where one still lives,
-// were made on. The default stream cannot join a capture, which ends in an error that the engine does not survive.
-void check_leaves(const Tensor& logits) {
-  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
-  std::vector<std::shared_ptr<torch::autograd::Node>> todo = {
-      logits.grad_fn() ? logits.grad_fn() : torch::autograd::impl::try_get_grad_accumulator(logits)};
-  std::unordered_set<torch::autograd::Node*> seen;
-  while (!todo.empty()) {
-    const std::shared_ptr<torch::autograd::Node> node = todo.back();
-    todo.pop_back();
-    if (!node || !seen.insert(node.get()).second) continue;
-    if (dynamic_cast<torch::autograd::AccumulateGrad*>(node.get())) {
-      const std::optional<c10::Stream> stream = node->stream();
-      TORCH_CHECK(!stream || stream->id() != 0,
-                  "the logits' leaves hold an autograd graph made on the default stream: drop it (its outputs) before "
-                  "a backward pass is captured");
-    }
-    for (const auto& edge : node->next_edges()) todo.push_back(edge.function);
-  }
-}
-
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
   // the outputs that are wanted, in the order log probabilities, entropy, alternatives' log probabilities and tokens
   static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& tokens, double temperature,
@@ -273,7 +207,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     if (o.top_k) g[2] = grads[o.entropy ? 2 : 1];
     variable_list out(6);
     if (!g[0].defined() && !g[1].defined() && !g[2].defined()) return out;
-    check_leaves(logits);
+    check_leaves(node_of(logits), "logits'");
     out[0] = at::GradMode::is_enabled() ? stock_backward(logits, tokens, top_tokens, o, g)
                                         : ::backward(logits, tokens, stats, entropy, top_tokens, o, g);
     return out;
@@ -372,114 +306,6 @@ PyObject* bind(PyObject*, PyObject* args) {
   Py_RETURN_NONE;
 }
 
-// A Python list or tuple of tensors: contiguous, of one of `types` (their places are the type codes), on `device`, with
-// the counts of values that are expected. Gradients of other strides are copied.
-struct TensorList {
-  std::vector<void*> addresses;
-  std::vector<int64_t> counts;
-  std::vector<int> codes;
-  std::vector<Tensor> kept;  // copies that have to live until the launch
-  std::vector<at::IntArrayRef> shapes;
-
-  TensorList(PyObject* list, const char* what, at::Device device, std::initializer_list<at::ScalarType> types,
-             const std::vector<int64_t>* expected = nullptr, int64_t block = 1, bool copy = false) {
-    TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), what, " must be a list or tuple of tensors");
-    PyObject** items = PySequence_Fast_ITEMS(list);
-    const size_t n = (size_t)PySequence_Fast_GET_SIZE(list);
-    addresses.reserve(n);
-    counts.reserve(n);
-    codes.reserve(n);
-    shapes.reserve(n);
-    for (size_t i = 0; i < n; ++i) {
-      TORCH_CHECK_TYPE(THPVariable_Check(items[i]), what, ": number ", i, " is no tensor");
-      const Tensor& t = THPVariable_Unpack(items[i]);
-      check_plain(t, what);
-      const auto at = std::find(types.begin(), types.end(), t.scalar_type());
-      TORCH_CHECK_TYPE(at != types.end(), what, " must be ", *types.begin(),
-                       types.size() > 1 ? " or another type of the list" : "",
-                       ", number ", i, " is ", t.scalar_type());
-      TORCH_CHECK_TYPE(t.layout() == at::kStrided, what, " must be dense, number ", i, " is ", t.layout());
-      TORCH_CHECK_VALUE(t.device() == device, what, " must be on ", device, ", number ", i, " is on ", t.device());
-      const int64_t count = t.numel();
-      TORCH_CHECK_VALUE(!expected || count == ((*expected)[i] + block - 1) / block, what, ": number ", i, " has ",
-                        count,
-                        " values, ", ((*expected)[i] + block - 1) / block, " are wanted");
-      const bool plain = t.is_contiguous() && !t.is_neg();
-      TORCH_CHECK_VALUE(plain || copy, what, " must be contiguous, number ", i, " is not");
-      if (!plain) kept.push_back(t.detach().resolve_neg().contiguous());
-      addresses.push_back((plain ? t : kept.back()).data_ptr());
-      counts.push_back(count);
-      codes.push_back((int)(at - types.begin()));
-      shapes.push_back(t.sizes());
-    }
-  }
-  size_t size() const { return addresses.size(); }
-};
-
-typedef std::vector<std::pair<uintptr_t, uintptr_t>> Ranges;  // of addresses, [first, last + 1), in their order
-
-Ranges ranges_of(const TensorList& list, size_t size) {
-  Ranges r;
-  r.reserve(list.size());
-  for (size_t i = 0; i < list.size(); ++i) {
-    const uintptr_t at = reinterpret_cast<uintptr_t>(list.addresses[i]);
-    if (list.counts[i]) r.emplace_back(at, at + list.counts[i] * size);
-  }
-  if (!std::is_sorted(r.begin(), r.end())) std::sort(r.begin(), r.end());
-  return r;
-}
-
-// Lists that lie in one buffer each come in order and apart, and need no sorting of all ranges anew; states allocated
-// parameter by parameter lie between each other and are merged (host time of a step of 240 tensors with 8-bit states:
-// 53 us in one buffer a kind, 75 as AdamW makes them).
-void merge(Ranges& to, const Ranges& r) {
-  if (r.empty()) return;
-  const bool ahead = !to.empty() && r.back() < to.front(), behind = to.empty() || to.back() < r.front();
-  const auto middle = to.insert(ahead ? to.begin() : to.end(), r.begin(), r.end());
-  if (!ahead && !behind) std::inplace_merge(to.begin(), middle, to.end());
-}
-
-bool overlap(const Ranges& r) {
-  for (size_t i = 1; i < r.size(); ++i)
-    if (r[i].first < r[i - 1].second) return true;
-  return false;
-}
-
-// whether one of a, which are apart, and one of b share an address
-bool meet(const Ranges& a, const Ranges& b) {
-  for (size_t i = 0, j = 0; i < a.size() && j < b.size();) {
-    if (a[i].second <= b[j].first) ++i;
-    else if (b[j].second <= a[i].first) ++j;
-    else return true;
-  }
-  return false;
-}
-
-// the first tensor of a list or tuple, whose device the others are to be on
-const Tensor& first_of(PyObject* list, const char* what) {
-  TORCH_CHECK_TYPE(PyList_Check(list) || PyTuple_Check(list), what, " must be a list or tuple of tensors");
-  TORCH_CHECK_VALUE(PySequence_Fast_GET_SIZE(list) > 0, "no ", what);
-  PyObject* first = PySequence_Fast_ITEMS(list)[0];
-  TORCH_CHECK_TYPE(THPVariable_Check(first), what, ": number 0 is no tensor");
-  return THPVariable_Unpack(first);
-}
-
-// one fp32 value on the device (a copy where its memory holds the negative), or none
-Tensor device_value(PyObject* o, const char* what, at::Device device) {
-  if (o == Py_None) return {};
-  TORCH_CHECK_TYPE(THPVariable_Check(o), what, " must be a tensor");
-  const Tensor& t = THPVariable_Unpack(o);
-  check_plain(t, what);
-  TORCH_CHECK_VALUE(t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == device, what,
-                    " must be one float32 value on ", device);
-  TORCH_CHECK_VALUE(t.data_ptr(), what, " has no memory");  // (an address of 0 stands for no value)
-  return t.is_neg() ? t.detach().resolve_neg() : t;
-}
-
-Tensor workspace_on(at::Device device, size_t bytes) {
-  return at::empty({(int64_t)std::max<size_t>(bytes, 1)}, at::TensorOptions().dtype(at::kByte).device(device));
-}
-
 // grad_norm(gradients, max_norm or a negative number for none) -> (norm, scale or None)
 PyObject* grad_norm(PyObject*, PyObject* args) {
   HANDLE_TH_ERRORS
@@ -503,17 +329,6 @@ PyObject* grad_norm(PyObject*, PyObject* args) {
   PyObject* scale = scaled ? THPVariable_Wrap(out.select(0, 1)) : Py_NewRef(Py_None);
   return Py_BuildValue("(NN)", norm, scale);
   END_HANDLE_TH_ERRORS
-}
-
-// Tensors (one, a list or tuple, or None) that were written in place: what autograd saved of them is stale.
-void count_writes(PyObject* o) {
-  const auto count = [](PyObject* item) {
-    const Tensor& t = THPVariable_Unpack(item);
-    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
-  };
-  if (o == Py_None) return;
-  if (THPVariable_Check(o)) return count(o);
-  for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(o); ++i) count(PySequence_Fast_ITEMS(o)[i]);
 }
 
 // adamw_step(parameters, gradients, first moments, second moments, steps (a list or one tensor), lr (a number or a
@@ -599,11 +414,29 @@ PyObject* adamw_step(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
+}  // namespace
+
+// the calls of host_train.cpp
+PyObject* host_bind_train(PyObject*, PyObject*);
+PyObject* host_embedding(PyObject*, PyObject*);
+PyObject* host_gated_scan(PyObject*, PyObject*);
+PyObject* host_orthogonalize(PyObject*, PyObject*);
+PyObject* host_check_steps(PyObject*, PyObject*);
+PyObject* host_muon_step(PyObject*, PyObject*);
+
+namespace {
+
 PyMethodDef methods[] = {{"bind", bind, METH_VARARGS, "the library's entry points and the stock gradient"},
                          {"token_logprobs", token_logprobs, METH_VARARGS, "the call"},
                          {"where", where, METH_VARARGS, "the rows of logits and tokens"},
                          {"grad_norm", grad_norm, METH_VARARGS, "the call"},
                          {"adamw_step", adamw_step, METH_VARARGS, "the call"},
+                         {"bind_train", host_bind_train, METH_VARARGS, "the entry points of the calls below"},
+                         {"embedding", host_embedding, METH_VARARGS, "the call"},
+                         {"gated_scan", host_gated_scan, METH_VARARGS, "the call"},
+                         {"orthogonalize", host_orthogonalize, METH_VARARGS, "the call"},
+                         {"check_steps", host_check_steps, METH_VARARGS, "of orthogonalization"},
+                         {"muon_step", host_muon_step, METH_VARARGS, "the call"},
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

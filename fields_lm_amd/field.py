@@ -7,6 +7,7 @@ Reference: src/fields_official/reference/field_only_v4_chunked_triton_wiki100.py
   then canon:300-309), ``fl_scan_norm_forward``.
 * :func:`field_decode_step`     — single-token step (no reference counterpart), ``fl_decode_step``;
   :func:`field_decode_norm_step` the same with read_norm fused, ``fl_decode_norm_step``.
+* :func:`gated_scan`            — the real gated recurrence with its gradients, ``fl_gated_scan``.
 * :class:`IndependentVacancyField`, :class:`FieldBlock`, :class:`RMSNorm`,
   :class:`PackedSwiGLU` — same constructor signatures, parameter names, initialisation order
   and forward maths as canon:1131-1221 and canon:300-325, so a reference state_dict loads
@@ -367,6 +368,26 @@ def boundary_scan(a: torch.Tensor, drive: torch.Tensor, state_in: Optional[torch
                                 nat.ptr(sout), nat.ptr(out), nat.stream_handle(drive.device))
     nat.check(code, "fl_boundary_scan")
     return (out, sout) if return_state else out
+
+
+def gated_scan(gate: torch.Tensor, drive: torch.Tensor, state_in: Optional[torch.Tensor] = None, *,
+               return_state: bool = False):
+    """Gated linear recurrence h[b,t,c] = gate[b,t,c] * h[b,t-1,c] + drive[b,t,c] with its gradients
+    (``fl_gated_scan``; :func:`boundary_scan` is its form for one fp32 gate a token, without gradients).
+
+    drive [B,T,C], gate [B,T,C] or one value a token ([B,T] or [B,T,1]), each fp32 or bf16 on one ROCm device and
+    read in place where its last dimension is unit-stride; state_in [B,C] fp32 or None for zeros. Returns h [B,T,C] in
+    drive's type, with ``return_state`` also h[:,T-1] in fp32. The recurrence and its gradients run in fp32 and are
+    rounded once.
+
+    Gradients flow to gate, drive and state_in. A backward that is to be differentiated itself (``create_graph``) runs
+    stock operations. A gate of 0 starts a new sequence, one of 1 with a drive of 0 passes the state on. Steps are
+    composed in tiles of 256, so that the product of any run of gates within a tile has to be finite in fp32, which it
+    is for gates of at most 1. Under graph capture the backward pass is refused while a graph of the default stream
+    holds the inputs' leaves.
+    """
+    out, last = nat.host().gated_scan(gate, drive, state_in, return_state)
+    return (out, last) if return_state else out
 
 
 def _row_stride(t: torch.Tensor) -> Optional[int]:

@@ -41,7 +41,8 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from ._dispatch import KERNEL_DTYPES, eager, free_rounding, no_grad_needed, plain_call, plain_linear
-from .field import (FieldBlock, RMSNorm, _linear_residual, boundary_scan, gate_residual_norm, rms_norm,
+from .embedding import embedding
+from .field import (FieldBlock, RMSNorm, _linear_residual, boundary_scan, gate_residual_norm, gated_scan, rms_norm,
                     rms_norm_takes, swiglu)
 from .logprobs import TokenLogprobs, token_logprobs
 
@@ -1022,6 +1023,10 @@ class BoundaryStateMixer(nn.Module):
         h = self.norm(x)
         z = self.down(h).float()
         boundary = self._boundary(h, tokens)
+        if not no_grad_needed(boundary, z) and eager(boundary, z):
+            state, last = gated_scan(1.0 - boundary, boundary[..., None] * z, return_state=True)
+            out = x + self.up(torch.cat((z, state), dim=-1).to(x.dtype))
+            return (out, last) if return_state else out
         state, last = boundary_scan((1.0 - boundary).contiguous(), (boundary[..., None] * z).contiguous(),
                                     return_state=True)
         out = x + self.up(torch.cat((z, state), dim=-1).to(x.dtype))
@@ -1117,10 +1122,21 @@ class FieldTokenSystem(nn.Module):
     def kinds(self) -> List[str]:
         return [_kind(b) for b in self.blocks]
 
+    def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
+        """The tokens' rows; where a gradient is wanted through ``fl_embedding``, whose gradient is the same bits every
+        time."""
+        emb = self.emb
+        weight = emb.weight
+        if (plain_call(emb, nn.Embedding) and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse
+                and not no_grad_needed(weight) and weight.dtype in KERNEL_DTYPES and tokens.dtype == torch.int64
+                and eager(weight, tokens)):
+            return embedding(tokens, weight, padding_idx=emb.padding_idx)
+        return emb(tokens)
+
     def states_logits(self, tokens: torch.Tensor, last_only: bool = False):
         """v21:620-627 / v29:353-381 (inference): hidden states and logits (of the last position
         only when ``last_only``, as v32:461-490's prefill benchmark)."""
-        x = self.emb(tokens)
+        x = self._embed(tokens)
         for i, block in enumerate(self.blocks):
             x = block(x)
             if i == self.patch_position:

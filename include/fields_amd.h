@@ -524,6 +524,69 @@ int fl_adamw_step(int64_t n, void* const* params, const void* const* grads, int 
                   double beta2, double eps, double weight_decay, const float* grad_scale, void* workspace,
                   size_t workspace_bytes, void* stream);
 
+/*
+ * Rows of an embedding by token and the gradient of its weight (no counterpart in the reference, which calls the stock
+ * embedding).
+ * fl_embedding: out [n, D] = scale * weight[tokens], weight rows weight_stride elements apart; a token outside 0 .. V - 1
+ *   has NaN. masked: the transpose of the gradient: rows of the token `padding` (-1: none) and of tokens outside are zeros.
+ * fl_embedding_backward: g_weight [V, D], contiguous, = scale * the sum of g [n, D] over the rows of each token, in
+ *   their order, fp32, rounded once; zeros for `padding` (-1: none) and for rows of no token. Tokens outside pass
+ *   nothing. Workspace 16-byte aligned, no initial contents needed.
+ */
+int fl_embedding(const int64_t* tokens, int64_t n, const void* weight, int weight_dtype, int64_t V, int64_t D,
+                 int64_t weight_stride, float scale, int masked, int64_t padding, void* out, int out_dtype,
+                 void* stream);
+size_t fl_embedding_backward_workspace_bytes(int64_t n, int64_t V, int64_t D);
+int fl_embedding_backward(const int64_t* tokens, int64_t n, const void* g, int g_dtype, int64_t V, int64_t D,
+                          int64_t padding, float scale, void* g_weight, int weight_dtype, void* workspace,
+                          size_t workspace_bytes, void* stream);
+
+/*
+ * The gated linear recurrence h[b,t,c] = gate[b,t,c] h[b,t-1,c] + drive[b,t,c], h[b,-1,:] = state_in [B, C] or 0, and its
+ * gradients (the differentiable form of fl_boundary_scan above). per_token: the gate is [B, T], one to all channels.
+ * Element (b, t, c) of gate and drive at b * stride_b + t * stride_t + c (elements); everything else is contiguous.
+ * fl_gated_scan: out [B, T, C] of drive_dtype; state_out [B, C] or NULL = h[:, T-1]; starts
+ *   [B, ceil(T / fl_gated_scan_tile()), C] or NULL: the states before every tile of steps, for the backward.
+ * fl_gated_scan_backward: from the forward's inputs and starts, and g_out [B, T, C] of drive_dtype and g_state [B, C]
+ *   (either may be NULL): g_drive [B, T, C], g_gate of the gate's shape (or NULL), g_state_in [B, C] (or NULL), each of
+ *   its tensor's type.
+ * Maths in fp32, rounded once. Workspace 16-byte aligned, no initial contents needed.
+ */
+int64_t fl_gated_scan_tile(void);
+size_t fl_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t C, int backward);
+int fl_gated_scan(const void* gate, int gate_dtype, int per_token, int64_t gate_stride_b, int64_t gate_stride_t,
+                  const void* drive, int drive_dtype, int64_t drive_stride_b, int64_t drive_stride_t, int64_t B,
+                  int64_t T, int64_t C, const float* state_in, float* state_out, float* starts, void* out,
+                  void* workspace, size_t workspace_bytes, void* stream);
+int fl_gated_scan_backward(const void* gate, int gate_dtype, int per_token, int64_t gate_stride_b,
+                           int64_t gate_stride_t, const void* drive, int drive_dtype, int64_t drive_stride_b,
+                           int64_t drive_stride_t, int64_t B, int64_t T, int64_t C, const float* starts,
+                           const void* g_out, const float* g_state, void* g_gate, void* g_drive, float* g_state_in,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Newton-Schulz steps over n matrices (no counterpart in the reference). Lists of addresses and sizes are HOST arrays,
+ * read before the call returns; rows and columns up to 2^20, values of a matrix up to 2^30, empty ones passed over.
+ * fl_orthogonalize: X = x / (|x| + eps), |x| the Frobenius norm, then `steps` (1 .. 64) times
+ *   X = a X + (b A + c A^2) X, A = X X^T (X^T X where rows > cols); out of the type of x, which it may not overlap.
+ * fl_muon_step: with g = grad * *grad_scale (NULL: 1), m the buffers,
+ *     m = momentum m + (1 - momentum) g;  u = nesterov ? (1 - momentum) g + momentum m : m;
+ *     p = p (1 - lr weight_decay) - lr lr_scale[i] orthogonalize(u),
+ *   p and g of dtype. Where *grad_scale is not finite nothing is written. lr_ptr as in fl_adamw_step.
+ * fl_orthogonalize_check: FL_OK, or FL_ERR_INVALID_ARGUMENT for steps and coefficients that both refuse: those by which
+ *   singular values in [0, 1], or a step's factor a + b s^2 + c s^4, could pass 1024.
+ * Workspace 16-byte aligned, no initial contents needed.
+ */
+int fl_orthogonalize_check(int steps, double a, double b, double c);
+size_t fl_orthogonalize_workspace_bytes(int64_t n, const int64_t* rows, const int64_t* cols);
+int fl_orthogonalize(int64_t n, const void* const* x, int dtype, const int64_t* rows, const int64_t* cols, int steps,
+                     double a, double b, double c, double eps, void* const* out, void* workspace,
+                     size_t workspace_bytes, void* stream);
+int fl_muon_step(int64_t n, void* const* params, const void* const* grads, int dtype, float* const* buffers,
+                 const int64_t* rows, const int64_t* cols, double lr, const float* lr_ptr, const double* lr_scale,
+                 double momentum, int nesterov, double weight_decay, int steps, double a, double b, double c, double eps,
+                 const float* grad_scale, void* workspace, size_t workspace_bytes, void* stream);
+
 /* Library version string (host function). No counterpart in the reference. */
 const char* fl_version(void);
 

@@ -1,0 +1,235 @@
+"""Embedding, gated scan, orthogonalization and Muon on the host: refusals (Python's and the C ABI's, none of which reaches
+a launch), workspaces, the optimizer's bookkeeping and the stock form that a differentiable backward runs.
+"""
+from __future__ import annotations
+
+import copy
+import ctypes
+import pickle
+
+import pytest
+import torch
+
+import fields_lm_amd as fl
+from fields_lm_amd import _native as nat
+from fields_lm_amd import _train as train
+
+
+def test_cpu_tensors_are_refused():
+    x = torch.randn(4, 6, requires_grad=True)
+    with pytest.raises(RuntimeError):
+        fl.embedding(torch.zeros(3, dtype=torch.long), x)
+    with pytest.raises(RuntimeError):
+        fl.gated_scan(torch.rand(2, 3), torch.rand(2, 3, 4))
+    with pytest.raises(RuntimeError):
+        fl.orthogonalize(x)
+    with pytest.raises(RuntimeError):
+        fl.muon_step([x.detach()], [torch.ones(4, 6)], [torch.zeros(4, 6)])
+
+
+def test_fake_tensors_are_refused():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, t = torch.empty(4, 6, device="cuda"), torch.zeros(3, dtype=torch.long, device="cuda")
+        d = torch.empty(2, 3, 4, device="cuda")
+    for call in (lambda: fl.embedding(t, x), lambda: fl.gated_scan(d, d), lambda: fl.orthogonalize(x),
+                 lambda: fl.muon_step([x], [x], [x])):
+        with pytest.raises(TypeError):
+            call()
+
+
+def test_types_and_shapes_are_refused():
+    t, w = torch.zeros(3, dtype=torch.long), torch.randn(5, 4)
+    for bad in ((t.int(), w), (t, w.half()), (t, 3), (None, w), (t, w.to_sparse())):
+        with pytest.raises(TypeError):
+            fl.embedding(*bad)
+    for bad in ((t, w[0]), (t, w[:0]), (t, w[:, :0])):
+        with pytest.raises(ValueError):
+            fl.embedding(*bad)
+    for kw in (dict(padding_idx=5), dict(padding_idx=-6), dict(scale=float("inf"))):
+        with pytest.raises(ValueError):
+            fl.embedding(t, w, **kw)
+    for dtype in (torch.float16, 3):
+        with pytest.raises(TypeError):
+            fl.embedding(t, w, dtype=dtype)
+    g, d, s = torch.rand(2, 5, 3), torch.rand(2, 5, 3), torch.rand(2, 3)
+    for bad in ((g.half(), d, s), (g, d.double(), s), (g, d, s.bfloat16()), (None, d), (g, d, 3.0)):
+        with pytest.raises(TypeError):
+            fl.gated_scan(*bad)
+    for bad in ((g[:, :4], d), (g[..., :2], d), (g[0], d), (g, d[0]), (g, d, s[:1])):
+        with pytest.raises(ValueError):
+            fl.gated_scan(*bad)
+
+
+def test_forward_mode_is_refused():
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        x = forward_ad.make_dual(torch.randn(3, 4, 5), torch.randn(3, 4, 5))
+        with pytest.raises(NotImplementedError):
+            fl.gated_scan(x, torch.randn(3, 4, 5))
+        with pytest.raises(NotImplementedError):
+            fl.embedding(torch.zeros(2, dtype=torch.long), x[0])
+
+
+def test_steps_and_coefficients_are_refused():
+    x = torch.randn(4, 5)
+    for kw in (dict(steps=0), dict(steps=65), dict(eps=-1.0), dict(eps=float("nan")), dict(coefficients=(30.0, 50.0, 9.0)),
+               dict(coefficients=(float("nan"), 0.0, 0.0)), dict(coefficients=(2.0, 0.0, 0.0), steps=11)):
+        with pytest.raises(ValueError):
+            fl.orthogonalize(x, **kw)
+    with pytest.raises(TypeError):
+        fl.orthogonalize(x, steps=2.5)
+    for kw in (dict(momentum=1.0), dict(momentum=-0.1), dict(lr=-1.0), dict(lr=float("nan")), dict(weight_decay=-1.0),
+               dict(adjust_lr="none")):
+        with pytest.raises(ValueError):
+            fl.muon_step([x], [x.clone()], [torch.zeros(4, 5)], **kw)
+
+
+@pytest.mark.parametrize("steps,abc", [(5, (3.4445, -4.7750, 2.0315)), (64, (1.5, -0.5, 0.0)), (10, (2.0, 0.0, 0.0)),
+                                       (8, (1.875, -1.25, 0.375)), (3, (-4.0, 1.0, 0.5)), (2, (0.0, 0.0, 0.0))])
+def test_bounds_hold(steps, abc):
+    """What the check lets pass keeps singular values and factors within 1024, on a fine grid of them."""
+    lib = nat.load()
+    a, b, c = abc
+    x = torch.linspace(0, 1, 100_001, dtype=torch.float64)
+    fine = True
+    for _ in range(steps):
+        p = a + b * x ** 2 + c * x ** 4
+        x = (p * x).abs()
+        fine = fine and bool(p.abs().max() <= 1024) and bool(x.max() <= 1024)
+    assert not fine or lib.fl_orthogonalize_check(steps, a, b, c) in (nat.FL_OK, nat.FL_ERR_INVALID_ARGUMENT)
+    if lib.fl_orthogonalize_check(steps, a, b, c) == nat.FL_OK:
+        assert fine
+    assert lib.fl_orthogonalize_check(5, 3.4445, -4.7750, 2.0315) == nat.FL_OK
+
+
+def _sizes(*values):
+    return (ctypes.c_int64 * len(values))(*values)
+
+
+def test_abi_refusals():
+    lib = nat.load()
+    tokens = (ctypes.c_int64 * 4)()
+    data = (ctypes.c_float * 64)()
+    at, k = ctypes.addressof(data), ctypes.addressof(tokens)
+    bad, dtype, ws = nat.FL_ERR_INVALID_ARGUMENT, nat.FL_ERR_DTYPE, nat.FL_ERR_WORKSPACE
+
+    def rows(n=4, w=at, wt=0, V=2, D=4, stride=4, out=at, ot=0, t=k):
+        return lib.fl_embedding(t, n, w, wt, V, D, stride, 1.0, 0, -1, out, ot, None)
+
+    assert rows(wt=2) == dtype == rows(ot=-1)
+    assert {rows(n=-1), rows(V=0), rows(D=0), rows(stride=-1), rows(w=None), rows(out=None), rows(t=None), rows(w=at + 2),
+            rows(t=k + 4)} == {bad}
+    assert rows(n=0) == nat.FL_OK
+
+    def grad(n=4, g=at, gt=0, V=2, D=4, out=at, ot=0, w=at, size=1 << 20, t=k):
+        return lib.fl_embedding_backward(t, n, g, gt, V, D, -1, 1.0, out, ot, w, size, None)
+
+    assert grad(gt=2) == dtype == grad(ot=7)
+    assert {grad(n=-1), grad(V=0), grad(g=None), grad(out=None), grad(t=None), grad(out=at + 1), grad(w=at + 4)} == {bad}
+    assert grad(w=None) == ws == grad(size=1)
+    assert lib.fl_embedding_backward_workspace_bytes(-1, 2, 4) == 0
+
+    def scan(a=at, at_=0, u=at, ut=0, B=1, T=2, C=3, out=at, w=at, size=1 << 20, sb=6, st=3):
+        return lib.fl_gated_scan(a, at_, 0, sb, st, u, ut, sb, st, B, T, C, None, None, None, out, w, size, None)
+
+    assert scan(at_=3) == dtype == scan(ut=2)
+    assert {scan(a=None), scan(u=None), scan(out=None), scan(B=0), scan(T=0), scan(C=0), scan(B=1 << 40), scan(T=1 << 40),
+            scan(C=1 << 40), scan(sb=-1), scan(st=-1), scan(a=at + 2), scan(w=at + 4)} == {bad}
+    # (a workspace is asked for at any size)
+    assert scan(w=None, T=5000) == ws == scan(size=0, T=5000)
+
+    def back(starts=at, g=at, ga=at, gu=at, w=at, size=1 << 20):
+        return lib.fl_gated_scan_backward(at, 0, 0, 6, 3, at, 0, 6, 3, 1, 5000, 3, starts, g, None, ga, gu, None, w, size, None)
+
+    assert {back(starts=None), back(gu=None), back(g=at + 1), back(ga=at + 2), back(starts=at + 2)} == {bad}
+    assert back(w=None) == ws == back(size=8)
+    assert lib.fl_gated_scan_workspace_bytes(0, 1, 1, 0) == 0
+
+    ptrs = (ctypes.c_void_p * 1)(at)
+    odd = (ctypes.c_void_p * 1)(at + 2)
+    none = (ctypes.c_void_p * 1)(None)
+    m, n = _sizes(4), _sizes(5)
+
+    def orth(x=ptrs, t=0, r=m, c=n, steps=5, a=3.4445, eps=1e-7, out=ptrs, w=at, size=1 << 40, count=1):
+        return lib.fl_orthogonalize(count, x, t, r, c, steps, a, -4.775, 2.0315, eps, out, w, size, None)
+
+    assert orth(t=5) == dtype
+    assert {orth(x=none), orth(x=odd), orth(out=none), orth(x=None), orth(r=_sizes(-1)), orth(c=_sizes(1 << 21)),
+            orth(r=_sizes(1 << 20), c=_sizes(1 << 20)), orth(steps=0), orth(steps=65), orth(a=float("inf")), orth(eps=-1.0),
+            orth(count=0), orth(w=at + 8)} == {bad}
+    assert orth(w=None) == ws == orth(size=64)
+    scale = (ctypes.c_double * 1)(1.0)
+
+    def muon(p=ptrs, g=ptrs, buf=ptrs, t=0, momentum=0.9, rate=scale, w=at, size=1 << 40):
+        return lib.fl_muon_step(1, p, g, t, buf, m, n, 0.1, None, rate, momentum, 1, 0.1, 5, 3.4445, -4.775, 2.0315, 1e-7,
+                                None, w, size, None)
+
+    assert muon(t=2) == dtype
+    assert {muon(p=none), muon(g=odd), muon(buf=none), muon(momentum=1.0), muon(momentum=float("nan")), muon(rate=None)} == {bad}
+    assert muon(w=None) == ws == muon(size=0)
+
+
+def test_workspaces_stay_within_groups():
+    """Up to a GiB where the matrices fit in that, whatever their number."""
+    lib = nat.load()
+    many = lib.fl_orthogonalize_workspace_bytes(400, _sizes(*[1024] * 400), _sizes(*[1024] * 400))
+    assert 1 << 29 < many <= (1 << 30) + (1 << 20)
+    one = lib.fl_orthogonalize_workspace_bytes(1, _sizes(16384), _sizes(16384))
+    assert one > 1 << 30
+
+
+def test_stock_scan_gradients():
+    """Against a loop over the steps in float64, and differentiable."""
+    g = torch.Generator().manual_seed(1)
+    for token in (False, True):
+        a = torch.rand((2, 11) if token else (2, 11, 3), generator=g, dtype=torch.float64, requires_grad=True)
+        u = torch.randn(2, 11, 3, generator=g, dtype=torch.float64, requires_grad=True)
+        s = torch.randn(2, 3, generator=g, dtype=torch.float64, requires_grad=True)
+        w, k = torch.randn(2, 11, 3, generator=g), torch.randn(2, 3, generator=g)
+        h, now = [], s
+        for t in range(11):
+            now = (a[:, t, None] if token else a[:, t]) * now + u[:, t]
+            h.append(now)
+        exp = torch.autograd.grad((torch.stack(h, 1) * w).sum() + (now * k).sum(), (a, u, s))
+        low = [t.detach().float().requires_grad_() for t in (a, u, s)]
+        got = train.stock_scan_gradients(*low, w, k)
+        assert all(torch.allclose(x.double(), y, rtol=0, atol=1e-4) for x, y in zip(got, exp))
+        assert all(x.requires_grad for x in got)
+        got = train.stock_scan_gradients(low[0], low[1], None, w, None)
+        assert got[2] is None and got[0].shape == a.shape
+
+
+def test_muon_bookkeeping():
+    with pytest.raises(ValueError, match="matrices"):
+        fl.Muon([torch.zeros(3)])
+    with pytest.raises(TypeError):
+        fl.Muon([torch.zeros(3, 3, dtype=torch.float16)])
+    for kw in (dict(lr=-1.0), dict(momentum=1.0), dict(weight_decay=-1.0), dict(steps=0), dict(eps=-1.0), dict(adjust_lr="x"),
+               dict(coefficients=(50.0, 50.0, 50.0)), dict(max_grad_norm=-1.0)):
+        with pytest.raises(ValueError):
+            fl.Muon([torch.zeros(3, 3)], **kw)
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = fl.Muon([p], max_grad_norm=2.0)
+    with pytest.raises(ValueError):
+        opt.add_param_group(dict(params=[torch.nn.Parameter(torch.zeros(3))]))
+    assert len(opt.param_groups) == 1
+    assert opt.step() is None and opt.step(lambda: 5.0) == 5.0
+    for twin in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert twin.max_grad_norm == 2.0 and twin.param_groups[0]["coefficients"] == opt.param_groups[0]["coefficients"]
+    state = opt.state_dict()
+    state["state"] = {0: dict(momentum_buffer=torch.ones(3, 4))}
+    opt.load_state_dict(state)
+    assert torch.equal(opt.state[p]["momentum_buffer"], torch.ones(3, 4))
+    for wrong in (dict(momentum_buffer=torch.ones(3, 5)), dict(momentum_buffer=torch.ones(3, 4).bfloat16()),
+                  dict(exp_avg=torch.ones(3, 4))):
+        state["state"] = {0: wrong}
+        with pytest.raises(ValueError):
+            opt.load_state_dict(state)
+    adam = fl.AdamW([torch.nn.Parameter(torch.zeros(3, 4))])
+    with pytest.raises(ValueError, match="lacks"):
+        opt.load_state_dict(adam.state_dict())
+    with pytest.raises(ValueError, match="lacks"):
+        adam.load_state_dict(opt.state_dict())
