@@ -2,148 +2,464 @@
 //   h_t = a_t h_{t-1} + u_t,  h_{-1} = state_in or 0,          a gate to every channel or one to a token;
 //   g_t = dh_t + a_{t+1} g_{t+1}  (the last step's carry is the final state's gradient),
 //   du_t = g_t,  da_t = g_t h_{t-1} (summed over the channels where they share a gate),  dstate_in = a_0 g_0.
-// The time is cut into tiles; a tile is a map h -> P h + S (P the product of its gates, S its end from 0), and maps
-// compose. One launch forms the tiles' maps, one composes them, one runs every tile from its start.
+//
+// A run of steps is a map h -> P h + S (P the product of its gates, S its end from 0), and maps compose; the reverse
+// recurrence's maps have the same P. A block takes a tile of 256 steps and 64 channels and holds it in registers, 16 lanes
+// with four channels each to a segment of consecutive steps. It composes its segments' maps through the LDS, gets the
+// tile's start from the tiles before it, and runs its steps from there: inputs are read once. The backward pass forms the
+// states again from each tile's start, which the forward pass keeps (4 bytes to 256 steps), in place of reading them:
+// those are rounded to the drive's type, and cost as much to read as the drive.
+//
+// Tiles of a chain (a sequence's 64 channels) find their start by looking back: each publishes its map, then its end, as
+// words of a value and a mark that it is there, and composes the maps of those before it up to the first that has
+// published its end. Tiles are taken in the order in which blocks start, from a counter: a tile waits only for tiles that
+// are running or done, so that every wait ends. The words are cleared by a launch before.
 #include "fl_common.h"
+
+#include <type_traits>
 
 namespace {
 
 using namespace fl;
 
-constexpr int kTile = 256;  // steps
+constexpr int kTile = 256;     // steps
+constexpr int kChannels = 64;  // of a chain
+constexpr int kWords = 3 * kChannels;  // of a tile: P and S of its map, its end
+constexpr int kBehind = 4;     // tiles whose words are loaded at a time
+constexpr uint32_t kMaxPolls = 1u << 20;  // of a wait that never ends; its tile's results are NaN
 constexpr int64_t kMaxB = 65535, kMaxC = 64 * 65535, kMaxT = (int64_t)1 << 30;
 
 struct Scan {
   const void* gate;
   const void* drive;
   int64_t gate_b, gate_t, drive_b, drive_t;  // strides in elements
-  int64_t T, C, tiles;
-  float2* maps;  // [B, tiles, C]
+  int64_t T, C;
+  int tiles, groups;   // of a chain, of 64 channels
+  unsigned chains;
+  uint32_t* ticket;    // null where chains have one tile
+  uint64_t* words;     // [tiles, chains, kWords]
 };
 
-template <typename GT, bool TOKEN>
-__device__ __forceinline__ float gate_at(const Scan& s, int64_t b, int64_t t, int64_t c) {
-  return load_as<GT>(static_cast<const GT*>(s.gate) + b * s.gate_b + t * s.gate_t + (TOKEN ? 0 : c));
-}
-template <typename DT>
-__device__ __forceinline__ float drive_at(const Scan& s, int64_t b, int64_t t, int64_t c) {
-  return load_as<DT>(static_cast<const DT*>(s.drive) + b * s.drive_b + t * s.drive_t + c);
-}
-
-template <typename GT, typename DT, bool TOKEN>
-__global__ __launch_bounds__(64) void fl_gated_map_kernel(const Scan s) {
-  const int64_t b = blockIdx.z, tile = blockIdx.x, c = (int64_t)blockIdx.y * 64 + threadIdx.x;
-  if (c >= s.C) return;
-  const int64_t t0 = tile * kTile, t1 = t0 + kTile < s.T ? t0 + kTile : s.T;
-  float p = 1.f, h = 0.f;
-  for (int64_t t = t0; t < t1; ++t) {
-    const float a = gate_at<GT, TOKEN>(s, b, t, c);
-    h = fmaf(a, h, drive_at<DT>(s, b, t, c));
-    p *= a;
-  }
-  s.maps[(b * s.tiles + tile) * s.C + c] = make_float2(p, h);
-}
-
-// the states that tiles start from
-__global__ __launch_bounds__(64) void fl_gated_carry_kernel(const float2* __restrict__ maps, int64_t tiles, int64_t C,
-                                                            const float* __restrict__ state_in,
-                                                            float* __restrict__ starts, float* __restrict__ state_out) {
-  const int64_t b = blockIdx.y, c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (c >= C) return;
-  float h = state_in ? state_in[b * C + c] : 0.f;
-  for (int64_t i = 0; i < tiles; ++i) {
-    const int64_t at = (b * tiles + i) * C + c;
-    const float2 m = maps[at];
-    starts[at] = h;
-    h = fmaf(m.x, h, m.y);
-  }
-  if (state_out) state_out[b * C + c] = h;
-}
-
-template <typename GT, typename DT, bool TOKEN>
-__global__ __launch_bounds__(64) void fl_gated_scan_kernel(const Scan s, const float* __restrict__ starts,
-                                                           DT* __restrict__ out) {
-  const int64_t b = blockIdx.z, tile = blockIdx.x, c = (int64_t)blockIdx.y * 64 + threadIdx.x;
-  if (c >= s.C) return;
-  const int64_t t0 = tile * kTile, t1 = t0 + kTile < s.T ? t0 + kTile : s.T;
-  float h = starts[(b * s.tiles + tile) * s.C + c];
-  for (int64_t t = t0; t < t1; ++t) {
-    h = fmaf(gate_at<GT, TOKEN>(s, b, t, c), h, drive_at<DT>(s, b, t, c));
-    store_as(out + (b * s.T + t) * s.C + c, h);
-  }
-}
-
-// the reverse map of a tile: what its steps' gradients and the carry into its end make of the carry out of its start
-template <typename GT, typename DT, bool TOKEN>
-__global__ __launch_bounds__(64) void fl_gated_back_map_kernel(const Scan s, const DT* __restrict__ g_out) {
-  const int64_t b = blockIdx.z, tile = blockIdx.x, c = (int64_t)blockIdx.y * 64 + threadIdx.x;
-  if (c >= s.C) return;
-  const int64_t t0 = tile * kTile, t1 = t0 + kTile < s.T ? t0 + kTile : s.T;
-  float p = 1.f, k = 0.f;
-  for (int64_t t = t1 - 1; t >= t0; --t) {
-    const float a = gate_at<GT, TOKEN>(s, b, t, c);
-    k = a * (k + (g_out ? load_as<DT>(g_out + (b * s.T + t) * s.C + c) : 0.f));
-    p *= a;
-  }
-  s.maps[(b * s.tiles + tile) * s.C + c] = make_float2(p, k);
-}
-
-__global__ __launch_bounds__(64) void fl_gated_back_carry_kernel(float2* __restrict__ maps, int64_t tiles, int64_t C,
-                                                                 const float* __restrict__ g_state,
-                                                                 float* __restrict__ g_state_in) {
-  const int64_t b = blockIdx.y, c = (int64_t)blockIdx.x * 64 + threadIdx.x;
-  if (c >= C) return;
-  float k = g_state ? g_state[b * C + c] : 0.f;
-  for (int64_t i = tiles - 1; i >= 0; --i) {
-    const int64_t at = (b * tiles + i) * C + c;
-    const float2 m = maps[at];
-    maps[at].x = k;  // the carry into the tile's end
-    k = fmaf(m.x, k, m.y);
-  }
-  if (g_state_in) g_state_in[b * C + c] = k;
-}
-
-// A tile's states again, kept in the LDS, then its steps from the last to the first.
-template <typename GT, typename DT, bool TOKEN>
-__global__ __launch_bounds__(64) void fl_gated_back_kernel(const Scan s, const float* __restrict__ starts,
-                                                           const DT* __restrict__ g_out, GT* __restrict__ g_gate,
-                                                           float* __restrict__ part, DT* __restrict__ g_drive) {
-  __shared__ float s_h[kTile][64];
-  const int lane = threadIdx.x;
-  const int64_t b = blockIdx.z, tile = blockIdx.x, c = (int64_t)blockIdx.y * 64 + lane;
-  const bool ok = c < s.C;
-  const int64_t cc = ok ? c : s.C - 1;
-  const int64_t t0 = tile * kTile, t1 = t0 + kTile < s.T ? t0 + kTile : s.T;
-  float h = starts[(b * s.tiles + tile) * s.C + cc];
-  for (int64_t t = t0; t < t1; ++t) {
-    s_h[t - t0][lane] = h;  // the state before the step
-    h = fmaf(gate_at<GT, TOKEN>(s, b, t, cc), h, drive_at<DT>(s, b, t, cc));
-  }
-  float k = s.maps[(b * s.tiles + tile) * s.C + cc].x;
-  for (int64_t t = t1 - 1; t >= t0; --t) {
-    const int64_t at = (b * s.T + t) * s.C + cc;
-    const float g = (g_out ? load_as<DT>(g_out + at) : 0.f) + k;
-    const float da = g * s_h[t - t0][lane];
-    if (ok) store_as(g_drive + at, g);
-    if (!g_gate) {
-    } else if constexpr (TOKEN) {
-      const float sum = wave_sum(ok ? da : 0.f);
-      if (lane == 0) part[((int64_t)blockIdx.y * gridDim.z + b) * s.T + t] = sum;
+// four values of a row as they lie, `left` of them there
+template <typename T>
+struct Four;
+template <>
+struct Four<float> {
+  float v[4];
+  __device__ __forceinline__ void load(const float* p, int64_t left) {
+    if (left >= 4) {
+      const u32x4 r = *reinterpret_cast<const u32x4_any*>(p);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
     } else {
-      if (ok) store_as(g_gate + at, da);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.f;
     }
-    k = gate_at<GT, TOKEN>(s, b, t, cc) * g;
   }
+  __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = x;
+  }
+  __device__ __forceinline__ float operator[](int i) const { return v[i]; }
+};
+template <>
+struct Four<bf16_bits> {
+  uint32_t w[2];
+  __device__ __forceinline__ void load(const bf16_bits* p, int64_t left) {
+    if (left >= 4) {
+      const u32x2 r = *reinterpret_cast<const u32x2_any*>(p);
+      w[0] = r[0];
+      w[1] = r[1];
+    } else {
+      w[0] = w[1] = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < left) w[i >> 1] |= (uint32_t)p[i] << (16 * (i & 1));
+    }
+  }
+  __device__ __forceinline__ void fill(float x) { w[0] = w[1] = bf16_bits_of(x) * 0x10001u; }
+  __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
+};
+__device__ __forceinline__ void store4(float* p, int64_t left, const float* v) {
+  if (left >= 4) {
+    *reinterpret_cast<u32x4_any*>(p) =
+        u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) p[i] = v[i];
+  }
+}
+__device__ __forceinline__ void store4(bf16_bits* p, int64_t left, const float* v) {
+  if (left >= 4) {
+    *reinterpret_cast<u32x2_any*>(p) = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < left) store_as(p + i, v[i]);
+  }
+}
+
+// lane J of each 16 in all of them (every lane has to be there)
+template <int J>
+__device__ __forceinline__ float of_lane(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x150 + J, 0xf, 0xf, true));
+}
+// the sum over each 16 lanes, in all of them
+__device__ __forceinline__ float row_sum(float v) {
+  v = dpp_add<0xb1>(v);
+  v = dpp_add<0x4e>(v);
+  v = dpp_add<0x141>(v);
+  return dpp_add<0x140>(v);
+}
+
+// The gates of a segment's STEPS steps: a value to every channel, or (TOKEN) one to a step, held by the lane of its number.
+template <typename GT, bool TOKEN, int STEPS>
+struct Gates;
+template <typename GT, int STEPS>
+struct Gates<GT, false, STEPS> {
+  Four<GT> v[STEPS];
+  __device__ __forceinline__ void load(const GT* p, int64_t step, int n, int, int64_t left) {
+#pragma unroll
+    for (int j = 0; j < STEPS; ++j) {
+      v[j].fill(1.f);
+      if (j < n && left > 0) v[j].load(p + j * step, left);
+    }
+  }
+  template <int J>
+  __device__ __forceinline__ float at(int i) const { return v[J][i]; }
+};
+template <typename GT, int STEPS>
+struct Gates<GT, true, STEPS> {
+  float v;
+  __device__ __forceinline__ void load(const GT* p, int64_t step, int n, int lane, int64_t) {
+    v = lane < n ? load_as<GT>(p + lane * step) : 1.f;
+  }
+  template <int J>
+  __device__ __forceinline__ float at(int) const { return of_lane<J>(v); }
+};
+
+// The product of two runs' gates. One too small for a float is kept off 0, which is a closed gate's alone: an infinite state
+// before such a run is infinite behind it, as it is step by step.
+__device__ __forceinline__ float kept(float product, bool closed) {
+  return product == 0.f && !closed ? __builtin_copysignf(0x1p-149f, product) : product;
+}
+__device__ __forceinline__ float times(float p, float q) { return kept(p * q, p == 0.f || q == 0.f); }
+
+template <int N, int I = 0, typename F>
+__device__ __forceinline__ void each(F f) {
+  if constexpr (I < N) {
+    f(std::integral_constant<int, I>());
+    each<N, I + 1>(f);
+  }
+}
+template <int N, typename F>
+__device__ __forceinline__ void each_back(F f) {
+  each<N>([&](auto i) { f(std::integral_constant<int, N - 1 - decltype(i)::value>()); });
+}
+
+__device__ __forceinline__ void publish(uint64_t* to, float v) {
+  __hip_atomic_store(to, (uint64_t)__float_as_uint(v) << 32 | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ uint64_t published(const uint64_t* from) {
+  return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ bool there(uint64_t w) { return __all((uint32_t)w == 1u); }
+__device__ __forceinline__ float value_of(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
+
+// What enters the tile at place `place` of its chain: the maps of the tiles before it, nearest first, up to one that has
+// published its end. `words`: the tile's own, lane's channel; `back`: words from a tile to the one before it.
+__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, int place) {
+  float p = 1.f, s = 0.f;
+  uint32_t polls = 0;
+  for (int i = 1;;) {
+    uint64_t w[kBehind][3];
+#pragma unroll
+    for (int q = 0; q < kBehind; ++q) {
+      const uint64_t* from = words - (int64_t)min(i + q, place) * back;
+#pragma unroll
+      for (int k = 0; k < 3; ++k) w[q][k] = published(from + k * kChannels);
+    }
+    int q = 0;
+    bool stop = false;
+#pragma unroll
+    for (int r = 0; r < kBehind; ++r) {
+      if (stop || i + r > place) continue;
+      if (there(w[r][2])) return fmaf(p, value_of(w[r][2]), s);
+      if (there(w[r][0]) && there(w[r][1])) {
+        s = fmaf(p, value_of(w[r][1]), s);
+        p = times(p, value_of(w[r][0]));
+        q = r + 1;
+      } else {
+        stop = true;
+      }
+    }
+    i += q;
+    if (q == 0) {
+      if (++polls >= kMaxPolls) return __uint_as_float(0x7fc00000u);
+      __builtin_amdgcn_s_sleep(1);
+    }
+  }
+}
+
+// Where a block's tile lies
+struct Place {
+  int place, tile;  // in the order of the scan, in time
+  unsigned chain;
+  int64_t b, c0;
+};
+template <bool BACK>
+__device__ __forceinline__ Place place_of(const Scan& s, uint32_t* s_ticket) {
+  unsigned t = blockIdx.x;
+  if (s.ticket) {
+    if (threadIdx.x == 0)
+      *s_ticket = __hip_atomic_fetch_add(s.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    t = (unsigned)uniform((int)*s_ticket);
+  }
+  Place r;
+  r.place = (int)(t / s.chains);
+  r.chain = t - (unsigned)r.place * s.chains;
+  r.tile = BACK ? s.tiles - 1 - r.place : r.place;
+  r.b = r.chain / (unsigned)s.groups;
+  r.c0 = (int64_t)(r.chain - (unsigned)r.b * (unsigned)s.groups) * kChannels;
+  return r;
+}
+
+constexpr int kForwardSteps = 16, kBackSteps = 8;  // of a segment
+constexpr int kForwardThreads = kTile / kForwardSteps * 16, kBackThreads = kTile / kBackSteps * 16;
+
+template <typename GT, typename DT, bool TOKEN>
+__global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Scan s, const float* __restrict__ state_in,
+                                                                        float* __restrict__ state_out,
+                                                                        float* __restrict__ starts,
+                                                                        DT* __restrict__ out) {
+  constexpr int STEPS = kForwardSteps, SEGS = kTile / STEPS;
+  __shared__ float s_p[SEGS][kChannels], s_s[SEGS][kChannels];
+  __shared__ uint32_t s_ticket;
+  const Place at = place_of<false>(s, &s_ticket);
+  const int seg = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int64_t c = at.c0 + lane * 4, left = s.C - c, t0 = (int64_t)at.tile * kTile + seg * STEPS;
+  const int n = (int)(s.T - t0 < STEPS ? (s.T > t0 ? s.T - t0 : 0) : STEPS);
+  Gates<GT, TOKEN, STEPS> a;
+  Four<DT> u[STEPS];
+  a.load(static_cast<const GT*>(s.gate) + at.b * s.gate_b + t0 * s.gate_t + (TOKEN ? 0 : c), s.gate_t, n, lane, left);
+  const DT* from = static_cast<const DT*>(s.drive) + at.b * s.drive_b + t0 * s.drive_t + c;
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) {
+    u[j].fill(0.f);
+    if (j < n && left > 0) u[j].load(from + j * s.drive_t, left);
+  }
+  f32x4 p = {1.f, 1.f, 1.f, 1.f}, least = p, h = {0.f, 0.f, 0.f, 0.f};
+  each<STEPS>([&](auto j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float g = a.template at<decltype(j)::value>(i);
+      h[i] = fmaf(g, h[i], u[decltype(j)::value][i]);
+      p[i] *= g;
+      least[i] = fminf(least[i], fabsf(g));
+    }
+  });
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = kept(p[i], least[i] == 0.f);
+  *reinterpret_cast<f32x4*>(&s_p[seg][lane * 4]) = p;
+  *reinterpret_cast<f32x4*>(&s_s[seg][lane * 4]) = h;
+  __syncthreads();
+  if (threadIdx.x < kChannels) {
+    const int ch = threadIdx.x;
+    const int64_t k = at.c0 + ch;
+    float ps[SEGS], ss[SEGS], pt = 1.f, st = 0.f;
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+      ps[i] = s_p[i][ch];
+      ss[i] = s_s[i][ch];
+    }
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+      const float pi = ps[i], si = ss[i];
+      ps[i] = pt;
+      ss[i] = st;
+      st = fmaf(pi, st, si);
+      pt = times(pt, pi);
+    }
+    uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
+    float first;
+    const bool more = at.place + 1 < s.tiles;
+    if (at.place == 0) {
+      first = state_in && k < s.C ? state_in[at.b * s.C + k] : 0.f;
+    } else {
+      if (more) {
+        publish(words, pt);
+        publish(words + kChannels, st);
+      }
+      first = look_back(words, (int64_t)s.chains * kWords, at.place);
+    }
+    const float last = fmaf(pt, first, st);
+    if (more) publish(words + 2 * kChannels, last);
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) s_s[i][ch] = fmaf(ps[i], first, ss[i]);
+    if (k < s.C) {
+      if (starts) starts[(at.b * s.tiles + at.tile) * s.C + k] = first;
+      if (state_out && !more) state_out[at.b * s.C + k] = last;
+    }
+  }
+  __syncthreads();
+  h = *reinterpret_cast<const f32x4*>(&s_s[seg][lane * 4]);
+  DT* to = out + (at.b * s.T + t0) * s.C + c;
+  each<STEPS>([&](auto j) {
+    float v[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      h[i] = fmaf(a.template at<decltype(j)::value>(i), h[i], u[decltype(j)::value][i]);
+      v[i] = h[i];
+    }
+    if (decltype(j)::value < n && left > 0) store4(to + decltype(j)::value * s.C, left, v);
+  });
+}
+
+// Wave 0 composes the tile's maps forward from the state it starts from, wave 1 backward from the carry into its end.
+template <typename GT, typename DT, bool TOKEN>
+__global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
+    const Scan s, const float* __restrict__ starts, const DT* __restrict__ g_out, const float* __restrict__ g_state,
+    GT* __restrict__ g_gate, float* __restrict__ part, DT* __restrict__ g_drive, float* __restrict__ g_state_in) {
+  constexpr int STEPS = kBackSteps, SEGS = kTile / STEPS;
+  __shared__ float s_p[SEGS][kChannels], s_h[SEGS][kChannels], s_k[SEGS][kChannels];
+  __shared__ uint32_t s_ticket;
+  const Place at = place_of<true>(s, &s_ticket);
+  const int seg = threadIdx.x >> 4, lane = threadIdx.x & 15;
+  const int64_t c = at.c0 + lane * 4, left = s.C - c, t0 = (int64_t)at.tile * kTile + seg * STEPS;
+  const int n = (int)(s.T - t0 < STEPS ? (s.T > t0 ? s.T - t0 : 0) : STEPS);
+  Gates<GT, TOKEN, STEPS> a;
+  Four<DT> u[STEPS], d[STEPS];
+  a.load(static_cast<const GT*>(s.gate) + at.b * s.gate_b + t0 * s.gate_t + (TOKEN ? 0 : c), s.gate_t, n, lane, left);
+  const DT* from = static_cast<const DT*>(s.drive) + at.b * s.drive_b + t0 * s.drive_t + c;
+  const DT* up = g_out + (at.b * s.T + t0) * s.C + c;
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) {
+    d[j].fill(0.f);
+    if (g_out && j < n && left > 0) d[j].load(up + j * s.C, left);
+  }
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) {
+    u[j].fill(0.f);
+    if (j < n && left > 0) u[j].load(from + j * s.drive_t, left);
+  }
+  f32x4 p = {1.f, 1.f, 1.f, 1.f}, least = p, h = {0.f, 0.f, 0.f, 0.f}, k = {0.f, 0.f, 0.f, 0.f};
+  each<STEPS>([&](auto j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float g = a.template at<decltype(j)::value>(i);
+      h[i] = fmaf(g, h[i], u[decltype(j)::value][i]);
+      p[i] *= g;
+      least[i] = fminf(least[i], fabsf(g));
+    }
+  });
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = kept(p[i], least[i] == 0.f);
+  each_back<STEPS>([&](auto j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = a.template at<decltype(j)::value>(i) * (k[i] + d[decltype(j)::value][i]);
+  });
+  *reinterpret_cast<f32x4*>(&s_p[seg][lane * 4]) = p;
+  *reinterpret_cast<f32x4*>(&s_h[seg][lane * 4]) = h;
+  *reinterpret_cast<f32x4*>(&s_k[seg][lane * 4]) = k;
+  __syncthreads();
+  const int ch = threadIdx.x & 63;
+  const int64_t cc = at.c0 + ch;
+  if (threadIdx.x < 64) {
+    float now = cc < s.C ? starts[(at.b * s.tiles + at.tile) * s.C + cc] : 0.f, ps[SEGS], hs[SEGS];
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+      ps[i] = s_p[i][ch];
+      hs[i] = s_h[i][ch];
+    }
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+      s_h[i][ch] = now;
+      now = fmaf(ps[i], now, hs[i]);
+    }
+  } else if (threadIdx.x < 128) {
+    float ps[SEGS], ks[SEGS], pt = 1.f, kt = 0.f;
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) {
+      ps[i] = s_p[i][ch];
+      ks[i] = s_k[i][ch];
+    }
+#pragma unroll
+    for (int i = SEGS - 1; i >= 0; --i) {
+      const float pi = ps[i], ki = ks[i];
+      ps[i] = pt;
+      ks[i] = kt;
+      kt = fmaf(pi, kt, ki);
+      pt = times(pt, pi);
+    }
+    uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
+    float first;
+    const bool more = at.place + 1 < s.tiles;
+    if (at.place == 0) {
+      first = g_state && cc < s.C ? g_state[at.b * s.C + cc] : 0.f;
+    } else {
+      if (more) {
+        publish(words, pt);
+        publish(words + kChannels, kt);
+      }
+      first = look_back(words, (int64_t)s.chains * kWords, at.place);
+    }
+    const float last = fmaf(pt, first, kt);
+    if (more) publish(words + 2 * kChannels, last);
+#pragma unroll
+    for (int i = 0; i < SEGS; ++i) s_k[i][ch] = fmaf(ps[i], first, ks[i]);
+    if (g_state_in && !more && cc < s.C) g_state_in[at.b * s.C + cc] = last;
+  }
+  __syncthreads();
+  h = *reinterpret_cast<const f32x4*>(&s_h[seg][lane * 4]);
+  k = *reinterpret_cast<const f32x4*>(&s_k[seg][lane * 4]);
+  f32x4 before[STEPS];
+  each<STEPS>([&](auto j) {
+    before[decltype(j)::value] = h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = fmaf(a.template at<decltype(j)::value>(i), h[i], u[decltype(j)::value][i]);
+  });
+  const int64_t row = at.b * s.T + t0;
+  each_back<STEPS>([&](auto jj) {
+    constexpr int j = decltype(jj)::value;
+    float g[4], da[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      g[i] = d[j][i] + k[i];
+      da[i] = g[i] * before[j][i];
+      k[i] = a.template at<j>(i) * g[i];
+    }
+    if (j < n && left > 0) store4(g_drive + (row + j) * s.C + c, left, g);
+    if constexpr (TOKEN) {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum += i < left ? da[i] : 0.f;
+      sum = row_sum(sum);
+      if (g_gate && j < n && lane == 0) {
+        if (s.groups == 1)
+          store_as(g_gate + row + j, sum);
+        else
+          part[(at.c0 / kChannels) * ((int64_t)(s.chains / (unsigned)s.groups) * s.T) + row + j] = sum;
+      }
+    } else {
+      if (g_gate && j < n && left > 0) store4(g_gate + (row + j) * s.C + c, left, da);
+    }
+  });
+}
+
+__global__ __launch_bounds__(256) void fl_gated_clear_kernel(u32x4* __restrict__ p, int64_t n) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) p[i] = u32x4{0, 0, 0, 0};
 }
 
 // the gradient of a token's gate: the sums of its groups of channels, in their order
 template <typename GT>
-__global__ __launch_bounds__(256) void fl_gated_token_kernel(const float* __restrict__ part, int64_t n, int64_t groups,
+__global__ __launch_bounds__(256) void fl_gated_token_kernel(const float* __restrict__ part, int64_t n, int groups,
                                                              GT* __restrict__ g_gate) {
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= n) return;
   float sum = 0.f;
-  for (int64_t k = 0; k < groups; ++k) sum += part[k * n + i];
+  for (int k = 0; k < groups; ++k) sum += part[k * n + i];
   store_as(g_gate + i, sum);
 }
 
@@ -151,40 +467,67 @@ struct Call {
   Scan s;
   int64_t B;
   hipStream_t stream;
-  dim3 tiles() const { return dim3((unsigned)s.tiles, (unsigned)cdiv(s.C, 64), (unsigned)B); }
-  dim3 chains() const { return dim3((unsigned)cdiv(s.C, 64), (unsigned)B); }
+  unsigned blocks() const { return (unsigned)s.tiles * s.chains; }
 };
 
+// bytes of the ticket's line and the words; 0 where chains have one tile
+size_t word_bytes(int64_t B, int64_t T, int64_t C) {
+  const int64_t tiles = cdiv(T, kTile);
+  return tiles > 1 ? 128 + (size_t)(tiles * B * cdiv(C, kChannels)) * kWords * 8 : 0;
+}
+
+void clear(const Call& c, size_t bytes) {
+  if (!c.s.ticket) return;
+  const int64_t n = (int64_t)(bytes / 16);
+  const unsigned blocks = (unsigned)(cdiv(n, 256) < 2048 ? cdiv(n, 256) : 2048);
+  fl_gated_clear_kernel<<<blocks, 256, 0, c.stream>>>(reinterpret_cast<u32x4*>(c.s.ticket), n);
+}
+
 template <typename GT, typename DT, bool TOKEN>
-int forward(const Call& c, const float* state_in, float* state_out, float* starts, void* out) {
-  fl_gated_map_kernel<GT, DT, TOKEN><<<c.tiles(), 64, 0, c.stream>>>(c.s);
-  fl_gated_carry_kernel<<<c.chains(), 64, 0, c.stream>>>(c.s.maps, c.s.tiles, c.s.C, state_in, starts, state_out);
-  fl_gated_scan_kernel<GT, DT, TOKEN><<<c.tiles(), 64, 0, c.stream>>>(c.s, starts, static_cast<DT*>(out));
+int forward(const Call& c, size_t bytes, const float* state_in, float* state_out, float* starts, void* out) {
+  clear(c, bytes);
+  fl_gated_scan_kernel<GT, DT, TOKEN><<<c.blocks(), kForwardThreads, 0, c.stream>>>(c.s, state_in, state_out, starts,
+                                                                                     static_cast<DT*>(out));
   return hip_status(hipGetLastError());
 }
 
 template <typename GT, typename DT, bool TOKEN>
-int backward(const Call& c, const float* starts, const void* g_out, const float* g_state, void* g_gate, void* g_drive,
-             float* g_state_in, float* part) {
-  const DT* g = static_cast<const DT*>(g_out);
-  fl_gated_back_map_kernel<GT, DT, TOKEN><<<c.tiles(), 64, 0, c.stream>>>(c.s, g);
-  fl_gated_back_carry_kernel<<<c.chains(), 64, 0, c.stream>>>(c.s.maps, c.s.tiles, c.s.C, g_state, g_state_in);
-  fl_gated_back_kernel<GT, DT, TOKEN><<<c.tiles(), 64, 0, c.stream>>>(c.s, starts, g, static_cast<GT*>(g_gate), part,
-                                                                       static_cast<DT*>(g_drive));
-  if (TOKEN && g_gate) {
+int backward(const Call& c, size_t bytes, const float* starts, const void* g_out, const float* g_state, void* g_gate,
+             void* g_drive, float* g_state_in, float* part) {
+  clear(c, bytes);
+  fl_gated_back_kernel<GT, DT, TOKEN><<<c.blocks(), kBackThreads, 0, c.stream>>>(
+      c.s, starts, static_cast<const DT*>(g_out), g_state, static_cast<GT*>(g_gate), part, static_cast<DT*>(g_drive),
+      g_state_in);
+  if (TOKEN && g_gate && c.s.groups > 1) {
     const int64_t n = c.B * c.s.T;
-    fl_gated_token_kernel<GT><<<(unsigned)cdiv(n, 256), 256, 0, c.stream>>>(part, n, cdiv(c.s.C, 64),
+    fl_gated_token_kernel<GT><<<(unsigned)cdiv(n, 256), 256, 0, c.stream>>>(part, n, c.s.groups,
                                                                             static_cast<GT*>(g_gate));
   }
   return hip_status(hipGetLastError());
 }
 
 bool sizes_ok(int64_t B, int64_t T, int64_t C) {
-  return B > 0 && T > 0 && C > 0 && B <= kMaxB && C <= kMaxC && T <= kMaxT;
+  return B > 0 && T > 0 && C > 0 && B <= kMaxB && C <= kMaxC && T <= kMaxT &&
+         cdiv(T, kTile) * B <= (((int64_t)1 << 31) - 1) / cdiv(C, kChannels);  // blocks of a launch
 }
 
 bool tensor_ok(const void* p, int dtype, int64_t stride_b, int64_t stride_t) {
   return p && aligned(p, esize(dtype)) && stride_b >= 0 && stride_t >= 0;
+}
+
+// a call without a workspace's need takes any
+bool workspace_ok(const void* workspace, size_t have, size_t need) { return need == 0 || (workspace && have >= need); }
+
+Call call_of(const void* gate, int64_t gate_b, int64_t gate_t, const void* drive, int64_t drive_b, int64_t drive_t,
+             int64_t B, int64_t T, int64_t C, void* workspace, void* stream) {
+  Call c = {};
+  const bool one = cdiv(T, kTile) == 1;
+  c.s = Scan{gate, drive, gate_b, gate_t, drive_b, drive_t, T, C, (int)cdiv(T, kTile), (int)cdiv(C, kChannels),
+             (unsigned)(B * cdiv(C, kChannels)), one ? nullptr : static_cast<uint32_t*>(workspace),
+             one ? nullptr : reinterpret_cast<uint64_t*>(static_cast<char*>(workspace) + 128)};
+  c.B = B;
+  c.stream = static_cast<hipStream_t>(stream);
+  return c;
 }
 
 }  // namespace
@@ -195,8 +538,8 @@ int64_t fl_gated_scan_tile(void) { return kTile; }
 
 size_t fl_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t C, int backward) {
   if (!sizes_ok(B, T, C)) return 0;
-  return (size_t)(B * cdiv(T, kTile) * C) * 8 + (size_t)(B * cdiv(T, kTile) * C) * 4 +
-         (backward ? (size_t)(cdiv(C, 64) * B * T) * 4 : 0);
+  const int64_t groups = cdiv(C, kChannels);
+  return word_bytes(B, T, C) + (backward && groups > 1 ? (size_t)(groups * B * T) * 4 : 0);
 }
 
 #define FL_GATED(CALL, ...)                                                                        \
@@ -217,14 +560,12 @@ int fl_gated_scan(const void* gate, int gate_dtype, int per_token, int64_t gate_
       !tensor_ok(drive, drive_dtype, drive_stride_b, drive_stride_t) || !tensor_ok(out, drive_dtype, 0, 0) ||
       !aligned(state_in, 4) || !aligned(state_out, 4) || !aligned(starts, 4))
     return FL_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < fl_gated_scan_workspace_bytes(B, T, C, 0)) return FL_ERR_WORKSPACE;
+  if (!workspace_ok(workspace, workspace_bytes, fl_gated_scan_workspace_bytes(B, T, C, 0))) return FL_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return FL_ERR_INVALID_ARGUMENT;
-  const int64_t tiles = cdiv(T, kTile);
-  float2* maps = static_cast<float2*>(workspace);
-  if (!starts) starts = reinterpret_cast<float*>(maps + B * tiles * C);
-  const Call c{{gate, drive, gate_stride_b, gate_stride_t, drive_stride_b, drive_stride_t, T, C, tiles, maps}, B,
-               static_cast<hipStream_t>(stream)};
-  FL_GATED(forward, c, state_in, state_out, starts, out)
+  const Call c = call_of(gate, gate_stride_b, gate_stride_t, drive, drive_stride_b, drive_stride_t, B, T, C, workspace,
+                         stream);
+  const size_t bytes = word_bytes(B, T, C);
+  FL_GATED(forward, c, bytes, state_in, state_out, starts, out)
 }
 
 int fl_gated_scan_backward(const void* gate, int gate_dtype, int per_token, int64_t gate_stride_b,
@@ -238,14 +579,13 @@ int fl_gated_scan_backward(const void* gate, int gate_dtype, int per_token, int6
       !tensor_ok(g_drive, drive_dtype, 0, 0) || !aligned(g_out, esize(drive_dtype)) || !starts || !aligned(starts, 4) ||
       !aligned(g_state, 4) || !aligned(g_state_in, 4))
     return FL_ERR_INVALID_ARGUMENT;
-  if (!workspace || workspace_bytes < fl_gated_scan_workspace_bytes(B, T, C, 1)) return FL_ERR_WORKSPACE;
+  if (!workspace_ok(workspace, workspace_bytes, fl_gated_scan_workspace_bytes(B, T, C, 1))) return FL_ERR_WORKSPACE;
   if (!aligned(workspace, 16)) return FL_ERR_INVALID_ARGUMENT;
-  const int64_t tiles = cdiv(T, kTile);
-  float2* maps = static_cast<float2*>(workspace);
-  float* part = reinterpret_cast<float*>(maps + B * tiles * C);
-  const Call c{{gate, drive, gate_stride_b, gate_stride_t, drive_stride_b, drive_stride_t, T, C, tiles, maps}, B,
-               static_cast<hipStream_t>(stream)};
-  FL_GATED(backward, c, starts, g_out, g_state, g_gate, g_drive, g_state_in, part)
+  const Call c = call_of(gate, gate_stride_b, gate_stride_t, drive, drive_stride_b, drive_stride_t, B, T, C, workspace,
+                         stream);
+  const size_t bytes = word_bytes(B, T, C);
+  float* part = reinterpret_cast<float*>(static_cast<char*>(workspace) + bytes);
+  FL_GATED(backward, c, bytes, starts, g_out, g_state, g_gate, g_drive, g_state_in, part)
 }
 
 #undef FL_GATED
