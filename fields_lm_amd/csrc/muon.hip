@@ -17,6 +17,9 @@
 
 #include <math.h>
 
+#include <algorithm>
+#include <vector>
+
 namespace {
 
 using namespace fl;
@@ -28,7 +31,10 @@ typedef _Float16 half_t;
 constexpr int kStage = 3;      // steps between two products with X
 constexpr int kPad = 32;       // rows of planes are a multiple of this long, zeros behind the matrix
 constexpr int kSquares = 5;    // m x m matrices of the workspace
-constexpr int kTile = 128;     // rows and columns of a product's tile
+#ifndef FORCE_TILE
+#define FORCE_TILE 0
+#endif
+constexpr int kForceTile = FORCE_TILE;
 constexpr int kCopyTile = 64;  // of the tile that is laid out by a block
 constexpr int kTable = 56;     // matrices to a launch that sets up their table
 constexpr int kNormChunk = 16384;  // values of a block of the norm
@@ -38,7 +44,7 @@ constexpr int kMaxSteps = 64;
 constexpr double kMaxBound = 1024.0;  // of singular values
 
 struct Mat {
-  half_t* base;    // its planes: X [m, ldn], X^T [n, ldm] twice, squares [m, ldm], each high then low
+  half_t* base;    // X [m, ldn], X^T [n, ldm] twice, squares [m, ldm], 2 ld halves to a row: 32 high parts, their low ones
   const void* g;
   float* buf;
   void* p;
@@ -114,16 +120,21 @@ __global__ __launch_bounds__(256) void fl_muon_norm_kernel(const Mat* __restrict
   if (threadIdx.x == 0) part[blockIdx.x] = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
 }
 
-// high and low part of v
-__device__ __forceinline__ void split(float v, half_t& hi, half_t& lo) {
-  hi = (half_t)v;
-  lo = (half_t)(v - (float)hi);
+// high and low part of v, in bits 15..0 and 31..16
+__device__ __forceinline__ uint32_t split(float v) {
+  const half_t hi = (half_t)v, lo = (half_t)(v - (float)hi);
+  return (uint32_t)__builtin_bit_cast(unsigned short, hi) | (uint32_t)__builtin_bit_cast(unsigned short, lo) << 16;
 }
+// where a row of halves has the high part of column c; its low part is kPad further on
+__device__ __forceinline__ int64_t column(int64_t c) { return (c >> 5) * 64 + (c & 31); }
+// the high (or low) parts of two values
+__device__ __forceinline__ uint32_t highs(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x05040100); }
+__device__ __forceinline__ uint32_t lows(uint32_t a, uint32_t b) { return __builtin_amdgcn_perm(b, a, 0x07060302); }
 
 // X = G / (|G| + eps) times x_scale, as planes of X and of X^T, a tile of 64 x 64 to a block.
 __global__ __launch_bounds__(256) void fl_muon_copy_kernel(const Mat* __restrict__ mats, int n, const Update u,
                                                            const double* __restrict__ part, double eps, float x_scale) {
-  __shared__ float s_x[kCopyTile][kCopyTile + 1];
+  __shared__ uint32_t s_x[kCopyTile][kCopyTile + 1];
   __shared__ double s_sum[4];
   const int i = matrix_of<&Mat::first_copy>(mats, n, blockIdx.x);
   const Mat& k = mats[i];
@@ -148,7 +159,6 @@ __global__ __launch_bounds__(256) void fl_muon_copy_kernel(const Mat* __restrict
   const int across = (int)((ld_r + kCopyTile - 1) / kCopyTile), tile = (int)blockIdx.x - k.first_copy;
   const int r0 = tile / across * kCopyTile, c0 = tile % across * kCopyTile;
   const float scale = u.grad_scale ? *u.grad_scale : 1.f;
-  const int64_t plane_s = rows * ld_r, plane_t = cols * ld_c;
   for (int j = threadIdx.x; j < kCopyTile * kCopyTile; j += 256) {
     const int r = r0 + j / kCopyTile, c = c0 + j % kCopyTile;
     float v = 0.f;
@@ -161,22 +171,28 @@ __global__ __launch_bounds__(256) void fl_muon_copy_kernel(const Mat* __restrict
       }
       v = (float)((double)v * inv);
     }
-    s_x[j / kCopyTile][j % kCopyTile] = v;
-    if (r < rows && c < ld_r) {
-      half_t hi, lo;
-      split(v, hi, lo);
-      straight[r * ld_r + c] = hi;
-      straight[plane_s + r * ld_r + c] = lo;
-    }
+    s_x[j / kCopyTile][j % kCopyTile] = split(v);
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < kCopyTile * kCopyTile; j += 256) {
-    const int c = c0 + j / kCopyTile, r = r0 + j % kCopyTile;
-    if (c < cols && r < ld_c) {
-      half_t hi, lo;
-      split(s_x[j % kCopyTile][j / kCopyTile], hi, lo);
-      turned[c * ld_c + r] = hi;
-      turned[plane_t + c * ld_c + r] = lo;
+  // 32 columns of a row to a line of 128 bytes: its high and low parts, eight lanes with 16 bytes each
+  for (int j = threadIdx.x; j < kCopyTile * 2 * 8; j += 256) {
+    const int line = j >> 3, part = j & 7, i = line >> 1, half = line & 1, from = half * 32 + (part & 3) * 8;
+    u32x4 v;
+    if (r0 + i < rows && c0 + half * 32 < ld_r) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t x0 = s_x[i][from + 2 * q], x1 = s_x[i][from + 2 * q + 1];
+        v[q] = part < 4 ? highs(x0, x1) : lows(x0, x1);
+      }
+      *reinterpret_cast<u32x4*>(straight + (int64_t)(r0 + i) * 2 * ld_r + (c0 / 32 + half) * 64 + part * 8) = v;
+    }
+    if (c0 + i < cols && r0 + half * 32 < ld_c) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t x0 = s_x[from + 2 * q][i], x1 = s_x[from + 2 * q + 1][i];
+        v[q] = part < 4 ? highs(x0, x1) : lows(x0, x1);
+      }
+      *reinterpret_cast<u32x4*>(turned + (int64_t)(c0 + i) * 2 * ld_c + (r0 / 32 + half) * 64 + part * 8) = v;
     }
   }
 }
@@ -184,28 +200,59 @@ __global__ __launch_bounds__(256) void fl_muon_copy_kernel(const Mat* __restrict
 // What a product is formed of: L R^T of rows of X, of X^T or of a square.
 struct Product {
   int left[2], right[2], out[2];  // squares' numbers, for up to two products of a launch
+  float norm[2], out_scale[2];    // 1 / (the operands' scales); the result's
+  float a, b, c, in_scale;        // of the polynomial, and 1 / the scale of the square that it reads
   int source;                     // which X^T
-  float norm;                     // 1 / (the operands' scales)
-  float a, b, c;                  // of the polynomial
-  float in_scale, out_scale;      // of the square that it reads, and of the result
 };
 
 enum Kind { kGram, kPoly, kSquare, kApply, kFinal };
 
+// A tile's sizes: TILE rows and columns by WR x WC waves, and how many steps of 32 columns a buffer of the LDS holds.
+template <int TILE>
+struct Shape;
+template <>
+struct Shape<256> {
+  static constexpr int WR = 2, WC = 4, BATCH = 1;
+};
+template <>
+struct Shape<128> {
+  static constexpr int WR = 2, WC = 2, BATCH = 1;
+};
+template <>
+struct Shape<64> {
+  static constexpr int WR = 2, WC = 2, BATCH = 4;
+};
+template <int TILE>
+constexpr int threads_of() { return Shape<TILE>::WR * Shape<TILE>::WC * 64; }
+
+// The blocks of a launch come to the card's eight dies in turn, so that runs of kRun tiles, which read the same rows, are
+// given to one of them.
+constexpr int kRun = 8;
+__device__ __forceinline__ int tile_of(int block) {
+  const int die = block & 7, i = block >> 3;
+  return (i / kRun * 8 + die) * kRun + i % kRun;
+}
+
 // One tile of L R^T. Rows past an operand's last are read as its last one; what they give is not written.
-// The LDS holds two steps of 32 columns: while a step is multiplied the next one's rows are loaded straight into it. A
-// row's four packs of 16 bytes change places by its number, so that eight rows' equal packs lie in different banks.
-template <int KIND>
-__global__ __launch_bounds__(256) void fl_muon_product_kernel(const Mat* __restrict__ mats, int n, const Product q,
-                                                              const Update u) {
+// The LDS holds two buffers: while one is multiplied the next is loaded straight into the other. 32 columns of a row are a
+// line of 128 bytes, high parts before low ones, whose eight packs change places by the row's number, so that eight
+// rows' equal packs lie in different banks.
+template <int KIND, int TILE>
+__global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(const Mat* __restrict__ mats, int n,
+                                                                             int tiles, const Product q,
+                                                                             const Update u) {
   constexpr bool kSymmetric = KIND <= kSquare;
-  constexpr int kStep = 32, kRow = kStep * 2;  // halves, bytes
-  constexpr int kPlane = kTile * kRow, kOperand = 2 * kPlane, kBuffer = 2 * kOperand;
-  __shared__ __attribute__((aligned(16))) char s_tile[2 * kBuffer];
+  constexpr int WR = Shape<TILE>::WR, WC = Shape<TILE>::WC, BATCH = Shape<TILE>::BATCH, kWaves = WR * WC;
+  constexpr int NI = TILE / WR / 32, NJ = TILE / WC / 32;
+  constexpr int kLine = 128, kStepBytes = TILE * kLine, kOperand = BATCH * kStepBytes, kBuffer = 2 * kOperand;
+  constexpr int kTurn = 36;  // words of a row of the tile that is turned in the LDS
+  static_assert(kWaves * 32 * kTurn * 4 <= 2 * kBuffer, "");
+  __shared__ __attribute__((aligned(128))) char s_tile[2 * kBuffer];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-  const int job = blockIdx.y;
-  const int which = kSymmetric ? matrix_of<&Mat::first_square>(mats, n, blockIdx.x)
-                               : matrix_of<&Mat::first_apply>(mats, n, blockIdx.x);
+  const int job = blockIdx.y, index = tile_of((int)blockIdx.x);
+  if (index >= tiles) return;
+  const int which = kSymmetric ? matrix_of<&Mat::first_square>(mats, n, index)
+                               : matrix_of<&Mat::first_apply>(mats, n, index);
   const Mat& k = mats[which];
   const int m = k.m, cols = k.n;
   const int64_t ldn = padded(cols), ldm = padded(m);
@@ -216,12 +263,11 @@ __global__ __launch_bounds__(256) void fl_muon_product_kernel(const Mat* __restr
 
   // operands: rows, their count, their length
   const half_t *lp, *rp;
-  int l_rows, r_rows;
+  int l_rows, r_rows, ti, tj;
   int64_t ld;
-  int ti, tj;
   const bool turn = KIND == kFinal && k.tall;
   if constexpr (kSymmetric) {
-    const int t = (int)blockIdx.x - k.first_square;
+    const int t = index - k.first_square;
     ti = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
     while (ti * (ti + 1) / 2 > t) --ti;
     while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
@@ -242,119 +288,99 @@ __global__ __launch_bounds__(256) void fl_muon_product_kernel(const Mat* __restr
     l_rows = turn ? cols : m;
     r_rows = turn ? m : cols;
     ld = ldm;
-    const int across = (r_rows + kTile - 1) / kTile, t = (int)blockIdx.x - k.first_apply;
+    const int across = (r_rows + TILE - 1) / TILE, t = index - k.first_apply;
     ti = t / across;
     tj = t - ti * across;
   }
-  const int r0 = ti * kTile, c0 = tj * kTile;
+  ti = uniform(ti);
+  tj = uniform(tj);
+  const int r0 = ti * TILE, c0 = tj * TILE;
+  const int steps = (int)(ld / 32);
 
-  // 16 rows of one plane to an instruction: 16 instructions an operand and buffer, four to a wave and operand
-  const int load_row = lane >> 2, load_pack = (lane & 3) ^ ((load_row >> 1) & 3);
+  // eight lines to an instruction
+  const int load_row = lane >> 3, load_pack = (lane & 7) ^ load_row;
   auto load = [&](int buffer, int step) {
+    constexpr int kPieces = TILE / 8 / kWaves;  // of an operand's step, to a wave
 #pragma unroll
-    for (int o = 0; o < 2; ++o) {
-      const half_t* base = o ? rp : lp;
-      const int rows = o ? r_rows : l_rows, first = o ? c0 : r0;
-      const int64_t plane = (int64_t)rows * ld;
+    for (int b = 0; b < BATCH; ++b) {
+      if (BATCH > 1 && step + b >= steps) break;
 #pragma unroll
-      for (int j = 0; j < kTile / 32; ++j) {
-        const int piece = wave * (kTile / 32) + j;  // of 2 planes x kTile / 16
-        const int p = piece / (kTile / 16), rr = piece % (kTile / 16) * 16;
-        const int row = min(first + rr + load_row, rows - 1);
-        const half_t* from = base + p * plane + row * ld + step * kStep + load_pack * 8;
-        __builtin_amdgcn_global_load_lds(
-            (const __attribute__((address_space(1))) void*)from,
-            (__attribute__((address_space(3))) void*)(s_tile + buffer * kBuffer + o * kOperand + p * kPlane + rr * kRow),
-            16, 0, 0);
+      for (int o = 0; o < 2; ++o) {
+        const half_t* base = o ? rp : lp;
+        const int rows = o ? r_rows : l_rows, first = o ? c0 : r0;
+#pragma unroll
+        for (int j = 0; j < kPieces; ++j) {
+          const int rr = (wave * kPieces + j) * 8;
+          const int row = min(first + rr + load_row, rows - 1);
+          const half_t* from = base + row * 2 * ld + (step + b) * 64 + load_pack * 8;
+          __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
+                                           (__attribute__((address_space(3))) void*)(s_tile + buffer * kBuffer +
+                                                                                     o * kOperand + b * kStepBytes +
+                                                                                     rr * kLine),
+                                           16, 0, 0);
+        }
       }
     }
   };
 
-  const int wr = (wave >> 1) * 64, wc = (wave & 1) * 64;
-  f32x16 acc[2][2];
+  const int wr = wave / WC * (TILE / WR), wc = wave % WC * (TILE / WC);
+  f32x16 acc[NI][NJ];
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+  for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < NJ; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  const int steps = (int)(ld / kStep);
+  const char* l_at = s_tile + (wr + (lane & 31)) * kLine;
+  const char* r_at = s_tile + kOperand + (wc + (lane & 31)) * kLine;
   load(0, 0);
-  for (int s = 0; s < steps; ++s) {
+  int buffer = 0;
+  for (int s = 0; s < steps; s += BATCH, buffer ^= 1) {
     __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();  // the step's rows are there, and nobody reads the other buffer any more
-    if (s + 1 < steps) load((s + 1) & 1, s + 1);
-    const char* buf = s_tile + (s & 1) * kBuffer;
+    __syncthreads();  // the buffer is there, and nobody reads the other one any more
+    if (s + BATCH < steps) load(buffer ^ 1, s + BATCH);
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      f16x8 l[2][2], r[2][2];
+    for (int b = 0; b < BATCH; ++b) {
+      if (BATCH > 1 && s + b >= steps) break;
+      const int at = buffer * kBuffer + b * kStepBytes;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int lr = wr + i * 32 + (lane & 31), rr = wc + i * 32 + (lane & 31);
-        const int pack = kk * 2 + (lane >> 5);
+      for (int kk = 0; kk < 2; ++kk) {
+        f16x8 l[NI][2], r[NJ][2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          l[i][p] = *reinterpret_cast<const f16x8*>(buf + p * kPlane + lr * kRow + (pack ^ ((lr >> 1) & 3)) * 16);
-          r[i][p] = *reinterpret_cast<const f16x8*>(buf + kOperand + p * kPlane + rr * kRow + (pack ^ ((rr >> 1) & 3)) * 16);
+          const int pack = ((p * 4 + kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16 + at;
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) r[j][p] = *reinterpret_cast<const f16x8*>(r_at + j * 32 * kLine + pack);
+#pragma unroll
+          for (int i = 0; i < NI; ++i) l[i][p] = *reinterpret_cast<const f16x8*>(l_at + i * 32 * kLine + pack);
         }
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][0], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][1], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][1], r[j][0], acc[i][j], 0, 0, 0);
+          }
       }
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][0], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][1], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][1], r[j][0], acc[i][j], 0, 0, 0);
-        }
     }
   }
 
-  const float lr = KIND == kFinal && u.muon ? (u.lr_ptr ? *u.lr_ptr : u.lr) : 0.f;
-  const float keep = 1.f - lr * u.decay, rate = lr * k.lr_scale;
-  const bool skip = KIND == kFinal && u.muon && skipped(u);
+  if constexpr (KIND == kFinal) {
+    const float lr = u.muon ? (u.lr_ptr ? *u.lr_ptr : u.lr) : 0.f;
+    const float keep = 1.f - lr * u.decay, rate = lr * k.lr_scale;
+    if (u.muon && skipped(u)) return;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int row = r0 + wr + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-        const int col = c0 + wc + j * 32 + (lane & 31);
-        float v = acc[i][j][e] * q.norm;
-        if constexpr (kSymmetric) {
-          // the lower half and its mirror, with the zeros behind each row
-          if (row < col || row >= ldm || col >= m) continue;
-          const bool in = row < m;
-          if constexpr (KIND == kPoly) {
-            const half_t* from = squares + q.left[job] * square + (int64_t)(in ? row : 0) * ldm + col;
-            v = q.b * ((float)from[0] + (float)from[m * ldm]) * q.in_scale + q.c * v + (row == col ? q.a : 0.f);
-          }
-          half_t hi, lo;
-          split(in ? v * q.out_scale : 0.f, hi, lo);
-          half_t* to = squares + q.out[job] * square;
-          if (in) {
-            to[row * ldm + col] = hi;
-            to[(m + row) * ldm + col] = lo;
-          }
-          to[col * ldm + row] = hi;
-          to[(m + col) * ldm + row] = lo;
-        } else if constexpr (KIND == kApply) {
-          // X and the other X^T
-          const bool in = row < m && col < cols;
-          half_t hi, lo;
-          split(in ? v * q.out_scale : 0.f, hi, lo);
-          if (row < m && col < ldn) {
-            x[row * ldn + col] = hi;
-            x[(m + row) * ldn + col] = lo;
-          }
-          half_t* to = xt[1 - q.source];
-          if (col < cols && row < ldm) {
-            to[col * ldm + row] = hi;
-            to[((int64_t)cols + col) * ldm + row] = lo;
-          }
-        } else {
-          if (row >= l_rows || col >= r_rows || skip) continue;
+        for (int e = 0; e < 16; ++e) {
+          const int row = r0 + wr + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
+          const int col = c0 + wc + j * 32 + (lane & 31);
+          if (row >= l_rows || col >= r_rows) continue;
+          float v = acc[i][j][e] * q.norm[0];
           const int64_t at = (int64_t)row * r_rows + col;
           if (u.muon) v = fmaf(-rate, v, load_any(k.p, at, u.is_bf16) * keep);
           if (u.is_bf16)
@@ -362,7 +388,75 @@ __global__ __launch_bounds__(256) void fl_muon_product_kernel(const Mat* __restr
           else
             store_as(static_cast<float*>(k.p) + at, v);
         }
+  } else {
+    // `straight` has the tile's rows, `turned` its columns; both get the zeros behind their rows. Of a square what
+    // is below the diagonal stands for what is above (which may differ in its last bits), so that no tile's size shows.
+    const int rows = m, columns = kSymmetric ? m : cols;
+    const int64_t ld_c = kSymmetric ? ldm : ldn, ld_r = ldm;
+    half_t* straight = kSymmetric ? squares + q.out[job] * square : x;
+    half_t* turned = kSymmetric ? straight : xt[1 - q.source];
+    const float norm = q.norm[job], out_scale = q.out_scale[job];
+    const half_t* poly = squares + q.left[job] * square;
+    uint32_t* s_turn = reinterpret_cast<uint32_t*>(s_tile) + wave * 32 * kTurn;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int rb = r0 + wr + i * 32, cb = c0 + wc + j * 32, col = cb + (lane & 31);
+        if (rb >= ld_r || cb >= ld_c || (kSymmetric && rb < cb)) continue;  // (the same in the whole wave)
+        const bool diagonal = kSymmetric && rb == cb;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const int row = rb + 8 * g + 4 * (lane >> 5);
+          f16x4 hi = {0, 0, 0, 0}, lo = {0, 0, 0, 0};
+          if constexpr (KIND == kPoly) {  // the square's own values, read as those across the diagonal
+            const half_t* from = poly + (int64_t)min(col, m - 1) * 2 * ldm + column(row);
+            hi = *reinterpret_cast<const f16x4*>(from);
+            lo = *reinterpret_cast<const f16x4*>(from + kPad);
+          }
+          u32x4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float v = acc[i][j][4 * g + e] * norm;
+            if constexpr (KIND == kPoly)
+              v = q.b * ((float)hi[e] + (float)lo[e]) * q.in_scale + q.c * v + (row + e == col ? q.a : 0.f);
+            w[e] = split(row + e < rows && col < columns ? v * out_scale : 0.f);
+          }
+          if (!diagonal && col < columns) {
+            half_t* to = turned + (int64_t)col * 2 * ld_r + column(row);
+            *reinterpret_cast<u32x2*>(to) = u32x2{highs(w[0], w[1]), highs(w[2], w[3])};
+            *reinterpret_cast<u32x2*>(to + kPad) = u32x2{lows(w[0], w[1]), lows(w[2], w[3])};
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s_turn[(8 * g + 4 * (lane >> 5) + e) * kTurn + (lane & 31)] = w[e];
+        }
+        // (a wave's own part of the LDS: its reads come behind its writes)
+        __builtin_amdgcn_wave_barrier();
+        const int row = rb + (lane >> 1), half = (lane & 1) * 16;
+        u32x4 w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[e] = *reinterpret_cast<const u32x4*>(s_turn + (lane >> 1) * kTurn + half + 4 * e);
+        if (diagonal) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (half + e > lane >> 1) w[e >> 2][e & 3] = s_turn[(half + e) * kTurn + (lane >> 1)];
+        }
+        __builtin_amdgcn_wave_barrier();
+        if (row < rows) {
+          half_t* to = straight + (int64_t)row * 2 * ld_c + column(cb) + half;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const u32x4 p = w[2 * e], o = w[2 * e + 1];
+            *reinterpret_cast<u32x4*>(to + 8 * e) =
+                u32x4{highs(p[0], p[1]), highs(p[2], p[3]), highs(o[0], o[1]), highs(o[2], o[3])};
+            *reinterpret_cast<u32x4*>(to + kPad + 8 * e) =
+                u32x4{lows(p[0], p[1]), lows(p[2], p[3]), lows(o[0], o[1]), lows(o[2], o[3])};
+          }
+        }
       }
+  }
 }
 
 // ---------------------------------------------------------------- host
@@ -434,22 +528,133 @@ bool bounds_of(int steps, double a, double b, double c, Bounds* o) {
 
 float scale_for(double bound) { return (float)exp2(14.0 - ceil(log2(fmax(bound, 1e-3)))); }
 
+template <int TILE>
+struct Launch {
+  const Mat* mats;
+  int count, squares, applies;  // matrices, tiles
+  const Update& u;
+  hipStream_t s;
+  template <int KIND>
+  void run(const Product& q, int jobs = 1) const {
+    const int tiles = KIND <= kSquare ? squares : applies;
+    const unsigned blocks = (unsigned)(cdiv(tiles, 8 * kRun) * 8 * kRun);
+    fl_muon_product_kernel<KIND, TILE><<<dim3(blocks, (unsigned)jobs), threads_of<TILE>(), 0, s>>>(mats, count, tiles, q, u);
+  }
+};
+
+// The steps of a group whose X is laid out.
+template <int TILE>
+void newton_schulz(const Launch<TILE>& launch, int steps, double a, double b, double c, const Bounds& bounds) {
+  const int stages = (int)cdiv(steps, kStage);
+  float x_scale = scale_for(1.0);
+  int source = 0;
+  for (int st = 0, k = 0; st < stages; ++st) {
+    const int len = (int)cdiv(steps - k, stages - st);  // the first ones are the longer ones
+    // squares: 0 A, 1 U = A P, the others in turn P and the product of the P so far
+    int poly_at = 2, product_at = -1, spare = 3;
+    double product_bound = 0.0;
+    float a_scale = scale_for(bounds.x[k] * bounds.x[k]), product_scale = 0.f;
+    Product q = {};
+    q.norm[0] = 1.f / (x_scale * x_scale);
+    q.out_scale[0] = a_scale;
+    launch.template run<kGram>(q);
+    for (int e = 0; e < len; ++e, ++k) {
+      const float p_scale = scale_for(bounds.p[k]);
+      const bool last = e + 1 == len;
+      q = {};
+      q.out[0] = poly_at;
+      q.norm[0] = 1.f / (a_scale * a_scale);
+      q.a = (float)a;
+      q.b = (float)b;
+      q.c = (float)c;
+      q.in_scale = 1.f / a_scale;
+      q.out_scale[0] = p_scale;
+      launch.template run<kPoly>(q);
+      q = {};
+      int jobs = 0;
+      const float u_scale = scale_for(bounds.x[k] * bounds.x[k] * bounds.p[k]);
+      const auto product = [&](int left, float left_scale, int out, float out_scale) {
+        q.left[jobs] = left;
+        q.right[jobs] = poly_at;
+        q.out[jobs] = out;
+        q.norm[jobs] = 1.f / (left_scale * p_scale);
+        q.out_scale[jobs] = out_scale;
+        ++jobs;
+      };
+      if (!last) product(0, a_scale, 1, u_scale);
+      if (e == 0) {
+        product_at = poly_at;
+        product_scale = p_scale;
+        product_bound = bounds.p[k];
+      } else {
+        product_bound *= bounds.p[k];
+        const float scale = scale_for(product_bound);
+        product(product_at, product_scale, spare, scale);
+        const int old = product_at;
+        product_at = spare;
+        spare = old;
+        product_scale = scale;
+      }
+      if (jobs) launch.template run<kSquare>(q, jobs);
+      if (!last) {  // A = U P
+        q = {};
+        jobs = 0;
+        a_scale = scale_for(bounds.x[k + 1] * bounds.x[k + 1]);
+        product(1, u_scale, 0, a_scale);
+        launch.template run<kSquare>(q);
+        if (e == 0) poly_at = 4;
+      }
+    }
+    q = {};
+    q.left[0] = product_at;
+    q.source = source;
+    q.norm[0] = 1.f / (product_scale * x_scale);
+    if (k < steps) {
+      x_scale = scale_for(bounds.x[k]);
+      q.out_scale[0] = x_scale;
+      launch.template run<kApply>(q);
+      source = 1 - source;
+    } else {
+      launch.template run<kFinal>(q);
+    }
+  }
+}
+
+// The tiles of a group's squares, lower half
+int64_t square_tiles(const std::vector<int64_t>& order, const int64_t* rows, const int64_t* cols, int tile) {
+  int64_t n = 0;
+  for (int64_t i : order) {
+    const int64_t side = cdiv(rows[i] < cols[i] ? rows[i] : cols[i], tile);
+    n += side * (side + 1) / 2;
+  }
+  return n;
+}
+
 int run(int64_t n, const void* const* g, void* const* p, float* const* buf, const int64_t* rows, const int64_t* cols,
         const double* lr_scale, int steps, double a, double b, double c, double eps, const Update& u, void* workspace,
         hipStream_t s) {
   Bounds bounds;
   if (!bounds_of(steps, a, b, c, &bounds)) return FL_ERR_INVALID_ARGUMENT;
-  for (int64_t i = 0; i < n;) {
-    const Group group = group_from(i, n, rows, cols);
+  std::vector<int64_t> order;
+  for (int64_t from = 0; from < n;) {
+    const Group group = group_from(from, n, rows, cols);
     if (group.count == 0) break;
+    order.clear();
+    for (int64_t i = from; i < group.end; ++i)
+      if (rows[i] * cols[i]) order.push_back(i);
+    from = group.end;
+    // the longest first, whose tiles take longest
+    std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
+      return std::max(rows[i], cols[i]) > std::max(rows[j], cols[j]);
+    });
+    const int tile = kForceTile ? kForceTile : square_tiles(order, rows, cols, 256) >= 192 ? 256 : square_tiles(order, rows, cols, 128) >= 128 ? 128 : 64;
     char* at = static_cast<char*>(workspace);
     half_t* planes = reinterpret_cast<half_t*>(at);
     double* sums = reinterpret_cast<double*>(at + group.planes);
     Mat* mats = reinterpret_cast<Mat*>(at + group.planes + (size_t)group.sums * 8);
     int64_t first_norm = 0, first_copy = 0, first_square = 0, first_apply = 0, done = 0;
     Table t = {};
-    for (; i < group.end; ++i) {
-      if (rows[i] * cols[i] == 0) continue;
+    for (int64_t i : order) {
       Mat& k = t.mat[t.n++];
       const bool tall = rows[i] > cols[i];
       k.base = planes;
@@ -467,111 +672,39 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
       planes += planes_bytes(rows[i], cols[i]) / sizeof(half_t);
       first_norm += norm_blocks(rows[i], cols[i]);
       first_copy += cdiv(padded(rows[i]), kCopyTile) * cdiv(padded(cols[i]), kCopyTile);
-      const int64_t side = cdiv(k.m, kTile);
+      const int64_t side = cdiv(k.m, tile);
       first_square += side * (side + 1) / 2;
-      first_apply += side * cdiv(k.n, kTile);
-      if (t.n == kTable || i + 1 == group.end) {
+      first_apply += side * cdiv(k.n, tile);
+      if (t.n == kTable || done + t.n == group.count) {
         fl_muon_table_kernel<<<1, 64, 0, s>>>(t, mats + done);
         done += t.n;
         t.n = 0;
       }
     }
-    if (t.n) {
-      fl_muon_table_kernel<<<1, 64, 0, s>>>(t, mats + done);
-      done += t.n;
-    }
     const int count = (int)group.count;
     fl_muon_norm_kernel<<<(unsigned)first_norm, 256, 0, s>>>(mats, count, u, sums);
-    float x_scale = scale_for(1.0);
-    fl_muon_copy_kernel<<<(unsigned)first_copy, 256, 0, s>>>(mats, count, u, sums, eps, x_scale);
-    int source = 0;
-    const dim3 squares((unsigned)first_square), apply((unsigned)first_apply);
-    const int stages = (int)cdiv(steps, kStage);
-    for (int st = 0, k = 0; st < stages; ++st) {
-      const int len = (steps - k + stages - st - 1) / (stages - st);  // the first ones are the longer ones
-      // squares: A, U, then three in turn for P and the product of the P so far
-      int poly_at = 2, product_at = -1, spare = 3, other = 4;
-      double product_bound = 0.0;
-      float a_scale = scale_for(bounds.x[k] * bounds.x[k]), product_scale = 0.f;
-      Product q = {};
-      q.out[0] = 0;
-      q.norm = 1.f / (x_scale * x_scale);
-      q.out_scale = a_scale;
-      fl_muon_product_kernel<kGram><<<squares, 256, 0, s>>>(mats, count, q, u);
-      for (int e = 0; e < len; ++e, ++k) {
-        const float p_scale = scale_for(bounds.p[k]);
-        q = {};
-        q.left[0] = q.right[0] = 0;
-        q.out[0] = poly_at;
-        q.norm = 1.f / (a_scale * a_scale);
-        q.a = (float)a;
-        q.b = (float)b;
-        q.c = (float)c;
-        q.in_scale = 1.f / a_scale;
-        q.out_scale = p_scale;
-        fl_muon_product_kernel<kPoly><<<squares, 256, 0, s>>>(mats, count, q, u);
-        const bool last = e + 1 == len;
-        const float u_scale = scale_for(bounds.x[k] * bounds.x[k] * bounds.p[k]);
-        if (!last) {  // U = A P
-          q = {};
-          q.left[0] = 0;
-          q.right[0] = poly_at;
-          q.out[0] = 1;
-          q.norm = 1.f / (a_scale * p_scale);
-          q.out_scale = u_scale;
-          fl_muon_product_kernel<kSquare><<<squares, 256, 0, s>>>(mats, count, q, u);
-        }
-        if (product_at < 0) {
-          product_at = poly_at;
-          product_scale = p_scale;
-          product_bound = bounds.p[k];
-        } else {  // the product of the P
-          product_bound *= bounds.p[k];
-          const float scale = scale_for(product_bound);
-          q = {};
-          q.left[0] = product_at;
-          q.right[0] = poly_at;
-          q.out[0] = spare;
-          q.norm = 1.f / (product_scale * p_scale);
-          q.out_scale = scale;
-          fl_muon_product_kernel<kSquare><<<squares, 256, 0, s>>>(mats, count, q, u);
-          const int free_at = product_at;
-          product_at = spare;
-          spare = free_at;
-          product_scale = scale;
-        }
-        if (!last) {  // A = U P
-          const float next = scale_for(bounds.x[k + 1] * bounds.x[k + 1]);
-          q = {};
-          q.left[0] = 1;
-          q.right[0] = poly_at;
-          q.out[0] = 0;
-          q.norm = 1.f / (u_scale * p_scale);
-          q.out_scale = next;
-          fl_muon_product_kernel<kSquare><<<squares, 256, 0, s>>>(mats, count, q, u);
-          a_scale = next;
-          if (product_at == poly_at) {
-            poly_at = other;
-          }
-        }
-      }
-      q = {};
-      q.left[0] = product_at;
-      q.source = source;
-      q.norm = 1.f / (product_scale * x_scale);
-      if (k < steps) {
-        x_scale = scale_for(bounds.x[k]);
-        q.out_scale = x_scale;
-        fl_muon_product_kernel<kApply><<<apply, 256, 0, s>>>(mats, count, q, u);
-        source = 1 - source;
-      } else {
-        fl_muon_product_kernel<kFinal><<<apply, 256, 0, s>>>(mats, count, q, u);
-      }
-    }
+    fl_muon_copy_kernel<<<(unsigned)first_copy, 256, 0, s>>>(mats, count, u, sums, eps, scale_for(1.0));
+    const int squares = (int)first_square, applies = (int)first_apply;
+    if (tile == 256)
+      newton_schulz(Launch<256>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+    else if (tile == 128)
+      newton_schulz(Launch<128>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+    else
+      newton_schulz(Launch<64>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_status(e);
   }
   return FL_OK;
+}
+
+// no exception leaves a C entry (the host's lists are all that allocates)
+template <typename F>
+int caught(F f) {
+  try {
+    return f();
+  } catch (...) {
+    return FL_ERR_HIP_BASE + (int)hipErrorOutOfMemory;
+  }
 }
 
 bool addresses_ok(int64_t n, const void* const* p, const int64_t* rows, const int64_t* cols, size_t size) {
@@ -612,8 +745,10 @@ int fl_orthogonalize(int64_t n, const void* const* x, int dtype, const int64_t* 
   if (!aligned(workspace, 16)) return FL_ERR_INVALID_ARGUMENT;
   Update u = {};
   u.is_bf16 = dtype == FL_DTYPE_BF16;
-  return run(n, x, out, nullptr, rows, cols, nullptr, steps, a, b, c, eps, u, workspace,
-             static_cast<hipStream_t>(stream));
+  return caught([&] {
+    return run(n, x, out, nullptr, rows, cols, nullptr, steps, a, b, c, eps, u, workspace,
+               static_cast<hipStream_t>(stream));
+  });
 }
 
 int fl_muon_step(int64_t n, void* const* params, const void* const* grads, int dtype, float* const* buffers,
@@ -638,8 +773,10 @@ int fl_muon_step(int64_t n, void* const* params, const void* const* grads, int d
   u.lr_ptr = lr_ptr;
   u.lr = (float)lr;
   u.decay = (float)weight_decay;
-  return run(n, grads, params, buffers, rows, cols, lr_scale, steps, a, b, c, eps, u, workspace,
-             static_cast<hipStream_t>(stream));
+  return caught([&] {
+    return run(n, grads, params, buffers, rows, cols, lr_scale, steps, a, b, c, eps, u, workspace,
+               static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"
