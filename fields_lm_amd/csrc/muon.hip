@@ -31,10 +31,6 @@ typedef _Float16 half_t;
 constexpr int kStage = 3;      // steps between two products with X
 constexpr int kPad = 32;       // rows of planes are a multiple of this long, zeros behind the matrix
 constexpr int kSquares = 5;    // m x m matrices of the workspace
-#ifndef FORCE_TILE
-#define FORCE_TILE 0
-#endif
-constexpr int kForceTile = FORCE_TILE;
 constexpr int kCopyTile = 64;  // of the tile that is laid out by a block
 constexpr int kTable = 56;     // matrices to a launch that sets up their table
 constexpr int kNormChunk = 16384;  // values of a block of the norm
@@ -207,13 +203,41 @@ struct Product {
 
 enum Kind { kGram, kPoly, kSquare, kApply, kFinal };
 
+// 16 values of a parameter, `left` of them there: p keep - rate v, or v itself
+template <typename T>
+__device__ __forceinline__ void update16(T* p, int left, const float* v, int muon, float keep, float rate) {
+  if (left >= 16) {
+    constexpr int N = 16 / sizeof(T);
+    u32x4_any* to = reinterpret_cast<u32x4_any*>(p);
+    u32x4 old[16 / N];
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) old[i] = muon ? (u32x4)to[i] : u32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < 16 / N; ++i) {
+      u32x4 r;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (N == 4) {
+          const float x = v[4 * i + k];
+          r[k] = __float_as_uint(muon ? fmaf(-rate, x, __uint_as_float(old[i][k]) * keep) : x);
+        } else {
+          const float x = v[8 * i + 2 * k], y = v[8 * i + 2 * k + 1];
+          r[k] = muon ? bf16_pair(fmaf(-rate, x, bf16_lo(old[i][k]) * keep), fmaf(-rate, y, bf16_hi(old[i][k]) * keep))
+                      : bf16_pair(x, y);
+        }
+      }
+      to[i] = r;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (i < left) store_as(p + i, muon ? fmaf(-rate, v[i], load_as<T>(p + i) * keep) : v[i]);
+  }
+}
+
 // A tile's sizes: TILE rows and columns by WR x WC waves, and how many steps of 32 columns a buffer of the LDS holds.
 template <int TILE>
 struct Shape;
-template <>
-struct Shape<256> {
-  static constexpr int WR = 2, WC = 4, BATCH = 1;
-};
 template <>
 struct Shape<128> {
   static constexpr int WR = 2, WC = 2, BATCH = 1;
@@ -227,7 +251,7 @@ constexpr int threads_of() { return Shape<TILE>::WR * Shape<TILE>::WC * 64; }
 
 // The blocks of a launch come to the card's eight dies in turn, so that runs of kRun tiles, which read the same rows, are
 // given to one of them.
-constexpr int kRun = 8;
+constexpr int kRun = 16;
 __device__ __forceinline__ int tile_of(int block) {
   const int die = block & 7, i = block >> 3;
   return (i / kRun * 8 + die) * kRun + i % kRun;
@@ -235,8 +259,8 @@ __device__ __forceinline__ int tile_of(int block) {
 
 // One tile of L R^T. Rows past an operand's last are read as its last one; what they give is not written.
 // The LDS holds two buffers: while one is multiplied the next is loaded straight into the other. 32 columns of a row are a
-// line of 128 bytes, high parts before low ones, whose eight packs change places by the row's number, so that eight
-// rows' equal packs lie in different banks.
+// line of 128 bytes, high parts before low ones, whose eight packs change places by half the row's number, so that sixteen
+// rows' equal packs lie in different banks of the 64.
 template <int KIND, int TILE>
 __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(const Mat* __restrict__ mats, int n,
                                                                              int tiles, const Product q,
@@ -298,7 +322,7 @@ __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(con
   const int steps = (int)(ld / 32);
 
   // eight lines to an instruction
-  const int load_row = lane >> 3, load_pack = (lane & 7) ^ load_row;
+  const int load_row = lane >> 3;
   auto load = [&](int buffer, int step) {
     constexpr int kPieces = TILE / 8 / kWaves;  // of an operand's step, to a wave
 #pragma unroll
@@ -312,7 +336,8 @@ __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(con
         for (int j = 0; j < kPieces; ++j) {
           const int rr = (wave * kPieces + j) * 8;
           const int row = min(first + rr + load_row, rows - 1);
-          const half_t* from = base + row * 2 * ld + (step + b) * 64 + load_pack * 8;
+          const int pack = (lane & 7) ^ (((rr + load_row) >> 1) & 7);
+          const half_t* from = base + row * 2 * ld + (step + b) * 64 + pack * 8;
           __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
                                            (__attribute__((address_space(3))) void*)(s_tile + buffer * kBuffer +
                                                                                      o * kOperand + b * kStepBytes +
@@ -349,7 +374,7 @@ __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(con
         f16x8 l[NI][2], r[NJ][2];
 #pragma unroll
         for (int p = 0; p < 2; ++p) {
-          const int pack = ((p * 4 + kk * 2 + (lane >> 5)) ^ (lane & 7)) * 16 + at;
+          const int pack = ((p * 4 + kk * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 + at;
 #pragma unroll
           for (int j = 0; j < NJ; ++j) r[j][p] = *reinterpret_cast<const f16x8*>(r_at + j * 32 * kLine + pack);
 #pragma unroll
@@ -371,23 +396,34 @@ __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(con
     const float lr = u.muon ? (u.lr_ptr ? *u.lr_ptr : u.lr) : 0.f;
     const float keep = 1.f - lr * u.decay, rate = lr * k.lr_scale;
     if (u.muon && skipped(u)) return;
+    float* s_turn = reinterpret_cast<float*>(s_tile) + wave * 32 * kTurn;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < NI; ++i)
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j) {
+        const int rb = r0 + wr + i * 32, cb = c0 + wc + j * 32;
+        if (rb >= l_rows || cb >= r_rows) continue;  // (the same in the whole wave)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int row = r0 + wr + i * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3);
-          const int col = c0 + wc + j * 32 + (lane & 31);
-          if (row >= l_rows || col >= r_rows) continue;
-          float v = acc[i][j][e] * q.norm[0];
-          const int64_t at = (int64_t)row * r_rows + col;
-          if (u.muon) v = fmaf(-rate, v, load_any(k.p, at, u.is_bf16) * keep);
-          if (u.is_bf16)
-            store_as(static_cast<bf16_bits*>(k.p) + at, v);
-          else
-            store_as(static_cast<float*>(k.p) + at, v);
+        for (int e = 0; e < 16; ++e)
+          s_turn[(8 * (e >> 2) + 4 * (lane >> 5) + (e & 3)) * kTurn + (lane & 31)] = acc[i][j][e] * q.norm[0];
+        __builtin_amdgcn_wave_barrier();
+        const int row = rb + (lane >> 1), col = cb + (lane & 1) * 16;
+        float v[16];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f32x4 w = *reinterpret_cast<const f32x4*>(s_turn + (lane >> 1) * kTurn + (lane & 1) * 16 + 4 * e);
+#pragma unroll
+          for (int f = 0; f < 4; ++f) v[4 * e + f] = w[f];
         }
+        __builtin_amdgcn_wave_barrier();
+        if (row >= l_rows) continue;
+        const int64_t at = (int64_t)row * r_rows + col;
+        if (u.is_bf16)
+          update16(static_cast<bf16_bits*>(k.p) + at, r_rows - col, v, u.muon, keep, rate);
+        else
+          update16(static_cast<float*>(k.p) + at, r_rows - col, v, u.muon, keep, rate);
+      }
   } else {
     // `straight` has the tile's rows, `turned` its columns; both get the zeros behind their rows. Of a square what
     // is below the diagonal stands for what is above (which may differ in its last bits), so that no tile's size shows.
@@ -647,7 +683,7 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
     std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
       return std::max(rows[i], cols[i]) > std::max(rows[j], cols[j]);
     });
-    const int tile = kForceTile ? kForceTile : square_tiles(order, rows, cols, 256) >= 192 ? 256 : square_tiles(order, rows, cols, 128) >= 128 ? 128 : 64;
+    const int tile = square_tiles(order, rows, cols, 128) >= 100 ? 128 : 64;
     char* at = static_cast<char*>(workspace);
     half_t* planes = reinterpret_cast<half_t*>(at);
     double* sums = reinterpret_cast<double*>(at + group.planes);
@@ -685,9 +721,7 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
     fl_muon_norm_kernel<<<(unsigned)first_norm, 256, 0, s>>>(mats, count, u, sums);
     fl_muon_copy_kernel<<<(unsigned)first_copy, 256, 0, s>>>(mats, count, u, sums, eps, scale_for(1.0));
     const int squares = (int)first_square, applies = (int)first_apply;
-    if (tile == 256)
-      newton_schulz(Launch<256>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
-    else if (tile == 128)
+    if (tile == 128)
       newton_schulz(Launch<128>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
     else
       newton_schulz(Launch<64>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
