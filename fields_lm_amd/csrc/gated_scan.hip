@@ -25,7 +25,9 @@ using namespace fl;
 constexpr int kTile = 256;     // steps
 constexpr int kChannels = 64;  // of a chain
 constexpr int kWords = 3 * kChannels;  // of a tile: P and S of its map, its end
-constexpr int kBehind = 4;     // tiles whose words are loaded at a time
+constexpr int kShort = 8;      // steps up to which no tile is formed (64 sequences of 1,024 channels, one step: 3.2 us, a
+                               // tile each 8.1)
+constexpr int kBehind = 2;     // tiles whose words are loaded at a time
 constexpr uint32_t kMaxPolls = 1u << 20;  // of a wait that never ends; its tile's results are NaN
 constexpr int64_t kMaxB = 65535, kMaxC = 64 * 65535, kMaxT = (int64_t)1 << 30;
 
@@ -80,10 +82,12 @@ struct Four<bf16_bits> {
   __device__ __forceinline__ void fill(float x) { w[0] = w[1] = bf16_bits_of(x) * 0x10001u; }
   __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
 };
+// Streaming stores: B=8, T=2,048, C=1,024 in fp32 with gradients 109 us, 123 with plain ones, B=1, T=65,536 285 and 292; what
+// reads the result next is as fast behind either (2 to 270 MB).
 __device__ __forceinline__ void store4(float* p, int64_t left, const float* v) {
   if (left >= 4) {
-    *reinterpret_cast<u32x4_any*>(p) =
-        u32x4{__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    const u32x4 r = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};
+    __builtin_nontemporal_store(r, reinterpret_cast<u32x4_any*>(p));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -92,7 +96,8 @@ __device__ __forceinline__ void store4(float* p, int64_t left, const float* v) {
 }
 __device__ __forceinline__ void store4(bf16_bits* p, int64_t left, const float* v) {
   if (left >= 4) {
-    *reinterpret_cast<u32x2_any*>(p) = u32x2{bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+    const u32x2 r = {bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3])};
+    __builtin_nontemporal_store(r, reinterpret_cast<u32x2_any*>(p));
   } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
@@ -317,6 +322,41 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
   });
 }
 
+// A few steps: 16 lanes to a chain, step by step.
+template <typename GT, typename DT, bool TOKEN>
+__global__ __launch_bounds__(256) void fl_gated_short_kernel(const Scan s, const float* __restrict__ state_in,
+                                                             float* __restrict__ state_out, float* __restrict__ starts,
+                                                             DT* __restrict__ out) {
+  constexpr int STEPS = kShort;
+  const unsigned chain = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const int lane = threadIdx.x & 15;
+  const int64_t b = chain / (unsigned)s.groups, c0 = (int64_t)(chain - (unsigned)b * (unsigned)s.groups) * kChannels;
+  const int64_t c = c0 + lane * 4, left = s.C - c;
+  const int n = chain < s.chains ? (int)s.T : 0;
+  Gates<GT, TOKEN, STEPS> a;
+  Four<DT> u[STEPS];
+  Four<float> h;
+  a.load(static_cast<const GT*>(s.gate) + b * s.gate_b + (TOKEN ? 0 : c), s.gate_t, n, lane, left);
+  const DT* from = static_cast<const DT*>(s.drive) + b * s.drive_b + c;
+#pragma unroll
+  for (int j = 0; j < STEPS; ++j) {
+    u[j].fill(0.f);
+    if (j < n && left > 0) u[j].load(from + j * s.drive_t, left);
+  }
+  h.fill(0.f);
+  const bool ok = n > 0 && left > 0;
+  if (ok && state_in) h.load(state_in + b * s.C + c, left);
+  if (ok && starts) store4(starts + b * s.C + c, left, h.v);
+  DT* to = out + b * s.T * s.C + c;
+  each<STEPS>([&](auto j) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      h.v[i] = fmaf(a.template at<decltype(j)::value>(i), h.v[i], u[decltype(j)::value][i]);
+    if (decltype(j)::value < n && left > 0) store4(to + decltype(j)::value * s.C, left, h.v);
+  });
+  if (ok && state_out) store4(state_out + b * s.C + c, left, h.v);
+}
+
 // Wave 0 composes the tile's maps forward from the state it starts from, wave 1 backward from the carry into its end.
 template <typename GT, typename DT, bool TOKEN>
 __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
@@ -485,6 +525,11 @@ void clear(const Call& c, size_t bytes) {
 
 template <typename GT, typename DT, bool TOKEN>
 int forward(const Call& c, size_t bytes, const float* state_in, float* state_out, float* starts, void* out) {
+  if (c.s.T <= kShort) {
+    fl_gated_short_kernel<GT, DT, TOKEN><<<(unsigned)cdiv(c.s.chains, 16), 256, 0, c.stream>>>(
+        c.s, state_in, state_out, starts, static_cast<DT*>(out));
+    return hip_status(hipGetLastError());
+  }
   clear(c, bytes);
   fl_gated_scan_kernel<GT, DT, TOKEN><<<c.blocks(), kForwardThreads, 0, c.stream>>>(c.s, state_in, state_out, starts,
                                                                                      static_cast<DT*>(out));
