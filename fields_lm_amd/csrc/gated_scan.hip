@@ -29,7 +29,7 @@ constexpr int kShort = 8;      // steps up to which no tile is formed (64 sequen
                                // tile each 8.1)
 constexpr int kBehind = 2;     // tiles whose words are loaded at a time
 constexpr uint32_t kMaxPolls = 1u << 20;  // of a wait that never ends; its tile's results are NaN
-constexpr int64_t kMaxB = 65535, kMaxC = 64 * 65535, kMaxT = (int64_t)1 << 30;
+constexpr int64_t kMaxB = 1 << 24, kMaxC = 1 << 24, kMaxT = (int64_t)1 << 30;
 
 struct Scan {
   const void* gate;
@@ -553,7 +553,8 @@ int backward(const Call& c, size_t bytes, const float* starts, const void* g_out
 
 bool sizes_ok(int64_t B, int64_t T, int64_t C) {
   return B > 0 && T > 0 && C > 0 && B <= kMaxB && C <= kMaxC && T <= kMaxT &&
-         cdiv(T, kTile) * B <= (((int64_t)1 << 31) - 1) / cdiv(C, kChannels);  // blocks of a launch
+         cdiv(T, kTile) * B <= (((int64_t)1 << 31) - 1) / cdiv(C, kChannels) &&  // blocks of a launch
+         T * B <= ((int64_t)1 << 40) / C;
 }
 
 bool tensor_ok(const void* p, int dtype, int64_t stride_b, int64_t stride_t) {

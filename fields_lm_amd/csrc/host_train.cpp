@@ -338,7 +338,8 @@ PyObject* host_gated_scan(PyObject*, PyObject* args) {
   const bool grad = at::GradMode::is_enabled() &&
                     (gate.requires_grad() || drive.requires_grad() || (state.defined() && state.requires_grad()));
   if (drive.numel() == 0) {  // no step or no channel: nothing changes the state
-    out = {drive.clone()};
+    const Tensor none = (gate.dim() == 2 ? gate.unsqueeze(2) : gate).to(drive.scalar_type()) * 0;
+    out = {drive + none};  // (on the graph of both)
     if (return_state)
       out.push_back(state.defined() ? state.clone()
                                     : at::zeros({B, C}, at::TensorOptions().dtype(at::kFloat).device(drive.device())));

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void fl_muon_copy_kernel(const Mat* __restrict
   if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
   __syncthreads();
   sum = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-  const double inv = (double)x_scale / (sqrt(sum) + eps);
+  const double inv = sum == 0.0 ? 0.0 : (double)x_scale / (sqrt(sum) + eps);  // (zeros stay zeros, whatever eps is)
 
   // the matrix as it lies: rows x cols
   const int rows = k.tall ? k.n : k.m, cols = k.tall ? k.m : k.n;

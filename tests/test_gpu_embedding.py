@@ -95,6 +95,27 @@ def test_gradient_of_counts_and_vocabularies(dev, n, V):
         check_grad(got, tokens, g, 1.0, None)
 
 
+@pytest.mark.parametrize("V,D,n", [(1 << 23, 3, 5000), ((1 << 23) - 5, 1, 70), (3, 5000, 700), (1, 1, 200_000), (4097, 33, 100_000)])
+def test_ends_of_the_ranges(dev, V, D, n):
+    """The largest vocabulary, wide rows, many tokens, a bucket of few rows and one of thousands."""
+    print(f"[case] embedding gradient V={V} D={D} n={n}", flush=True)
+    gen = torch.Generator(device=dev).manual_seed(n)
+    g = torch.randn(n, D, device=dev, generator=gen)
+    tokens = torch.randint(0, V, (n,), device=dev, generator=gen)
+    tokens[::3] = V - 1
+    tokens[1::7] = max(0, V - 1500)
+    weight = torch.zeros(V, D, device=dev, requires_grad=True)
+    got, = torch.autograd.grad(fl.embedding(tokens, weight), weight, g)
+    check_grad(got, tokens, g, 1.0, None)
+
+
+def test_refuses_a_vocabulary_past_the_largest(dev):
+    print("[case] embedding, vocabulary past the largest", flush=True)
+    w = torch.empty(1, 1, device=dev).expand((1 << 23) + 1, 1)
+    with pytest.raises(ValueError):
+        fl.embedding(torch.zeros(1, dtype=torch.long, device=dev), w)
+
+
 def test_tokens_outside(dev):
     print("[case] embedding, tokens outside", flush=True)
     weight = torch.randn(9, 20, device=dev, requires_grad=True)

@@ -106,7 +106,7 @@ def inputs(dev, B, T, C, token, gt, dt, state, seed, low=0.0):
     return gate.to(gt), drive.to(dt), first, g_out, g_last
 
 
-SHAPES = [(1, 1, 1), (64, 1, 96), (2, 2, 3), (3, 15, 5), (1, 16, 64), (2, 17, 65), (1, 63, 7), (2, 64, 64), (1, 65, 130),
+SHAPES = [(70_001, 2, 3), (1, 8, 70), (2, 9, 70), (1, 1, 1), (64, 1, 96), (2, 2, 3), (3, 15, 5), (1, 16, 64), (2, 17, 65), (1, 63, 7), (2, 64, 64), (1, 65, 130),
           (3, 255, 31), (1, 256, 4), (2, 257, 66), (1, 300, 1), (2, 511, 62), (1, 513, 257), (3, 1025, 64), (1, 4099, 33),
           (2, 2048, 192)]
 
@@ -235,6 +235,10 @@ def test_empty(dev):
     assert bool((got == 1).all())
     out, last = fl.gated_scan(torch.rand(0, 4, 5, device=dev), torch.rand(0, 4, 5, device=dev), return_state=True)
     assert out.shape == (0, 4, 5) and last.shape == (0, 5)
+    for shape in ((2, 0, 5), (2, 0)):
+        gate, drive = torch.rand(shape, device=dev, requires_grad=True), torch.rand(2, 0, 5, device=dev, requires_grad=True)
+        got = torch.autograd.grad(fl.gated_scan(gate, drive).sum(), (gate, drive))
+        assert got[0].shape == shape and got[1].shape == (2, 0, 5)
 
 
 def test_special_values(dev):

@@ -172,7 +172,8 @@ def test_sizes_of_values(dev):
     """Zeros, large and small scales, a row or column alone, an identity; NaN and infinities spoil their matrix alone."""
     print("[case] orthogonalize, values", flush=True)
     x = matrices(dev, (60, 80), 6)
-    assert bool((fl.orthogonalize(torch.zeros(5, 60, 80, device=dev)) == 0).all())
+    for eps in (1e-7, 0.0):
+        assert bool((fl.orthogonalize(torch.zeros(5, 60, 80, device=dev), eps=eps) == 0).all())
     base = fl.orthogonalize(x, eps=0.0)
     for scale in (2.0 ** 100, 2.0 ** -100):
         assert torch.equal(fl.orthogonalize(x * scale, eps=0.0), base)

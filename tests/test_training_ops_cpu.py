@@ -93,16 +93,16 @@ def test_bounds_hold(steps, abc):
     """What the check lets pass keeps singular values and factors within 1024, on a fine grid of them."""
     lib = nat.load()
     a, b, c = abc
-    x = torch.linspace(0, 1, 100_001, dtype=torch.float64)
-    fine = True
-    for _ in range(steps):
-        p = a + b * x ** 2 + c * x ** 4
-        x = (p * x).abs()
-        fine = fine and bool(p.abs().max() <= 1024) and bool(x.max() <= 1024)
-    assert not fine or lib.fl_orthogonalize_check(steps, a, b, c) in (nat.FL_OK, nat.FL_ERR_INVALID_ARGUMENT)
     if lib.fl_orthogonalize_check(steps, a, b, c) == nat.FL_OK:
-        assert fine
-    assert lib.fl_orthogonalize_check(5, 3.4445, -4.7750, 2.0315) == nat.FL_OK
+        x = torch.linspace(0, 1, 100_001, dtype=torch.float64)
+        for _ in range(steps):
+            p = a + b * x ** 2 + c * x ** 4
+            x = (p * x).abs()
+            assert float(p.abs().max()) <= 1024 and float(x.max()) <= 1024
+    else:
+        assert (steps, abc) == (3, (-4.0, 1.0, 0.5))
+    assert lib.fl_orthogonalize_check(10, 2.0, 0.0, 0.0) == nat.FL_OK
+    assert lib.fl_orthogonalize_check(11, 2.0, 0.0, 0.0) == nat.FL_ERR_INVALID_ARGUMENT
 
 
 def _sizes(*values):
