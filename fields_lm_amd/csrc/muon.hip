@@ -35,7 +35,10 @@ constexpr int kCopyTile = 64;  // of the tile that is laid out by a block
 constexpr int kTable = 56;     // matrices to a launch that sets up their table
 constexpr int kNormChunk = 4096;  // values of a block of the norm (one matrix of 256 x 632: 3.6 us, 12 with 16,384 values read one by one)
 constexpr int64_t kMaxMatrices = 1 << 20, kMaxSide = 1 << 20, kMaxValues = (int64_t)1 << 30;
-constexpr size_t kGroupBytes = (size_t)1 << 30;  // matrices are taken in groups of about this much workspace
+constexpr int kTile = 128, kSmallTile = 64;  // rows and columns of a product's tile
+constexpr int64_t kSlots = 512, kIdle = 150;  // tiles that run at a time (two to a CU)
+// (110 matrices of a model: groups of 1 GiB 15.3 ms, 2 GiB 14.7, 4 GiB 14.6)
+constexpr size_t kGroupBytes = (size_t)2 << 30;  // matrices are taken in groups of at most about this much workspace
 constexpr int kMaxSteps = 64;
 constexpr double kMaxBound = 1024.0;  // of singular values
 
@@ -289,11 +292,11 @@ __device__ __forceinline__ void update16(T* p, int left, const float* v, int muo
 template <int TILE>
 struct Shape;
 template <>
-struct Shape<128> {
+struct Shape<kTile> {
   static constexpr int WR = 2, WC = 2, BATCH = 1;
 };
 template <>
-struct Shape<64> {
+struct Shape<kSmallTile> {
   static constexpr int WR = 2, WC = 2, BATCH = 4;
 };
 template <int TILE>
@@ -569,17 +572,41 @@ struct Group {
   size_t bytes() const { return planes + (size_t)sums * 8 + (size_t)count * sizeof(Mat); }
 };
 
+// lower half of an m x m square in tiles
+int64_t square_tiles(int64_t m, int tile) {
+  const int64_t side = cdiv(m, tile);
+  return side * (side + 1) / 2;
+}
+
+// What a group's product of squares takes, in tiles of a card that runs kSlots at a time, a launch's start and end counted
+// as kIdle.
+int64_t cost(int64_t tiles) { return tiles ? cdiv(tiles, kSlots) * kSlots + kIdle : 0; }
+
+// As many matrices as kGroupBytes hold, or fewer where their tiles fill the card better: 21 matrices of 1,024 x 2,438 (756
+// tiles, two rounds of which the second is half empty) take 110 us a product, 14 of them 55. All that are left are taken at
+// once unless two groups are better.
 Group group_from(int64_t i, int64_t n, const int64_t* rows, const int64_t* cols) {
-  Group g = {i, 0, 0, 0};
+  Group g = {i, 0, 0, 0}, best = g;
+  int64_t tiles = 0, best_tiles = 0;
+  bool all = true;
   for (; g.end < n; ++g.end) {
     if (rows[g.end] * cols[g.end] == 0) continue;
     const size_t bytes = planes_bytes(rows[g.end], cols[g.end]);
-    if (g.count && g.planes + bytes > kGroupBytes) break;
+    if (g.count && g.planes + bytes > kGroupBytes) {
+      all = false;
+      break;
+    }
     g.planes += bytes;
     g.sums += norm_blocks(rows[g.end], cols[g.end]);
     ++g.count;
+    tiles += square_tiles(std::min(rows[g.end], cols[g.end]), kTile);
+    if (best_tiles == 0 || tiles * cost(best_tiles) >= best_tiles * cost(tiles)) {
+      best = g;
+      ++best.end;
+      best_tiles = tiles;
+    }
   }
-  return g;
+  return all && cost(tiles) <= cost(best_tiles) + cost(tiles - best_tiles) ? g : best;
 }
 
 // Bounds of what the steps form, from singular values in [0, 1], and the powers of two that bring them below 2^15.
@@ -706,16 +733,6 @@ void newton_schulz(const Launch<TILE>& launch, int steps, double a, double b, do
   }
 }
 
-// The tiles of a group's squares, lower half
-int64_t square_tiles(const std::vector<int64_t>& order, const int64_t* rows, const int64_t* cols, int tile) {
-  int64_t n = 0;
-  for (int64_t i : order) {
-    const int64_t side = cdiv(rows[i] < cols[i] ? rows[i] : cols[i], tile);
-    n += side * (side + 1) / 2;
-  }
-  return n;
-}
-
 int run(int64_t n, const void* const* g, void* const* p, float* const* buf, const int64_t* rows, const int64_t* cols,
         const double* lr_scale, int steps, double a, double b, double c, double eps, const Update& u, void* workspace,
         hipStream_t s) {
@@ -733,7 +750,11 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
     std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
       return std::max(rows[i], cols[i]) > std::max(rows[j], cols[j]);
     });
-    const int tile = square_tiles(order, rows, cols, 128) >= 100 ? 128 : 64;
+    // small tiles while the large ones leave most of the card idle. us, 64 | 128: 36 tiles of 128 (1,024 x 1,024) 291 | 550,
+    // 72 494 | 555, 108 569 | 565, 144 767 | 616, 200 (20 matrices of 400 x 400) 445 | 396
+    int64_t large = 0;
+    for (int64_t i : order) large += square_tiles(std::min(rows[i], cols[i]), kTile);
+    const int tile = large >= 100 ? kTile : kSmallTile;
     char* at = static_cast<char*>(workspace);
     half_t* planes = reinterpret_cast<half_t*>(at);
     double* sums = reinterpret_cast<double*>(at + group.planes);
@@ -758,9 +779,8 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
       planes += planes_bytes(rows[i], cols[i]) / sizeof(half_t);
       first_norm += norm_blocks(rows[i], cols[i]);
       first_copy += cdiv(padded(rows[i]), kCopyTile) * cdiv(padded(cols[i]), kCopyTile);
-      const int64_t side = cdiv(k.m, tile);
-      first_square += side * (side + 1) / 2;
-      first_apply += side * cdiv(k.n, tile);
+      first_square += square_tiles(k.m, tile);
+      first_apply += cdiv(k.m, tile) * cdiv(k.n, tile);
       if (t.n == kTable || done + t.n == group.count) {
         fl_muon_table_kernel<<<1, 64, 0, s>>>(t, mats + done);
         done += t.n;
@@ -771,10 +791,10 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
     fl_muon_norm_kernel<<<(unsigned)first_norm, 256, 0, s>>>(mats, count, u, sums);
     fl_muon_copy_kernel<<<(unsigned)first_copy, 256, 0, s>>>(mats, count, u, sums, eps, scale_for(1.0));
     const int squares = (int)first_square, applies = (int)first_apply;
-    if (tile == 128)
-      newton_schulz(Launch<128>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+    if (tile == kTile)
+      newton_schulz(Launch<kTile>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
     else
-      newton_schulz(Launch<64>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+      newton_schulz(Launch<kSmallTile>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_status(e);
   }

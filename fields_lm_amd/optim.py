@@ -101,7 +101,7 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float,
 
     Everything is computed in fp32 and in products of 22 bits and rounded once, to x's type; a matrix of zeros stays
     zeros, one with NaN or infinities becomes NaN. Coefficients with which singular values, or a step's factor, could
-    pass 1024 are refused. Not differentiable. A call takes up to a GiB of workspace, or what its largest matrix needs.
+    pass 1024 are refused. Not differentiable. A call takes up to 2 GiB of workspace, or what its largest matrix needs.
     """
     a, b, c = coefficients
     return nat.host().orthogonalize(x, steps, a, b, c, eps)
