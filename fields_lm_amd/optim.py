@@ -95,9 +95,10 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
 
 def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float, float, float] = NEWTON_SCHULZ,
                   eps: float = 1e-7) -> torch.Tensor:
-    """Matrices [..., M, N] (up to 2^20 of them, sides up to 2^20, 2^30 values each; fp32 or bf16, on a ROCm device) brought near their closest semi-orthogonal ones by
-    Newton-Schulz steps (``fl_orthogonalize``): from X = x / (|x| + eps), |x| the Frobenius norm, ``steps`` (1 to 64)
-    times X = a X + (b A + c A^2) X with A = X X^T (X^T X for a tall matrix), (a, b, c) the ``coefficients``.
+    """Matrices [..., M, N] (up to 2^20 of them, sides up to 2^20, 2^30 values each; fp32 or bf16, on a ROCm device)
+    brought near their closest semi-orthogonal ones by Newton-Schulz steps (``fl_orthogonalize``): from
+    X = x / (|x| + eps), |x| the Frobenius norm, ``steps`` (1 to 64) times X = a X + (b A + c A^2) X with A = X X^T
+    (X^T X for a tall matrix), (a, b, c) the ``coefficients``.
 
     Everything is computed in fp32 and in products of 22 bits and rounded once, to x's type; a matrix of zeros stays
     zeros, one with NaN or infinities becomes NaN. Coefficients with which singular values, or a step's factor, could

@@ -526,11 +526,11 @@ int fl_adamw_step(int64_t n, void* const* params, const void* const* grads, int 
 
 /*
  * Rows of an embedding by token and the gradient of its weight (no counterpart in the reference, which calls the stock
- * embedding).
+ * embedding). V up to 2^23, n up to 2^30, D up to 2^24.
  * fl_embedding: out [n, D] = scale * weight[tokens], weight rows weight_stride elements apart; a token outside 0 .. V - 1
  *   has NaN. masked: the transpose of the gradient: rows of the token `padding` (-1: none) and of tokens outside are zeros.
- * fl_embedding_backward: g_weight [V, D], contiguous, = scale * the sum of g [n, D] over the rows of each token, in
- *   their order, fp32, rounded once; zeros for `padding` (-1: none) and for rows of no token. Tokens outside pass
+ * fl_embedding_backward: g_weight [V, D], contiguous, = scale * the sum of g [n, D] over the rows of each token, in an
+ *   order of the tokens' alone, fp32, rounded once; zeros for `padding` (-1: none) and for rows of no token. Tokens outside pass
  *   nothing. Workspace 16-byte aligned, no initial contents needed.
  */
 int fl_embedding(const int64_t* tokens, int64_t n, const void* weight, int weight_dtype, int64_t V, int64_t D,
@@ -550,7 +550,9 @@ int fl_embedding_backward(const int64_t* tokens, int64_t n, const void* g, int g
  * fl_gated_scan_backward: from the forward's inputs and starts, and g_out [B, T, C] of drive_dtype and g_state [B, C]
  *   (either may be NULL): g_drive [B, T, C], g_gate of the gate's shape (or NULL), g_state_in [B, C] (or NULL), each of
  *   its tensor's type.
- * Maths in fp32, rounded once. Workspace 16-byte aligned, no initial contents needed.
+ * Maths in fp32, rounded once. B, C up to 2^24, T up to 2^30. Workspace 16-byte aligned, no initial contents needed (0
+ * bytes: NULL will do). Tiles of a chain wait for those before them; a wait that does not end within 2^20 polls leaves
+ * its tile's results NaN.
  */
 int64_t fl_gated_scan_tile(void);
 size_t fl_gated_scan_workspace_bytes(int64_t B, int64_t T, int64_t C, int backward);
