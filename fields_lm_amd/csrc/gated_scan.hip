@@ -11,9 +11,14 @@
 // those are rounded to the drive's type, and cost as much to read as the drive.
 //
 // Tiles of a chain (a sequence's 64 channels) find their start by looking back: each publishes its map, then its end, as
-// words of a value and a mark that it is there, and composes the maps of those before it up to the first that has
+// words of a value and a mark that it is there, and takes the maps of those before it up to the first that has
 // published its end. Tiles are taken in the order in which blocks start, from a counter: a tile waits only for tiles that
 // are running or done, so that every wait ends. The words are cleared by a launch before.
+//
+// Bound by memory: B=8, T=2,048, C=1,024 in fp32 44 us forward (4.6 TB/s) and 60 us back (5.6 TB/s); B=1, T=65,536, fp32 gates
+// and bf16 drives 99 us (5.4 TB/s) and 174 us (5.4 TB/s), where three launches over the same tiles (maps, composition,
+// steps) took 2.8 ms. Two blocks of 256 steps fit a CU (200 registers a lane): with fewer registers and more blocks
+// more tiles look back at once and further, 352 us in place of 292 for the long one.
 #include "fl_common.h"
 
 #include <type_traits>
@@ -28,6 +33,7 @@ constexpr int kWords = 3 * kChannels;  // of a tile: P and S of its map, its end
 constexpr int kShort = 8;      // steps up to which no tile is formed (64 sequences of 1,024 channels, one step: 3.2 us, a
                                // tile each 8.1)
 constexpr int kBehind = 2;     // tiles whose words are loaded at a time
+constexpr int kHeld = 16;      // tiles whose maps a tile holds; it waits for an end where it would need more
 constexpr uint32_t kMaxPolls = 1u << 20;  // of a wait that never ends; its tile's results are NaN
 constexpr int64_t kMaxB = 1 << 24, kMaxC = 1 << 24, kMaxT = (int64_t)1 << 30;
 
@@ -172,10 +178,14 @@ __device__ __forceinline__ uint64_t published(const uint64_t* from) {
 __device__ __forceinline__ bool there(uint64_t w) { return __all((uint32_t)w == 1u); }
 __device__ __forceinline__ float value_of(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
 
-// What enters the tile at place `place` of its chain: the maps of the tiles before it, nearest first, up to one that has
-// published its end. `words`: the tile's own, lane's channel; `back`: words from a tile to the one before it.
-__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, int place) {
-  float p = 1.f, s = 0.f;
+// A state behind a run. One of 0 passes none of the run's product, which may have overflowed.
+__device__ __forceinline__ float through(float p, float h, float s) { return h == 0.f ? s : fmaf(p, h, s); }
+
+// What enters the tile at place `place` of its chain: the end of the nearest tile before it that has published one, through
+// the maps of those between, which are held in `hold_p` and `hold_s` (kHeld rows of kChannels, the lane's column). Each
+// map is applied as its own tile applies it, so that the bits are the same wherever an end was found. `words`: the
+// tile's own, lane's channel; `back`: words from a tile to the one before it.
+__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, int place, float* hold_p, float* hold_s) {
   uint32_t polls = 0;
   for (int i = 1;;) {
     uint64_t w[kBehind][3];
@@ -190,10 +200,14 @@ __device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, 
 #pragma unroll
     for (int r = 0; r < kBehind; ++r) {
       if (stop || i + r > place) continue;
-      if (there(w[r][2])) return fmaf(p, value_of(w[r][2]), s);
-      if (there(w[r][0]) && there(w[r][1])) {
-        s = fmaf(p, value_of(w[r][1]), s);
-        p = times(p, value_of(w[r][0]));
+      if (there(w[r][2])) {
+        float h = value_of(w[r][2]);
+        for (int m = i + r - 2; m >= 0; --m) h = through(hold_p[m * kChannels], h, hold_s[m * kChannels]);
+        return h;
+      }
+      if (i + r <= kHeld && there(w[r][0]) && there(w[r][1])) {
+        hold_p[(i + r - 1) * kChannels] = value_of(w[r][0]);
+        hold_s[(i + r - 1) * kChannels] = value_of(w[r][1]);
         q = r + 1;
       } else {
         stop = true;
@@ -212,10 +226,11 @@ struct Place {
   int place, tile;  // in the order of the scan, in time
   unsigned chain;
   int64_t b, c0;
+  bool there;
 };
 template <bool BACK>
 __device__ __forceinline__ Place place_of(const Scan& s, uint32_t* s_ticket) {
-  unsigned t = blockIdx.x;
+  unsigned t = blockIdx.y * gridDim.x + blockIdx.x;
   if (s.ticket) {
     if (threadIdx.x == 0)
       *s_ticket = __hip_atomic_fetch_add(s.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -223,6 +238,7 @@ __device__ __forceinline__ Place place_of(const Scan& s, uint32_t* s_ticket) {
     t = (unsigned)uniform((int)*s_ticket);
   }
   Place r;
+  r.there = t < (unsigned)s.tiles * s.chains;
   r.place = (int)(t / s.chains);
   r.chain = t - (unsigned)r.place * s.chains;
   r.tile = BACK ? s.tiles - 1 - r.place : r.place;
@@ -240,9 +256,11 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
                                                                         float* __restrict__ starts,
                                                                         DT* __restrict__ out) {
   constexpr int STEPS = kForwardSteps, SEGS = kTile / STEPS;
+  static_assert(SEGS >= kHeld, "rows for the maps looked back at");
   __shared__ float s_p[SEGS][kChannels], s_s[SEGS][kChannels];
   __shared__ uint32_t s_ticket;
   const Place at = place_of<false>(s, &s_ticket);
+  if (!at.there) return;  // (the whole block)
   const int seg = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const int64_t c = at.c0 + lane * 4, left = s.C - c, t0 = (int64_t)at.tile * kTile + seg * STEPS;
   const int n = (int)(s.T - t0 < STEPS ? (s.T > t0 ? s.T - t0 : 0) : STEPS);
@@ -284,7 +302,7 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
       const float pi = ps[i], si = ss[i];
       ps[i] = pt;
       ss[i] = st;
-      st = fmaf(pi, st, si);
+      st = through(pi, st, si);
       pt = times(pt, pi);
     }
     uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
@@ -297,12 +315,12 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
         publish(words, pt);
         publish(words + kChannels, st);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, at.place);
+      first = look_back(words, (int64_t)s.chains * kWords, at.place, &s_p[0][ch], &s_s[0][ch]);
     }
-    const float last = fmaf(pt, first, st);
+    const float last = through(pt, first, st);
     if (more) publish(words + 2 * kChannels, last);
 #pragma unroll
-    for (int i = 0; i < SEGS; ++i) s_s[i][ch] = fmaf(ps[i], first, ss[i]);
+    for (int i = 0; i < SEGS; ++i) s_s[i][ch] = through(ps[i], first, ss[i]);
     if (k < s.C) {
       if (starts) starts[(at.b * s.tiles + at.tile) * s.C + k] = first;
       if (state_out && !more) state_out[at.b * s.C + k] = last;
@@ -328,7 +346,7 @@ __global__ __launch_bounds__(256) void fl_gated_short_kernel(const Scan s, const
                                                              float* __restrict__ state_out, float* __restrict__ starts,
                                                              DT* __restrict__ out) {
   constexpr int STEPS = kShort;
-  const unsigned chain = blockIdx.x * 16 + (threadIdx.x >> 4);
+  const unsigned chain = (blockIdx.y * gridDim.x + blockIdx.x) * 16 + (threadIdx.x >> 4);
   const int lane = threadIdx.x & 15;
   const int64_t b = chain / (unsigned)s.groups, c0 = (int64_t)(chain - (unsigned)b * (unsigned)s.groups) * kChannels;
   const int64_t c = c0 + lane * 4, left = s.C - c;
@@ -363,9 +381,11 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
     const Scan s, const float* __restrict__ starts, const DT* __restrict__ g_out, const float* __restrict__ g_state,
     GT* __restrict__ g_gate, float* __restrict__ part, DT* __restrict__ g_drive, float* __restrict__ g_state_in) {
   constexpr int STEPS = kBackSteps, SEGS = kTile / STEPS;
+  static_assert(SEGS >= 2 * kHeld, "rows for the maps looked back at");
   __shared__ float s_p[SEGS][kChannels], s_h[SEGS][kChannels], s_k[SEGS][kChannels];
   __shared__ uint32_t s_ticket;
   const Place at = place_of<true>(s, &s_ticket);
+  if (!at.there) return;  // (the whole block)
   const int seg = threadIdx.x >> 4, lane = threadIdx.x & 15;
   const int64_t c = at.c0 + lane * 4, left = s.C - c, t0 = (int64_t)at.tile * kTile + seg * STEPS;
   const int n = (int)(s.T - t0 < STEPS ? (s.T > t0 ? s.T - t0 : 0) : STEPS);
@@ -416,7 +436,7 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
 #pragma unroll
     for (int i = 0; i < SEGS; ++i) {
       s_h[i][ch] = now;
-      now = fmaf(ps[i], now, hs[i]);
+      now = through(ps[i], now, hs[i]);
     }
   } else if (threadIdx.x < 128) {
     float ps[SEGS], ks[SEGS], pt = 1.f, kt = 0.f;
@@ -430,7 +450,7 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
       const float pi = ps[i], ki = ks[i];
       ps[i] = pt;
       ks[i] = kt;
-      kt = fmaf(pi, kt, ki);
+      kt = through(pi, kt, ki);
       pt = times(pt, pi);
     }
     uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
@@ -443,12 +463,12 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
         publish(words, pt);
         publish(words + kChannels, kt);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, at.place);
+      first = look_back(words, (int64_t)s.chains * kWords, at.place, &s_k[0][ch], &s_k[kHeld][ch]);
     }
-    const float last = fmaf(pt, first, kt);
+    const float last = through(pt, first, kt);
     if (more) publish(words + 2 * kChannels, last);
 #pragma unroll
-    for (int i = 0; i < SEGS; ++i) s_k[i][ch] = fmaf(ps[i], first, ks[i]);
+    for (int i = 0; i < SEGS; ++i) s_k[i][ch] = through(ps[i], first, ks[i]);
     if (g_state_in && !more && cc < s.C) g_state_in[at.b * s.C + cc] = last;
   }
   __syncthreads();
@@ -507,8 +527,13 @@ struct Call {
   Scan s;
   int64_t B;
   hipStream_t stream;
-  unsigned blocks() const { return (unsigned)s.tiles * s.chains; }
 };
+
+// rows of 2^22 blocks: a row's threads have to be fewer than 2^32
+dim3 grid_of(int64_t blocks) {
+  const int64_t row = (int64_t)1 << 22;
+  return blocks <= row ? dim3((unsigned)blocks) : dim3((unsigned)row, (unsigned)cdiv(blocks, row));
+}
 
 // bytes of the ticket's line and the words; 0 where chains have one tile
 size_t word_bytes(int64_t B, int64_t T, int64_t C) {
@@ -526,12 +551,12 @@ void clear(const Call& c, size_t bytes) {
 template <typename GT, typename DT, bool TOKEN>
 int forward(const Call& c, size_t bytes, const float* state_in, float* state_out, float* starts, void* out) {
   if (c.s.T <= kShort) {
-    fl_gated_short_kernel<GT, DT, TOKEN><<<(unsigned)cdiv(c.s.chains, 16), 256, 0, c.stream>>>(
+    fl_gated_short_kernel<GT, DT, TOKEN><<<grid_of(cdiv((int64_t)c.s.chains, (int64_t)16)), 256, 0, c.stream>>>(
         c.s, state_in, state_out, starts, static_cast<DT*>(out));
     return hip_status(hipGetLastError());
   }
   clear(c, bytes);
-  fl_gated_scan_kernel<GT, DT, TOKEN><<<c.blocks(), kForwardThreads, 0, c.stream>>>(c.s, state_in, state_out, starts,
+  fl_gated_scan_kernel<GT, DT, TOKEN><<<grid_of((int64_t)c.s.tiles * c.s.chains), kForwardThreads, 0, c.stream>>>(c.s, state_in, state_out, starts,
                                                                                      static_cast<DT*>(out));
   return hip_status(hipGetLastError());
 }
@@ -540,7 +565,7 @@ template <typename GT, typename DT, bool TOKEN>
 int backward(const Call& c, size_t bytes, const float* starts, const void* g_out, const float* g_state, void* g_gate,
              void* g_drive, float* g_state_in, float* part) {
   clear(c, bytes);
-  fl_gated_back_kernel<GT, DT, TOKEN><<<c.blocks(), kBackThreads, 0, c.stream>>>(
+  fl_gated_back_kernel<GT, DT, TOKEN><<<grid_of((int64_t)c.s.tiles * c.s.chains), kBackThreads, 0, c.stream>>>(
       c.s, starts, static_cast<const DT*>(g_out), g_state, static_cast<GT*>(g_gate), part, static_cast<DT*>(g_drive),
       g_state_in);
   if (TOKEN && g_gate && c.s.groups > 1) {

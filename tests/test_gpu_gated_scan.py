@@ -253,6 +253,72 @@ def test_special_values(dev):
     assert bool(out.isfinite().all())
 
 
+@pytest.mark.parametrize("token", [False, True])
+def test_same_bits(dev, token):
+    """Wherever a tile finds the state that enters it, the results are the same bits."""
+    print(f"[case] gated_scan, same bits, token={token}", flush=True)
+    gate, drive, first, g_out, g_last = inputs(dev, 3, 9000, 300, token, F32, F32, True, 16)
+    gate = 1.0 - (1.0 - gate.abs()) * 1e-3
+    leaves = [t.detach().requires_grad_() for t in (gate, drive, first)]
+    busy = torch.randn(2048, 2048, device=dev)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    kept = None
+    for i in range(12):
+        if i % 3:
+            with torch.cuda.stream(side):  # other work takes some of the card
+                for _ in range(i):
+                    busy.mm(busy)
+        out, last = fl.gated_scan(*leaves, return_state=True)
+        got = [out.detach(), last.detach(), *torch.autograd.grad([out, last], leaves, [g_out, g_last])]
+        kept = kept or got
+        assert all(torch.equal(a, b) for a, b in zip(got, kept))
+    torch.cuda.synchronize()
+
+
+def test_states_of_zero_before_growing_gates(dev):
+    """A state of 0 stays 0 whatever the product of the gates behind it; products over several tiles may overflow."""
+    print("[case] gated_scan, growing gates", flush=True)
+    gate, drive = torch.full((1, 2000, 3), 2.0, device=dev), torch.zeros(1, 2000, 3, device=dev)
+    drive[0, 1990] = 1.0
+    leaves = [t.requires_grad_() for t in (gate, drive)]
+    out = fl.gated_scan(*leaves)
+    exp = torch.zeros_like(drive)
+    exp[0, 1990:] = 2.0 ** torch.arange(10.0, device=dev)[:, None]
+    assert torch.equal(out, exp)
+    up = torch.zeros_like(drive)
+    up[0, 5] = 1.0
+    got = torch.autograd.grad(out, leaves, up)
+    back = torch.zeros_like(drive)
+    back[0, :6] = 2.0 ** torch.arange(5.0, -1.0, -1.0, device=dev)[:, None]
+    assert torch.equal(got[1], back) and bool((got[0] == 0).all())
+    # 2^-60 times 2^90 over 1,920 steps: the product over eight tiles is 2^90, over the steps after the first tile 2^78;
+    # a gate of 2^(3 / 64) is off by a rounding a step, so that 1,920 steps are off by 1,920 * 2^-24 and their own roundings
+    gate = torch.full((1, 1920), 2.0 ** (3 / 64), device=dev)
+    first = torch.full((1, 3), 2.0 ** -60, device=dev)
+    out, last = fl.gated_scan(gate, torch.zeros(1, 1920, 3, device=dev), first, return_state=True)
+    assert bool(((last / 2.0 ** 30 - 1).abs() <= 1920 * 2.0 ** -22).all())
+
+
+def test_many_sequences(dev):
+    """More threads than one dimension of a launch holds: 2^23 chains of one tile back, 2^26 of one step forward."""
+    print("[case] gated_scan, 2^23 + 5 sequences", flush=True)
+    B = 2 ** 23 + 5
+    gen = torch.Generator(device=dev).manual_seed(17)
+    leaves = [torch.rand(shape, device=dev, generator=gen).requires_grad_() for shape in ((B, 1), (B, 1, 1), (B, 1))]
+    out = fl.gated_scan(*leaves)
+    exp = torch.addcmul(leaves[1].detach().double()[:, 0], leaves[0].detach().double(), leaves[2].detach().double())
+    assert bool(((out.detach()[:, 0] - exp).abs() <= exp * 2.0 ** -24).all())
+    got = torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert torch.equal(got[0], leaves[2]) and bool((got[1] == 1).all()) and torch.equal(got[2], leaves[0])
+    del leaves, out, exp, got
+    print("[case] gated_scan, 2^24 sequences of 257 channels", flush=True)
+    B, C = 2 ** 24, 257
+    drive = torch.randn(2 ** 20, C, device=dev, dtype=BF16, generator=gen).repeat(B // 2 ** 20, 1).view(B, 1, C)
+    out = fl.gated_scan(torch.rand(B, 1, device=dev, generator=gen), drive)
+    assert torch.equal(out, drive)
+
+
 def test_gradients_by_differences(dev):
     """The loss's quotient of differences, in a direction of each input. It is off by the outputs' roundings over the step,
     and by what the same quotient in 64 bits is off the derivative."""
