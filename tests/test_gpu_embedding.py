@@ -281,3 +281,16 @@ def test_refuses(dev):
         fl.embedding(t, w, scale=float("nan"))
     with pytest.raises(RuntimeError):
         torch.jit.trace(lambda x: fl.embedding(t, x), w)
+
+
+def test_more_rows_than_a_launch_holds(dev):
+    """2^26 + 8 rows of 512, a wave to each."""
+    print("[case] embedding, 2^26 + 8 tokens", flush=True)
+    n, V = 2 ** 26 + 8, 1000
+    weight = torch.randn(V, 512, device=dev, dtype=torch.bfloat16)
+    tokens = torch.randint(V, (n,), device=dev)
+    out = fl.embedding(tokens, weight)
+    for at in (0, 2 ** 25 - 4, 2 ** 26 - 4):
+        assert torch.equal(out[at:at + 12], weight[tokens[at:at + 12]])
+    some = torch.arange(0, n, 4099, device=dev)
+    assert torch.equal(out[some], weight[tokens[some]])
