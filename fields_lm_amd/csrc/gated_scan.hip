@@ -32,7 +32,6 @@ constexpr int kChannels = 64;  // of a chain
 constexpr int kWords = 3 * kChannels;  // of a tile: P and S of its map, its end
 constexpr int kShort = 8;      // steps up to which no tile is formed (64 sequences of 1,024 channels, one step: 3.2 us, a
                                // tile each 8.1)
-constexpr int kBehind = 2;     // tiles whose words are loaded at a time
 constexpr int kHeld = 16;      // tiles whose maps a tile holds; it waits for an end where it would need more
 constexpr uint32_t kMaxPolls = 1u << 20;  // of a wait that never ends; its tile's results are NaN
 constexpr int64_t kMaxB = 1 << 24, kMaxC = 1 << 24, kMaxT = (int64_t)1 << 30;
@@ -181,43 +180,32 @@ __device__ __forceinline__ float value_of(uint64_t w) { return __uint_as_float((
 // A state behind a run. One of 0 passes none of the run's product, which may have overflowed.
 __device__ __forceinline__ float through(float p, float h, float s) { return h == 0.f ? s : fmaf(p, h, s); }
 
-// What enters the tile at place `place` of its chain: the end of the nearest tile before it that has published one, through
+// What enters a tile behind its chain's first: the end of the nearest tile before it that has published one, through
 // the maps of those between, which are held in `hold_p` and `hold_s` (kHeld rows of kChannels, the lane's column). Each
-// map is applied as its own tile applies it, so that the bits are the same wherever an end was found. `words`: the
+// map is applied as its own tile applies it, so that the bits are the same wherever an end was found (one product of the
+// maps took 2 us less of 286, with bits that varied). `words`: the
 // tile's own, lane's channel; `back`: words from a tile to the one before it.
-__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, int place, float* hold_p, float* hold_s) {
+__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, float* hold_p, float* hold_s) {
   uint32_t polls = 0;
-  for (int i = 1;;) {
-    uint64_t w[kBehind][3];
-#pragma unroll
-    for (int q = 0; q < kBehind; ++q) {
-      const uint64_t* from = words - (int64_t)min(i + q, place) * back;
-#pragma unroll
-      for (int k = 0; k < 3; ++k) w[q][k] = published(from + k * kChannels);
-    }
-    int q = 0;
-    bool stop = false;
-#pragma unroll
-    for (int r = 0; r < kBehind; ++r) {
-      if (stop || i + r > place) continue;
-      if (there(w[r][2])) {
-        float h = value_of(w[r][2]);
-        for (int m = i + r - 2; m >= 0; --m) h = through(hold_p[m * kChannels], h, hold_s[m * kChannels]);
-        return h;
-      }
-      if (i + r <= kHeld && there(w[r][0]) && there(w[r][1])) {
-        hold_p[(i + r - 1) * kChannels] = value_of(w[r][0]);
-        hold_s[(i + r - 1) * kChannels] = value_of(w[r][1]);
-        q = r + 1;
-      } else {
-        stop = true;
-      }
-    }
-    i += q;
-    if (q == 0) {
+  for (int i = 0;;) {
+    words -= back;  // (the first tile of a chain has an end, and is the last to be looked at)
+    uint64_t p, s, end;
+    for (;;) {
+      p = published(words);
+      s = published(words + kChannels);
+      end = published(words + 2 * kChannels);
+      if (there(end) || (i < kHeld && there(p) && there(s))) break;
       if (++polls >= kMaxPolls) return __uint_as_float(0x7fc00000u);
       __builtin_amdgcn_s_sleep(1);
     }
+    if (there(end)) {
+      float h = value_of(end);
+      for (; i > 0; --i) h = through(hold_p[(i - 1) * kChannels], h, hold_s[(i - 1) * kChannels]);
+      return h;
+    }
+    hold_p[i * kChannels] = value_of(p);
+    hold_s[i * kChannels] = value_of(s);
+    ++i;
   }
 }
 
@@ -315,7 +303,7 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
         publish(words, pt);
         publish(words + kChannels, st);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, at.place, &s_p[0][ch], &s_s[0][ch]);
+      first = look_back(words, (int64_t)s.chains * kWords, &s_p[0][ch], &s_s[0][ch]);
     }
     const float last = through(pt, first, st);
     if (more) publish(words + 2 * kChannels, last);
@@ -463,7 +451,7 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
         publish(words, pt);
         publish(words + kChannels, kt);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, at.place, &s_k[0][ch], &s_k[kHeld][ch]);
+      first = look_back(words, (int64_t)s.chains * kWords, &s_k[0][ch], &s_k[kHeld][ch]);
     }
     const float last = through(pt, first, kt);
     if (more) publish(words + 2 * kChannels, last);
