@@ -17,7 +17,7 @@
 // Bound by the matrix units: 64 squares of 1,024 x 1,024 take 157 to 165 us a product (1.4 to 1.5 PFLOP/s of fp16, of which a
 // third counts; registers alone reach 1.7 on such values), the matrix units 88% busy while a CU has tiles. 110 matrices of
 // a model, 0.27 G values, take 14.7 ms, steps on X in fp32 library products 80; a single 256 x 632 matrix, 20 dependent
-// launches, 126 us (1,175). What was tried and is no faster (110 matrices, 15.9 ms at the time): tiles of 256 x 256 (15.2
+// launches, 123 us (1,175). What was tried and is no faster (110 matrices, 15.9 ms at the time): tiles of 256 x 256 (15.2
 // to 19.0), 256 x 128 with three buffers (18.3), 128 x 128 with four and one block to a CU (17.8), all of a step's reads
 // ahead of its products (17.2), wave priority (1% slower), waves above the diagonal left idle (4% slower).
 #include "fl_common.h"
@@ -71,13 +71,19 @@ __global__ __launch_bounds__(64) void fl_muon_table_kernel(const Table t, Mat* _
   if ((int)threadIdx.x < t.n) out[threadIdx.x] = t.mat[threadIdx.x];
 }
 
-// the matrix whose blocks, counted by FIRST, hold `block`: as many begin at or before it, less one
+// the matrix whose blocks, counted by FIRST, hold `block`: the last that begins at or before it, 64 of them tried at
+// a time (4,096 matrices of 64 x 64 1.5 ms, 3.9 by counting all that begin before it)
 template <int Mat::*FIRST>
 __device__ __forceinline__ int matrix_of(const Mat* mats, int n, int block) {
   const int lane = threadIdx.x & 63;
-  int begun = 0;
-  for (int i = 0; i < n; i += 64) begun += __popcll(__ballot(i + lane < n && mats[min(i + lane, n - 1)].*FIRST <= block));
-  return uniform(begun - 1);
+  int at = 0;
+  for (int left = n; left > 1;) {
+    const int step = (left + 63) / 64, k = lane * step;
+    const int last = __popcll(__ballot(k < left && mats[at + min(k, left - 1)].*FIRST <= block)) - 1;
+    at += last * step;
+    left = min(step, left - last * step);
+  }
+  return uniform(at);
 }
 
 struct Update {

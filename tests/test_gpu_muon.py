@@ -168,6 +168,31 @@ def test_stacks_and_strides(dev):
     assert not wide.requires_grad
 
 
+@pytest.mark.parametrize("n", [63, 64, 65, 128, 4096, 4097, 10_000])
+def test_many_matrices(dev, n):
+    """A stack's matrices are found at any count of them, with one tile and with several to each."""
+    for shape in ((5, 9), (65, 130)):
+        print(f"[case] orthogonalize, {n} of {shape}", flush=True)
+        x = matrices(dev, (n, *shape), n)
+        got = fl.orthogonalize(x)
+        check(got, x)
+        for i in (0, 1, n // 2, n - 2, n - 1):
+            assert torch.equal(fl.orthogonalize(x[i]), got[i])
+
+
+def test_many_ragged_matrices(dev):
+    print("[case] muon_step, 5,000 ragged matrices", flush=True)
+    shapes = [(1 + i % 13, 1 + i * 7 % 90) for i in range(4990)] + [(140, 300)] * 10
+    params, grads, bufs = model(dev, F32, 9, shapes)
+    before = [p.clone() for p in params]
+    fl.muon_step(params, grads, bufs, lr=0.5, weight_decay=0.0, momentum=0.0, nesterov=False)
+    for i in (*range(0, 5000, 333), 4988, 4989, 4990, 4999):
+        r, c = shapes[i]
+        step = 0.5 * max(1.0, r / c) ** 0.5 * fl.orthogonalize(grads[i])
+        # the parameter's rounding and that of r as it is multiplied
+        assert torch.allclose(params[i], before[i] - step, rtol=2.0 ** -22, atol=2.0 ** -22)
+
+
 def test_sizes_of_values(dev):
     """Zeros, large and small scales, a row or column alone, an identity; NaN and infinities spoil their matrix alone."""
     print("[case] orthogonalize, values", flush=True)
