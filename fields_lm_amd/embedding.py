@@ -8,15 +8,18 @@ import torch
 
 from . import _native as nat
 
+MAX_ROWS = 1 << 23  # of a weight
+
 
 def embedding(tokens: torch.Tensor, weight: torch.Tensor, *, scale: float = 1.0, padding_idx: Optional[int] = None,
               dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``weight[tokens] * scale``: [..., D] in ``dtype`` (the weight's unless given), computed in fp32 and rounded once.
 
-    tokens [...] int64, weight [V, D] (V up to 2^23) fp32 or bf16, both on one ROCm device. The gradient of ``weight`` is dense, in its
-    type: every row sums its tokens' gradients in fp32 in an order that the tokens alone decide, times ``scale``, rounded
-    once, so that it is the same bits every time. Rows of no token are zeros. The row of ``padding_idx`` (from the end where negative)
-    is read like any other and gets no gradient. A token outside 0 .. V - 1 has a row of NaN and passes no gradient.
+    tokens [...] int64 (up to 2^30), weight [V, D] (V up to 2^23) fp32 or bf16, both on one ROCm device. The gradient of
+    ``weight`` is dense, in its type: every row sums its tokens' gradients in fp32 in an order that the tokens alone
+    decide, times ``scale``, rounded once, so that it is the same bits every time. Rows of no token are zeros. The row of
+    ``padding_idx`` (from the end where negative) is read like any other and gets no gradient. A token outside 0 .. V - 1
+    has a row of NaN and passes no gradient.
 
     Backward passes can themselves be differentiated. Under graph capture the backward pass is refused while a graph of
     the default stream holds the weight's leaves.

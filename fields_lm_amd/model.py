@@ -41,7 +41,7 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from ._dispatch import KERNEL_DTYPES, eager, free_rounding, no_grad_needed, plain_call, plain_linear
-from .embedding import embedding
+from .embedding import MAX_ROWS, embedding
 from .field import (FieldBlock, RMSNorm, _linear_residual, boundary_scan, gate_residual_norm, gated_scan, rms_norm,
                     rms_norm_takes, swiglu)
 from .logprobs import TokenLogprobs, token_logprobs
@@ -1129,6 +1129,7 @@ class FieldTokenSystem(nn.Module):
         weight = emb.weight
         if (plain_call(emb, nn.Embedding) and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse
                 and not no_grad_needed(weight) and weight.dtype in KERNEL_DTYPES and tokens.dtype == torch.int64
+                and 0 < weight.shape[0] <= MAX_ROWS and weight.shape[1] > 0
                 and eager(weight, tokens)):
             return embedding(tokens, weight, padding_idx=emb.padding_idx)
         return emb(tokens)

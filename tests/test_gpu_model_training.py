@@ -130,3 +130,18 @@ def test_training_steps(dev):
     muon.step()
     adam.step()
     assert all(bool(p.isfinite().all()) for p in named.values())
+
+
+@pytest.mark.parametrize("rows", [2 ** 23, 2 ** 23 + 1])
+def test_the_largest_vocabulary(dev, rows):
+    """Past the kernel's rows the model's embedding is the stock one."""
+    print(f"[case] model's embedding of {rows} rows", flush=True)
+    core = small_model(dev)
+    core.emb = torch.nn.Embedding(rows, 5, device=dev)
+    tokens = torch.tensor([[0, rows - 1, 7, rows - 1]], device=dev)
+    up = torch.randn(1, 4, 5, device=dev)
+    x = core._embed(tokens)
+    assert torch.equal(x, core.emb.weight[tokens])
+    got, = torch.autograd.grad(x, core.emb.weight, up)
+    assert torch.equal(got[[0, 7]], up[0, [0, 2]]) and torch.equal(got[rows - 1], up[0, 1] + up[0, 3])
+    assert int(got.ne(0).any(1).sum()) == 3
