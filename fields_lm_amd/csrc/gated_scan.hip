@@ -17,8 +17,9 @@
 //
 // Bound by memory: B=8, T=2,048, C=1,024 in fp32 44 us forward (4.6 TB/s) and 60 us back (5.6 TB/s); B=1, T=65,536, fp32 gates
 // and bf16 drives 99 us (5.4 TB/s) and 174 us (5.4 TB/s), where three launches over the same tiles (maps, composition,
-// steps) took 2.8 ms. Two blocks of 256 steps fit a CU (200 registers a lane): with fewer registers and more blocks
-// more tiles look back at once and further, 352 us in place of 292 for the long one.
+// steps) took 2.8 ms. Of the forward's blocks with a gate a channel two fit a CU (190 registers a lane), by a limit: with
+// three more tiles look back at once and further (42.5 us for the first in place of 39.5 without gradients kept). With a
+// gate a token four do (126), and of the backward's blocks, twice as many threads, one does (158 and 128).
 #include "fl_common.h"
 
 #include <type_traits>
@@ -149,12 +150,16 @@ struct Gates<GT, true, STEPS> {
   __device__ __forceinline__ float at(int) const { return of_lane<J>(v); }
 };
 
-// The product of two runs' gates. One too small for a float is kept off 0, which is a closed gate's alone: an infinite state
-// before such a run is infinite behind it, as it is step by step.
-__device__ __forceinline__ float kept(float product, bool closed) {
-  return product == 0.f && !closed ? __builtin_copysignf(0x1p-149f, product) : product;
+// A run's product of gates is held in fp64: in fp32 that of ordinary ones leaves the range (0.5^256), and a large state, or
+// gates above 1 that follow, would bring what is lost of it back. One too small for that too is kept off 0, which is a
+// closed gate's alone: an infinite state before such a run is infinite behind it, as it is step by step, and a finite
+// one passes nothing (2^-1022 of it). One too large is kept finite, so that a state of 0 passes 0 and any other infinity.
+// The last bit stays clear, for `publish`.
+constexpr double kLeast = 0x1p-1022, kMost = 0x1.ffffffffffffep1023;
+__device__ __forceinline__ double kept(double product, bool closed) {
+  const double size = fmin(fmax(fabs(product), kLeast), kMost);
+  return closed ? 0.0 : __longlong_as_double(__double_as_longlong(copysign(size, product)) & ~1ll);
 }
-__device__ __forceinline__ float times(float p, float q) { return kept(p * q, p == 0.f || q == 0.f); }
 
 template <int N, int I = 0, typename F>
 __device__ __forceinline__ void each(F f) {
@@ -168,24 +173,28 @@ __device__ __forceinline__ void each_back(F f) {
   each<N>([&](auto i) { f(std::integral_constant<int, N - 1 - decltype(i)::value>()); });
 }
 
-__device__ __forceinline__ void publish(uint64_t* to, float v) {
-  __hip_atomic_store(to, (uint64_t)__float_as_uint(v) << 32 | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// a word: the last bit says that it is there, the others are a product's, or a float's in the upper half
+__device__ __forceinline__ void publish(uint64_t* to, uint64_t bits) {
+  __hip_atomic_store(to, bits | 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+__device__ __forceinline__ void publish(uint64_t* to, float v) { publish(to, (uint64_t)__float_as_uint(v) << 32); }
+__device__ __forceinline__ void publish(uint64_t* to, double p) { publish(to, (uint64_t)__double_as_longlong(p)); }
 __device__ __forceinline__ uint64_t published(const uint64_t* from) {
   return __hip_atomic_load(from, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-__device__ __forceinline__ bool there(uint64_t w) { return __all((uint32_t)w == 1u); }
+__device__ __forceinline__ bool there(uint64_t w) { return __all(w & 1u); }
 __device__ __forceinline__ float value_of(uint64_t w) { return __uint_as_float((uint32_t)(w >> 32)); }
+__device__ __forceinline__ double product_of(uint64_t w) { return __longlong_as_double((long long)(w & ~(uint64_t)1)); }
 
-// A state behind a run. One of 0 passes none of the run's product, which may have overflowed.
-__device__ __forceinline__ float through(float p, float h, float s) { return h == 0.f ? s : fmaf(p, h, s); }
+// a state behind a run
+__device__ __forceinline__ double through(double p, double h, double s) { return fma(p, h, s); }
 
 // What enters a tile behind its chain's first: the end of the nearest tile before it that has published one, through
 // the maps of those between, which are held in `hold_p` and `hold_s` (kHeld rows of kChannels, the lane's column). Each
 // map is applied as its own tile applies it, so that the bits are the same wherever an end was found (one product of the
 // maps took 2 us less of 286, with bits that varied). `words`: the
 // tile's own, lane's channel; `back`: words from a tile to the one before it.
-__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, float* hold_p, float* hold_s) {
+__device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, double* hold_p, float* hold_s) {
   uint32_t polls = 0;
   for (int i = 0;;) {
     words -= back;  // (the first tile of a chain has an end, and is the last to be looked at)
@@ -200,12 +209,33 @@ __device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, 
     }
     if (there(end)) {
       float h = value_of(end);
-      for (; i > 0; --i) h = through(hold_p[(i - 1) * kChannels], h, hold_s[(i - 1) * kChannels]);
+      for (; i > 0; --i) h = (float)through(hold_p[(i - 1) * kChannels], h, hold_s[(i - 1) * kChannels]);
       return h;
     }
-    hold_p[i * kChannels] = value_of(p);
+    hold_p[i * kChannels] = product_of(p);
     hold_s[i * kChannels] = value_of(s);
     ++i;
+  }
+}
+
+// What enters a tile's segments: `first` through the products of those before each (BACK: behind each), whose ends are in `ends`.
+// The products are the bare ones, which may have left fp64: a state of 0 passes none, and for infinite ones they are formed again.
+template <int SEGS, bool BACK>
+__device__ __forceinline__ void enter(const double (*each_p)[kChannels], const double (*run_p)[kChannels],
+                                      float (*ends)[kChannels], int ch, float first) {
+  if (__any(fabsf(first) == __builtin_inff())) {
+    double run = 1.0;
+    for (int i = 0; i < SEGS; ++i) {
+      const int seg = BACK ? SEGS - 1 - i : i;
+      if (first != 0.f) ends[seg][ch] = (float)through(run, first, ends[seg][ch]);
+      run = kept(run * each_p[seg][ch], run == 0.0 || each_p[seg][ch] == 0.0);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < SEGS; ++i) {
+    const float end = ends[i][ch], now = (float)through(run_p[i][ch], first, end);
+    ends[i][ch] = first == 0.f ? end : now;
   }
 }
 
@@ -239,13 +269,14 @@ constexpr int kForwardSteps = 16, kBackSteps = 8;  // of a segment
 constexpr int kForwardThreads = kTile / kForwardSteps * 16, kBackThreads = kTile / kBackSteps * 16;
 
 template <typename GT, typename DT, bool TOKEN>
-__global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Scan s, const float* __restrict__ state_in,
+__global__ __launch_bounds__(kForwardThreads) __attribute__((amdgpu_waves_per_eu(2, TOKEN ? 4 : 2)))
+void fl_gated_scan_kernel(const Scan s, const float* __restrict__ state_in,
                                                                         float* __restrict__ state_out,
                                                                         float* __restrict__ starts,
                                                                         DT* __restrict__ out) {
   constexpr int STEPS = kForwardSteps, SEGS = kTile / STEPS;
-  static_assert(SEGS >= kHeld, "rows for the maps looked back at");
-  __shared__ float s_p[SEGS][kChannels], s_s[SEGS][kChannels];
+  __shared__ double s_p[SEGS][kChannels], s_before[SEGS][kChannels], s_hold_p[kHeld][kChannels];
+  __shared__ float s_s[SEGS][kChannels], s_hold_s[kHeld][kChannels];
   __shared__ uint32_t s_ticket;
   const Place at = place_of<false>(s, &s_ticket);
   if (!at.there) return;  // (the whole block)
@@ -261,7 +292,8 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
     u[j].fill(0.f);
     if (j < n && left > 0) u[j].load(from + j * s.drive_t, left);
   }
-  f32x4 p = {1.f, 1.f, 1.f, 1.f}, least = p, h = {0.f, 0.f, 0.f, 0.f};
+  double p[4] = {1.0, 1.0, 1.0, 1.0};
+  f32x4 least = {1.f, 1.f, 1.f, 1.f}, h = {0.f, 0.f, 0.f, 0.f};
   each<STEPS>([&](auto j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -272,27 +304,25 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
     }
   });
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = kept(p[i], least[i] == 0.f);
-  *reinterpret_cast<f32x4*>(&s_p[seg][lane * 4]) = p;
+  for (int i = 0; i < 4; ++i) s_p[seg][lane * 4 + i] = kept(p[i], least[i] == 0.f);
   *reinterpret_cast<f32x4*>(&s_s[seg][lane * 4]) = h;
   __syncthreads();
   if (threadIdx.x < kChannels) {
     const int ch = threadIdx.x;
     const int64_t k = at.c0 + ch;
-    float ps[SEGS], ss[SEGS], pt = 1.f, st = 0.f;
+    double run = 1.0, smallest = 1.0, end = 0.0;
 #pragma unroll
     for (int i = 0; i < SEGS; ++i) {
-      ps[i] = s_p[i][ch];
-      ss[i] = s_s[i][ch];
+      const double pi = s_p[i][ch];
+      const float si = s_s[i][ch];
+      s_before[i][ch] = run;
+      s_s[i][ch] = (float)end;
+      end = through(pi, end, si);
+      run *= pi;
+      smallest = fmin(smallest, fabs(pi));
     }
-#pragma unroll
-    for (int i = 0; i < SEGS; ++i) {
-      const float pi = ps[i], si = ss[i];
-      ps[i] = pt;
-      ss[i] = st;
-      st = through(pi, st, si);
-      pt = times(pt, pi);
-    }
+    const double pt = kept(run, smallest == 0.0);
+    const float st = (float)end;
     uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
     float first;
     const bool more = at.place + 1 < s.tiles;
@@ -303,12 +333,11 @@ __global__ __launch_bounds__(kForwardThreads) void fl_gated_scan_kernel(const Sc
         publish(words, pt);
         publish(words + kChannels, st);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, &s_p[0][ch], &s_s[0][ch]);
+      first = look_back(words, (int64_t)s.chains * kWords, &s_hold_p[0][ch], &s_hold_s[0][ch]);
     }
-    const float last = through(pt, first, st);
+    const float last = (float)through(pt, first, st);
     if (more) publish(words + 2 * kChannels, last);
-#pragma unroll
-    for (int i = 0; i < SEGS; ++i) s_s[i][ch] = through(ps[i], first, ss[i]);
+    enter<SEGS, false>(s_p, s_before, s_s, ch, first);
     if (k < s.C) {
       if (starts) starts[(at.b * s.tiles + at.tile) * s.C + k] = first;
       if (state_out && !more) state_out[at.b * s.C + k] = last;
@@ -369,8 +398,8 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
     const Scan s, const float* __restrict__ starts, const DT* __restrict__ g_out, const float* __restrict__ g_state,
     GT* __restrict__ g_gate, float* __restrict__ part, DT* __restrict__ g_drive, float* __restrict__ g_state_in) {
   constexpr int STEPS = kBackSteps, SEGS = kTile / STEPS;
-  static_assert(SEGS >= 2 * kHeld, "rows for the maps looked back at");
-  __shared__ float s_p[SEGS][kChannels], s_h[SEGS][kChannels], s_k[SEGS][kChannels];
+  __shared__ double s_p[SEGS][kChannels], s_after[SEGS][kChannels], s_hold_p[kHeld][kChannels];
+  __shared__ float s_h[SEGS][kChannels], s_k[SEGS][kChannels], s_hold_k[kHeld][kChannels];
   __shared__ uint32_t s_ticket;
   const Place at = place_of<true>(s, &s_ticket);
   if (!at.there) return;  // (the whole block)
@@ -392,7 +421,8 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
     u[j].fill(0.f);
     if (j < n && left > 0) u[j].load(from + j * s.drive_t, left);
   }
-  f32x4 p = {1.f, 1.f, 1.f, 1.f}, least = p, h = {0.f, 0.f, 0.f, 0.f}, k = {0.f, 0.f, 0.f, 0.f};
+  double p[4] = {1.0, 1.0, 1.0, 1.0};
+  f32x4 least = {1.f, 1.f, 1.f, 1.f}, h = {0.f, 0.f, 0.f, 0.f}, k = h;
   each<STEPS>([&](auto j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -403,44 +433,38 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
     }
   });
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = kept(p[i], least[i] == 0.f);
+  for (int i = 0; i < 4; ++i) s_p[seg][lane * 4 + i] = kept(p[i], least[i] == 0.f);
   each_back<STEPS>([&](auto j) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) k[i] = a.template at<decltype(j)::value>(i) * (k[i] + d[decltype(j)::value][i]);
   });
-  *reinterpret_cast<f32x4*>(&s_p[seg][lane * 4]) = p;
   *reinterpret_cast<f32x4*>(&s_h[seg][lane * 4]) = h;
   *reinterpret_cast<f32x4*>(&s_k[seg][lane * 4]) = k;
   __syncthreads();
   const int ch = threadIdx.x & 63;
   const int64_t cc = at.c0 + ch;
   if (threadIdx.x < 64) {
-    float now = cc < s.C ? starts[(at.b * s.tiles + at.tile) * s.C + cc] : 0.f, ps[SEGS], hs[SEGS];
+    double now = cc < s.C ? starts[(at.b * s.tiles + at.tile) * s.C + cc] : 0.f;
 #pragma unroll
     for (int i = 0; i < SEGS; ++i) {
-      ps[i] = s_p[i][ch];
-      hs[i] = s_h[i][ch];
-    }
-#pragma unroll
-    for (int i = 0; i < SEGS; ++i) {
-      s_h[i][ch] = now;
-      now = through(ps[i], now, hs[i]);
+      const float hi = s_h[i][ch];
+      s_h[i][ch] = (float)now;
+      now = through(s_p[i][ch], now, hi);
     }
   } else if (threadIdx.x < 128) {
-    float ps[SEGS], ks[SEGS], pt = 1.f, kt = 0.f;
-#pragma unroll
-    for (int i = 0; i < SEGS; ++i) {
-      ps[i] = s_p[i][ch];
-      ks[i] = s_k[i][ch];
-    }
+    double run = 1.0, smallest = 1.0, end = 0.0;
 #pragma unroll
     for (int i = SEGS - 1; i >= 0; --i) {
-      const float pi = ps[i], ki = ks[i];
-      ps[i] = pt;
-      ks[i] = kt;
-      kt = through(pi, kt, ki);
-      pt = times(pt, pi);
+      const double pi = s_p[i][ch];
+      const float ki = s_k[i][ch];
+      s_after[i][ch] = run;
+      s_k[i][ch] = (float)end;
+      end = through(pi, end, ki);
+      run *= pi;
+      smallest = fmin(smallest, fabs(pi));
     }
+    const double pt = kept(run, smallest == 0.0);
+    const float kt = (float)end;
     uint64_t* words = s.words + ((int64_t)at.place * s.chains + at.chain) * kWords + ch;
     float first;
     const bool more = at.place + 1 < s.tiles;
@@ -451,12 +475,11 @@ __global__ __launch_bounds__(kBackThreads) void fl_gated_back_kernel(
         publish(words, pt);
         publish(words + kChannels, kt);
       }
-      first = look_back(words, (int64_t)s.chains * kWords, &s_k[0][ch], &s_k[kHeld][ch]);
+      first = look_back(words, (int64_t)s.chains * kWords, &s_hold_p[0][ch], &s_hold_k[0][ch]);
     }
-    const float last = through(pt, first, kt);
+    const float last = (float)through(pt, first, kt);
     if (more) publish(words + 2 * kChannels, last);
-#pragma unroll
-    for (int i = 0; i < SEGS; ++i) s_k[i][ch] = through(ps[i], first, ks[i]);
+    enter<SEGS, true>(s_p, s_after, s_k, ch, first);
     if (g_state_in && !more && cc < s.C) g_state_in[at.b * s.C + cc] = last;
   }
   __syncthreads();

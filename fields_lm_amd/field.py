@@ -382,9 +382,9 @@ def gated_scan(gate: torch.Tensor, drive: torch.Tensor, state_in: Optional[torch
 
     Gradients flow to gate, drive and state_in. A backward that is to be differentiated itself (``create_graph``) runs
     stock operations. A gate of 0 starts a new sequence, one of 1 with a drive of 0 passes the state on. Steps are
-    composed in tiles of 256, so that a state that is not 0 needs products of the gates within a tile that are finite in
-    fp32, which they are for gates of at most 1. The same inputs give the same bits. Under graph capture the backward pass
-    is refused while a graph of the default stream holds the inputs' leaves.
+    composed in tiles of 256 by products of the gates in fp64: a state that leaves fp32's range and would come back to it
+    within a tile may do so. The same inputs give the same bits. Under graph capture the backward pass is refused while a
+    graph of the default stream holds the inputs' leaves.
     """
     out, last = nat.host().gated_scan(gate, drive, state_in, return_state)
     return (out, last) if return_state else out

@@ -300,6 +300,54 @@ def test_states_of_zero_before_growing_gates(dev):
     assert bool(((last / 2.0 ** 30 - 1).abs() <= 1920 * 2.0 ** -22).all())
 
 
+def gates(dev, T, *runs):
+    """[1, T] of 1, but (from, to, value) for each of `runs`."""
+    gate = torch.ones(1, T, device=dev)
+    for lo, hi, value in runs:
+        gate[:, lo:hi] = value
+    return gate
+
+
+# with a state of `size` before and a gradient of the last state of as much; every state, gradient and product of both is an
+# ordinary number in fp32, the products of gates over a segment or a tile are not
+RUNS = [(1e15, (3, 19, 1e-3)), (1e15, (250, 266, 1e-3)), (1e15, (3, 19, 1e-3), (300, 305, 1e3)),
+        (1e15, (3, 19, 1e-3), (40, 45, 1e3)), (1e15, (3, 19, -1e-3), (530, 533, -1e3)), (1e-30, (3, 48, 10.0)),
+        (1e-30, (3, 33, 10.0), (40, 55, -10.0)), (1e-30, (240, 285, 10.0))]
+
+
+@pytest.mark.parametrize("token", [False, True])
+@pytest.mark.parametrize("size,runs", [(r[0], r[1:]) for r in RUNS], ids=str)
+def test_products_outside_fp32(dev, size, runs, token):
+    print(f"[case] gated_scan, products of {runs} token={token}", flush=True)
+    T, C = 700, 5
+    gate = gates(dev, T, *runs)
+    if not token:
+        gate = gate[..., None].expand(1, T, C).contiguous()
+    first = torch.linspace(0.5, 1.5, C, device=dev)[None] * size
+    drive, g_out, g_last = torch.zeros(1, T, C, device=dev), torch.zeros(1, T, C, device=dev), first.flip(1)
+    exp = expected(gate, drive, first, g_out, g_last)
+    leaves = [t.detach().requires_grad_() for t in (gate, drive, first)]
+    out, last = fl.gated_scan(*leaves, return_state=True)
+    close(out.detach(), exp["out"], "out")
+    close(last.detach(), exp["state"], "state")
+    got = torch.autograd.grad([out, last], leaves, [g_out, g_last])
+    for name, g in zip(("gate", "drive", "state_in"), got):
+        close(g, exp[name], name)
+
+
+@pytest.mark.parametrize("value", [1e-3, -1e-3, 1e-30])
+def test_infinite_states_before_small_gates(dev, value):
+    """Infinite step by step, also where a tile's product of gates is too small for any number; a finite state is gone."""
+    print(f"[case] gated_scan, infinite states before gates of {value}", flush=True)
+    gate, drive = torch.full((1, 700), value, device=dev), torch.ones(1, 700, 2, device=dev)
+    first = torch.tensor([[float("inf"), 1e30]], device=dev)
+    out, last = fl.gated_scan(gate, drive, first, return_state=True)
+    sign = torch.full((700,), value, device=dev).sign().cumprod(0)
+    assert torch.equal(out[0, :, 0], sign * float("inf")) and torch.equal(last[0, 0], out[0, -1, 0])
+    exp = expected(gate, drive[..., 1:].contiguous(), first[:, 1:], None, None)
+    close(out[..., 1:], exp["out"], "out")
+
+
 def test_many_sequences(dev):
     """More threads than one dimension of a launch holds: 2^23 chains of one tile back, 2^26 of one step forward."""
     print("[case] gated_scan, 2^23 + 5 sequences", flush=True)
