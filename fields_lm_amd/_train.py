@@ -158,33 +158,52 @@ def transition_ops(radius_logit, theta):
     return (radius * torch.cos(theta)).contiguous(), (radius * torch.sin(theta)).contiguous(), gamma.contiguous()
 
 
+SCAN_TILE = 256  # steps that the stock form composes at once: products of more gates leave fp32's range sooner
+
+
 def gated_scan_ops(gate, drive, state):
-    """(all states, the last one) of the gated scan in stock ops, by doubling: after k rounds a step holds what the last
-    2^k steps make of it."""
-    p = (gate if gate.ndim == 3 else gate[..., None]).float()
-    s = drive.float()
-    if state is not None:
-        s = torch.cat(((p[:, 0] * state + s[:, 0])[:, None], s[:, 1:]), 1)
-    reach = 1
-    while reach < s.shape[1]:
-        s = torch.cat((s[:, :reach], p[:, reach:] * s[:, :-reach] + s[:, reach:]), 1)
-        p = torch.cat((p[:, :reach], p[:, reach:] * p[:, :-reach]), 1)
-        reach *= 2
-    return s.to(drive.dtype), s[:, -1]
+    """(all states, the last one) of the gated scan in stock ops: tile by tile, each by doubling: after k rounds a step
+    holds what the last 2^k steps make of it. (For a use that the kernels do not take; gates of at most 1, or whose
+    products over a tile are finite.)"""
+    gate = (gate if gate.ndim == 3 else gate[..., None]).float()
+    drive_type, drive = drive.dtype, drive.float()
+    last, done = state, [drive[:, :0]]
+    for lo in range(0, drive.shape[1], SCAN_TILE):
+        p, s = gate[:, lo:lo + SCAN_TILE], drive[:, lo:lo + SCAN_TILE]
+        if last is not None:
+            s = torch.cat(((p[:, 0] * last + s[:, 0])[:, None], s[:, 1:]), 1)
+        reach = 1
+        while reach < s.shape[1]:
+            s = torch.cat((s[:, :reach], p[:, reach:] * s[:, :-reach] + s[:, reach:]), 1)
+            p = torch.cat((p[:, :reach], p[:, reach:] * p[:, :-reach]), 1)
+            reach *= 2
+        done.append(s)
+        last = s[:, -1]
+    if last is None:
+        last = drive.new_zeros(drive.shape[0], drive.shape[2])
+    return torch.cat(done, 1).to(drive_type), last
 
 
 def stock_scan_gradients(gate, drive, state, g_out, g_last):
-    """The gradients of gate, drive and state (or None) in stock ops, for a backward that must itself be
-    differentiable; an upstream gradient may be None."""
-    given = [(i, g) for i, g in enumerate((g_out, g_last)) if g is not None]
+    """The gradients of gate, drive and state (or None) of the gated scan, for a backward that must itself be
+    differentiable; an upstream gradient may be None. They are products of two scans, the states and the same
+    recurrence from the end, g_t = dh_t + a_{t+1} g_{t+1}, in fp32: the kernels' own on the device, so that they hold
+    wherever those do, the stock form elsewhere; everything around them is stock ops."""
+    from .field import gated_scan
 
-    def fn(a, u, *first):
-        outs = gated_scan_ops(a, u, *(first or (None,)))
-        return tuple(outs[i] for i, _ in given)
-
-    inputs = (gate, drive) if state is None else (gate, drive, state)
-    got = _stock_grads(fn, inputs, tuple(g for _, g in given))
-    return (*got, *[None] * (3 - len(got)))
+    scan = gated_scan if drive.is_cuda else lambda *args: gated_scan_ops(*args)[0]
+    a, u = gate.float(), drive.float()
+    g_out = torch.zeros_like(u) if g_out is None else g_out.float()
+    after = torch.cat((a[:, 1:], torch.ones_like(a[:, :1])), 1)  # (the last step's carry is g_last)
+    g = scan(after.flip(1), g_out.flip(1), g_last).flip(1)
+    d_gate = d_state = None
+    if gate.requires_grad:
+        before = torch.cat(((torch.zeros_like(u[:, 0]) if state is None else state)[:, None], scan(a, u, state)[:, :-1]), 1)
+        d_gate = g * before
+        d_gate = (d_gate.sum(-1) if gate.ndim == 2 else d_gate).to(gate.dtype)
+    if state is not None:
+        d_state = (a[:, 0] if a.ndim == 3 else a[:, :1]) * g[:, 0]
+    return d_gate, g.to(drive.dtype), d_state
 
 
 class Transition(torch.autograd.Function):

@@ -199,7 +199,7 @@ variable_list scan_gradients(const Tensor& gate, const Tensor& drive, const Tens
   return r;
 }
 
-// The gradients in stock operations, which can be differentiated again: the function of Python that was handed over.
+// The gradients in operations that can be differentiated again: the function of Python that was handed over.
 variable_list stock_scan(const Tensor& gate, const Tensor& drive, const Tensor& state, const Tensor& g_out,
                          const Tensor& g_last) {
   const PyGILState_STATE gil = PyGILState_Ensure();
@@ -460,7 +460,7 @@ PyObject* host_muon_step(PyObject*, PyObject* args) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind_train(addresses of the library's entry points, the steps of a scan's tile, the scan's stock gradients)
+// bind_train(addresses of the library's entry points, the steps of a scan's tile, the scan's differentiable gradients)
 PyObject* host_bind_train(PyObject*, PyObject* args) {
   unsigned long long k[10];
   long long tile;

@@ -380,8 +380,8 @@ def gated_scan(gate: torch.Tensor, drive: torch.Tensor, state_in: Optional[torch
     drive's type, with ``return_state`` also h[:,T-1] in fp32. The recurrence and its gradients run in fp32 and are
     rounded once.
 
-    Gradients flow to gate, drive and state_in. A backward that is to be differentiated itself (``create_graph``) runs
-    stock operations. A gate of 0 starts a new sequence, one of 1 with a drive of 0 passes the state on. Steps are
+    Gradients flow to gate, drive and state_in. A backward that is to be differentiated itself (``create_graph``)
+    runs further scans. A gate of 0 starts a new sequence, one of 1 with a drive of 0 passes the state on. Steps are
     composed in tiles of 256 by products of the gates in fp64: a state that leaves fp32's range and would come back to it
     within a tile may do so. The same inputs give the same bits. Under graph capture the backward pass is refused while a
     graph of the default stream holds the inputs' leaves.

@@ -422,6 +422,65 @@ def test_differentiable_backward(dev, token):
         assert bool(((a.double().cpu() - b).abs() <= 400 * U * (s.abs() + 1)).all())
 
 
+@pytest.mark.parametrize("types", [(F32, F32), (BF16, F32), (F32, BF16)], ids=str)
+@pytest.mark.parametrize("token", [False, True])
+def test_differentiable_backward_over_tiles(dev, token, types):
+    """First derivatives of a backward with create_graph, by the bounds of an ordinary one: many tiles; and gates above 1
+    whose products leave fp32, with states of 0 and gradients that end early."""
+    print(f"[case] gated_scan, create_graph over tiles, token={token} {types}", flush=True)
+    for state in (False, True):
+        gate, drive, first, g_out, g_last = inputs(dev, 2, 1300, 9, token, *types, state, 41)
+        exp = expected(gate, drive, first, g_out, g_last)
+        leaves = [t.detach().requires_grad_() for t in (gate, drive, first) if t is not None]
+        outs = fl.gated_scan(*leaves, return_state=True)
+        got = torch.autograd.grad(outs, leaves, [g_out, g_last], create_graph=True)
+        for name, g, leaf in zip(("gate", "drive", "state_in"), got, leaves):
+            assert g.dtype == leaf.dtype and g.shape == leaf.shape and g.requires_grad
+            close(g.detach(), exp[name], name)
+    T = 2500
+    for value in (1.05, 2.0):
+        gate = torch.full((1, T) if token else (1, T, 3), value, device=dev, dtype=types[0], requires_grad=True)
+        drive = torch.zeros(1, T, 3, device=dev, dtype=types[1])
+        drive[:, T - 10:] = 0.5
+        drive.requires_grad_()
+        up = torch.zeros(1, T, 3, device=dev, dtype=types[1])
+        up[:, 5] = 1.0
+        exp = expected(gate.detach(), drive.detach(), None, up, None)
+        got = torch.autograd.grad(fl.gated_scan(gate, drive), (gate, drive), up, create_graph=True)
+        for name, g in zip(("gate", "drive"), got):
+            close(g.detach(), exp[name], name)
+
+
+@pytest.mark.parametrize("token", [False, True])
+def test_second_derivatives_over_tiles(dev, token):
+    """Of a sum of weighted gradients, against the same in 64 bits on the CPU; bounds as test_differentiable_backward's."""
+    print(f"[case] gated_scan, second derivatives over tiles, token={token}", flush=True)
+    gate, drive, first, w, _ = inputs(dev, 1, 530, 3, token, F32, F32, True, 42)
+    gen = torch.Generator(device=dev).manual_seed(43)
+    weights = [torch.randn(t.shape, device=dev, generator=gen) for t in (gate, drive, first)]
+
+    def second(op, ts, w, weights):
+        leaves = [t.detach().requires_grad_() for t in ts]
+        grads = torch.autograd.grad((op(*leaves) * w).sum(), leaves, create_graph=True)
+        return torch.autograd.grad(sum((g * v).sum() for g, v in zip(grads, weights)), leaves[:2])
+
+    def ops(a, u, s):
+        h, now = [], s
+        for t in range(u.shape[1]):
+            now = (a[:, t, None] if a.ndim == 2 else a[:, t]) * now + u[:, t]
+            h.append(now)
+        return torch.stack(h, 1)
+
+    got = second(fl.gated_scan, (gate, drive, first), w, weights)
+    args = [[t.double().cpu() for t in x] if isinstance(x, list) else x.double().cpu()
+            for x in ([gate, drive, first], w, weights)]
+    exp = second(ops, *args)
+    size = second(ops, *[[t.abs() for t in x] if isinstance(x, list) else x.abs() for x in args])
+    # four scans behind each other, each with 2 x 260 u of a tile and as many tiles as three: 4 * 3 * 520 u of the magnitudes
+    for a, b, s in zip(got, exp, size):
+        assert bool(((a.double().cpu() - b).abs() <= 6240 * U * (s.abs() + 1)).all())
+
+
 def test_stock_form(dev):
     print("[case] gated_scan, stock form", flush=True)
     for token in (False, True):

@@ -202,6 +202,41 @@ def test_stock_scan_gradients():
         assert got[2] is None and got[0].shape == a.shape
 
 
+def _steps64(a, u, s, w, k):
+    """The gradients of the scan, a loop over its steps in float64."""
+    a, u, s = (t.detach().double().requires_grad_() for t in (a, u, s))
+    h, now = [], s
+    for t in range(u.shape[1]):
+        now = (a[:, t, None] if a.ndim == 2 else a[:, t]) * now + u[:, t]
+        h.append(now)
+    return torch.autograd.grad((torch.stack(h, 1) * w).sum() + (now * k).sum(), (a, u, s))
+
+
+@pytest.mark.parametrize("token", [False, True])
+def test_stock_scan_gradients_over_tiles(token):
+    """Gates above 1, whose product over all steps leaves fp32 while those within a tile are finite, states of 0 before a late
+    drive, gradients that end early: everything the formulas form is an ordinary number."""
+    T, late, early = 2500, 2490, 5
+    a = torch.full((1, T) if token else (1, T, 2), 1.05, requires_grad=True)
+    u = torch.zeros(1, T, 2)
+    u[:, late:] = torch.linspace(0.5, 1.5, 20).view(1, 10, 2)
+    u.requires_grad_()
+    s = torch.zeros(1, 2, requires_grad=True)
+    w = torch.zeros(1, T, 2)
+    w[:, early] = 1.0
+    # forward sums at most 10 terms of at most 10 gates each, backward 6 gates: 30 roundings are ample
+    states, last = train.gated_scan_ops(a, u, s)
+    now = torch.zeros(2, dtype=torch.float64)
+    for t in range(late, T):
+        now = 1.05 * now + u.detach().double()[0, t]
+    assert bool(states.isfinite().all()) and torch.allclose(last.double()[0], now, rtol=30 * 2.0 ** -24, atol=0)
+    exp = _steps64(a, u, s, w, torch.zeros(1, 2))
+    got = train.stock_scan_gradients(a, u, s, w, None)
+    for x, y in zip(got, exp):
+        assert bool(x.isfinite().all())
+        assert bool(((x.detach().double() - y).abs() <= 30 * 2.0 ** -24 * y.abs() + 1e-30).all())
+
+
 def test_muon_bookkeeping():
     with pytest.raises(ValueError, match="matrices"):
         fl.Muon([torch.zeros(3)])
