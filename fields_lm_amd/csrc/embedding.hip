@@ -7,6 +7,8 @@
 // shared rows); 32,768 tokens and 131,072 rows in bf16 17 us (8.0 TB/s, part of it from the caches) and 87 us (335 MB).
 #include "fl_common.h"
 
+#include <algorithm>
+
 namespace {
 
 using namespace fl;
@@ -22,6 +24,8 @@ constexpr int kJoinThreads = 512;
 constexpr int kPiece = 32;        // entries of a list that a block takes
 constexpr int kAhead = 8;         // rows that a wave loads before it adds them
 constexpr size_t kPartBytes = (size_t)1 << 28;  // of parts, about; pieces grow where they would take more
+constexpr int64_t kMaxExtras = (int64_t)1 << 22;  // pieces behind their buckets' first: a launch's threads have to be fewer
+                                                  // than 2^32, and the join takes kJoinThreads to each
 constexpr int64_t kMaxTokens = (int64_t)1 << 30, kMaxVocab = (int64_t)kMaxBuckets * kMaxRows, kMaxDim = (int64_t)1 << 24;
 
 // Streaming stores: the gradient of 32,768 tokens, 131,072 rows of 1,024 in bf16 87 us, 108 with plain ones; a third of that
@@ -472,6 +476,8 @@ int embedding(const int64_t* tokens, int64_t n, const void* weight, int64_t V, i
   return FL_OK;
 }
 
+static_assert(kMaxExtras * kJoinThreads < (int64_t)1 << 32 && (kMaxExtras + kMaxBuckets) * kSumThreads < (int64_t)1 << 32, "");
+
 // how a call's tokens are sorted and summed
 struct Plan {
   Sort s;
@@ -491,9 +497,10 @@ Plan plan_of(int64_t n, int64_t V, int64_t D) {
   if (s.chunks < 1) s.chunks = 1;
   const size_t row_bytes = (size_t)D * 4 << s.shift;
   const int64_t most = (int64_t)(kPartBytes / row_bytes) > 32 ? (int64_t)(kPartBytes / row_bytes) : 32;
-  s.piece = (int)(cdiv(cdiv(2 * n, most), kPiece) * kPiece);
+  const int64_t least = std::max(cdiv(2 * n, most), cdiv(n, kMaxExtras));
+  s.piece = (int)(cdiv(least, kPiece) * kPiece);
   if (s.piece < kPiece) s.piece = kPiece;
-  p.extras = n / s.piece;
+  p.extras = n / s.piece;  // (at most kMaxExtras)
   const auto take = [&](size_t bytes) {
     const size_t at = p.bytes;
     p.bytes += (bytes + 15) / 16 * 16;

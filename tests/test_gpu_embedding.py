@@ -294,3 +294,18 @@ def test_more_rows_than_a_launch_holds(dev):
         assert torch.equal(out[at:at + 12], weight[tokens[at:at + 12]])
     some = torch.arange(0, n, 4099, device=dev)
     assert torch.equal(out[some], weight[tokens[some]])
+
+
+@pytest.mark.parametrize("n", [2 ** 28 + 2048, 2 ** 29 + 7])
+def test_gradient_of_more_pieces_than_a_launch_holds(dev, n):
+    """Narrow rows and so many tokens that pieces of 32 would need 2^32 threads and more; whole numbers, whose sums are exact."""
+    print(f"[case] embedding gradient, {n} tokens", flush=True)
+    V = 2048
+    tokens = torch.arange(n, device=dev) % V
+    g = torch.randint(-1, 2, (n, 1), device=dev, dtype=torch.int8).float()
+    weight = torch.zeros(V, 1, device=dev, requires_grad=True)
+    got, = torch.autograd.grad(fl.embedding(tokens, weight), weight, g)
+    whole = n // V * V
+    exp = g[:whole].view(-1, V).sum(0, dtype=torch.float64)
+    exp[:n - whole] += g[whole:, 0].double()
+    assert torch.equal(got[:, 0].double(), exp)

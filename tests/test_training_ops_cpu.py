@@ -172,6 +172,26 @@ def test_abi_refusals():
     assert muon(w=None) == ws == muon(size=0)
 
 
+@pytest.mark.parametrize("V", [1, 2048, 2049, 1 << 23])
+@pytest.mark.parametrize("D", [1, 2, 3, 4, 5, 64])
+def test_gradient_launches_hold_few_enough_threads(D, V):
+    """The gradient's sums are launched with 256 threads to each bucket and each piece behind a bucket's first, their join
+    with 512 to each such piece; a dimension of a launch holds fewer than 2^32 threads. The number of pieces is read off the
+    workspace: 4 bytes each, a bit to each of two pieces' rows in words of 4, and two places of fp32 rows."""
+    lib = nat.load()
+    rows = 1
+    while -(-V // rows) > 2048:
+        rows *= 2
+    buckets = -(-V // rows)
+    for n in (1 << 20, (1 << 28) - 1, 1 << 28, (1 << 28) + 1, 1 << 29, (1 << 30) - 1, 1 << 30):
+        size = lib.fl_embedding_backward_workspace_bytes(n, V, D)
+        fixed = 64 * 2048 * 4 + (buckets + 1) * 4 + 4 + buckets * 4 + n * 8
+        per = 4 + 2 * 4 * -(-rows // 32) + 2 * rows * D * 4
+        extras = (size - fixed) // per  # (rounded up by what the parts are aligned with: 6 times up to 15 bytes)
+        assert 0 < extras <= n // 32 + 8
+        assert extras * 512 < 1 << 32 and (extras + buckets) * 256 < 1 << 32, (n, extras)
+
+
 def test_workspaces_stay_within_groups():
     """Up to 2 GiB where the matrices fit in that, whatever their number."""
     lib = nat.load()
