@@ -145,9 +145,11 @@ def muon_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], mom
 class _Optimizer(torch.optim.Optimizer):
     """What the optimizers share: a step over parameters by group, type and device, with its clip, and checkpoints whose
     states keep their types. A subclass has ``_group`` (what a step reads of its group), ``_check_group``,
-    ``_check_parameter``, ``_wanted`` (a state's types and counts), ``_new`` (fresh states) and ``_step``."""
+    ``_check_parameter``, ``_wanted`` (a state's types and counts), ``_like_parameter`` (which of them have a value to each of
+    the parameter's), ``_new`` (fresh states) and ``_step``."""
 
     _group: Tuple[str, ...] = ()
+    _like_parameter: Tuple[str, ...] = ()
 
     def __init__(self, params, defaults: dict, max_grad_norm: Optional[float]) -> None:
         if max_grad_norm is not None and not float(max_grad_norm) >= 0.0:
@@ -190,11 +192,17 @@ class _Optimizer(torch.optim.Optimizer):
             if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.numel() != count:
                 got = f"{t.numel()} of {t.dtype}" if isinstance(t, torch.Tensor) else repr(t)
                 raise ValueError(f"{name} of a parameter of {p.numel()} values must be {count} of {dtype}, got {got}")
+            if name in self._like_parameter and not self._lies_as(t, p):
+                raise ValueError(f"{name} of a parameter of the shape {tuple(p.shape)} has the shape {tuple(t.shape)}")
+
+    def _lies_as(self, t: torch.Tensor, p: torch.Tensor) -> bool:
+        """Whether a saved state's values belong to the parameter's in their order."""
+        return t.shape == p.shape
 
     def load_state_dict(self, state_dict) -> None:
         """As the base class, hooks included, but every state keeps the type it was saved in, and a learning rate held in
-        a tensor comes to the parameters' device, as states do. What no step can go on from
-        (another optimizer's checkpoint, states of other types or sizes) is refused before anything is changed."""
+        a tensor comes to the parameters' device, as states do, which become contiguous. What no step can go on from
+        (another optimizer's checkpoint, states of other types, sizes or shapes) is refused before anything is changed."""
         loaded: dict = {}
 
         def last(_, final) -> None:  # behind the other pre-hooks: what the base class is about to load
@@ -214,8 +222,8 @@ class _Optimizer(torch.optim.Optimizer):
             ids = [i for g in loaded["param_groups"] for i in g["params"]]
             for i, p in zip(ids, (p for g in self.param_groups for p in g["params"])):
                 if i in loaded["state"]:
-                    self.state[p] = {k: v.detach().to(p.device, copy=True) if isinstance(v, torch.Tensor) else v
-                                     for k, v in loaded["state"][i].items()}
+                    self.state[p] = {k: v.detach().to(p.device, copy=True, memory_format=torch.contiguous_format)
+                                     if isinstance(v, torch.Tensor) else v for k, v in loaded["state"][i].items()}
 
         hooks = (self.register_load_state_dict_pre_hook(last),
                  self.register_load_state_dict_post_hook(first, prepend=True))
@@ -266,6 +274,7 @@ class AdamW(_Optimizer):
     """
 
     _group = ("lr", "betas", "eps", "weight_decay", "state_bits")
+    _like_parameter = ("exp_avg", "exp_avg_sq")
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
@@ -285,6 +294,9 @@ class AdamW(_Optimizer):
         if bits == 8:
             wanted.update(exp_avg_scale=(torch.float32, blocks), exp_avg_sq_scale=(torch.float32, blocks))
         return wanted
+
+    def _lies_as(self, t: torch.Tensor, p: torch.Tensor) -> bool:
+        return super()._lies_as(t, p) or t.ndim == 1  # (a step goes value by value)
 
     def _new(self, p: torch.Tensor, group: dict) -> dict:
         new = dict(device=p.device)
@@ -317,6 +329,7 @@ class Muon(_Optimizer):
     """
 
     _group = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "adjust_lr")
+    _like_parameter = ("momentum_buffer",)
 
     def __init__(self, params, lr: Union[float, torch.Tensor] = 1e-3, momentum: float = 0.95, nesterov: bool = True,
                  weight_decay: float = 0.1, *, steps: int = 5,

@@ -288,3 +288,37 @@ def test_muon_bookkeeping():
         opt.load_state_dict(adam.state_dict())
     with pytest.raises(ValueError, match="lacks"):
         adam.load_state_dict(opt.state_dict())
+
+
+@pytest.mark.parametrize("make,names", [(lambda p: fl.Muon([p]), ("momentum_buffer",)),
+                                        (lambda p: fl.AdamW([p]), ("exp_avg", "exp_avg_sq"))], ids=["Muon", "AdamW"])
+def test_states_of_other_shapes_and_strides(make, names):
+    """A state of as many values in another shape belongs to other positions: refused, and nothing is changed. One of other
+    strides is loaded as the contiguous one that a step takes."""
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    opt = make(p)
+    turned = torch.arange(12.0).view(4, 3)
+    rest = {} if len(names) == 1 else {"step": torch.ones((), dtype=torch.int64)}
+    saved = opt.state_dict()
+    for wrong in (turned, turned.view(2, 6), turned.view(1, 3, 4), turned.view(3, 4)[None].transpose(0, 1)):
+        for name in names:
+            state = {**rest, **{n: torch.zeros(3, 4) for n in names}, name: wrong}
+            with pytest.raises(ValueError, match="shape"):
+                opt.load_state_dict({**saved, "state": {0: state}})
+            assert not opt.state
+    opt.load_state_dict({**saved, "state": {0: {**rest, **{n: turned.t() for n in names}}}})
+    for name in names:
+        got = opt.state[p][name]
+        assert got.is_contiguous() and torch.equal(got, turned.t())
+
+
+def test_flat_states():
+    """AdamW goes value by value, and takes a state that lies flat; a flat momentum says nothing of rows and columns."""
+    p = torch.nn.Parameter(torch.zeros(3, 4))
+    adam, muon = fl.AdamW([p]), fl.Muon([p])
+    flat = torch.arange(12.0)
+    adam.load_state_dict({**adam.state_dict(), "state": {0: dict(step=torch.ones((), dtype=torch.int64), exp_avg=flat,
+                                                                 exp_avg_sq=flat)}})
+    assert torch.equal(adam.state[p]["exp_avg"].view(-1), flat)
+    with pytest.raises(ValueError, match="shape"):
+        muon.load_state_dict({**muon.state_dict(), "state": {0: dict(momentum_buffer=flat)}})
