@@ -41,6 +41,7 @@ import torch.nn.functional as F
 
 from . import _native as nat
 from ._dispatch import KERNEL_DTYPES, eager, free_rounding, no_grad_needed, plain_call, plain_linear
+from ._train import gated_scan_ops
 from .embedding import MAX_ROWS, embedding
 from .field import (FieldBlock, RMSNorm, _linear_residual, boundary_scan, gate_residual_norm, gated_scan, rms_norm,
                     rms_norm_takes, swiglu)
@@ -1023,12 +1024,13 @@ class BoundaryStateMixer(nn.Module):
         h = self.norm(x)
         z = self.down(h).float()
         boundary = self._boundary(h, tokens)
-        if not no_grad_needed(boundary, z) and eager(boundary, z):
-            state, last = gated_scan(1.0 - boundary, boundary[..., None] * z, return_state=True)
-            out = x + self.up(torch.cat((z, state), dim=-1).to(x.dtype))
-            return (out, last) if return_state else out
-        state, last = boundary_scan((1.0 - boundary).contiguous(), (boundary[..., None] * z).contiguous(),
-                                    return_state=True)
+        gate, drive = 1.0 - boundary, boundary[..., None] * z
+        if no_grad_needed(gate, drive) or not drive.is_cuda:
+            state, last = boundary_scan(gate.contiguous(), drive.contiguous(), return_state=True)
+        elif eager(boundary, z):
+            state, last = gated_scan(gate, drive, return_state=True)
+        else:  # (boundary_scan has no gradient)
+            state, last = gated_scan_ops(gate, drive, None)
         out = x + self.up(torch.cat((z, state), dim=-1).to(x.dtype))
         return (out, last) if return_state else out
 

@@ -98,6 +98,62 @@ def test_the_recurrence_passes_its_gradient(dev):
     assert float((full - less).norm()) > 0.05 * float(less.norm())
 
 
+def _contexts():
+    import contextlib
+
+    from torch.utils._python_dispatch import TorchDispatchMode
+    from torch.utils.flop_counter import FlopCounterMode
+
+    class Watch(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    return {"nothing": contextlib.nullcontext, "a dispatch mode": Watch, "a flop counter": lambda: FlopCounterMode(display=False)}
+
+
+@pytest.mark.parametrize("watched", ["nothing", "a dispatch mode", "a flop counter", "selective checkpoints",
+                                     "torch.func", "compilation"])
+def test_the_recurrence_passes_its_gradient_to_whatever_watches(dev, watched):
+    """Where the kernels do not run the gradient is that of stock operations: both round the recurrence's 300 steps, each at
+    most by 2 u of what a sum of magnitudes is, and the rest alike: 1,000 u of the norm."""
+    print(f"[case] softpatch gradient under {watched}", flush=True)
+    mixer = small_model(dev).softpatch
+    gen = torch.Generator(device=dev).manual_seed(6)
+    x = torch.randn(2, 300, 128, device=dev, generator=gen)
+    tokens = torch.zeros(2, 300, dtype=torch.long, device=dev)
+    w = torch.randn(2, 300, 128, device=dev, generator=gen)
+    named = dict(mixer.named_parameters())
+
+    def gradients(run):
+        out = run(x)
+        return torch.autograd.grad((out * w).sum(), list(named.values()))
+
+    want = gradients(lambda y: mixer(y, tokens))
+    if watched == "selective checkpoints":
+        import functools
+
+        from torch.utils.checkpoint import CheckpointPolicy, checkpoint, create_selective_checkpoint_contexts
+
+        contexts = functools.partial(create_selective_checkpoint_contexts,
+                                     lambda ctx, op, *a, **k: CheckpointPolicy.PREFER_RECOMPUTE)
+        got = gradients(lambda y: checkpoint(mixer, y, tokens, use_reentrant=False, context_fn=contexts))
+    elif watched == "compilation":
+        got = gradients(lambda y: torch.compile(mixer, backend="aot_eager")(y, tokens))
+    elif watched == "torch.func":
+        def loss(params):
+            return (torch.func.functional_call(mixer, params, (x, tokens)) * w).sum()
+
+        got = list(torch.func.grad(loss)({n: p.detach() for n, p in named.items()}).values())
+        with pytest.raises(RuntimeError):  # a batched tensor says of no gradient: refused, not lost
+            torch.vmap(lambda a, t: mixer(a[None], t[None])[0])(x, tokens)
+    else:
+        with _contexts()[watched]():
+            got = gradients(lambda y: mixer(y, tokens))
+    for (name, _), a, b in zip(named.items(), got, want):
+        assert float((a - b).norm()) <= 1000 * U * float(b.norm()), name
+    assert float(dict(zip(named, got))["down.weight"].norm()) > 0
+
+
 def test_training_steps(dev):
     """Every parameter gets a gradient and a step, Muon's is muon_step's, and checkpoints carry on."""
     print("[case] training steps", flush=True)
