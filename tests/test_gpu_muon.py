@@ -150,6 +150,132 @@ def test_steps_and_coefficients(dev, steps, abc):
         check(fl.orthogonalize(x, steps=steps, coefficients=abc), x, steps, abc)
 
 
+def divided(fn, l):
+    """|fn[l_i, l_j]|, the divided differences of a polynomial; its slope where two are close."""
+    f, d = fn(l), l[:, None] - l[None, :]
+    close = d.abs() < 1e-6 * l.abs().max()
+    mid, h = (l[:, None] + l[None, :]) / 2, 1e-5 * l.abs().max()
+    slope = (fn(mid + h) - fn(mid - h)) / (2 * h)
+    return torch.where(close, slope, (f[:, None] - f[None, :]) / torch.where(close, 1.0, d)).abs()
+
+
+def held(k):
+    """Of a product over k terms, relative to |L| |R| (one of them the Frobenius, one the spectral norm): what is stored of it
+    is two parts of 11 bits, 2^-22 off at most; the product of both low parts, left out, is as much; sums in fp32 are off
+    by sqrt(k) u and their scales by 4 u. Mirroring half a square makes that sqrt(2) as much at most."""
+    return 1.5 * (2.0 ** -21 + (math.sqrt(k) + 4) * U)
+
+
+def off_at_most(x, steps, abc, eps=1e-7):
+    """Of the Frobenius norm of one matrix's error, to first order, from its own singular values s; l = s^2. Everything of a
+    stage is a function of A, so that in A's eigenvectors an error E of what is held passes on entry by entry: that of A with
+    the divided differences of the factor still to come, times q s, what it meets on its right; that of a step's P as
+    itself in the product of the factors and as A P E + E P A in the next A; that of X by those of s -> Q(s^2) s, which
+    are, of a matrix that is not symmetric, (f_i - f_j) / (s_i - s_j), (f_i + f_j) / (s_i + s_j) and f_i / s_i."""
+    a, b, c = abc
+    m, n = min(x.shape), max(x.shape)
+    s = torch.linalg.svdvals(x.double().cpu())
+    s = s / (s.square().sum().sqrt() + eps)
+
+    def p(l):
+        return a + b * l + c * l * l
+
+    def factor(k):  # of k steps, from A's eigenvalues before them
+        def q(l):
+            out = torch.ones_like(l)
+            for _ in range(k):
+                out, l = out * p(l), l * p(l) ** 2
+            return out
+        return q
+
+    def size(v):
+        return float(v.square().sum().sqrt())
+
+    def top(v):
+        return float(v.abs().max())
+
+    err = 0.0
+    for k in stages(steps):
+        l, q = s * s, torch.ones_like(s)
+        f = factor(k)(l) * s
+        plus = (f[:, None] + f[None, :]) / (s[:, None] + s[None, :]).clamp_min(1e-300)
+        of_x = max(top(divided(lambda t: factor(k)(t * t) * t, s)), top(plus), top(factor(k)(l)))
+        total = of_x * (err + 2.0 ** -22 * size(s))
+        e_a = held(n) * size(s) * top(s)
+        for e in range(k):
+            total += float((divided(factor(k - e), l) * (q * s).abs()[None, :]).max()) * e_a
+            pl = p(l)
+            after = l * pl * pl
+            rest = factor(k - e - 1)(after)
+            e_p = (abs(c) * held(m) * size(l) * top(l) + 1.5 * 2.0 ** -21 * size(pl) +
+                   4 * U * (abs(a) * math.sqrt(m) + abs(b) * size(l)))
+            total += top(rest * q) * e_p * top(s)
+            if e:
+                total += held(m) * size(q) * top(pl) * top(rest) * top(s)  # the product of the factors, as it is held
+            e_a = (2 * top(l) * top(pl) * e_p + held(m) * size(l) * top(pl) * top(pl) + held(m) * size(l * pl) * top(pl))
+            q, l = q * pl, after
+        err = total + held(m) * min(size(q) * top(s), top(q) * size(s))
+        s = (q * s).abs()
+    return err
+
+
+def beyond(got, x, steps, abc):
+    """How far a matrix is past that and its type's rounding, and both, relative to the result's norm."""
+    exp = polar64(x, steps, abc)
+    size, bound = float(exp.norm()), off_at_most(x, steps, abc)
+    return float((got.double() - exp).norm()) / size - bound / size - half_step(got.dtype), bound / size
+
+
+def spectrum(dev, shape, seed):
+    """Singular values over six decades."""
+    gen = torch.Generator(device="cpu").manual_seed(seed)
+    m = min(shape)
+    u, v = (torch.linalg.qr(torch.randn(k, m, generator=gen, dtype=torch.float64))[0] for k in shape)
+    return ((u * torch.logspace(0, -6, m, dtype=torch.float64)) @ v.t()).float().to(dev)
+
+
+ABCS = [ABC, (1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.0, -1.5, 0.5)]
+NEAR_SHAPES = [(1, 1), (1, 9), (9, 1), (7, 5), (33, 200), (130, 60), (257, 255), (640, 640), (1000, 301)]
+# at most this much of the result, so that the bound says something: small singular values that the usual coefficients
+# raise by 3.4 a step, over more than five steps, may end as far off as they are large
+SAYS = 0.3
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 4, 5, 6, 7, 10])
+@pytest.mark.parametrize("abc", ABCS, ids=str)
+def test_near_at_every_step(dev, steps, abc):
+    print(f"[case] orthogonalize, by its own singular values: {steps} steps of {abc}", flush=True)
+    tried = 0
+    for shape in NEAR_SHAPES:
+        for i, kind in enumerate(("plain", "rows", "low", "wide")):
+            x = spectrum(dev, shape, steps) if kind == "wide" else matrices(dev, shape, 10 * steps + i, kind)
+            for dtype in (F32, BF16):
+                y = x.to(dtype)
+                far, bound = beyond(fl.orthogonalize(y, steps=steps, coefficients=abc), y, steps, abc)
+                assert far <= 0 or bound > SAYS, (shape, kind, dtype, far, bound)
+                tried += bound <= SAYS
+    assert tried >= (20 if steps > 7 and abc == ABC else 50)
+
+
+@pytest.mark.parametrize("shape", [(3, 1024, 1100), (40, 300, 200), (18, 500, 130)], ids=str)
+def test_near_in_large_tiles(dev, shape):
+    """Enough matrices for tiles of 128; in bf16 each value is, besides, the nearest to one within the bound."""
+    print(f"[case] orthogonalize, by their own singular values: {shape}", flush=True)
+    x = matrices(dev, shape, 7)
+    for steps in (5, 7):
+        got = fl.orthogonalize(x, steps=steps)
+        for i in range(shape[0]):
+            far, bound = beyond(got[i], x[i], steps, ABC)
+            assert far <= 0 and bound <= SAYS, (i, steps, far, bound)
+    y = x.bfloat16()
+    got = fl.orthogonalize(y)
+    for i in range(shape[0]):
+        exp = polar64(y[i])
+        off = (got[i].double() - exp).abs()
+        assert bool((off <= half_step(BF16) * exp.abs() + 1.01 * off_at_most(y[i], 5, ABC)).all())
+    assert all(torch.equal(fl.orthogonalize(y), got) for _ in range(3))
+
+
 def test_stacks_and_strides(dev):
     print("[case] orthogonalize, stacks and strides", flush=True)
     x = matrices(dev, (3, 2, 50, 70), 5)

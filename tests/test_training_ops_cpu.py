@@ -322,3 +322,48 @@ def test_flat_states():
     assert torch.equal(adam.state[p]["exp_avg"].view(-1), flat)
     with pytest.raises(ValueError, match="shape"):
         muon.load_state_dict({**muon.state_dict(), "state": {0: dict(momentum_buffer=flat)}})
+
+
+def _polar_of_high_parts(x, steps, abc):
+    """Steps whose products' operands have the 11 bits of fp16."""
+    def high(t):
+        return (t * 1024).half().float() / 1024
+
+    tall = x.shape[0] > x.shape[1]
+    y = x.t() if tall else x
+    y = (y / (y.double().norm() + 1e-7)).float()
+    for _ in range(steps):
+        y = high(y)
+        gram = high(y @ y.t())
+        y = high(abc[0] * torch.eye(len(y)) + abc[1] * gram + abc[2] * (gram @ gram)) @ y
+    return y.t() if tall else y
+
+
+@pytest.mark.parametrize("steps", [1, 2, 3, 5, 7, 10])
+def test_the_bound_of_orthogonalization_finds_mistakes(steps):
+    """What the GPU tests' bound lets pass is neither zeros nor a step fewer nor, where errors are not magnified past
+    it, operands of 11 bits."""
+    import test_gpu_muon as muon
+
+    cpu = torch.device("cpu")
+    found = {"zeros": 0, "fewer": 0, "high": 0}
+    for abc in muon.ABCS:
+        for shape in ((7, 5), (33, 200), (130, 60), (150, 140)):
+            for kind in ("plain", "rows", "low", "wide"):
+                x = muon.spectrum(cpu, shape, steps) if kind == "wide" else muon.matrices(cpu, shape, steps, kind)
+
+                def far(got):
+                    return muon.beyond(got, x, steps, abc)[0]
+
+                right = muon.polar64(x, steps, abc)
+                bound = muon.beyond(right, x, steps, abc)[1]
+                assert far(right.float()) <= 0
+                if bound > muon.SAYS:
+                    continue
+                assert far(torch.zeros_like(right)) > 0
+                found["zeros"] += 1
+                if abc == muon.ABC:  # (the others stand still where they have arrived)
+                    assert far(muon.polar64(x, steps - 1, abc)) > 0
+                    found["fewer"] += 1
+                found["high"] += far(_polar_of_high_parts(x, steps, abc)) > 0
+    assert found["zeros"] >= 48 and found["fewer"] >= 8 and found["high"] >= (48 if steps <= 3 else 20), found
