@@ -1080,6 +1080,12 @@ def _kind(block: nn.Module) -> str:
     return "field"
 
 
+# Rows and gradient, us, kernels | stock: 65,536 rows of 1,024 fp32 values 66 | 53 with 192 tokens, 67 | 66 with 384, 67 | 76
+# with 512; 131,072 rows 117 | 89 with 64 and 121 | 116 with 384. Of smaller weights both are host time (52 | 47 up to 512
+# tokens, 52 | 76 with 1,024), and in bf16 the stock sums are rounded to it one by one (300 tokens of four rows: 5.7e-3 off for 1.6e-3).
+_FEW_TOKENS, _LARGE_WEIGHT = 384, 1 << 25
+
+
 class FieldTokenSystem(nn.Module):
     """Embedding, 24 blocks, softpatch after block ``patch_position``, final norm, tied head."""
 
@@ -1125,13 +1131,14 @@ class FieldTokenSystem(nn.Module):
         return [_kind(b) for b in self.blocks]
 
     def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
-        """The tokens' rows; where a gradient is wanted through ``fl_embedding``, whose gradient is the same bits every
-        time."""
+        """The tokens' rows; where a gradient is wanted through ``fl_embedding``, whose gradient is summed in fp32 and the
+        same bits every time. A few tokens' gradient of a large fp32 weight is the stock one: zeros with some rows added."""
         emb = self.emb
         weight = emb.weight
         if (plain_call(emb, nn.Embedding) and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse
                 and not no_grad_needed(weight) and weight.dtype in KERNEL_DTYPES and tokens.dtype == torch.int64
                 and 0 < weight.shape[0] <= MAX_ROWS and weight.shape[1] > 0
+                and not (weight.dtype == torch.float32 and tokens.numel() < _FEW_TOKENS and weight.numel() >= _LARGE_WEIGHT)
                 and eager(weight, tokens)):
             return embedding(tokens, weight, padding_idx=emb.padding_idx)
         return emb(tokens)

@@ -201,3 +201,23 @@ def test_the_largest_vocabulary(dev, rows):
     got, = torch.autograd.grad(x, core.emb.weight, up)
     assert torch.equal(got[[0, 7]], up[0, [0, 2]]) and torch.equal(got[rows - 1], up[0, 1] + up[0, 3])
     assert int(got.ne(0).any(1).sum()) == 3
+
+
+@pytest.mark.parametrize("rows,tokens,dtype,kernels", [(1 << 15, 383, torch.float32, False), (1 << 15, 384, torch.float32, True),
+                                                       ((1 << 15) - 1, 383, torch.float32, True),
+                                                       (1 << 15, 383, torch.bfloat16, True)], ids=str)
+def test_a_few_tokens_of_a_large_weight(dev, monkeypatch, rows, tokens, dtype, kernels):
+    """Whose gradient the kernels make, and that either is the sum of the tokens' (whole numbers, exact in any order)."""
+    print(f"[case] model's embedding of {rows} rows, {tokens} tokens, {dtype}", flush=True)
+    core = small_model(dev)
+    core.emb = torch.nn.Embedding(rows, 1024, device=dev, dtype=dtype)
+    gen = torch.Generator(device=dev).manual_seed(8)
+    ids = torch.randint(0, 9, (1, tokens), device=dev, generator=gen) * (rows // 9)
+    up = torch.randint(-1, 2, (1, tokens, 1024), device=dev, generator=gen).to(dtype)
+    calls = []
+    monkeypatch.setattr(M, "embedding", lambda *a, **k: (calls.append(1), fl.embedding(*a, **k))[1])
+    x = core._embed(ids)
+    assert bool(calls) == kernels and torch.equal(x, core.emb.weight[ids])
+    got, = torch.autograd.grad(x, core.emb.weight, up)
+    exp = torch.zeros(rows, 1024, device=dev).index_add_(0, ids[0], up[0].float())
+    assert torch.equal(got.float(), exp)
