@@ -7,8 +7,8 @@
 // P = a I + b A + c A^2 a step is X <- P X and makes A into P A P, and all of these commute and are symmetric. So k steps
 // are one product X X^T, products of symmetric matrices (of which the lower half is computed) and one product
 // (P_k .. P_1) X. A's small eigenvalues are squares of X's singular values, and a step lets their error grow a^2-fold
-// (12 for the usual a) where X's own grows a-fold: after at most kStage steps X is formed and A taken from it anew,
-// which keeps results as near to the formula's as steps on X in fp32 are.
+// (12 for the usual a) where X's own grows a-fold: after at most kStage steps, one where sums are short, X is formed and A
+// taken from it anew, which keeps results as near to the formula's as steps on X in fp32 are.
 //
 // Every matrix is held as two fp16 planes, high and low part of its values times a power of two (22 bits), and a product
 // is three of matrix instructions, high high + high low + low high, summed in fp32: bf16 operands end 3% from the result
@@ -25,6 +25,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -35,13 +36,16 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half_t;
 
-constexpr int kStage = 3;      // steps between two products with X
+constexpr int kStage = 3;      // steps between two products with X at most, where one
+                               // does not have to do:
+constexpr int64_t kLongSide = 256;  // where the short side is this long, or results are bf16
 constexpr int kPad = 32;       // rows of planes are a multiple of this long, zeros behind the matrix
 constexpr int kSquares = 5;    // m x m matrices of the workspace
 constexpr int kCopyTile = 64;  // of the tile that is laid out by a block
 constexpr int kTable = 56;     // matrices to a launch that sets up their table
 constexpr int kNormChunk = 4096;  // values of a block of the norm (one matrix of 256 x 632: 3.6 us, 12 with 16,384 values read one by one)
 constexpr int64_t kMaxMatrices = 1 << 20, kMaxSide = 1 << 20, kMaxValues = (int64_t)1 << 30;
+constexpr int kFold = 16;      // steps of 32 columns
 constexpr int kTile = 128, kSmallTile = 64;  // rows and columns of a product's tile
 constexpr int64_t kSlots = 512, kIdle = 150;  // tiles that run at a time (two to a CU)
 // (110 matrices of a model: groups of 1 GiB 15.3 ms, 2 GiB 14.7, 4 GiB 14.6)
@@ -328,7 +332,7 @@ __device__ __forceinline__ int tile_of(int block) {
 // line of 128 bytes, high parts before low ones, whose eight packs change places by half the row's number, so that sixteen
 // rows' equal packs lie in different banks of the 64.
 template <int KIND, int TILE>
-__global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(const Mat* __restrict__ mats, int n,
+__global__ __launch_bounds__(threads_of<TILE>(), TILE == kTile ? 2 : 1) void fl_muon_product_kernel(const Mat* __restrict__ mats, int n,
                                                                              int tiles, const Product q,
                                                                              const Update u) {
   constexpr bool kSymmetric = KIND <= kSquare;
@@ -415,48 +419,66 @@ __global__ __launch_bounds__(threads_of<TILE>()) void fl_muon_product_kernel(con
   };
 
   const int wr = wave / WC * (TILE / WR), wc = wave % WC * (TILE / WC);
-  f32x16 acc[NI][NJ];
+  const f32x16 none = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  f32x16 acc[NI][NJ], part[NI][NJ];
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+    for (int j = 0; j < NJ; ++j) acc[i][j] = part[i][j] = none;
 
   const char* l_at = s_tile + (wr + (lane & 31)) * kLine;
   const char* r_at = s_tile + kOperand + (wc + (lane & 31)) * kLine;
-  load(0, 0);
-  int buffer = 0;
-  for (int s = 0; s < steps; s += BATCH, buffer ^= 1) {
-    __builtin_amdgcn_s_waitcnt(0);
-    __syncthreads();  // the buffer is there, and nobody reads the other one any more
-    if (s + BATCH < steps) load(buffer ^ 1, s + BATCH);
+  // Sums: 512 columns at a time, which a second sum takes (a wide matrix's 1,286 columns in one: 3 times the error). While
+  // that is empty it holds the products with low parts, which are 2^-11 of the others and round nothing of them off.
+  const auto multiply = [&](int at, auto first) {
 #pragma unroll
-    for (int b = 0; b < BATCH; ++b) {
-      if (BATCH > 1 && s + b >= steps) break;
-      const int at = buffer * kBuffer + b * kStepBytes;
+    for (int kk = 0; kk < 2; ++kk) {
+      f16x8 l[NI][2], r[NJ][2];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        f16x8 l[NI][2], r[NJ][2];
+      for (int p = 0; p < 2; ++p) {
+        const int pack = ((p * 4 + kk * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 + at;
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          const int pack = ((p * 4 + kk * 2 + (lane >> 5)) ^ ((lane >> 1) & 7)) * 16 + at;
+        for (int j = 0; j < NJ; ++j) r[j][p] = *reinterpret_cast<const f16x8*>(r_at + j * 32 * kLine + pack);
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) r[j][p] = *reinterpret_cast<const f16x8*>(r_at + j * 32 * kLine + pack);
+        for (int i = 0; i < NI; ++i) l[i][p] = *reinterpret_cast<const f16x8*>(l_at + i * 32 * kLine + pack);
+      }
 #pragma unroll
-          for (int i = 0; i < NI; ++i) l[i][p] = *reinterpret_cast<const f16x8*>(l_at + i * 32 * kLine + pack);
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          f32x16& low = decltype(first)::value ? acc[i][j] : part[i][j];
+          part[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][0], part[i][j], 0, 0, 0);
+          low = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][1], low, 0, 0, 0);
+          low = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][1], r[j][0], low, 0, 0, 0);
         }
+    }
+  };
+  const auto fold = [&] {
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
+    for (int i = 0; i < NI; ++i)
 #pragma unroll
-          for (int j = 0; j < NJ; ++j) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][0], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][0], r[j][1], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(l[i][1], r[j][0], acc[i][j], 0, 0, 0);
-          }
+      for (int j = 0; j < NJ; ++j) {
+        acc[i][j] += part[i][j];
+        part[i][j] = none;
+      }
+  };
+  load(0, 0);
+  int buffer = 0, s = 0;
+  const auto sum = [&](int end, auto first) {
+    for (; s < end; s += BATCH, buffer ^= 1) {
+      __builtin_amdgcn_s_waitcnt(0);
+      __syncthreads();  // the buffer is there, and nobody reads the other one any more
+      if (s + BATCH < steps) load(buffer ^ 1, s + BATCH);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        if (BATCH > 1 && s + b >= steps) break;
+        multiply(buffer * kBuffer + b * kStepBytes, first);
       }
     }
-  }
+    fold();
+  };
+  sum(min(steps, kFold), std::true_type());
+  while (s < steps) sum(min(steps, s + kFold), std::false_type());
 
   if constexpr (KIND == kFinal) {
     const float lr = u.muon ? (u.lr_ptr ? *u.lr_ptr : u.lr) : 0.f;
@@ -595,15 +617,25 @@ int64_t square_tiles(int64_t m, int tile) {
 // as kIdle.
 int64_t cost(int64_t tiles) { return tiles ? cdiv(tiles, kSlots) * kSlots + kIdle : 0; }
 
+// Stages of one step lose nothing on steps on X in fp32, those of three nothing visible in bf16 and little where sums
+// are long. Error over that of steps on X, 1 step | 3: 65 x 65 0.7 | 2.2, 160 x 1,900 0.7 | 1.5, 200 x 200 0.5 | 1.4,
+// 256 x 256 0.5 | 1.3, 256 x 632 0.5 | 1.0, 512 x 512 0.5 | 1.1, 1,024 x 1,536 0.4 | 0.8; us, one of 64 x 64 76 | 92, 2,000
+// of 100 x 100 1,425 | 1,584, 200 of 128 x 1,024 876 | 567, one of 256 x 632 127 | 123, 110 matrices of a model 19,200 |
+// 14,600. Matrices of both kinds are taken in groups of their own, so that a matrix's result is a matter of itself alone.
+enum Pick { kAll, kLongSides, kShortSides };
+bool picked(Pick pick, int64_t rows, int64_t cols) {
+  return rows * cols != 0 && (pick == kAll || (std::min(rows, cols) < kLongSide) == (pick == kShortSides));
+}
+
 // As many matrices as kGroupBytes hold, or fewer where their tiles fill the card better: 21 matrices of 1,024 x 2,438 (756
 // tiles, two rounds of which the second is half empty) take 110 us a product, 14 of them 55. All that are left are taken at
 // once unless two groups are better.
-Group group_from(int64_t i, int64_t n, const int64_t* rows, const int64_t* cols) {
+Group group_from(int64_t i, int64_t n, const int64_t* rows, const int64_t* cols, Pick pick) {
   Group g = {i, 0, 0, 0}, best = g;
   int64_t tiles = 0, best_tiles = 0;
   bool all = true;
   for (; g.end < n; ++g.end) {
-    if (rows[g.end] * cols[g.end] == 0) continue;
+    if (!picked(pick, rows[g.end], cols[g.end])) continue;
     const size_t bytes = planes_bytes(rows[g.end], cols[g.end]);
     if (g.count && g.planes + bytes > kGroupBytes) {
       all = false;
@@ -668,10 +700,10 @@ struct Launch {
   }
 };
 
-// The steps of a group whose X is laid out.
+// The steps of a group whose X is laid out, at most `stage` between two products with X.
 template <int TILE>
-void newton_schulz(const Launch<TILE>& launch, int steps, double a, double b, double c, const Bounds& bounds) {
-  const int stages = (int)cdiv(steps, kStage);
+void newton_schulz(const Launch<TILE>& launch, int stage, int steps, double a, double b, double c, const Bounds& bounds) {
+  const int stages = (int)cdiv(steps, stage);
   float x_scale = scale_for(1.0);
   int source = 0;
   for (int st = 0, k = 0; st < stages; ++st) {
@@ -746,18 +778,18 @@ void newton_schulz(const Launch<TILE>& launch, int steps, double a, double b, do
   }
 }
 
-int run(int64_t n, const void* const* g, void* const* p, float* const* buf, const int64_t* rows, const int64_t* cols,
-        const double* lr_scale, int steps, double a, double b, double c, double eps, const Update& u, void* workspace,
+int run(Pick pick, int64_t n, const void* const* g, void* const* p, float* const* buf, const int64_t* rows,
+        const int64_t* cols, const double* lr_scale, int steps, double a, double b, double c, double eps, const Update& u, void* workspace,
         hipStream_t s) {
   Bounds bounds;
   if (!bounds_of(steps, a, b, c, &bounds)) return FL_ERR_INVALID_ARGUMENT;
   std::vector<int64_t> order;
   for (int64_t from = 0; from < n;) {
-    const Group group = group_from(from, n, rows, cols);
+    const Group group = group_from(from, n, rows, cols, pick);
     if (group.count == 0) break;
     order.clear();
     for (int64_t i = from; i < group.end; ++i)
-      if (rows[i] * cols[i]) order.push_back(i);
+      if (picked(pick, rows[i], cols[i])) order.push_back(i);
     from = group.end;
     // the longest first, whose tiles take longest
     std::stable_sort(order.begin(), order.end(), [&](int64_t i, int64_t j) {
@@ -803,15 +835,26 @@ int run(int64_t n, const void* const* g, void* const* p, float* const* buf, cons
     const int count = (int)group.count;
     fl_muon_norm_kernel<<<(unsigned)first_norm, 256, 0, s>>>(mats, count, u, sums);
     fl_muon_copy_kernel<<<(unsigned)first_copy, 256, 0, s>>>(mats, count, u, sums, eps, scale_for(1.0));
-    const int squares = (int)first_square, applies = (int)first_apply;
+    const int squares = (int)first_square, applies = (int)first_apply, stage = pick == kShortSides ? 1 : kStage;
     if (tile == kTile)
-      newton_schulz(Launch<kTile>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+      newton_schulz(Launch<kTile>{mats, count, squares, applies, u, s}, stage, steps, a, b, c, bounds);
     else
-      newton_schulz(Launch<kSmallTile>{mats, count, squares, applies, u, s}, steps, a, b, c, bounds);
+      newton_schulz(Launch<kSmallTile>{mats, count, squares, applies, u, s}, stage, steps, a, b, c, bounds);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return hip_status(e);
   }
   return FL_OK;
+}
+
+int run(int64_t n, const void* const* g, void* const* p, float* const* buf, const int64_t* rows, const int64_t* cols,
+        const double* lr_scale, int steps, double a, double b, double c, double eps, const Update& u, void* workspace,
+        hipStream_t s) {
+  const auto of = [&](Pick pick) {
+    return run(pick, n, g, p, buf, rows, cols, lr_scale, steps, a, b, c, eps, u, workspace, s);
+  };
+  if (u.is_bf16) return of(kAll);
+  const int status = of(kLongSides);
+  return status == FL_OK ? of(kShortSides) : status;
 }
 
 // no exception leaves a C entry (the host's lists are all that allocates)
@@ -838,11 +881,12 @@ extern "C" {
 size_t fl_orthogonalize_workspace_bytes(int64_t n, const int64_t* rows, const int64_t* cols) {
   if (!lists_ok(n, rows, cols)) return 0;
   size_t most = 256;
-  for (int64_t i = 0; i < n;) {
-    const Group g = group_from(i, n, rows, cols);
-    most = g.bytes() > most ? g.bytes() : most;
-    i = g.end;
-  }
+  for (Pick pick : {kAll, kLongSides, kShortSides})
+    for (int64_t i = 0; i < n;) {
+      const Group g = group_from(i, n, rows, cols, pick);
+      most = g.bytes() > most ? g.bytes() : most;
+      i = g.end;
+    }
   return most;
 }
 

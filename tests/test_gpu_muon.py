@@ -47,8 +47,8 @@ def polar64(x, steps=5, abc=ABC, eps=1e-7):
     return x.mT if tall else x
 
 
-def stages(steps):
-    n = -(-steps // 3)
+def stages(steps, most=3):
+    n = -(-steps // most)
     out, left = [], steps
     for i in range(n):
         out.append(-(-left // (n - i)))
@@ -172,6 +172,7 @@ def off_at_most(x, steps, abc, eps=1e-7):
     the divided differences of the factor still to come, times q s, what it meets on its right; that of a step's P as
     itself in the product of the factors and as A P E + E P A in the next A; that of X by those of s -> Q(s^2) s, which
     are, of a matrix that is not symmetric, (f_i - f_j) / (s_i - s_j), (f_i + f_j) / (s_i + s_j) and f_i / s_i."""
+    # (a stage has one step where the short side of an fp32 matrix is below 256, at most three elsewhere)
     a, b, c = abc
     m, n = min(x.shape), max(x.shape)
     s = torch.linalg.svdvals(x.double().cpu())
@@ -195,7 +196,7 @@ def off_at_most(x, steps, abc, eps=1e-7):
         return float(v.abs().max())
 
     err = 0.0
-    for k in stages(steps):
+    for k in stages(steps, 1 if x.dtype == F32 and m < 256 else 3):
         l, q = s * s, torch.ones_like(s)
         f = factor(k)(l) * s
         plus = (f[:, None] + f[None, :]) / (s[:, None] + s[None, :]).clamp_min(1e-300)
@@ -255,6 +256,55 @@ def test_near_at_every_step(dev, steps, abc):
                 assert far <= 0 or bound > SAYS, (shape, kind, dtype, far, bound)
                 tried += bound <= SAYS
     assert tried >= (20 if steps > 7 and abc == ABC else 50)
+
+
+def steps32(x, steps=5, abc=ABC):
+    """The formula's steps on one X in fp32."""
+    tall = x.shape[0] > x.shape[1]
+    y = x.t().contiguous() if tall else x
+    y = (y / (y.double().norm() + 1e-7)).float()
+    for _ in range(steps):
+        gram = y @ y.t()
+        y = abc[0] * y + (abc[1] * gram + abc[2] * (gram @ gram)) @ y
+    return y.t() if tall else y
+
+
+@pytest.mark.parametrize("shape", [(8, 10), (18, 15), (24, 25), (33, 20), (65, 65), (100, 100), (11, 1286), (1654, 40), (160, 1900),
+                                   (200, 200), (255, 300), (256, 256), (300, 1500), (700, 600)], ids=str)
+def test_errors_are_those_of_steps_in_fp32(dev, shape):
+    """In the mean square over matrices that look like gradients, at most twice as far as steps on X in fp32. What is held
+    of a value is off by 0.35 of fp32's last place in the mean square (up to half of it, less where the low part is
+    small) where fp32 is off by 0.29; a sum is rounded once to 16 terms where fp32's is to each; matrices of more
+    than one step a stage are those whose sums, a few hundred terms at least, make up for what a stage adds."""
+    print(f"[case] orthogonalize, errors beside fp32 {shape}", flush=True)
+    gen = torch.Generator(device=dev).manual_seed(sum(shape))
+    count = 32 if max(shape) < 300 else 6
+    x = torch.randn(count, *shape, device=dev, generator=gen)
+    x = x * torch.exp(0.5 * torch.randn(count, shape[0], 1, device=dev, generator=gen))
+    x = x * torch.exp(0.5 * torch.randn(count, 1, shape[1], device=dev, generator=gen))
+    x = x + 0.5 * torch.matmul(torch.randn(count, shape[0], 4, device=dev, generator=gen),
+                               torch.randn(count, 4, shape[1], device=dev, generator=gen))
+    got = fl.orthogonalize(x)
+    own = stock = 0.0
+    for i in range(count):
+        exp = polar64(x[i])
+        own += float(((got[i].double() - exp).norm() / exp.norm()) ** 2)
+        stock += float(((steps32(x[i]).double() - exp).norm() / exp.norm()) ** 2)
+    assert own <= 4 * stock, math.sqrt(own / stock)
+    print(f"[measured] {math.sqrt(own / stock):.2f} of fp32's {math.sqrt(stock / count):.1e}", flush=True)
+
+
+def test_results_are_a_matter_of_the_matrix_alone(dev):
+    """In lists of long and short sides, in either tile, in fp32 and in bf16."""
+    print("[case] muon_step, long and short sides", flush=True)
+    shapes = [(255, 300), (256, 300), (300, 255), (40, 40), (257, 256), (1, 700), (0, 3), (1024, 1024)] + [(64, 200)] * 30
+    for dtype in (F32, BF16):
+        params, grads, bufs = model(dev, dtype, 21, shapes)
+        before = [(p.clone(), b.clone()) for p, b in zip(params, bufs)]
+        fl.muon_step(params, grads, bufs, lr=0.1)
+        for (p, b), g, now, buf in zip(before, grads, params, bufs):
+            fl.muon_step([p], [g], [b], lr=0.1)
+            assert torch.equal(p, now) and torch.equal(b, buf)
 
 
 @pytest.mark.parametrize("shape", [(3, 1024, 1100), (40, 300, 200), (18, 500, 130)], ids=str)
