@@ -218,16 +218,17 @@ __device__ __forceinline__ float look_back(const uint64_t* words, int64_t back, 
   }
 }
 
-// What enters a tile's segments: `first` through the products of those before each (BACK: behind each), whose ends are in `ends`.
-// The products are the bare ones, which may have left fp64: a state of 0 passes none, and for infinite ones they are formed again.
+// What enters a tile's segments: `first` through the products of those before each (BACK: behind each), whose ends are in
+// `ends`. The products are the bare ones, which may have left fp64: a state of 0 passes none, and for an infinite one, in its
+// own lane, they are formed again.
 template <int SEGS, bool BACK>
 __device__ __forceinline__ void enter(const double (*each_p)[kChannels], const double (*run_p)[kChannels],
                                       float (*ends)[kChannels], int ch, float first) {
-  if (__any(fabsf(first) == __builtin_inff())) {
+  if (fabsf(first) == __builtin_inff()) {
     double run = 1.0;
     for (int i = 0; i < SEGS; ++i) {
       const int seg = BACK ? SEGS - 1 - i : i;
-      if (first != 0.f) ends[seg][ch] = (float)through(run, first, ends[seg][ch]);
+      ends[seg][ch] = (float)through(run, first, ends[seg][ch]);
       run = kept(run * each_p[seg][ch], run == 0.0 || each_p[seg][ch] == 0.0);
     }
     return;

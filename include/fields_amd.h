@@ -550,7 +550,7 @@ int fl_embedding_backward(const int64_t* tokens, int64_t n, const void* g, int g
  * fl_gated_scan_backward: from the forward's inputs and starts, and g_out [B, T, C] of drive_dtype and g_state [B, C]
  *   (either may be NULL): g_drive [B, T, C], g_gate of the gate's shape (or NULL), g_state_in [B, C] (or NULL), each of
  *   its tensor's type.
- * Maths in fp32, rounded once. B, C up to 2^24, T up to 2^30. Workspace 16-byte aligned, no initial contents needed (0
+ * Maths in fp32 (products of a tile's gates in fp64), rounded once. B, C up to 2^24, T up to 2^30. Workspace 16-byte aligned, no initial contents needed (0
  * bytes: NULL will do). Tiles of a chain wait for those before them; a wait that does not end within 2^20 polls leaves
  * its tile's results NaN.
  */

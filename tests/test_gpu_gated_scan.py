@@ -348,6 +348,22 @@ def test_infinite_states_before_small_gates(dev, value):
     close(out[..., 1:], exp["out"], "out")
 
 
+def test_infinities_stay_in_their_channel(dev):
+    """Bits of the channels beside an infinite state, forward and back."""
+    print("[case] gated_scan, infinities beside", flush=True)
+    gate, drive, first, g_out, g_last = inputs(dev, 2, 1500, 70, False, F32, F32, True, 51, low=1e-3)
+    wild, wild_last = first.clone(), g_last.clone()
+    wild[:, ::7], wild_last[:, ::7] = float("inf"), float("-inf")
+    rest = torch.arange(70, device=dev) % 7 != 0
+    kept = None
+    for f, k in ((first, g_last), (wild, wild_last)):
+        leaves = [t.detach().requires_grad_() for t in (gate, drive, f)]
+        outs = fl.gated_scan(*leaves, return_state=True)
+        got = [t[..., rest] for t in (*(o.detach() for o in outs), *torch.autograd.grad(outs, leaves, [g_out, k]))]
+        kept = kept or got
+        assert all(torch.equal(a, b) for a, b in zip(got, kept))
+
+
 def test_many_sequences(dev):
     """More threads than one dimension of a launch holds: 2^23 chains of one tile back, 2^26 of one step forward."""
     print("[case] gated_scan, 2^23 + 5 sequences", flush=True)
