@@ -1138,8 +1138,8 @@ class FieldTokenSystem(nn.Module):
         if (plain_call(emb, nn.Embedding) and emb.max_norm is None and not emb.scale_grad_by_freq and not emb.sparse
                 and not no_grad_needed(weight) and weight.dtype in KERNEL_DTYPES and tokens.dtype == torch.int64
                 and 0 < weight.shape[0] <= MAX_ROWS and weight.shape[1] > 0
-                and not (weight.dtype == torch.float32 and tokens.numel() < _FEW_TOKENS and weight.numel() >= _LARGE_WEIGHT)
-                and eager(weight, tokens)):
+                and eager(weight, tokens)
+                and not (weight.dtype == torch.float32 and tokens.numel() < _FEW_TOKENS and weight.numel() >= _LARGE_WEIGHT)):
             return embedding(tokens, weight, padding_idx=emb.padding_idx)
         return emb(tokens)
 
