@@ -2,9 +2,11 @@
 // tokens k_n,
 //   out[n] = s W[k_n],    dW[v] = s sum over n with k_n = v of g[n], in an order of the tokens' alone.
 //
-// Both directions are bound by memory, each row touched once: 8,192 tokens of 1,024 fp32 values take 11 us forward
-// (6.0 TB/s), and with 16,384 rows 33 us back (100 MB: 18 us of sums at 5.6 TB/s behind 10 us of sorting, 5 us of joining
-// shared rows); 32,768 tokens and 131,072 rows in bf16 17 us (8.0 TB/s, part of it from the caches) and 87 us (335 MB).
+// Both directions are bound by memory, each row touched once: 8,192 tokens of 1,024 fp32 values take 12 us forward
+// (5.4 TB/s), and with 16,384 rows 35 us back (100 MB: 18 us of sums at 5.7 TB/s behind 11 us of sorting, 6 us of joining
+// shared rows); 32,768 tokens and 131,072 rows in bf16 23 us (5.8 TB/s) and 107 us (335 MB: 81 us of sums at 4.1 TB/s, 14 and
+// 12). A row that many tokens share is joined by one wave: 32,768 tokens, 16,384 rows of 1,024 fp32 values, both directions,
+// 97 us; with a quarter of the tokens alike 137, half of them 175, all 265 (as padding 80).
 #include "fl_common.h"
 
 #include <algorithm>
@@ -28,8 +30,8 @@ constexpr int64_t kMaxExtras = (int64_t)1 << 22;  // pieces behind their buckets
                                                   // than 2^32, and the join takes kJoinThreads to each
 constexpr int64_t kMaxTokens = (int64_t)1 << 30, kMaxVocab = (int64_t)kMaxBuckets * kMaxRows, kMaxDim = (int64_t)1 << 24;
 
-// Streaming stores: the gradient of 32,768 tokens, 131,072 rows of 1,024 in bf16 87 us, 108 with plain ones; a third of that
-// as fast either way.
+// Streaming stores: a fifth less time for the gradient of 32,768 tokens, 131,072 rows of 1,024 in bf16; a third of that as
+// fast either way.
 __device__ __forceinline__ void store_once(u32x4_any* p, u32x4 v) { __builtin_nontemporal_store(v, p); }
 __device__ __forceinline__ void store_once(u32x2_any* p, u32x2 v) { __builtin_nontemporal_store(v, p); }
 

@@ -15,9 +15,9 @@
 // published its end. Tiles are taken in the order in which blocks start, from a counter: a tile waits only for tiles that
 // are running or done, so that every wait ends. The words are cleared by a launch before.
 //
-// Bound by memory: B=8, T=2,048, C=1,024 in fp32 44 us forward (4.6 TB/s) and 60 us back (5.6 TB/s); B=1, T=65,536, fp32 gates
-// and bf16 drives 99 us (5.4 TB/s) and 174 us (5.4 TB/s), where three launches over the same tiles (maps, composition,
-// steps) took 2.8 ms. Of the forward's blocks with a gate a channel two fit a CU (190 registers a lane), by a limit: with
+// Bound by memory, in rounds of blocks that read, wait and write in turn: B=8, T=2,048, C=1,024 in fp32 47 us forward
+// (4.3 TB/s) and 68 us back (5.0 TB/s); B=1, T=65,536, fp32 gates and bf16 drives 106 us (5.1 TB/s) and 185 us (5.1 TB/s),
+// where three launches over the same tiles (maps, composition, steps) took 2.8 ms. Of the forward's blocks with a gate a channel two fit a CU (190 registers a lane), by a limit: with
 // three more tiles look back at once and further (42.5 us for the first in place of 39.5 without gradients kept). With a
 // gate a token four do (126), and of the backward's blocks, twice as many threads, one does (158 and 128).
 #include "fl_common.h"
@@ -88,8 +88,8 @@ struct Four<bf16_bits> {
   __device__ __forceinline__ void fill(float x) { w[0] = w[1] = bf16_bits_of(x) * 0x10001u; }
   __device__ __forceinline__ float operator[](int i) const { return i & 1 ? bf16_hi(w[i >> 1]) : bf16_lo(w[i >> 1]); }
 };
-// Streaming stores: B=8, T=2,048, C=1,024 in fp32 with gradients 109 us, 123 with plain ones, B=1, T=65,536 285 and 292; what
-// reads the result next is as fast behind either (2 to 270 MB).
+// Streaming stores: 11% less time for B=8, T=2,048, C=1,024 in fp32 with gradients, 2% for B=1, T=65,536; what reads the result
+// next is as fast behind either (2 to 270 MB).
 __device__ __forceinline__ void store4(float* p, int64_t left, const float* v) {
   if (left >= 4) {
     const u32x4 r = {__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])};

@@ -14,10 +14,11 @@
 // is three of matrix instructions, high high + high low + low high, summed in fp32: bf16 operands end 3% from the result
 // where singular values are alike, and as far as it is long where a few are strong.
 //
-// Bound by the matrix units: 64 squares of 1,024 x 1,024 take 157 to 165 us a product (1.4 to 1.5 PFLOP/s of fp16, of which a
-// third counts; registers alone reach 1.7 on such values), the matrix units 88% busy while a CU has tiles. 110 matrices of
-// a model, 0.27 G values, take 14.7 ms, steps on X in fp32 library products 80; a single 256 x 632 matrix, 20 dependent
-// launches, 123 us (1,175). What was tried and is no faster (110 matrices, 15.9 ms at the time): tiles of 256 x 256 (15.2
+// Bound by the operands, past the L2: 64 squares of 1,024 x 1,024 take 157 to 165 us a product (1.4 to 1.5 PFLOP/s of fp16, of
+// which a third counts; registers alone reach 1.7 on such values), and 110 matrices of a model, 0.27 G values, 14.7 ms
+// (steps on X in fp32 library products 80), in which matrix instructions hold their units for 41 to 55% of the cycles in which a
+// CU has work: a product with X moves 10.6 GB in 2.1 ms (5.0 TB/s), five times its operands, the others move 2.8 to 4.3
+// TB/s. A single 256 x 632 matrix, 20 dependent launches, takes 123 us (1,175). What was tried and is no faster (110 matrices, 15.9 ms at the time): tiles of 256 x 256 (15.2
 // to 19.0), 256 x 128 with three buffers (18.3), 128 x 128 with four and one block to a CU (17.8), all of a step's reads
 // ahead of its products (17.2), wave priority (1% slower), waves above the diagonal left idle (4% slower).
 #include "fl_common.h"
