@@ -100,8 +100,8 @@ def orthogonalize(x: torch.Tensor, *, steps: int = 5, coefficients: Tuple[float,
     X = x / (|x| + eps), |x| the Frobenius norm, ``steps`` (1 to 64) times X = a X + (b A + c A^2) X with A = X X^T
     (X^T X for a tall matrix), (a, b, c) the ``coefficients``.
 
-    Everything is computed in fp32 and in products of 22 bits and rounded once, to x's type; a matrix of zeros stays
-    zeros, one with NaN or infinities becomes NaN. Coefficients with which singular values, or a step's factor, could
+    Everything is computed in fp32 and in products of 22 bits, whose errors are about those of the same steps in fp32 (0.4
+    to 1.3 times), and rounded once, to x's type; a matrix of zeros stays zeros, one with NaN or infinities becomes NaN. Coefficients with which singular values, or a step's factor, could
     pass 1024 are refused. Not differentiable. A call takes up to 2 GiB of workspace, or what its largest matrix needs.
     """
     a, b, c = coefficients
